@@ -203,6 +203,29 @@ int nb200_op_q4k_matvec(float *out, const float *x, const uint8_t *w_blocks, uin
 int nb200_op_q4k_quantize_blocks(uint8_t *blocks, const float *x, uint64_t nblocks);
 int nb200_op_q4k_matvec_blocks(float *out, const uint8_t *x_blocks, const uint8_t *w_blocks, uint32_t n, uint32_t d);
 
+/* ---- operators on device memory ----
+ * Pointers named in these calls lie in the memory of the current CUDA device (cudaSetDevice) unless the comment says host; `stream` is a cudaStream_t of that
+ * device, NULL its default stream.  A call checks its arguments, queues its kernels and returns: it allocates no device memory, waits for nothing, keeps
+ * nothing (what lies in host arrays has been read when it returns), and may be captured into a CUDA graph.  Calls on different streams are independent.
+ * What is refused is refused before anything is queued. */
+#define NB200_T_F32 0u
+#define NB200_T_BF16 1u
+#define NB200_T_F16 2u
+
+/* Log probabilities of given tokens, entropy and the `top` (<= 32) most probable alternatives of `rows` rows of logits: row r is the `vocab` numbers of `type` at
+ * logits + r * row_stride elements, any alignment of the type.  tokens [rows]: 32-bit or 64-bit ids (token_bytes 4 or 8); an id outside [0, vocab) has log
+ * probability NaN.  logprob [rows], entropy [rows], top_logprob [rows][top], top_id [rows][top] may each be NULL.  Alternatives are ordered by logit, descending,
+ * equal ones by id.  Natural logarithms; sums in fp32.  A logit of -inf is a masked token; a row of nothing else has log probabilities -inf and entropy 0; a row
+ * with NaN or +inf has NaN. */
+int nb200_dev_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_id, const void *logits, uint32_t type, uint64_t row_stride,
+                             uint32_t rows, uint32_t vocab, const void *tokens, uint32_t token_bytes, uint32_t top, void *stream);
+
+/* Copies pages of a cache: page src[i] over page dst[i], i < n, in each of n_pools pools; page p of pool k is the page_bytes[k] bytes at pools[k] + p *
+ * page_stride[k], p < n_pages[k].  All arrays are on the host.  A source may appear many times (a prompt's page forked for several continuations); a destination
+ * that is a source too or appears twice is refused. */
+int nb200_dev_pages_copy(void *const *pools, const uint64_t *page_bytes, const uint64_t *page_stride, const uint32_t *n_pages, uint32_t n_pools,
+                         const uint32_t *src, const uint32_t *dst, uint32_t n, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

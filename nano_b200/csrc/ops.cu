@@ -1,0 +1,431 @@
+// ops.cu -- operators on device memory: log probabilities of given tokens, copies of cache pages, and their C entry points.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "family.h"
+#include "ops.h"
+
+namespace nb {
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// Log probabilities.  For a row x of V logits with maximum M, Z = sum exp(x_i - M):
+//     log p_t = (x_t - M) - log Z,    H = log Z + (1/Z) sum exp(x_i - M) (M - x_i),    alternatives in the order (x descending, index ascending).
+// One pass: every thread keeps (m, z, s) of what it has seen -- z = sum exp(x - m), s = sum exp(x - m) (x - m) -- and rescales them when m grows; two such
+// triples join as  z = z1 f1 + z2 f2,  s = f1 (s1 + z1 (m1 - m)) + f2 (...),  f = exp(m_i - m).  Sums are fp32.
+// The alternatives ride on the same pass: each warp keeps its 32 best in registers (lane i the i-th), as 64-bit keys (ordered bits of x, complement of the index),
+// and looks at a vector of logits one by one only when its largest reaches the k-th best that any warp of the block has.
+// A row belongs to a cluster of C blocks, whose parts are joined over distributed shared memory: one launch, no workspace, no order of arrival in the result.
+// -inf (a masked token) adds nothing; a row of nothing else has log probabilities -inf and entropy 0; NaN or +inf anywhere makes a row's numbers NaN (its order
+// of alternatives counts NaN as -inf).
+// ------------------------------------------------------------------------------------------------
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpMaxCluster = 16;
+constexpr int kLpUnroll = 4;          // 16-byte vectors in flight per thread
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void widen(const uint4 &v, float *x) { x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w); }
+    static __device__ __forceinline__ float one(const float *p) { return __ldg(p); }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void widen(const uint4 &v, float *x) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+};
+template <> struct Elem<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void widen(const uint4 &v, float *x) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i])); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+    }
+    static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
+};
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+constexpr float kLog2e = 1.4426950408889634f;
+
+// keys: larger is better.  Bits of x ordered as unsigned numbers (-0 as 0, NaN as -inf), then the complement of the index; 0 is "none"
+__device__ __forceinline__ unsigned long long top_key(float x, uint32_t idx) {
+    x = x != x ? -INFINITY : x + 0.0f;
+    uint32_t u = __float_as_uint(x);
+    u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    return ((unsigned long long)u << 32) | (uint32_t)~idx;
+}
+__device__ __forceinline__ float key_value(unsigned long long k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
+
+// 32 lanes' keys into descending order
+__device__ __forceinline__ unsigned long long warp_sort(unsigned long long v) {
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (uint32_t size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (uint32_t step = size >> 1; step > 0; step >>= 1) {
+            const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, step);
+            const bool down = (lane & size) == 0, first = (lane & step) == 0;
+            v = (down == first) == (v > o) ? v : o;
+        }
+    return v;
+}
+// the 32 best of two descending lists, descending
+__device__ __forceinline__ unsigned long long warp_merge(unsigned long long a, unsigned long long b) {
+    const uint32_t lane = threadIdx.x & 31u;
+    b = __shfl_xor_sync(0xffffffffu, b, 31u);
+    unsigned long long v = a > b ? a : b;
+#pragma unroll
+    for (uint32_t step = 16; step > 0; step >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, step);
+        v = ((lane & step) == 0) == (v > o) ? v : o;
+    }
+    return v;
+}
+
+struct TopList {
+    unsigned long long list = 0, kth = 0;
+    uint32_t top;
+    __device__ __forceinline__ void take(unsigned long long key) {          // every lane brings one key (0: none)
+        uint32_t more = __ballot_sync(0xffffffffu, key > kth);
+        if (!more) return;
+        if (__popc(more) > 5) list = warp_merge(list, warp_sort(key));
+        else
+            for (; more; more &= more - 1u) {
+                const unsigned long long k = __shfl_sync(0xffffffffu, key, __ffs(more) - 1), up = __shfl_up_sync(0xffffffffu, list, 1);
+                if (!(list > k)) list = (threadIdx.x & 31u) == 0 || up > k ? k : up;
+            }
+        kth = __shfl_sync(0xffffffffu, list, top - 1u);
+    }
+};
+
+struct Sums { float m, z, s; };
+__device__ __forceinline__ Sums join(const Sums &a, const Sums &b) {
+    Sums r;
+    r.m = fmaxf(a.m, b.m);
+    const float da = a.m - r.m, db = b.m - r.m, fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
+    r.z = a.z * fa + b.z * fb;
+    r.s = (fa > 0.0f ? fa * fmaf(a.z, da, a.s) : 0.0f) + (fb > 0.0f ? fb * fmaf(b.z, db, b.s) : 0.0f);
+    if (r.m == INFINITY) r.z = NAN;
+    return r;
+}
+__device__ __forceinline__ Sums shfl(const Sums &a, int step) {
+    return Sums{__shfl_xor_sync(0xffffffffu, a.m, step), __shfl_xor_sync(0xffffffffu, a.z, step), __shfl_xor_sync(0xffffffffu, a.s, step)};
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+template <typename W>
+__device__ __forceinline__ W peer_word(const W *mine, uint32_t rank) {          // the word at the same place of block `rank`'s shared memory
+    uint32_t at = (uint32_t)__cvta_generic_to_shared(mine), there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    W v;
+    if constexpr (sizeof(W) == 8) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(there) : "memory");
+    else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+
+// grid (C, rows), clusters of C blocks
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads, 2) k_logprobs(const LogprobArgs a, const uint32_t C) {
+    constexpr int N = Elem<T>::N;
+    __shared__ unsigned long long lists[kLpWarps][32];
+    __shared__ float red[3][kLpWarps], part[3];
+    __shared__ float floor_s;          // no alternative lies below it: the largest k-th best of the block's warps
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = C > 1 ? cluster_rank() : 0u;
+    const T *row = static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.row_stride;
+    if (TOP) { if (tid == 0) floor_s = -INFINITY; __syncthreads(); }
+
+    long long token = -1;
+    float xt = NAN;
+    if (rank == 0 && tid == 0 && a.tokens) {          // (asked for now, used at the end)
+        token = a.token_bytes == 8 ? static_cast<const long long *>(a.tokens)[blockIdx.y] : (long long)static_cast<const int *>(a.tokens)[blockIdx.y];
+        if (token >= 0 && token < (long long)a.vocab) xt = Elem<T>::one(row + token);
+    }
+
+    // the row as 16-byte vectors of memory: vector v holds the elements [v N - head, v N - head + N), the first and the last possibly in part
+    const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T)), nv = (head + a.vocab + N - 1u) / N, each = (nv + C - 1u) / C;
+    const uint32_t v0 = min(nv, rank * each), v1 = min(nv, v0 + each);
+    const uint4 *vecs = reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15u);
+    Sums t{-FLT_MAX, 0.0f, 0.0f};
+    TopList best;
+    best.top = a.top;
+    // (every warp walks as many steps as its first lane has vectors: the list is a warp's work)
+    for (uint32_t vb = v0 + warp * 32u; vb < v1; vb += kLpThreads * kLpUnroll) {
+        uint4 raw[kLpUnroll] = {};
+        float x[kLpUnroll][N], vm[kLpUnroll];
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++) {          // all loads of the step are in flight at once; the row's first and last vector are read by the element
+            const uint32_t v = vb + j * kLpThreads + lane;
+            if (v > 0 && v + 1u < nv && v < v1) raw[j] = __ldg(vecs + v);
+        }
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++) {
+            const uint32_t v = vb + j * kLpThreads + lane;
+            Elem<T>::widen(raw[j], x[j]);
+            if (!(v > 0 && v + 1u < nv && v < v1)) {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const uint32_t i = v * N + e - head;          // wraps below the row's start
+                    x[j][e] = v < v1 && i < a.vocab ? Elem<T>::one(row + i) : -INFINITY;
+                }
+            }
+        }
+        float bm = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++) {
+            vm[j] = x[j][0];
+#pragma unroll
+            for (int e = 1; e < N; e++) vm[j] = fmaxf(vm[j], x[j][e]);
+            bm = fmaxf(bm, vm[j]);
+        }
+        if (bm > t.m) {
+            const float d = t.m - bm, f = ex2(d * kLog2e);
+            t.s = f > 0.0f ? f * fmaf(t.z, d, t.s) : 0.0f; t.z *= f; t.m = bm;
+        }
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float d = x[j][e] - t.m, p = ex2(d * kLog2e);
+                t.z += p;
+                t.s = fmaf(p, fmaxf(d, -1e4f), t.s);          // (p is 0 below -104; -inf would make 0 * -inf of it)
+            }
+        if constexpr (TOP) {
+            const float low = *(volatile float *)&floor_s;
+#pragma unroll
+            for (int j = 0; j < kLpUnroll; j++) {
+                if (!__any_sync(0xffffffffu, !(vm[j] < low))) continue;
+                const uint32_t first = (vb + j * kLpThreads + lane) * N - head;
+                const bool mine = vb + j * kLpThreads + lane < v1;
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const bool in = mine && first + e < a.vocab && !(x[j][e] < low);
+                    if (__any_sync(0xffffffffu, in)) best.take(in ? top_key(x[j][e], first + e) : 0ull);
+                }
+                if (best.kth && lane == 0) {          // (racing warps may leave the smaller of two floors, which is one too)
+                    const float f = key_value(best.kth);
+                    if (f > *(volatile float *)&floor_s) *(volatile float *)&floor_s = f;
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t = join(t, shfl(t, o));
+    if (lane == 0) { red[0][warp] = t.m; red[1][warp] = t.z; red[2][warp] = t.s; }
+    if (TOP) lists[warp][lane] = best.list;
+    __syncthreads();
+    if constexpr (TOP) {
+#pragma unroll
+        for (uint32_t half = kLpWarps / 2; half > 0; half >>= 1) {
+            if (warp < half) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + half][lane]);
+            __syncthreads();
+        }
+    }
+    if (warp == 0) {
+        t = Sums{lane < kLpWarps ? red[0][lane] : -FLT_MAX, lane < kLpWarps ? red[1][lane] : 0.0f, lane < kLpWarps ? red[2][lane] : 0.0f};
+#pragma unroll
+        for (int o = kLpWarps / 2; o > 0; o >>= 1) t = join(t, shfl(t, o));
+        if (lane == 0) { part[0] = t.m; part[1] = t.z; part[2] = t.s; }
+    }
+    if (C > 1) {
+        cluster_sync();
+        if (rank == 0) {
+            if (TOP && warp < C && warp > 0) {          // (the block's own list stays where it is)
+                const unsigned long long k = peer_word(&lists[0][lane], warp);
+                __syncwarp();
+                lists[warp][lane] = k;
+            }
+            if (warp == 0) {
+                t = Sums{lane < C ? peer_word(&part[0], lane) : -FLT_MAX, lane < C ? peer_word(&part[1], lane) : 0.0f, lane < C ? peer_word(&part[2], lane) : 0.0f};
+#pragma unroll
+                for (int o = kLpMaxCluster / 2; o > 0; o >>= 1) t = join(t, shfl(t, o));
+            }
+            if constexpr (TOP) {
+                __syncthreads();
+                for (uint32_t half = C / 2; half > 0; half >>= 1) {
+                    if (warp < half) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + half][lane]);
+                    __syncthreads();
+                }
+            }
+        }
+        cluster_sync();          // nobody leaves while its shared memory is read
+    }
+    if (rank || warp) return;
+    t.m = __shfl_sync(0xffffffffu, t.m, 0); t.z = __shfl_sync(0xffffffffu, t.z, 0); t.s = __shfl_sync(0xffffffffu, t.s, 0);
+    const bool empty = t.z == 0.0f;          // (a NaN is no zero)
+    const float lz = logf(t.z);
+    const uint64_t r = blockIdx.y;
+    if (lane == 0) {
+        if (a.logprob) a.logprob[r] = xt != xt ? NAN : empty ? -INFINITY : (xt - t.m) - lz;
+        if (a.entropy) a.entropy[r] = empty ? 0.0f : lz - t.s / t.z;
+    }
+    if (TOP && lane < a.top) {
+        const unsigned long long k = lists[0][lane];
+        if (a.top_logprob) a.top_logprob[r * a.top + lane] = empty ? -INFINITY : (key_value(k) - t.m) - lz;
+        if (a.top_id) a.top_id[r * a.top + lane] = (int32_t)~(uint32_t)k;
+    }
+}
+
+template <typename T, bool TOP>
+cudaError_t logprobs_launch_t(const LogprobArgs &a, cudaStream_t stream) {
+    const uint32_t nv = (a.vocab + Elem<T>::N - 1u) / Elem<T>::N;
+    // blocks to a row: as long as each thread keeps a vector of it and the device is not full of them
+    uint32_t C = 1;
+    while (C < kLpMaxCluster && nv >= 2u * C * kLpThreads && (uint64_t)a.rows * C < 148u * 4u) C *= 2;
+    if (C > 8) {          // more than eight blocks to a cluster are to be asked for, on every device that runs them
+        cudaError_t e = cudaFuncSetAttribute(k_logprobs<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    for (uint32_t r0 = 0; r0 < a.rows; r0 += 65535u) {          // (the grid's second dimension)
+        LogprobArgs b = a;
+        b.rows = std::min(65535u, a.rows - r0);
+        b.logits = static_cast<const char *>(a.logits) + (uint64_t)r0 * a.row_stride * sizeof(T);
+        if (a.tokens) b.tokens = static_cast<const char *>(a.tokens) + (uint64_t)r0 * a.token_bytes;
+        if (a.logprob) b.logprob += r0;
+        if (a.entropy) b.entropy += r0;
+        if (a.top_logprob) b.top_logprob += (uint64_t)r0 * a.top;
+        if (a.top_id) b.top_id += (uint64_t)r0 * a.top;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(C, b.rows); cfg.blockDim = dim3(kLpThreads); cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_logprobs<T, TOP>, b, C);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Copies of pages.  Pure movement: a block takes 8 KB of one page of one pool, with every load in flight before the first store.  The pairs and the pools
+// travel with the launch, so the call reads no memory of the caller's later and copies nothing to the device.
+// ------------------------------------------------------------------------------------------------
+constexpr uint32_t kCopyThreads = 256, kCopyVecs = 2, kCopyChunk = kCopyThreads * kCopyVecs * 16u;
+template <uint32_t PAIRS>
+struct PageArgs { PagePool pool[kPagePools]; uint32_t src[PAIRS], dst[PAIRS]; };
+template <uint32_t PAIRS, bool VEC>
+__global__ void __launch_bounds__(kCopyThreads) k_pages_copy(const __grid_constant__ PageArgs<PAIRS> a) {
+    const PagePool &p = a.pool[blockIdx.z];
+    const uint64_t at = (uint64_t)blockIdx.x * kCopyChunk;
+    if (at >= p.page_bytes) return;
+    const uint64_t n = min((uint64_t)kCopyChunk, p.page_bytes - at);
+    const char *from = static_cast<const char *>(p.base) + a.src[blockIdx.y] * p.page_stride + at;
+    char *to = static_cast<char *>(p.base) + a.dst[blockIdx.y] * p.page_stride + at;
+    if constexpr (VEC) {
+        uint4 v[kCopyVecs];
+#pragma unroll
+        for (uint32_t i = 0; i < kCopyVecs; i++) { const uint32_t o = (threadIdx.x + i * kCopyThreads) * 16u; if (o < n) v[i] = __ldcs(reinterpret_cast<const uint4 *>(from + o)); }
+#pragma unroll
+        for (uint32_t i = 0; i < kCopyVecs; i++) { const uint32_t o = (threadIdx.x + i * kCopyThreads) * 16u; if (o < n) *reinterpret_cast<uint4 *>(to + o) = v[i]; }
+    } else
+        for (uint32_t o = threadIdx.x; o < n; o += kCopyThreads) to[o] = from[o];
+}
+template <uint32_t PAIRS, bool VEC>
+cudaError_t pages_launch(const PagePool *pools, uint32_t n_pools, const uint32_t *src, const uint32_t *dst, uint32_t n, uint64_t bytes, cudaStream_t stream) {
+    PageArgs<PAIRS> a;
+    for (uint32_t i = 0; i < n_pools; i++) a.pool[i] = pools[i];
+    std::copy(src, src + n, a.src);
+    std::copy(dst, dst + n, a.dst);
+    k_pages_copy<PAIRS, VEC><<<dim3((uint32_t)((bytes + kCopyChunk - 1u) / kCopyChunk), n, n_pools), kCopyThreads, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t logprobs_launch(const LogprobArgs &a, cudaStream_t stream) {
+    if (!a.rows) return cudaSuccess;
+    switch (a.type) {
+        case T_F32: return a.top ? logprobs_launch_t<float, true>(a, stream) : logprobs_launch_t<float, false>(a, stream);
+        case T_BF16: return a.top ? logprobs_launch_t<__nv_bfloat16, true>(a, stream) : logprobs_launch_t<__nv_bfloat16, false>(a, stream);
+        default: return a.top ? logprobs_launch_t<__half, true>(a, stream) : logprobs_launch_t<__half, false>(a, stream);
+    }
+}
+
+cudaError_t pages_copy_launch(const PagePool *pools, uint32_t n_pools, const uint32_t *src, const uint32_t *dst, uint32_t n, cudaStream_t stream, uint32_t *launches) {
+    for (uint32_t p0 = 0; p0 < n_pools; p0 += kPagePools) {
+        const uint32_t np = std::min(kPagePools, n_pools - p0);
+        uint64_t bytes = 0;
+        bool vec = true;
+        for (uint32_t i = 0; i < np; i++) {
+            const PagePool &p = pools[p0 + i];
+            bytes = std::max(bytes, p.page_bytes);
+            vec = vec && ((reinterpret_cast<uintptr_t>(p.base) | p.page_bytes | p.page_stride) & 15u) == 0;
+        }
+        if (!bytes) continue;
+        for (uint32_t i = 0; i < n; i += kPagePairs) {
+            const uint32_t m = std::min(kPagePairs, n - i);
+            cudaError_t e;
+            if (m <= 64u) e = vec ? pages_launch<64, true>(pools + p0, np, src + i, dst + i, m, bytes, stream) : pages_launch<64, false>(pools + p0, np, src + i, dst + i, m, bytes, stream);
+            else e = vec ? pages_launch<kPagePairs, true>(pools + p0, np, src + i, dst + i, m, bytes, stream) : pages_launch<kPagePairs, false>(pools + p0, np, src + i, dst + i, m, bytes, stream);
+            if (e != cudaSuccess) return e;
+            if (launches) ++*launches;
+        }
+    }
+    return cudaSuccess;
+}
+
+}  // namespace nb
+
+using nb::fail;
+
+extern "C" {
+
+int nb200_dev_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_id, const void *logits, uint32_t type, uint64_t row_stride,
+                             uint32_t rows, uint32_t vocab, const void *tokens, uint32_t token_bytes, uint32_t top, void *stream) {
+    if (type > nb::T_F16) return fail(NB200_EINVAL, "logits are fp32, bf16 or fp16 (type %u)", type);
+    if (rows && (!logits || !vocab || vocab > 0x7fffffffu)) return fail(NB200_EINVAL, "bad logits (%u rows of %u)", rows, vocab);
+    if (reinterpret_cast<uintptr_t>(logits) % nb::elem_size(type)) return fail(NB200_EINVAL, "logits are not aligned to their type");
+    if (tokens && token_bytes != 4 && token_bytes != 8) return fail(NB200_EINVAL, "tokens are 32-bit or 64-bit numbers");
+    if (tokens && reinterpret_cast<uintptr_t>(tokens) % token_bytes) return fail(NB200_EINVAL, "tokens are not aligned to their type");
+    if (top > nb::kTopMax || (rows && top > vocab)) return fail(NB200_EINVAL, "%u alternatives asked for: at most %u, and no more than the vocabulary has", top, nb::kTopMax);
+    if (logprob && !tokens) return fail(NB200_EINVAL, "log probabilities need tokens");
+    if (top && !top_logprob && !top_id) top = 0;
+    if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
+    const nb::LogprobArgs a{logits, row_stride, type, rows, vocab, logprob ? tokens : nullptr, token_bytes, top, logprob, entropy, top_logprob, top_id};
+    NB_CK(nb::logprobs_launch(a, static_cast<cudaStream_t>(stream)));
+    return 0;
+}
+
+int nb200_dev_pages_copy(void *const *pools, const uint64_t *page_bytes, const uint64_t *page_stride, const uint32_t *n_pages, uint32_t n_pools, const uint32_t *src,
+                         const uint32_t *dst, uint32_t n, void *stream) {
+    if ((n_pools && (!pools || !page_bytes || !page_stride || !n_pages)) || (n && (!src || !dst))) return fail(NB200_EINVAL, "null argument");
+    try {
+        uint32_t pages = n_pools ? 0xffffffffu : 0u;
+        std::vector<nb::PagePool> list(n_pools);
+        for (uint32_t i = 0; i < n_pools; i++) {
+            if (!pools[i] && page_bytes[i] && n_pages[i]) return fail(NB200_EINVAL, "pool %u is null", i);
+            if (page_bytes[i] > (1ull << 32) || page_stride[i] < page_bytes[i]) return fail(NB200_EINVAL, "pool %u: pages of %llu bytes every %llu", i, (unsigned long long)page_bytes[i], (unsigned long long)page_stride[i]);
+            list[i] = nb::PagePool{pools[i], page_bytes[i], page_stride[i]};
+            pages = std::min(pages, n_pages[i]);
+        }
+        if (!n_pools || !n) return 0;
+        std::vector<bool> used(pages, false);
+        for (uint32_t i = 0; i < n; i++) {
+            if (src[i] >= pages || dst[i] >= pages) return fail(NB200_EINVAL, "pair %u copies page %u to %u: the smallest pool has %u", i, src[i], dst[i], pages);
+            used[src[i]] = true;
+        }
+        for (uint32_t i = 0; i < n; i++) {
+            if (used[dst[i]]) return fail(NB200_EINVAL, "page %u is written and read, or written twice, by one call", dst[i]);
+            used[dst[i]] = true;
+        }
+        if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
+        NB_CK(nb::pages_copy_launch(list.data(), n_pools, src, dst, n, static_cast<cudaStream_t>(stream), nullptr));
+    } catch (const std::bad_alloc &) { return fail(NB200_ENOMEM, "out of host memory"); }
+    return 0;
+}
+
+}  // extern "C"

@@ -33,6 +33,7 @@ EXPORTS = [
     "nb200_lora_load", "nb200_lora_enable", "nb200_lora_unload",
     "nb200_engine_create_tp", "nb200_tp_export", "nb200_tp_attach_ipc", "nb200_tp_attach_local",
     "nb200_engine_create_dir", "nb200_seq_open", "nb200_seq_close", "nb200_step", "nb200_step_timed", "nb200_read_residual",
+    "nb200_dev_token_logprobs", "nb200_dev_pages_copy",
 ]
 
 
@@ -117,6 +118,8 @@ def lib(layered_ok: bool = False):
         L.nb200_step.argtypes = [C.c_void_p, C.c_uint32, u32p, C.c_uint32, u32p, C.c_uint32, f32p]
         L.nb200_step_timed.argtypes = [C.c_void_p, C.c_uint32, u32p, C.c_uint32, C.c_uint32, f32p]
         L.nb200_read_residual.argtypes = [C.c_void_p, C.c_uint32, f32p, C.c_uint32]
+        L.nb200_dev_token_logprobs.argtypes = [C.c_void_p] * 5 + [C.c_uint32, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]
+        L.nb200_dev_pages_copy.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), u32p, C.c_uint32, u32p, u32p, C.c_uint32, C.c_void_p]
         L.nb200_lora_load.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64]
         L.nb200_lora_enable.argtypes = [C.c_void_p, C.c_int]
         L.nb200_lora_unload.argtypes = [C.c_void_p]
