@@ -226,6 +226,38 @@ int nb200_dev_token_logprobs(float *logprob, float *entropy, float *top_logprob,
 int nb200_dev_pages_copy(void *const *pools, const uint64_t *page_bytes, const uint64_t *page_stride, const uint32_t *n_pages, uint32_t n_pools,
                          const uint32_t *src, const uint32_t *dst, uint32_t n, void *stream);
 
+/* A paged key/value cache held in 4 bits.  A pool is n_pages pages of 32 tokens; a page, page_stride bytes after the one before, holds for each of kv_heads heads one
+ * block of 40 * head_dim bytes: key codes, key pairs, value codes, value pairs.  32 neighbouring coordinates x of a token's head share a pair (s, m) of fp16 numbers,
+ * m = min x and s = (max x - min x) / 15, both rounded; a coordinate is the nearest of the sixteen c s + m (5 bits in all).  A group that holds a number beyond +-32768, an infinity or
+ * a NaN stands for NaN.  Where in a block a coordinate lies is told in csrc/kv4.h; bytes of pages may be copied, nothing else in them is to be relied on.
+ * nb200_dev_kv4_write puts row t of keys and values, kv_heads x head_dim numbers of `type` each (strides in numbers), at place slots[t] = page * 32 + place in the page; rows whose
+ * slot lies outside the pool (-1: padding) are skipped; no slot may be given twice.  nb200_dev_kv4_read writes what the places stand for to k and v, zeros for skipped rows. */
+typedef struct nb200_kv4_rows {
+    void *pool; uint64_t page_stride; uint32_t n_pages, kv_heads, head_dim;      /* head_dim: a multiple of 32 up to 256 */
+    uint32_t type, tokens; const int32_t *slots;                                 /* [tokens] */
+    void *k, *v; uint64_t k_token, k_head, v_token, v_head;
+} nb200_kv4_rows;
+int nb200_dev_kv4_write(const nb200_kv4_rows *rows, void *stream);
+int nb200_dev_kv4_read(const nb200_kv4_rows *rows, void *stream);
+
+/* Attention over such a cache: `tokens` queries of each of `batch` sequences, query t of sequence b at position lens[b] - tokens + t of its sequence (the keys and values of the new
+ * tokens have been written before).  lens [batch] counts all its tokens, table [batch][width] (rows table_stride numbers apart) names its pages.  Query head h reads
+ * key/value head h / (heads / kv_heads).  A query sees the keys of positions up to its own, of these only the last `window` (0: all) and those in its own block of `block` positions
+ * counted from 0 (0: all); scores are scale q . k, with softcap > 0 softcap tanh(scale q . k / softcap); sinks [heads] (or NULL) join the softmax denominator as exp(sink).
+ * A query at a negative position, or one that sees no key, has an output of zeros; a length beyond width * 32 counts as that; the tokens of a page number outside the pool
+ * are not seen.  A key or value that stands for NaN makes the rows that see it NaN, and no others.
+ * type: of q and out, fp32 or bf16.  Either way products take operands of 11 bits (c s + m, queries, softmax weights rounded to fp16 significands) and sum in fp32.
+ * Strides are in numbers; out's base and strides are multiples of four numbers.  The workspace's bytes do not depend on what lies in device memory;
+ * two calls that may run at the same time need one each. */
+typedef struct nb200_kv4_attention {
+    const void *q; void *out; uint64_t q_batch, q_token, q_head, o_batch, o_token, o_head;
+    const void *pool; uint64_t page_stride; uint32_t n_pages, kv_heads, head_dim;                 /* head_dim 32, 64, 96, 128 or 256 */
+    uint32_t type, batch, tokens, heads, width; uint64_t table_stride; const int32_t *table, *lens; const float *sinks;
+    float scale, softcap; uint32_t window, block;
+} nb200_kv4_attention;
+int nb200_dev_kv4_attention_workspace(const nb200_kv4_attention *p, uint64_t *bytes);
+int nb200_dev_kv4_attention(const nb200_kv4_attention *p, void *workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

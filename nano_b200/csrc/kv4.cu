@@ -1,0 +1,732 @@
+// kv4.cu -- writing, reading and attending to a paged key/value cache held in 4 bits (layout and formulas: kv4.h).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "family.h"
+#include "kv4.h"
+
+namespace nb {
+namespace {
+
+__device__ __forceinline__ void pdl_enter4() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ------------------------------------------------------------------------------------------------
+// Writing.  Four lanes hold a group, eight coordinates each: the extremes take two shuffles, a lane's codes are one word of a key row (two halves of a
+// word of a value row).  The code is round_half_even((x - m) / s) of the numbers themselves: the fp32 quotient decides it unless it lies within 1e-4 of a
+// border between two codes (its own error is below 1e-5), where the quotient is taken in 64 bits.
+// ------------------------------------------------------------------------------------------------
+constexpr float kKv4Most = 32768.0f;          // c s + m of a written group stays inside fp16
+constexpr uint32_t kRowThreads = 256;
+
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+
+// the place of token t in the pool, or -1
+__device__ __forceinline__ long long kv4_place(const Kv4Rows &a, uint32_t t) {
+    if (a.slots) {
+        const int s = a.slots[t];
+        return s >= 0 && (uint32_t)s / kKv4Page < a.n_pages ? (long long)s : -1;
+    }
+    const uint32_t pos = a.pos0 + t + (a.pos_ptr ? *a.pos_ptr : 0u), page = a.table[pos / kKv4Page];
+    return page < a.n_pages ? (long long)page * kKv4Page + pos % kKv4Page : -1;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) k_kv4_write(const Kv4Rows a) {
+    pdl_enter4();
+    const uint32_t n = a.D / kKv4Group, b = threadIdx.x & 3u;
+    const uint64_t items = (uint64_t)a.T * a.G * n, item = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 2;
+    const bool live = item < items, value = blockIdx.y != 0;
+    const uint32_t t = live ? (uint32_t)(item / (a.G * n)) : 0u, e = live ? (uint32_t)(item % (a.G * n)) : 0u, g = e / n, j = e % n;
+    const long long place = live ? kv4_place(a, t) : -1;
+    float x[8] = {};
+    if (place >= 0) {
+        const T *src = static_cast<const T *>(value ? a.v : a.k) + (value ? t * a.v_token + g * a.v_head : t * a.k_token + g * a.k_head) + j * kKv4Group + b * 8u;
+        if constexpr (VEC) {
+            __align__(16) T raw[8];
+#pragma unroll
+            for (uint32_t i = 0; i < sizeof raw / 16; i++) reinterpret_cast<uint4 *>(raw)[i] = reinterpret_cast<const uint4 *>(src)[i];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = widen(raw[i]);
+        } else
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = widen(src[i]);
+    }
+    float lo = x[0], hi = x[0];
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 8; i++) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); fine = fine && fabsf(x[i]) <= kKv4Most; }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        fine = __shfl_xor_sync(0xffffffffu, (int)fine, o) && fine;
+    }
+    if (place < 0) return;
+    __half m = __float2half_rn(lo), s = __float2half_rn((hi - lo) * (1.0f / 15.0f));
+    uint32_t word = 0;
+    if (!fine) m = s = __ushort_as_half(0x7fff);
+    else if (__half2float(s) > 0.0f) {
+        const float mf = __half2float(m), sf = __half2float(s), inv = 1.0f / sf;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float q = (x[i] - mf) * inv;
+            float r = rintf(q);
+            if (fabsf(q - r) > 0.4999f) r = (float)rint(((double)x[i] - (double)mf) / (double)sf);
+            word |= (uint32_t)fminf(fmaxf(r, 0.0f), 15.0f) << (4 * i);
+        }
+    }
+    unsigned char *block = a.pool + (uint64_t)(place / kKv4Page) * a.page_stride + (uint64_t)g * kv4_block_bytes(a.D) + (value ? 640u * n : 0u);
+    const uint32_t at = (uint32_t)(place % kKv4Page);
+    unsigned char *codes = block + at * 16u * n;
+    if (value) {
+        reinterpret_cast<uint16_t *>(codes)[2u * b * n + j] = (uint16_t)word;
+        reinterpret_cast<uint16_t *>(codes)[(2u * b + 1u) * n + j] = (uint16_t)(word >> 16);
+    } else reinterpret_cast<uint32_t *>(codes)[b * n + j] = word;
+    if (b == 0) reinterpret_cast<__half2 *>(block + 512u * n)[at * n + j] = __halves2half2(s, m);
+}
+
+// Reading back: a thread per eight neighbouring coordinates.  c s is exact in fp32, so one rounding is left
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) k_kv4_read(const Kv4Rows a) {
+    const uint32_t n = a.D / kKv4Group, b = threadIdx.x & 3u;
+    const uint64_t items = (uint64_t)a.T * a.G * n, item = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 2;
+    if (item >= items) return;
+    const bool value = blockIdx.y != 0;
+    const uint32_t t = (uint32_t)(item / (a.G * n)), e = (uint32_t)(item % (a.G * n)), g = e / n, j = e % n;
+    const long long place = kv4_place(a, t);
+    float x[8] = {};
+    if (place >= 0) {
+        const unsigned char *block = a.pool + (uint64_t)(place / kKv4Page) * a.page_stride + (uint64_t)g * kv4_block_bytes(a.D) + (value ? 640u * n : 0u);
+        const uint32_t at = (uint32_t)(place % kKv4Page);
+        const unsigned char *codes = block + at * 16u * n;
+        const uint32_t word = value ? reinterpret_cast<const uint16_t *>(codes)[2u * b * n + j] | (uint32_t)reinterpret_cast<const uint16_t *>(codes)[(2u * b + 1u) * n + j] << 16
+                                    : reinterpret_cast<const uint32_t *>(codes)[b * n + j];
+        const float2 sm = __half22float2(reinterpret_cast<const __half2 *>(block + 512u * n)[at * n + j]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = fmaf((float)((word >> (4 * i)) & 15u), sm.x, sm.y);
+    }
+    T *dst = static_cast<T *>(value ? a.v : a.k) + (value ? t * a.v_token + g * a.v_head : t * a.k_token + g * a.k_head) + j * kKv4Group + b * 8u;
+    __align__(16) T y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = (T)x[i];
+    if constexpr (VEC) {
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof y / 16; i++) reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(y)[i];
+    } else
+#pragma unroll
+        for (int i = 0; i < 8; i++) dst[i] = y[i];
+}
+
+bool rows_at16(const Kv4Rows &a) {
+    const uint64_t unit = 16u / elem_size(a.type);
+    return ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15u) == 0 && a.k_token % unit == 0 && a.v_token % unit == 0 && a.k_head % unit == 0 && a.v_head % unit == 0;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Attention.  A warp multiplies the keys of one page at a time (32, in two tiles of 16 rows) with NT tiles of 8 columns -- column c of key/value head g is
+// query token c / rep, head g rep + c % rep, rep = H / G -- on the matrix instructions: keys and values are the row operand, made in registers from the codes
+// (a code c next to the exponent of 1024 is the fp16 number 1024 + c; minus 1024 and one fp16 multiply-add with the group's pair gives c s + m rounded once), queries
+// and weights the column operand.  Softmax in one pass: per column the running maximum m, the sum l and the weighted values o in fp32; log2 units, weights
+// times 2^kLift so that fp16 keeps small ones.  Rounding to 11 bits: the keys and values (c s + m), the queries (times a power of two per row, so that any
+// magnitude fits) and the weights; each rounding is at most 2^-11 of its number, against the 2^-8 of a bf16 output and the cache's own 1/30 of a group's range.
+// Each warp brings its own pages into its own ring of shared memory (cp.async, one group of copies to a page) and waits for nobody else until the end.
+// WK warps of a block share the columns and take every WK-th page (single tokens: the keys are what there is to share out); with WK = 1 each warp has columns of
+// its own.  The pages of a row are also split over nsplit blocks, whose parts k_kv4_join puts together.
+// Values that stand for NaN are taken out of the product (0 times NaN would reach columns that do not see them) and make the rows that do see them NaN.
+// ------------------------------------------------------------------------------------------------
+constexpr int kLift = 12;
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 half2_of(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
+// the codes at bits 0-3 and 16-19 (HIGH: 4-7 and 20-23) of w as c s + m
+template <bool HIGH>
+__device__ __forceinline__ uint32_t stand_for(uint32_t w, __half2 s, __half2 m) {
+    const __half2 h = half2_of((w & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+    const __half2 c = HIGH ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-64.0f)) : __hsub2(h, __float2half2_rn(1024.0f));
+    return bits(__hfma2(c, s, m));
+}
+// BYTES (a multiple of 2) bytes of shared memory in words
+template <int BYTES>
+__device__ __forceinline__ void take(const unsigned char *p, uint32_t (&w)[(BYTES + 3) / 4]) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; i++) { const uint4 v = reinterpret_cast<const uint4 *>(p)[i]; w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
+    } else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2 *>(p); w[0] = v.x; w[1] = v.y; }
+    else if constexpr (BYTES % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; i++) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 2; i++) {
+            const uint32_t v = reinterpret_cast<const uint16_t *>(p)[i];
+            if (i & 1) w[i / 2] |= v << 16; else w[i / 2] = v;
+        }
+    }
+}
+
+__device__ __forceinline__ int first_seen(int pos, uint32_t window, uint32_t block) {
+    int f = 0;
+    if (window && pos >= (int)window) f = pos - (int)window + 1;
+    if (block) f = max(f, pos - (int)((uint32_t)pos % block));
+    return f;
+}
+__device__ __forceinline__ int seq_len(const Kv4Attn &a, uint32_t b) {
+    const long long most = (long long)a.width * kKv4Page;
+    const long long n = a.lens ? a.lens[b] : (long long)a.pos0 + (a.pos_ptr ? *a.pos_ptr : 0u) + a.T;
+    return (int)(n < 0 ? 0 : n < most ? n : most);
+}
+// what is left to do with a column's sums: the sink, the division, the gate.  m in log2 units, l and the values times 2^kLift; returns the values' factor
+__device__ __forceinline__ float last_factor(const Kv4Attn &a, uint32_t t, uint32_t h, float m, float l) {
+    if (l == 0.0f) return 0.0f;          // no key in sight (a NaN is no zero)
+    float f = 1.0f;
+    if (a.sink) {
+        const float s = a.sink[h] * kLog2e, top = fmaxf(m, s);
+        f = ex2(m - top);
+        l = fmaf(l, f, ex2(s - top + (float)kLift));
+    }
+    f /= l;
+    if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[(uint64_t)t * a.ldg + h]));
+    return f;
+}
+__device__ __forceinline__ void store_four(const Kv4Attn &a, uint32_t b, uint32_t t, uint32_t h, uint32_t d, float x0, float x1, float x2, float x3) {
+    const uint64_t at = b * a.o_batch + t * a.o_token + h * a.o_head + d;
+    if (a.type == T_F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(x0, x1, x2, x3);
+    else {
+        const __nv_bfloat162 u = __floats2bfloat162_rn(x0, x1), v = __floats2bfloat162_rn(x2, x3);
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(a.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&u), *reinterpret_cast<const uint32_t *>(&v));
+    }
+}
+
+struct Shape { uint32_t nsplit, tiles, cols; };          // splits of the keys, blocks along the columns of a head, columns of a block
+constexpr int kStages = 3;
+template <int NG, int NT, int WK, int W>
+struct Room {
+    static constexpr uint32_t block = 1280u * NG, ring = W * kStages * block, merge = WK > 1 ? W * NT * 8u * (32u * NG + 2u) * 4u : 0u,
+                              q = (W / WK) * NT * NG * 512u, all = (ring > merge ? ring : merge) + q + (W / WK) * NT * 8u * 4u;
+};
+
+// grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
+template <int NG, int NT, int WK, int W>
+__global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shape sh) {
+    pdl_enter4();
+    using R = Room<NG, NT, WK, W>;
+    constexpr uint32_t D = 32u * NG, COLS = NT * 8u;
+    extern __shared__ __align__(16) unsigned char sm[];
+    __shared__ uint32_t known[W][kStages];          // whether the page in a stage is one of the pool's
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, wr = warp / WK, wk = warp % WK, gq = lane >> 2, tq = lane & 3u;
+    const uint32_t split = blockIdx.x % sh.nsplit, tile = blockIdx.x / sh.nsplit, g = blockIdx.y, b = blockIdx.z, rep = a.H / a.G, ncols = a.T * rep;
+    unsigned char *ring = sm + warp * kStages * R::block;
+    unsigned char *q_s = sm + (R::ring > R::merge ? R::ring : R::merge) + wr * NT * NG * 512u;
+    float *scale_s = reinterpret_cast<float *>(sm + (R::ring > R::merge ? R::ring : R::merge) + R::q) + wr * COLS;
+    const uint32_t c0 = tile * sh.cols + wr * COLS;
+    const int len = seq_len(a, b);
+
+    // the queries as the column operand, each row times the power of two that brings its largest number to [1, 2)
+    for (uint32_t c = wk; c < COLS; c += WK) {
+        const uint32_t col = c0 + c, t = col / rep, h = g * rep + col % rep;
+        float x[NG], most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            x[j] = 0.0f;
+            if (col < ncols) {
+                const uint64_t at = b * a.q_batch + t * a.q_token + h * a.q_head + j * 32u + lane;
+                x[j] = a.type == T_F32 ? static_cast<const float *>(a.q)[at] : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at]);
+            }
+            most = fmaxf(most, fabsf(x[j]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int e = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126) : 0;
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        // coordinate 32 j + 8 b + i (lane = 8 b + i): step i / 2 % 2 of the group, register i % 2, half i / 4
+        const uint32_t bq = lane >> 3, i = lane & 7u;
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+            *reinterpret_cast<__half *>(q_s + (((c >> 3) * NG + j) * 2u + ((i >> 1) & 1u)) * 256u + ((c & 7u) * 4u + bq) * 8u + (i & 1u) * 4u + (i >> 2) * 2u) = __float2half_rn(x[j] * down);
+        if (lane == 0) scale_s[c] = a.scale * __uint_as_float((uint32_t)(127 + e) << 23) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+    }
+    if constexpr (WK > 1) __syncthreads(); else __syncwarp();
+
+    // pages that any of this warp's columns sees, and the share of this split
+    const uint32_t c1 = min(c0 + COLS, ncols);
+    const int pos_a = c0 < ncols ? len - (int)a.T + (int)(c0 / rep) : -1, pos_b = c0 < ncols ? len - (int)a.T + (int)((c1 - 1u) / rep) : -1;
+    uint32_t p0 = 0, p1 = 0;
+    int low_b = 0;
+    if (pos_b >= 0) {
+        const uint32_t first = (uint32_t)first_seen(max(pos_a, 0), a.window, a.block) / kKv4Page, np = (uint32_t)pos_b / kKv4Page + 1u - first;
+        p0 = first + (uint32_t)((uint64_t)np * split / sh.nsplit); p1 = first + (uint32_t)((uint64_t)np * (split + 1u) / sh.nsplit);
+        low_b = first_seen(pos_b, a.window, a.block);
+    }
+    const uint32_t count = p0 + wk < p1 ? (p1 - p0 - wk + WK - 1u) / WK : 0u;
+
+    float m[NT][2], l[NT][2], o[2 * NG][NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        m[t][0] = m[t][1] = -INFINITY; l[t][0] = l[t][1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i++) { o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.0f; }
+    }
+    float f[NT][2]; int pos[NT][2];          // this thread's columns: 2 tq and 2 tq + 1 of each tile
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const uint32_t c = t * 8u + tq * 2u + x;
+            f[t][x] = scale_s[c];
+            pos[t][x] = c0 + c < ncols ? len - (int)a.T + (int)((c0 + c) / rep) : -1;
+        }
+
+    uint32_t ahead = 0;          // page numbers of 32 steps, one to a lane
+    const unsigned char *head = a.pool + (uint64_t)g * R::block;
+    const int32_t *table = a.table + (uint64_t)b * a.table_stride;
+    auto fetch = [&](uint32_t i) {
+        if (i < count) {
+            if ((i & 31u) == 0) { const uint32_t p = p0 + wk + (i + lane) * WK; ahead = p < p1 ? (uint32_t)table[p] : 0u; }
+            const uint32_t page = __shfl_sync(0xffffffffu, ahead, i & 31u), stage = i % kStages;
+            const bool ok = page < a.n_pages;
+            if (lane == 0) known[warp][stage] = ok;
+            if (ok) {
+                const unsigned char *src = head + (uint64_t)page * a.page_stride;
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * R::block);
+#pragma unroll
+                for (uint32_t v = 0; v < (80u * NG + 31u) / 32u; v++) { const uint32_t k = v * 32u + lane; if (80u * NG % 32u == 0 || k < 80u * NG) copy16(dst + k * 16u, src + k * 16u); }
+            }
+        }
+        copy_commit();
+    };
+    for (uint32_t i = 0; i < kStages - 1; i++) fetch(i);
+    uint32_t qf[NT == 1 ? 2 * NG : 1][2];
+    if constexpr (NT == 1)
+#pragma unroll
+        for (int j = 0; j < 2 * NG; j++) { const uint2 v = *reinterpret_cast<const uint2 *>(q_s + j * 256u + lane * 8u); qf[j][0] = v.x; qf[j][1] = v.y; }
+    const uint32_t row = (gq & 1u) * 4u + (gq >> 1);          // row r of eight is token 4 (r % 2) + r / 2 of eight: the transposed weights then pair tokens i and i + 4
+    for (uint32_t i = 0; i < count; i++) {
+        copy_wait<kStages - 2>();
+        __syncwarp();
+        fetch(i + kStages - 1);
+        const uint32_t stage = i % kStages;
+        if (!known[warp][stage]) continue;          // not a page of the pool: its keys are not seen
+        unsigned char *pg = ring + stage * R::block;
+        const int key0 = (int)((p0 + wk + i * WK) * kKv4Page);
+
+        // values that are no number
+        uint32_t bad = 0;
+        {
+            uint32_t w[NG];
+            take<4 * NG>(pg + 1152u * NG + lane * 4u * NG, w);
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < NG; j++) odd = odd || (w[j] & 0x7c00u) == 0x7c00u || (w[j] & 0x7c000000u) == 0x7c000000u;
+            bad = __ballot_sync(0xffffffffu, odd);
+            if (bad) {
+                if (odd)
+#pragma unroll
+                    for (int j = 0; j < NG; j++) reinterpret_cast<uint32_t *>(pg + 1152u * NG + lane * 4u * NG)[j] = 0u;
+                __syncwarp();
+            }
+        }
+
+        // scores: rows 16 k + row (+ 8) of the page
+        float s[2][NT][4];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) s[k][t][0] = s[k][t][1] = s[k][t][2] = s[k][t][3] = 0.0f;
+            const uint32_t ra = k * 16u + row, rb = ra + 8u;
+            uint32_t wa[NG], wb[NG], sa[NG], sb[NG];
+            take<4 * NG>(pg + ra * 16u * NG + tq * 4u * NG, wa); take<4 * NG>(pg + rb * 16u * NG + tq * 4u * NG, wb);
+            take<4 * NG>(pg + 512u * NG + ra * 4u * NG, sa); take<4 * NG>(pg + 512u * NG + rb * 4u * NG, sb);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const __half2 s_a = __low2half2(half2_of(sa[j])), m_a = __high2half2(half2_of(sa[j])), s_b = __low2half2(half2_of(sb[j])), m_b = __high2half2(half2_of(sb[j]));
+                const uint32_t x0 = stand_for<false>(wa[j], s_a, m_a), x1 = stand_for<true>(wa[j], s_a, m_a), x2 = stand_for<false>(wa[j] >> 8, s_a, m_a), x3 = stand_for<true>(wa[j] >> 8, s_a, m_a);
+                const uint32_t y0 = stand_for<false>(wb[j], s_b, m_b), y1 = stand_for<true>(wb[j], s_b, m_b), y2 = stand_for<false>(wb[j] >> 8, s_b, m_b), y3 = stand_for<true>(wb[j] >> 8, s_b, m_b);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    uint2 u, v;
+                    if constexpr (NT == 1) { u = make_uint2(qf[2 * j][0], qf[2 * j][1]); v = make_uint2(qf[2 * j + 1][0], qf[2 * j + 1][1]); }
+                    else { u = *reinterpret_cast<const uint2 *>(q_s + ((t * NG + j) * 2u) * 256u + lane * 8u); v = *reinterpret_cast<const uint2 *>(q_s + ((t * NG + j) * 2u + 1u) * 256u + lane * 8u); }
+                    mma(s[k][t], x0, y0, x1, y1, u.x, u.y);
+                    mma(s[k][t], x2, y2, x3, y3, v.x, v.y);
+                }
+            }
+        }
+
+        // weights, as the column operand of the second product
+        const bool whole = pos_a >= key0 + (int)kKv4Page - 1 && low_b <= key0;
+        uint32_t pw[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float top[2] = {m[t][0], m[t][1]};
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    float v = s[k][t][x] * f[t][x & 1];
+                    if (a.softcap > 0.0f) v = a.softcap * kLog2e * tanhf(v);
+                    if (!whole) {
+                        const int key = key0 + k * 16 + (x >> 1) * 8 + (int)row;
+                        if (key > pos[t][x & 1] || key < first_seen(max(pos[t][x & 1], 0), a.window, a.block)) v = -INFINITY;
+                    }
+                    s[k][t][x] = v;
+                    top[x & 1] = fmaxf(top[x & 1], v);
+                }
+            float corr[2], use[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], off));
+                use[x] = top[x] == -INFINITY ? 0.0f : top[x];
+                corr[x] = ex2(m[t][x] - use[x]);
+                m[t][x] = top[x];
+                use[x] -= (float)kLift;
+                l[t][x] *= corr[x];
+            }
+            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f))
+#pragma unroll
+                for (int d = 0; d < 2 * NG; d++) { o[d][t][0] *= corr[0]; o[d][t][1] *= corr[1]; o[d][t][2] *= corr[0]; o[d][t][3] *= corr[1]; }
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const float u = ex2(s[k][t][2 * r] - use[0]), v = ex2(s[k][t][2 * r + 1] - use[1]);
+                    l[t][0] += u; l[t][1] += v;
+                    if (bad && (bad >> (k * 16 + r * 8 + row) & 1u)) {          // seen, however little it weighs
+                        if (s[k][t][2 * r] != -INFINITY) l[t][0] = NAN;
+                        if (s[k][t][2 * r + 1] != -INFINITY) l[t][1] = NAN;
+                    }
+                    pw[t][2 * k + r] = transpose8(bits(__floats2half2_rn(u, v)));
+                }
+        }
+
+        // weighted values: depth step k takes tokens 16 k + tq + {0, 4, 8, 12}; rows are coordinates 32 j + 4 gq + {0 .. 3}
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            uint32_t w[4][(NG + 1) / 2], sp[4][NG];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const uint32_t r = k * 16u + tq + 4u * x;
+                take<2 * NG>(pg + 640u * NG + r * 16u * NG + gq * 2u * NG, w[x]);
+                take<4 * NG>(pg + 1152u * NG + r * 4u * NG, sp[x]);
+            }
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                const uint32_t ab = __byte_perm(w[0][j / 2], w[1][j / 2], sel), cd = __byte_perm(w[2][j / 2], w[3][j / 2], sel);
+                const __half2 s_ab = half2_of(__byte_perm(sp[0][j], sp[1][j], 0x5410u)), m_ab = half2_of(__byte_perm(sp[0][j], sp[1][j], 0x7632u));
+                const __half2 s_cd = half2_of(__byte_perm(sp[2][j], sp[3][j], 0x5410u)), m_cd = half2_of(__byte_perm(sp[2][j], sp[3][j], 0x7632u));
+                const uint32_t x0 = stand_for<false>(ab, s_ab, m_ab), x1 = stand_for<true>(ab, s_ab, m_ab), x2 = stand_for<false>(ab >> 8, s_ab, m_ab), x3 = stand_for<true>(ab >> 8, s_ab, m_ab);
+                const uint32_t y0 = stand_for<false>(cd, s_cd, m_cd), y1 = stand_for<true>(cd, s_cd, m_cd), y2 = stand_for<false>(cd >> 8, s_cd, m_cd), y3 = stand_for<true>(cd >> 8, s_cd, m_cd);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    mma(o[2 * j][t], x0, x1, y0, y1, pw[t][2 * k], pw[t][2 * k + 1]);
+                    mma(o[2 * j + 1][t], x2, x3, y2, y3, pw[t][2 * k], pw[t][2 * k + 1]);
+                }
+            }
+        }
+    }
+    copy_wait<0>();
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], off);
+
+    const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols, places = (uint64_t)a.B * a.G * sh.tiles * sh.nsplit * sh.cols;
+    float2 *ml = reinterpret_cast<float2 *>(a.part + places * D);
+    if constexpr (WK > 1) {
+        float *mo = reinterpret_cast<float *>(sm), *mm = mo + W * COLS * D;          // [warp][column][D], then [warp][column] (m, l): where the rings were
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t c = warp * COLS + t * 8u + tq * 2u + x;
+#pragma unroll
+                for (int j = 0; j < NG; j++)
+                    *reinterpret_cast<float4 *>(mo + c * D + j * 32u + gq * 4u) = make_float4(o[2 * j][t][x], o[2 * j][t][2 + x], o[2 * j + 1][t][x], o[2 * j + 1][t][2 + x]);
+                if (gq == 0) { mm[2 * c] = m[t][x]; mm[2 * c + 1] = l[t][x]; }
+            }
+        __syncthreads();
+        for (uint32_t e = tid; e < COLS * D / 4u; e += W * 32u) {
+            const uint32_t c = e / (D / 4u), d = e % (D / 4u) * 4u, col = c0 + c;
+            if (col >= ncols) break;
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) top = fmaxf(top, mm[2 * (w * COLS + c)]);
+            const float use = top == -INFINITY ? 0.0f : top;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float k = ex2(mm[2 * (w * COLS + c)] - use);
+                const float4 u = *reinterpret_cast<const float4 *>(mo + (w * COLS + c) * D + d);
+                sum = fmaf(mm[2 * (w * COLS + c) + 1], k, sum);
+                v.x = fmaf(u.x, k, v.x); v.y = fmaf(u.y, k, v.y); v.z = fmaf(u.z, k, v.z); v.w = fmaf(u.w, k, v.w);
+            }
+            if (sh.nsplit > 1) {
+                *reinterpret_cast<float4 *>(a.part + (where + c) * D + d) = v;
+                if (d == 0) ml[where + c] = make_float2(top, sum);
+            } else {
+                const uint32_t t = col / rep, h = g * rep + col % rep;
+                const float k = last_factor(a, t, h, top, sum);
+                const bool none = sum == 0.0f;
+                store_four(a, b, t, h, d, none ? 0.0f : v.x * k, none ? 0.0f : v.y * k, none ? 0.0f : v.z * k, none ? 0.0f : v.w * k);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t c = wr * COLS + t * 8u + tq * 2u + x, col = tile * sh.cols + c;
+                if (col >= ncols) continue;
+                const uint32_t tt = col / rep, h = g * rep + col % rep;
+                const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, tt, h, m[t][x], l[t][x]);
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    const float v0 = o[2 * j][t][x] * k, v1 = o[2 * j][t][2 + x] * k, v2 = o[2 * j + 1][t][x] * k, v3 = o[2 * j + 1][t][2 + x] * k;
+                    if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + (where + c) * D + j * 32u + gq * 4u) = make_float4(v0, v1, v2, v3);
+                    else store_four(a, b, tt, h, j * 32u + gq * 4u, v0, v1, v2, v3);
+                }
+                if (sh.nsplit > 1 && gq == 0) ml[where + c] = make_float2(m[t][x], l[t][x]);
+            }
+    }
+}
+
+// The parts of a row's splits put together: a warp per row.  grid (ceil(T rep / 8), G, B)
+__global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a, const Shape sh) {
+    pdl_enter4();
+    const uint32_t lane = threadIdx.x & 31u, rep = a.H / a.G, col = blockIdx.x * 8u + (threadIdx.x >> 5), g = blockIdx.y, b = blockIdx.z;
+    if (col >= a.T * rep) return;
+    const uint32_t t = col / rep, h = g * rep + col % rep;
+    const uint64_t places = (uint64_t)a.B * a.G * sh.tiles * sh.nsplit * sh.cols, where = ((uint64_t)(b * a.G + g) * sh.tiles + col / sh.cols) * sh.nsplit * sh.cols + col % sh.cols;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + places * a.D);
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t s = lane; s < sh.nsplit; s += 32u) top = fmaxf(top, ml[where + (uint64_t)s * sh.cols].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float use = top == -INFINITY ? 0.0f : top;
+    for (uint32_t d0 = 0; d0 < a.D; d0 += 128u) {
+        const uint32_t d = d0 + lane * 4u;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        sum = 0.0f;
+        for (uint32_t s = 0; s < sh.nsplit; s++) {
+            const float2 p = ml[where + (uint64_t)s * sh.cols];
+            const float k = ex2(p.x - use);
+            sum = fmaf(p.y, k, sum);
+            if (d < a.D) {
+                const float4 u = *reinterpret_cast<const float4 *>(a.part + (where + (uint64_t)s * sh.cols) * a.D + d);
+                v.x = fmaf(u.x, k, v.x); v.y = fmaf(u.y, k, v.y); v.z = fmaf(u.z, k, v.z); v.w = fmaf(u.w, k, v.w);
+            }
+        }
+        const float k = last_factor(a, t, h, top, sum);
+        if (d < a.D) store_four(a, b, t, h, d, v.x * k, v.y * k, v.z * k, v.w * k);
+    }
+}
+
+template <typename K, typename... A>
+cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream, bool pdl, const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+// ---- which instance, and how the work is shared out ----
+struct Plan { int nt; bool rows; Shape sh; };
+constexpr uint32_t kWarps = 4;
+Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
+    const uint32_t ncols = T * (H / G), most = D > 128 ? 2u : 4u;
+    Plan p{};
+    p.nt = ncols <= 8 ? 1 : ncols <= 16 || most == 2 ? 2 : 4;
+    p.rows = ncols > (uint32_t)p.nt * 8u;
+    p.sh.cols = (uint32_t)p.nt * 8u * (p.rows ? kWarps : 1u);
+    p.sh.tiles = (ncols + p.sh.cols - 1u) / p.sh.cols;
+    // pages that a block can have in sight
+    const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
+    const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
+    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = 3ull * sms;
+    const uint32_t least = p.rows ? 8u : 2u * kWarps;          // pages of a split
+    p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want / std::max<uint64_t>(1, blocks), std::max(1u, pages / least)));
+    return p;
+}
+
+template <int NG, int NT, int WK>
+cudaError_t attn_launch(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, bool pdl) {
+    constexpr int smem = (int)Room<NG, NT, WK, kWarps>::all;
+    const auto k = k_kv4_attn<NG, NT, WK, kWarps>;
+    const cudaError_t e = smem_at_least(reinterpret_cast<const void *>(k), smem);
+    return e != cudaSuccess ? e : launch_on(k, dim3(sh.nsplit * sh.tiles, a.G, a.B), kWarps * 32, smem, stream, pdl, a, sh);
+}
+template <int NG>
+cudaError_t attn_launch_nt(const Kv4Attn &a, const Plan &p, cudaStream_t stream, bool pdl) {
+    constexpr int most = NG > 4 ? 2 : 4;
+    if (p.rows) return attn_launch<NG, most, 1>(a, p.sh, stream, pdl);
+    if (p.nt == 1) return attn_launch<NG, 1, kWarps>(a, p.sh, stream, pdl);
+    if (p.nt == 2) return attn_launch<NG, 2, kWarps>(a, p.sh, stream, pdl);
+    return attn_launch<NG, most, kWarps>(a, p.sh, stream, pdl);
+}
+
+template <bool WRITE>
+cudaError_t rows_launch(const Kv4Rows &a, cudaStream_t stream, bool pdl) {
+    const uint64_t items = (uint64_t)a.T * a.G * (a.D / kKv4Group);
+    if (!items) return cudaSuccess;
+    const dim3 grid((uint32_t)((items * 4u + kRowThreads - 1u) / kRowThreads), 2);
+    const bool vec = rows_at16(a);
+#define KV4_ROWS(TYPE)                                                                                                                          \
+    (WRITE ? (vec ? launch_on(k_kv4_write<TYPE, true>, grid, kRowThreads, 0, stream, pdl, a) : launch_on(k_kv4_write<TYPE, false>, grid, kRowThreads, 0, stream, pdl, a)) \
+           : (vec ? launch_on(k_kv4_read<TYPE, true>, grid, kRowThreads, 0, stream, false, a) : launch_on(k_kv4_read<TYPE, false>, grid, kRowThreads, 0, stream, false, a)))
+    return a.type == T_F32 ? KV4_ROWS(float) : a.type == T_BF16 ? KV4_ROWS(__nv_bfloat16) : KV4_ROWS(__half);
+#undef KV4_ROWS
+}
+
+}  // namespace
+
+cudaError_t kv4_write_launch(const Kv4Rows &a, cudaStream_t stream, bool pdl) { return rows_launch<true>(a, stream, pdl); }
+cudaError_t kv4_read_launch(const Kv4Rows &a, cudaStream_t stream) { return rows_launch<false>(a, stream, false); }
+
+size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
+    const Plan p = plan_for(B, T, H, G, D, width, window, block, sms);
+    return p.sh.nsplit == 1 ? 0 : (size_t)B * G * p.sh.tiles * p.sh.nsplit * p.sh.cols * (D + 2u) * 4u;
+}
+
+cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, uint32_t *launches) {
+    const Plan p = plan_for(a.B, a.T, a.H, a.G, a.D, a.width, a.window, a.block, sms);
+    cudaError_t e;
+    switch (a.D / 32u) {
+        case 1: e = attn_launch_nt<1>(a, p, stream, pdl); break;
+        case 2: e = attn_launch_nt<2>(a, p, stream, pdl); break;
+        case 3: e = attn_launch_nt<3>(a, p, stream, pdl); break;
+        case 4: e = attn_launch_nt<4>(a, p, stream, pdl); break;
+        default: e = attn_launch_nt<8>(a, p, stream, pdl); break;
+    }
+    if (e == cudaSuccess && p.sh.nsplit > 1)
+        e = launch_on(k_kv4_join, dim3((a.T * (a.H / a.G) + 7u) / 8u, a.G, a.B), 256, 0, stream, true, a, p.sh);
+    if (launches) *launches = p.sh.nsplit > 1 ? 2 : 1;
+    return e;
+}
+
+}  // namespace nb
+
+using nb::fail;
+
+namespace {
+int kv4_pool_check(const void *pool, uint64_t page_stride, uint32_t n_pages, uint32_t kv_heads, uint32_t head_dim) {
+    if (!head_dim || head_dim % nb::kKv4Group || head_dim > 256u) return fail(NB200_EINVAL, "head_dim %u: a cache in 4 bits holds multiples of 32 up to 256", head_dim);
+    if (!kv_heads || kv_heads > 65535u) return fail(NB200_EINVAL, "kv_heads %u unusable", kv_heads);
+    if (n_pages > 0x7fffffffu / nb::kKv4Page) return fail(NB200_EINVAL, "%u pages: places are 32-bit numbers", n_pages);
+    if ((reinterpret_cast<uintptr_t>(pool) | page_stride) & 15u) return fail(NB200_EINVAL, "the pool's base and page stride are to be multiples of 16 bytes");
+    if (n_pages && (!pool || (n_pages > 1 && page_stride < (uint64_t)kv_heads * nb::kv4_block_bytes(head_dim)))) return fail(NB200_EINVAL, "null pool, or pages that overlap");
+    return 0;
+}
+int kv4_rows_check(const nb200_kv4_rows *r, nb::Kv4Rows *a) {
+    if (!r) return fail(NB200_EINVAL, "null argument");
+    int rc;
+    if ((rc = kv4_pool_check(r->pool, r->page_stride, r->n_pages, r->kv_heads, r->head_dim))) return rc;
+    if (r->type > nb::T_F16) return fail(NB200_EINVAL, "rows are fp32, bf16 or fp16 (type %u)", r->type);
+    if (r->tokens && (!r->k || !r->v || !r->slots)) return fail(NB200_EINVAL, "null argument");
+    if ((reinterpret_cast<uintptr_t>(r->k) | reinterpret_cast<uintptr_t>(r->v)) % nb::elem_size(r->type) || reinterpret_cast<uintptr_t>(r->slots) % 4u) return fail(NB200_EINVAL, "rows or slots are not aligned to their type");
+    if ((uint64_t)r->tokens * r->kv_heads * (r->head_dim / 8u) > 0x7fffffffull * nb::kRowThreads) return fail(NB200_EINVAL, "%u tokens are too many for one call", r->tokens);
+    if (r->tokens && nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
+    *a = nb::Kv4Rows{r->k, r->v, r->k_token, r->v_token, r->k_head, r->v_head, r->type, r->slots, nullptr, 0, nullptr, r->tokens, r->kv_heads, r->head_dim,
+                     static_cast<unsigned char *>(r->pool), r->page_stride, r->n_pages};
+    return 0;
+}
+int sm_count(uint32_t *sms) {
+    int dev = 0, n = 0;
+    NB_CK(cudaGetDevice(&dev));
+    NB_CK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    *sms = (uint32_t)n;
+    return 0;
+}
+int kv4_attention_check(const nb200_kv4_attention *p) {
+    if (!p) return fail(NB200_EINVAL, "null argument");
+    int rc;
+    if ((rc = kv4_pool_check(p->pool, p->page_stride, p->n_pages, p->kv_heads, p->head_dim))) return rc;
+    if (!nb::kv4_dim_ok(p->head_dim)) return fail(NB200_EINVAL, "head_dim %u has no attention kernel (32, 64, 96, 128 and 256 have)", p->head_dim);
+    if (p->type > nb::T_BF16) return fail(NB200_EINVAL, "queries are fp32 or bf16 (type %u)", p->type);
+    if (!p->heads || p->heads % p->kv_heads) return fail(NB200_EINVAL, "%u heads do not share %u key/value heads evenly", p->heads, p->kv_heads);
+    if (p->batch > 65535u) return fail(NB200_EINVAL, "%u sequences are too many for one call", p->batch);
+    if ((uint64_t)p->tokens * (p->heads / p->kv_heads) > (1u << 30) || p->tokens > (1u << 30)) return fail(NB200_EINVAL, "%u tokens are too many for one call", p->tokens);
+    if ((uint64_t)p->width * nb::kKv4Page > (1u << 30)) return fail(NB200_EINVAL, "%u pages to a sequence are too many", p->width);
+    if (p->window > (1u << 30) || p->block > (1u << 30)) return fail(NB200_EINVAL, "window or block above 2^30");
+    if (!(p->softcap >= 0.0f) || isinf(p->softcap) || !isfinite(p->scale)) return fail(NB200_EINVAL, "scale %g or softcap %g unusable", p->scale, p->softcap);
+    if (p->batch && p->tokens) {
+        if (!p->q || !p->out || !p->lens || (p->width && !p->table)) return fail(NB200_EINVAL, "null argument");
+        const uint32_t e = nb::elem_size(p->type), four = 4u * e;
+        if (reinterpret_cast<uintptr_t>(p->q) % e || reinterpret_cast<uintptr_t>(p->lens) % 4u || reinterpret_cast<uintptr_t>(p->table) % 4u || reinterpret_cast<uintptr_t>(p->sinks) % 4u) return fail(NB200_EINVAL, "an operand is not aligned to its type");
+        if (reinterpret_cast<uintptr_t>(p->out) % four || (p->o_batch | p->o_token | p->o_head) % 4u) return fail(NB200_EINVAL, "out's base and strides are to be multiples of four numbers");
+    }
+    return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int nb200_dev_kv4_write(const nb200_kv4_rows *rows, void *stream) {
+    nb::Kv4Rows a;
+    const int r = kv4_rows_check(rows, &a);
+    if (r) return r;
+    NB_CK(nb::kv4_write_launch(a, static_cast<cudaStream_t>(stream), false));
+    return 0;
+}
+
+int nb200_dev_kv4_read(const nb200_kv4_rows *rows, void *stream) {
+    nb::Kv4Rows a;
+    const int r = kv4_rows_check(rows, &a);
+    if (r) return r;
+    NB_CK(nb::kv4_read_launch(a, static_cast<cudaStream_t>(stream)));
+    return 0;
+}
+
+int nb200_dev_kv4_attention_workspace(const nb200_kv4_attention *p, uint64_t *bytes) {
+    int r;
+    uint32_t sms = 0;
+    if (!bytes) return fail(NB200_EINVAL, "null argument");
+    if ((r = kv4_attention_check(p))) return r;
+    *bytes = 0;
+    if (!p->batch || !p->tokens) return 0;
+    if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
+    if ((r = sm_count(&sms))) return r;
+    *bytes = nb::kv4_attn_workspace(p->batch, p->tokens, p->heads, p->kv_heads, p->head_dim, p->width, p->window, p->block, sms);
+    return 0;
+}
+
+int nb200_dev_kv4_attention(const nb200_kv4_attention *p, void *workspace, uint64_t workspace_bytes, void *stream) {
+    int r;
+    uint32_t sms = 0;
+    if ((r = kv4_attention_check(p))) return r;
+    if (!p->batch || !p->tokens) return 0;
+    if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
+    if ((r = sm_count(&sms))) return r;
+    const size_t need = nb::kv4_attn_workspace(p->batch, p->tokens, p->heads, p->kv_heads, p->head_dim, p->width, p->window, p->block, sms);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) & 15u)) return fail(NB200_EINVAL, "the workspace is to have %zu bytes at a multiple of 16", need);
+    const nb::Kv4Attn a{p->q, p->q_batch, p->q_token, p->q_head, p->type, p->out, p->o_batch, p->o_token, p->o_head, static_cast<const unsigned char *>(p->pool), p->page_stride, p->n_pages,
+                        p->table, p->table_stride, p->width, p->lens, 0, nullptr, p->batch, p->tokens, p->heads, p->kv_heads, p->head_dim, p->scale, p->softcap, p->sinks, p->window, p->block,
+                        nullptr, 0, static_cast<float *>(workspace)};
+    NB_CK(nb::kv4_attn_launch(a, sms, static_cast<cudaStream_t>(stream), false, nullptr));
+    return 0;
+}
+
+}  // extern "C"

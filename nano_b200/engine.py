@@ -34,6 +34,7 @@ EXPORTS = [
     "nb200_engine_create_tp", "nb200_tp_export", "nb200_tp_attach_ipc", "nb200_tp_attach_local",
     "nb200_engine_create_dir", "nb200_seq_open", "nb200_seq_close", "nb200_step", "nb200_step_timed", "nb200_read_residual",
     "nb200_dev_token_logprobs", "nb200_dev_pages_copy",
+    "nb200_dev_kv4_write", "nb200_dev_kv4_read", "nb200_dev_kv4_attention_workspace", "nb200_dev_kv4_attention",
 ]
 
 
@@ -41,6 +42,19 @@ class Config(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in (
         "arch", "quant", "group_size", "block_size", "vocab_size", "n_layer", "n_embd", "n_head", "n_kv_head",
         "n_hidden", "tied", "head_dim", "q_dim", "kv_dim", "max_seq_len", "tp_rank", "tp_size")] + [("reserved", C.c_uint32 * 7)]
+
+
+class Kv4Rows(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("page_stride", C.c_uint64), ("n_pages", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("type", C.c_uint32), ("tokens", C.c_uint32), ("slots", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_uint64) for n in ("k_token", "k_head", "v_token", "v_head")]
+
+
+class Kv4Attention(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p)] + [(n, C.c_uint64) for n in ("q_batch", "q_token", "q_head", "o_batch", "o_token", "o_head")] + \
+               [("pool", C.c_void_p), ("page_stride", C.c_uint64)] + [(n, C.c_uint32) for n in ("n_pages", "kv_heads", "head_dim", "type", "batch", "tokens", "heads", "width")] + \
+               [("table_stride", C.c_uint64), ("table", C.c_void_p), ("lens", C.c_void_p), ("sinks", C.c_void_p), ("scale", C.c_float), ("softcap", C.c_float),
+                ("window", C.c_uint32), ("block", C.c_uint32)]
 
 
 class NB200Error(RuntimeError):
@@ -120,6 +134,9 @@ def lib(layered_ok: bool = False):
         L.nb200_read_residual.argtypes = [C.c_void_p, C.c_uint32, f32p, C.c_uint32]
         L.nb200_dev_token_logprobs.argtypes = [C.c_void_p] * 5 + [C.c_uint32, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]
         L.nb200_dev_pages_copy.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), u32p, C.c_uint32, u32p, u32p, C.c_uint32, C.c_void_p]
+        L.nb200_dev_kv4_write.argtypes = L.nb200_dev_kv4_read.argtypes = [C.POINTER(Kv4Rows), C.c_void_p]
+        L.nb200_dev_kv4_attention_workspace.argtypes = [C.POINTER(Kv4Attention), C.POINTER(C.c_uint64)]
+        L.nb200_dev_kv4_attention.argtypes = [C.POINTER(Kv4Attention), C.c_void_p, C.c_uint64, C.c_void_p]
         L.nb200_lora_load.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64]
         L.nb200_lora_enable.argtypes = [C.c_void_p, C.c_int]
         L.nb200_lora_unload.argtypes = [C.c_void_p]
