@@ -47,6 +47,8 @@ extern "C" {
 #define NB200_FLAG_NO_PDL 0x4u     /* disable programmatic dependent launch */
 #define NB200_FLAG_F32 0x20u       /* model folders: true 32-bit compute (weights widened to fp32, fp32 FMA matrix products, no tensor-core rounding);
                                       the default keeps the file's bfloat16 weights and feeds the tensor cores bfloat16 operands with fp32 accumulation */
+#define NB200_FLAG_KV4 0x40u       /* model folders: the cache rows of grouped-query attention layers are held in 4 bits (see "operators on device memory"; 5 bits a coordinate instead
+                                      of 32), written and attended to by nb200_dev_kv4_*'s kernels.  Layers of equal dim and vdim of 32, 64, 96, 128 or 256; not with NB200_FLAG_F32 */
 #define NB200_FLAG_NO_STREAM 0x10u /* do not use the grid-wide streaming kernel (per-CTA TMA weight ring, one launch per run of tokens) */
 
 /* quantisation / architecture ids: identical to infer/tensor.h:72-76 and infer/infer.h:45-47 */
@@ -140,6 +142,16 @@ int nb200_step(nb200_engine *e, uint32_t seq, const uint32_t *tokens, uint32_t n
 /* the same step `reps` times from the same state (state and cache are restored in between), timed with CUDA events on the engine's
  * stream after one untimed run: ms[0] = mean milliseconds of one run.  For bench.py. */
 int nb200_step_timed(nb200_engine *e, uint32_t seq, const uint32_t *tokens, uint32_t n, uint32_t reps, float *ms);
+/* A second sequence that goes on from where `seq` stands, for several continuations of one prompt: full pages are shared, the page in progress and the state slot are
+ * copied.  Both go on independently; a page returns when the last sequence that reads it is closed. */
+int nb200_seq_fork(nb200_engine *e, uint32_t seq, uint32_t *fork);
+/* nb200_step that returns, instead of the logits at the n_want places want[], the log probability of the token targets[i] there, the entropy and the `top` (<= 32) most
+ * probable alternatives with theirs (logprob [n_want], entropy [n_want], top_logprob and top_id [n_want][top], host): what nb200_dev_token_logprobs says of the logits, which do not
+ * leave the device. */
+int nb200_step_scores(nb200_engine *e, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, const uint32_t *targets, uint32_t n_want, uint32_t top,
+                      float *logprob, float *entropy, float *top_logprob, int32_t *top_id);
+/* the same of the logits that nb200_read_logits would return (every family, one GPU) */
+int nb200_read_scores(nb200_engine *e, uint32_t target, uint32_t top, float *logprob, float *entropy, float *top_logprob, int32_t *top_id);
 /* parity tests: the residual stream after layer run `run` of the last step, [tokens of that step][width] (engine created with
  * NB200_KEEP_RESIDUALS=1 in the environment) */
 int nb200_read_residual(nb200_engine *e, uint32_t run, float *dst, uint32_t count);

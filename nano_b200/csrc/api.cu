@@ -112,6 +112,14 @@ int nb200_step(nb200_engine *e, uint32_t seq, const uint32_t *tokens, uint32_t n
 int nb200_step_timed(nb200_engine *e, uint32_t seq, const uint32_t *tokens, uint32_t n, uint32_t reps, float *ms) {
     NB_OP(e, step_timed); return base(e)->ops->step_timed(e, seq, tokens, n, reps, ms);
 }
+int nb200_seq_fork(nb200_engine *e, uint32_t seq, uint32_t *fork) { NB_OP(e, seq_fork); return base(e)->ops->seq_fork(e, seq, fork); }
+int nb200_step_scores(nb200_engine *e, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, const uint32_t *targets, uint32_t n_want, uint32_t top,
+                      float *logprob, float *entropy, float *top_logprob, int32_t *top_id) {
+    NB_OP(e, step_scores); return base(e)->ops->step_scores(e, seq, tokens, n, want, targets, n_want, top, logprob, entropy, top_logprob, top_id);
+}
+int nb200_read_scores(nb200_engine *e, uint32_t target, uint32_t top, float *logprob, float *entropy, float *top_logprob, int32_t *top_id) {
+    NB_OP(e, read_scores); return base(e)->ops->read_scores(e, target, top, logprob, entropy, top_logprob, top_id);
+}
 int nb200_read_residual(nb200_engine *e, uint32_t run, float *dst, uint32_t count) { NB_OP(e, read_residual); return base(e)->ops->read_residual(e, run, dst, count); }
 
 uint64_t nb200_kernel_launches(const nb200_engine *e) { return e ? base(e)->launches : 0; }

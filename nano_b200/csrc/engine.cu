@@ -30,6 +30,7 @@
 #include "stream_count.h"
 #include "stream_groups.h"
 #include "stream_host.h"
+#include "ops.h"
 #include "sample_host.h"
 #include "family.h"
 #include "prefill.h"
@@ -100,6 +101,7 @@ struct nb200_engine : nb::EngineBase {
     uint32_t st_smem = 0, st_grid = 0;
     uint32_t *st_err_host = nullptr, *st_err_dev = nullptr;      // mapped pinned word: the code a device-side spin recorded before trapping
     nb::StreamCount st_count;                                    // exchange epochs and barrier arrivals used up so far (stream.cuh)
+    float *score_host = nullptr, *score_dev = nullptr;      // nb200_read_scores: pinned and device words
     float *logits_host = nullptr; bool logits_on_host = false;   // pinned copy of the logits that one-token calls of the streaming kernel write; whether it holds the last step's
     void *samp_ws = nullptr; size_t samp_cub = 0; uint32_t *samp_host = nullptr;       // device-side sampler workspace (sample.cu), pinned result
     uint64_t stream_bytes = 0;
@@ -668,6 +670,7 @@ static void nano_destroy(nb200_engine *e) {
     if (e->samp_host) cudaFreeHost(e->samp_host);
     if (e->tok_host) cudaFreeHost(e->tok_host);
     if (e->logits_host) cudaFreeHost(e->logits_host);
+    if (e->score_host) cudaFreeHost(e->score_host);
     if (e->stream) cudaStreamDestroy(e->stream);
     delete e;
 }
@@ -682,6 +685,7 @@ static int create_impl(nb200_engine **out, const uint8_t *img, uint64_t image_by
     if (!out || !img || image_bytes < 260 || max_seq_len == 0) return fail(NB200_EINVAL, "bad arguments");
     if (tp_size < 1 || tp_size > (uint32_t)kTpMax || tp_rank >= tp_size) return fail(NB200_EINVAL, "bad tensor-parallel rank/size");
     *out = nullptr;
+    if (flags & NB200_FLAG_KV4) return fail(NB200_EINVAL, "a cache in 4 bits is for model folders");
     if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
     if (rd_u32(img) != 0x42443453u || rd_u32(img + 4) != 0x55524c4du) return fail(NB200_EINVAL, "bad magic (not a BD4SURLM file)");
     CK(cudaSetDevice(device));
@@ -1433,8 +1437,31 @@ int nb200_trace_token(nb200_engine *e, uint32_t token, uint32_t pos, unsigned lo
     return r;
 }
 
+// log probability of `target`, entropy and alternatives of the last step's logits, which stay on the device
+static int nano_read_scores(nb200_engine *e, uint32_t target, uint32_t top, float *logprob, float *entropy, float *top_logprob, int32_t *top_id) {
+    if (!e || !logprob || !entropy || (top && (!top_logprob || !top_id))) return fail(NB200_EINVAL, "null argument");
+    if (target >= e->d.V) return fail(NB200_EINVAL, "token id %u outside the vocabulary of %u", target, e->d.V);
+    if (top > kTopMax || top > e->d.V) return fail(NB200_EINVAL, "%u alternatives asked for: at most %u, and no more than the vocabulary has", top, kTopMax);
+    if (e->tp_size > 1) return fail(NB200_EINVAL, "scores are not available on tensor-parallel engines (logits are sharded)");
+    CK(cudaSetDevice(e->device));
+    constexpr size_t words = 3u + 2u * kTopMax;          // token, log probability, entropy, alternatives
+    if (!e->score_host) CK(cudaHostAlloc(&e->score_host, words * 4u, cudaHostAllocDefault));
+    if (!e->score_dev) DM(e->score_dev, words * 4u);
+    uint32_t *tok = reinterpret_cast<uint32_t *>(e->score_dev);
+    float *lp = e->score_dev + 1, *tl = lp + 2;
+    *reinterpret_cast<uint32_t *>(e->score_host) = target;
+    CK(cudaMemcpyAsync(tok, e->score_host, 4u, cudaMemcpyHostToDevice, e->stream));
+    CK(logprobs_launch(LogprobArgs{e->logits, e->d.V, T_F32, 1u, e->d.V, tok, 4u, top, lp, lp + 1, top ? tl : nullptr, top ? reinterpret_cast<int32_t *>(tl + top) : nullptr}, e->stream));
+    e->launches++;
+    CK(cudaMemcpyAsync(e->score_host + 1, lp, (2u + 2u * top) * 4u, cudaMemcpyDeviceToHost, e->stream));
+    CK(cudaStreamSynchronize(e->stream));
+    *logprob = e->score_host[1]; *entropy = e->score_host[2];
+    if (top) { memcpy(top_logprob, e->score_host + 3, top * 4u); memcpy(top_id, e->score_host + 3 + top, top * 4u); }
+    return 0;
+}
+
 const nb::EngineOps kNanoOps = {nano_destroy, nano_get_config, nano_forward, nano_read_logits, nano_next_greedy, nano_next_sampled,
-                               nano_decode_greedy, nullptr, nullptr, nullptr, nullptr, nullptr};
+                               nano_decode_greedy, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nano_read_scores};
 
 // ---------------------------------------------------------------------------------------------
 // op-level entry points

@@ -63,6 +63,10 @@ struct EngineOps {
     int (*step)(nb200_engine *, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, uint32_t n_want, float *logits);
     int (*read_residual)(nb200_engine *, uint32_t run, float *dst, uint32_t count);
     int (*step_timed)(nb200_engine *, uint32_t seq, const uint32_t *tokens, uint32_t n, uint32_t reps, float *ms);
+    int (*seq_fork)(nb200_engine *, uint32_t seq, uint32_t *fork);
+    int (*step_scores)(nb200_engine *, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, const uint32_t *targets, uint32_t n_want, uint32_t top,
+                       float *logprob, float *entropy, float *top_logprob, int32_t *top_id);
+    int (*read_scores)(nb200_engine *, uint32_t target, uint32_t top, float *logprob, float *entropy, float *top_logprob, int32_t *top_id);
 };
 
 struct EngineBase {

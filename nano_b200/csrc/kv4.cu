@@ -555,7 +555,7 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 
 // ---- which instance, and how the work is shared out ----
 struct Plan { int nt; bool rows; Shape sh; };
-constexpr uint32_t kWarps = 4;
+constexpr uint32_t kWarps = 4, kBlocksPerSm = 3;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G), most = D > 128 ? 2u : 4u;
     Plan p{};
@@ -566,7 +566,7 @@ Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32
     // pages that a block can have in sight
     const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
     const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
-    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = 3ull * sms;
+    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)kBlocksPerSm * sms;
     const uint32_t least = p.rows ? 8u : 2u * kWarps;          // pages of a split
     p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want / std::max<uint64_t>(1, blocks), std::max(1u, pages / least)));
     return p;
@@ -610,6 +610,9 @@ size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32
     const Plan p = plan_for(B, T, H, G, D, width, window, block, sms);
     return p.sh.nsplit == 1 ? 0 : (size_t)B * G * p.sh.tiles * p.sh.nsplit * p.sh.cols * (D + 2u) * 4u;
 }
+
+// (keys are split only while blocks times splits stays within kBlocksPerSm blocks to an SM)
+size_t kv4_attn_workspace_most(uint32_t B, uint32_t G, uint32_t D, uint32_t sms) { return (size_t)std::max(B * G, kBlocksPerSm * sms) * kWarps * 32u * (D + 2u) * 4u; }
 
 cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, uint32_t *launches) {
     const Plan p = plan_for(a.B, a.T, a.H, a.G, a.D, a.width, a.window, a.block, sms);

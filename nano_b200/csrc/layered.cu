@@ -62,6 +62,7 @@
 #include "attn_tc.h"
 #include "f32_split.h"
 #include "family.h"
+#include "kv4.h"
 #include "layered_kernels.cuh"
 #include "layered_mixers.cuh"
 #include "layered_mixers2.cuh"
@@ -71,6 +72,7 @@
 #include "layered_one.cuh"
 #include "layered_tc.h"
 #include "modeldir.h"
+#include "ops.h"
 #include "sample_host.h"
 
 using nb::fail;
@@ -171,7 +173,7 @@ struct LayeredEngine : nb::EngineBase {
     int device = 0, num_sms = 148;
     cudaStream_t stream = nullptr, side = nullptr, side2 = nullptr, cur = nullptr;      // cur: where launch() puts kernels (stream, or side for a layer's feed-forward branch)
     cudaEvent_t ev_fork = nullptr, ev_join = nullptr, ev_join2 = nullptr;
-    bool f32 = false;
+    bool f32 = false, kv4 = false;      // kv4: the rows of grouped-query attention layers are held in 4 bits (kv4.h; NB200_FLAG_KV4)
     uint32_t V = 0, E = 0; float eps = 0.0f;
     std::vector<Layer> layers; std::vector<Run> runs;
     bool keep_x0 = false;
@@ -180,7 +182,7 @@ struct LayeredEngine : nb::EngineBase {
     // state manager
     uint32_t max_tokens = 0, max_seqs = 0, n_pages = 0, chunk_cap = 0; size_t slot_floats = 0;
     float *state = nullptr, *state_bak = nullptr; uint32_t *table = nullptr;
-    std::vector<uint32_t> free_pages; std::vector<Seq> seqs;
+    std::vector<uint32_t> free_pages, page_refs; std::vector<Seq> seqs;      // page_refs: how many sequences read a page (forks share full pages)
     // scratch (chunk_cap tokens)
     float *x = nullptr, *x0 = nullptr, *hm = nullptr, *h2 = nullptr, *d = nullptr, *d2 = nullptr;
     float *b_yx = nullptr, *b_u = nullptr, *b_g = nullptr, *b_sy = nullptr;                          // recurrent block
@@ -201,6 +203,7 @@ struct LayeredEngine : nb::EngineBase {
     float *b_gcv = nullptr, *b_gblk = nullptr, *b_gv = nullptr, *b_gsp = nullptr, *b_gt = nullptr, *b_go = nullptr, *b_ga = nullptr;
     // matrix memory: per head and token the gates' sums, per chunk the state before it
     double *b_mfa = nullptr, *b_mfb = nullptr, *b_mfc = nullptr; float *b_mmt = nullptr, *b_mme = nullptr, *b_mS = nullptr, *b_mn = nullptr, *b_mo = nullptr;
+    float *b_krows = nullptr, *b_kpart = nullptr;               // cache in 4 bits: key and value rows of a portion, parts of the key splits
     float *b_gpart = nullptr; uint32_t *b_gtick = nullptr;      // grouped-query attention: partials and tickets of the key splits
     uint32_t *ids_dev = nullptr, *want_dev = nullptr, *next_dev = nullptr, *tok_host = nullptr; uint8_t *seen = nullptr;
     // pinned host memory that copies go through without a wait: a call's token ids and wanted places, the sequences' page tables, logits rows.
@@ -218,6 +221,8 @@ struct LayeredEngine : nb::EngineBase {
     // generation on the implicit sequence
     int gen_seq = -1;
     void *samp_ws = nullptr; size_t samp_cub = 0; uint32_t *samp_host = nullptr;
+    // scores of wanted places: [log probabilities | entropies | alternatives' log probabilities | their ids] of kWantBatch rows, on the device and pinned; tokens asked for
+    float *score_dev = nullptr, *score_host = nullptr; uint32_t *score_tok = nullptr;
     TcState tc;              // products of long portions on the tensor cores' own memory (layered_tc.cu)
     nb::TcAttnState ta;      // and their attention (attn_tc.cu)
     float *b_kv = nullptr; size_t kv_floats = 0;      // keys and values multiplied out of the latents
@@ -1473,6 +1478,23 @@ int gqa_branch(LayeredEngine *e, const Layer &L, const Run &run, const Ctx &cx, 
     GqaArgs a{e->b_p, P, 0u, H * D, H * D + G * D, L.c_hg, L.qn, L.kn, L.rot_tab, L.a_half, run.cache, cx.table, T, H, G, D, VD, L.RL, cx.pos0, cx.pos_ptr, e->eps,
               L.scale, L.softcap, L.sink, L.has_gate ? 1u : 0u, e->b_a, 1u, e->b_gpart, e->b_gtick, gqa_hb(L), L.block_size, L.head_norm ? 1u : 0u};
     int r;
+    if (e->kv4) {      // normed and turned rows beside the cache, the cache's bytes from them, attention over its pages
+        a.cache = e->b_krows; a.flat = 1u;
+        if ((r = launch<GqaArgs>(e, k_qk_norm_rope, dim3(T), dim3(256), 0, a))) return r;
+        nb::Kv4Rows kr{};
+        kr.k = e->b_krows; kr.v = e->b_krows + G * D; kr.k_token = kr.v_token = L.RL; kr.k_head = D; kr.v_head = VD; kr.type = nb::T_F32;
+        kr.table = cx.table; kr.pos0 = cx.pos0; kr.pos_ptr = cx.pos_ptr; kr.T = T; kr.G = G; kr.D = D; kr.pool = reinterpret_cast<unsigned char *>(run.cache); kr.page_stride = (uint64_t)G * nb::kv4_block_bytes(D); kr.n_pages = e->n_pages;
+        CK(nb::kv4_write_launch(kr, e->cur, e->use_pdl));
+        nb::Kv4Attn ka{};      // (queries carry the scale already)
+        ka.q = e->b_p; ka.q_token = P; ka.q_head = D; ka.type = nb::T_F32; ka.out = e->b_a; ka.o_token = H * VD; ka.o_head = VD; ka.pool = kr.pool; ka.page_stride = kr.page_stride; ka.n_pages = e->n_pages;
+        ka.table = reinterpret_cast<const int32_t *>(cx.table); ka.width = cx.pos_ptr ? e->n_pages : (cx.pos0 + T + kPage - 1u) / kPage; ka.pos0 = cx.pos0; ka.pos_ptr = cx.pos_ptr;
+        ka.B = 1; ka.T = T; ka.H = H; ka.G = G; ka.D = D; ka.scale = 1.0f; ka.softcap = L.softcap; ka.sink = L.sink; ka.block = L.block_size; ka.part = e->b_kpart;
+        if (L.has_gate) { ka.gate = e->b_p + L.c_hg; ka.ldg = P; }
+        uint32_t launches = 0;
+        CK(nb::kv4_attn_launch(ka, (uint32_t)e->num_sms, e->cur, e->use_pdl, &launches));
+        e->launches += 1u + launches;
+        return gemm(e, plain(e->b_a, H * VD, L.o, dst, e->E, T), 1, T);
+    }
     if (T <= kGemvMaxM) {      // a captured step does not know the position: blocks without a share of the keys leave at once
         uint32_t pages = ((cx.pos_ptr ? e->max_tokens : cx.pos0 + T) + kPage - 1u) / kPage;
         if (L.block_size) pages = std::min(pages, (L.block_size + kPage - 2u) / kPage + 1u);      // a block of positions may start inside a page
@@ -2014,7 +2036,7 @@ int reserve_pages(LayeredEngine *e, uint32_t seq, uint32_t tokens) {
     if (need <= have) return 0;
     if (need - have > e->free_pages.size()) return fail(NB200_ENOMEM, "the cache is full: %u tokens asked for sequence %u, %zu pages free", tokens, seq, e->free_pages.size());
     uint32_t *row = e->stage_pages + (size_t)seq * e->n_pages;
-    for (size_t i = have; i < need; i++) { s.pages.push_back(e->free_pages.back()); e->free_pages.pop_back(); row[i] = s.pages[i]; }
+    for (size_t i = have; i < need; i++) { s.pages.push_back(e->free_pages.back()); e->free_pages.pop_back(); row[i] = s.pages[i]; e->page_refs[row[i]] = 1; }
     CK(cudaMemcpyAsync(e->table + (size_t)seq * e->n_pages + have, row + have, (need - have) * 4, cudaMemcpyHostToDevice, e->stream));
     return 0;
 }
@@ -2038,13 +2060,95 @@ int lm_seq_close(nb200_engine *h, uint32_t seq) {
     int r;
     if ((r = seq_check(e, seq))) return r;
     Seq &s = e->seqs[seq];
-    for (size_t i = s.pages.size(); i > 0; i--) e->free_pages.push_back(s.pages[i - 1]);
+    for (size_t i = s.pages.size(); i > 0; i--) if (--e->page_refs[s.pages[i - 1]] == 0) e->free_pages.push_back(s.pages[i - 1]);
     s.pages.clear(); s.live = false; s.len = 0;
     if ((int)seq == e->gen_seq) e->gen_seq = -1;
     return 0;
 }
 
+// bytes of one page of a layer run's cache (0: the run has none, or reads another run's)
+size_t cache_page_bytes(const LayeredEngine *e, const Run &q) {
+    const Layer &L = e->layers[q.layer];
+    switch (L.type) {
+        case MIX_DIFF_ATTN: return L.kv_from >= 0 ? 0 : (size_t)kPage * L.RL * 4;
+        case MIX_LATENT_ATTN: return (size_t)kPage * L.RS * 4;
+        case MIX_ATTN_DELTA: case MIX_GQA: return e->kv4 ? (size_t)L.G * nb::kv4_block_bytes(L.dim) : (size_t)kPage * L.RL * 4;
+        case MIX_WINDOW_SSM: return (size_t)kPage * L.RL * 4;
+        default: return 0;
+    }
+}
+
+// A second sequence that goes on from where `seq` stands: full pages are shared (nothing writes them any more), the last page, if it is not full, is copied in every
+// run's cache, and so is the state slot.  One launch for the pages of 32 runs (kPagePools), whatever the length
+int lm_seq_fork(nb200_engine *h, uint32_t seq, uint32_t *fork) {
+    LayeredEngine *e = self(h);
+    int r;
+    if (!fork) return fail(NB200_EINVAL, "null argument");
+    if ((r = seq_check(e, seq))) return r;
+    const uint32_t len = e->seqs[seq].len, full = len / kPage;
+    const bool rest = len % kPage != 0;
+    if (rest && e->free_pages.empty()) return fail(NB200_ENOMEM, "the cache is full: a fork of sequence %u needs a page", seq);
+    CK(cudaSetDevice(e->device));
+    uint32_t s = 0;
+    if ((r = lm_seq_open(h, &s))) return r;
+    Seq &to = e->seqs[s];
+    const Seq &from = e->seqs[seq];
+    uint32_t *row = e->stage_pages + (size_t)s * e->n_pages;
+    auto queue = [&]() -> int {
+        std::vector<nb::PagePool> pools;
+        pools.reserve(e->runs.size()); to.pages.reserve(from.pages.size());
+        for (uint32_t i = 0; i < full; i++) { to.pages.push_back(from.pages[i]); row[i] = from.pages[i]; e->page_refs[row[i]]++; }
+        if (rest) { to.pages.push_back(e->free_pages.back()); e->free_pages.pop_back(); row[full] = to.pages[full]; e->page_refs[row[full]] = 1; }
+        to.len = len;
+        CK(cudaMemcpyAsync(e->state + (size_t)s * e->slot_floats, e->state + (size_t)seq * e->slot_floats, e->slot_floats * 4, cudaMemcpyDeviceToDevice, e->stream));
+        if (!to.pages.empty()) CK(cudaMemcpyAsync(e->table + (size_t)s * e->n_pages, row, to.pages.size() * 4, cudaMemcpyHostToDevice, e->stream));
+        if (rest) {
+            for (const Run &q : e->runs) if (const size_t bytes = cache_page_bytes(e, q)) pools.push_back(nb::PagePool{q.cache, bytes, bytes});
+            uint32_t launches = 0;
+            CK(nb::pages_copy_launch(pools.data(), (uint32_t)pools.size(), &from.pages[full], &to.pages[full], 1, e->stream, &launches));
+            e->launches += launches;
+        }
+        CK(cudaStreamSynchronize(e->stream));
+        return 0;
+    };
+    try { r = queue(); } catch (const std::bad_alloc &) { r = fail(NB200_ENOMEM, "out of host memory"); }
+    if (r) { lm_seq_close(h, s); return r; }
+    *fork = s;
+    return 0;
+}
+
 // ---------------- step ----------------
+// what a call wants of its places instead of their logits: log probability of targets[i], entropy, the `top` best alternatives of wanted place i
+struct ScoreReq { const uint32_t *targets; uint32_t top; float *logprob, *entropy, *top_logprob; int32_t *top_id; };
+int score_room(LayeredEngine *e) {
+    if (e->score_dev) return 0;
+    constexpr size_t bytes = (size_t)kWantBatch * (2u + 2u * nb::kTopMax) * 4u;
+    if (!e->score_host) CK(cudaHostAlloc(&e->score_host, bytes + kWantBatch * 4u, cudaHostAllocDefault));
+    if (!e->score_tok) DM(e->score_tok, kWantBatch * 4u);
+    DM(e->score_dev, bytes);
+    return 0;
+}
+int score_check(const LayeredEngine *e, uint32_t top, const float *top_logprob, const int32_t *top_id) {
+    if (top > nb::kTopMax || top > e->V) return fail(NB200_EINVAL, "%u alternatives asked for: at most %u, and no more than the vocabulary has", top, nb::kTopMax);
+    if (top && (!top_logprob || !top_id)) return fail(NB200_EINVAL, "null argument");
+    return 0;
+}
+// rows [0, nw) of e->logits are places i0 .. i0 + nw of the request; a wait for everything before them
+int score_rows(LayeredEngine *e, uint32_t nw, uint32_t i0, const ScoreReq &q) {
+    const size_t k = q.top;
+    float *lp = e->score_dev, *ent = lp + nw, *tl = ent + nw; int32_t *ti = reinterpret_cast<int32_t *>(tl + nw * k);
+    uint32_t *tok = reinterpret_cast<uint32_t *>(e->score_host) + (size_t)kWantBatch * (2u + 2u * nb::kTopMax);
+    memcpy(tok, q.targets + i0, nw * 4u);
+    CK(cudaMemcpyAsync(e->score_tok, tok, nw * 4u, cudaMemcpyHostToDevice, e->stream));
+    CK(nb::logprobs_launch(nb::LogprobArgs{e->logits, e->V, nb::T_F32, nw, e->V, e->score_tok, 4u, q.top, lp, ent, k ? tl : nullptr, k ? ti : nullptr}, e->stream));
+    e->launches++;
+    CK(cudaMemcpyAsync(e->score_host, e->score_dev, nw * (2u + 2u * k) * 4u, cudaMemcpyDeviceToHost, e->stream));
+    CK(cudaStreamSynchronize(e->stream));
+    memcpy(q.logprob + i0, e->score_host, nw * 4u);
+    memcpy(q.entropy + i0, e->score_host + nw, nw * 4u);
+    if (k) { memcpy(q.top_logprob + i0 * k, e->score_host + 2u * nw, nw * k * 4u); memcpy(q.top_id + i0 * k, e->score_host + nw * (2u + k), nw * k * 4u); }
+    return 0;
+}
 // the first nw rows of e->logits to the caller, and a wait for everything before them
 int fetch_logits(LayeredEngine *e, uint32_t nw, float *dst) {
     const bool staged = nw <= e->stage_rows;
@@ -2054,8 +2158,8 @@ int fetch_logits(LayeredEngine *e, uint32_t nw, float *dst) {
     return 0;
 }
 
-// tokens already on the device at tok_dev[0..n); want (host, ascending, may be null) -> logits_host [n_want][V]
-int step_dev(LayeredEngine *e, uint32_t seq, const uint32_t *tok_dev, uint32_t n, const uint32_t *want, uint32_t n_want, float *logits_host) {
+// tokens already on the device at tok_dev[0..n); want (host, ascending, may be null) -> logits_host [n_want][V], or what `score` asks for of them (its first place is want[0])
+int step_dev(LayeredEngine *e, uint32_t seq, const uint32_t *tok_dev, uint32_t n, const uint32_t *want, uint32_t n_want, float *logits_host, const ScoreReq *score = nullptr) {
     int r;
     Seq &s = e->seqs[seq];
     if ((r = reserve_pages(e, seq, s.len + n))) return r;
@@ -2071,7 +2175,7 @@ int step_dev(LayeredEngine *e, uint32_t seq, const uint32_t *tok_dev, uint32_t n
         while (wi < n_want && want[wi] < c0 + T) {
             uint32_t nw = 0;
             while (nw < kWantBatch && wi + nw < n_want && want[wi + nw] < c0 + T) nw++;
-            if ((r = head_rows(e, nw, e->want_dev + wi)) || (r = fetch_logits(e, nw, logits_host + (size_t)wi * e->V))) return r;
+            if ((r = head_rows(e, nw, e->want_dev + wi)) || (r = score ? score_rows(e, nw, wi, *score) : fetch_logits(e, nw, logits_host + (size_t)wi * e->V))) return r;
             wi += nw;
         }
     }
@@ -2083,17 +2187,17 @@ int check_tokens(LayeredEngine *e, const uint32_t *tokens, uint32_t n) {
     return 0;
 }
 
-int lm_step(nb200_engine *h, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, uint32_t n_want, float *logits) {
-    LayeredEngine *e = self(h);
+// logits, or score
+int step_any(LayeredEngine *e, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, uint32_t n_want, float *logits, const ScoreReq *score) {
     int r;
-    if (!tokens || n == 0 || (n_want && (!want || !logits))) return fail(NB200_EINVAL, "bad arguments");
+    if (!tokens || n == 0 || (n_want && (!want || (!logits && !score)))) return fail(NB200_EINVAL, "bad arguments");
     if ((r = seq_check(e, seq)) || (r = check_tokens(e, tokens, n))) return r;
     for (uint32_t i = 0; i < n_want; i++) if (want[i] >= n || (i && want[i] <= want[i - 1])) return fail(NB200_EINVAL, "want[] must be ascending indices into this step's tokens");
     CK(cudaSetDevice(e->device));
     if (n == 1) {          // a single token: the captured decode step
         Seq &s = e->seqs[seq];
         if ((r = reserve_pages(e, seq, s.len + 1))) return r;
-        if (n_want && e->use_graph && !e->keep) {
+        if (n_want && !score && e->use_graph && !e->keep) {
             if ((r = call_step(e, seq, s.len, tokens[0]))) return r;
             s.len += 1;
             CK(cudaStreamSynchronize(e->stream));
@@ -2102,7 +2206,7 @@ int lm_step(nb200_engine *h, uint32_t seq, const uint32_t *tokens, uint32_t n, c
         }
         if ((r = set_step(e, s.len, tokens[0])) || (r = decode_step(e, seq))) return r;
         s.len += 1;
-        if (n_want) return fetch_logits(e, 1, logits);
+        if (n_want) return score ? score_rows(e, 1, 0, *score) : fetch_logits(e, 1, logits);
         CK(cudaStreamSynchronize(e->stream));
         return 0;
     }
@@ -2117,10 +2221,26 @@ int lm_step(nb200_engine *h, uint32_t seq, const uint32_t *tokens, uint32_t n, c
         w1 = w0;
         done.clear();
         while (w1 < n_want && want[w1] < c0 + m) done.push_back(want[w1++] - c0);
-        if ((r = step_dev(e, seq, e->ids_dev, m, done.data(), (uint32_t)done.size(), logits ? logits + (size_t)w0 * e->V : nullptr))) return r;
+        ScoreReq part{};
+        if (score) part = ScoreReq{score->targets + w0, score->top, score->logprob + w0, score->entropy + w0, score->top_logprob ? score->top_logprob + (size_t)w0 * score->top : nullptr, score->top_id ? score->top_id + (size_t)w0 * score->top : nullptr};
+        if ((r = step_dev(e, seq, e->ids_dev, m, done.data(), (uint32_t)done.size(), logits ? logits + (size_t)w0 * e->V : nullptr, score ? &part : nullptr))) return r;
     }
     CK(cudaStreamSynchronize(e->stream));
     return tc_check(&e->tc);
+}
+int lm_step(nb200_engine *h, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, uint32_t n_want, float *logits) {
+    return step_any(self(h), seq, tokens, n, want, n_want, logits, nullptr);
+}
+int lm_step_scores(nb200_engine *h, uint32_t seq, const uint32_t *tokens, uint32_t n, const uint32_t *want, const uint32_t *targets, uint32_t n_want, uint32_t top, float *logprob,
+                   float *entropy, float *top_logprob, int32_t *top_id) {
+    LayeredEngine *e = self(h);
+    int r;
+    if (n_want && (!targets || !logprob || !entropy)) return fail(NB200_EINVAL, "bad arguments");
+    if ((r = score_check(e, top, top_logprob, top_id)) || (r = check_tokens(e, targets, n_want))) return r;
+    CK(cudaSetDevice(e->device));
+    if ((r = score_room(e))) return r;
+    const ScoreReq q{targets, top, logprob, entropy, top_logprob, top_id};
+    return step_any(e, seq, tokens, n, want, n_want, nullptr, &q);
 }
 
 int lm_step_timed(nb200_engine *h, uint32_t seq, const uint32_t *tokens, uint32_t n, uint32_t reps, float *ms) {
@@ -2218,6 +2338,16 @@ int lm_read_logits(nb200_engine *h, float *out) {
     if (!out) return fail(NB200_EINVAL, "null argument");
     CK(cudaSetDevice(e->device));
     return fetch_logits(e, 1, out);
+}
+
+int lm_read_scores(nb200_engine *h, uint32_t target, uint32_t top, float *logprob, float *entropy, float *top_logprob, int32_t *top_id) {
+    LayeredEngine *e = self(h);
+    int r;
+    if (!logprob || !entropy) return fail(NB200_EINVAL, "null argument");
+    if ((r = score_check(e, top, top_logprob, top_id)) || (r = check_tokens(e, &target, 1))) return r;
+    CK(cudaSetDevice(e->device));
+    if ((r = score_room(e))) return r;
+    return score_rows(e, 1, 0, ScoreReq{&target, top, logprob, entropy, top_logprob, top_id});
 }
 
 int mark_seen(LayeredEngine *e, const uint32_t *ids, uint32_t pos) {
@@ -2340,6 +2470,7 @@ void lm_destroy(nb200_engine *h) {
     for (void *p : e->allocs) cudaFree(p);
     for (void *p : {(void *)e->tok_host, (void *)e->stage_ids, (void *)e->stage_want, (void *)e->stage_pages, (void *)e->stage_logits}) if (p) cudaFreeHost(p);
     if (e->samp_host) cudaFreeHost(e->samp_host);
+    if (e->score_host) cudaFreeHost(e->score_host);
     nb::attn_tc_free(&e->ta);
     tc_free(&e->tc);
     if (e->ev_fork) cudaEventDestroy(e->ev_fork);
@@ -2352,7 +2483,7 @@ void lm_destroy(nb200_engine *h) {
 }
 
 const nb::EngineOps kLayeredOps = {lm_destroy, lm_get_config, lm_forward, lm_read_logits, lm_next_greedy, lm_next_sampled, lm_decode_greedy,
-                                   lm_seq_open, lm_seq_close, lm_step, lm_read_residual, lm_step_timed};
+                                   lm_seq_open, lm_seq_close, lm_step, lm_read_residual, lm_step_timed, lm_seq_fork, lm_step_scores, lm_read_scores};
 
 
 // What long portions need beside the engine: rounded rows of every product (rows: numbers), images of keys and values for as many keys as a sequence can hold
@@ -2373,7 +2504,7 @@ int portion_memory(LayeredEngine *e, Loader &ld, size_t rows) {
     bool grouped = false;
     for (const Layer &L : e->layers) {
         const bool up = L.type == MIX_LATENT_ATTN && latent_up(e, L);
-        if (!up && L.type != MIX_ATTN_DELTA && L.type != MIX_GQA) continue;
+        if (!up && (e->kv4 || (L.type != MIX_ATTN_DELTA && L.type != MIX_GQA))) continue;      // (a cache in 4 bits has no images)
         const uint32_t G = up ? L.H : L.G;
         image = std::max(image, nb::attn_tc_bytes(128, G, L.dim, L.vdim) / 128u); heads = std::max(heads, G);
         if (!up) { grouped = true; continue; }
@@ -2607,6 +2738,18 @@ int create(LayeredEngine *e, const nb::ModelDir *dir, uint32_t max_tokens) {
         for (uint32_t i = hi; i < NL; i++) { Run q; q.layer = i; e->runs.push_back(q); }
     }
 
+    if (e->kv4) {
+        bool any = false;
+        if (e->f32) return fail(NB200_EINVAL, "a cache in 4 bits and true 32-bit compute exclude each other");
+        for (size_t i = 0; i < e->layers.size(); i++) {
+            const Layer &L = e->layers[i];
+            if (L.type != MIX_GQA && L.type != MIX_ATTN_DELTA) continue;
+            any = true;
+            if (L.dim != L.vdim || !nb::kv4_dim_ok(L.dim)) return fail(NB200_EINVAL, "layer %zu: dim %u and vdim %u have no cache in 4 bits (equal ones of 32, 64, 96, 128 and 256 have)", i, L.dim, L.vdim);
+        }
+        if (!any) return fail(NB200_EINVAL, "the model has no grouped-query attention layer whose cache could be held in 4 bits");
+    }
+
     // state manager: slots and pages
     e->max_tokens = max_tokens;
     e->max_seqs = std::max(1u, env_u32("NB200_MAX_SEQS", 8));
@@ -2636,11 +2779,11 @@ int create(LayeredEngine *e, const nb::ModelDir *dir, uint32_t max_tokens) {
                 q.st_conv = off; off += (size_t)(L.d_taps - 1) * (2 * L.dG * L.dD + L.dH * L.dVD);
                 off = (off + 3) & ~(size_t)3;
                 q.st_S = off; off += (size_t)L.dH * L.dVD * L.dD;
-                if (L.type == MIX_ATTN_DELTA) { DM(q.cache, (size_t)e->n_pages * kPage * L.RL * 4); CK(cudaMemset(q.cache, 0, (size_t)e->n_pages * kPage * L.RL * 4)); }
-                break;
-            case MIX_GQA:            // rows of [normed and turned keys | values]
-                DM(q.cache, (size_t)e->n_pages * kPage * L.RL * 4);
-                CK(cudaMemset(q.cache, 0, (size_t)e->n_pages * kPage * L.RL * 4));
+                if (L.type == MIX_DELTA) break;
+                [[fallthrough]];
+            case MIX_GQA:            // rows of [normed and turned keys | values], or blocks of 4-bit codes
+                DM(q.cache, (size_t)e->n_pages * cache_page_bytes(e, q));
+                CK(cudaMemset(q.cache, 0, (size_t)e->n_pages * cache_page_bytes(e, q)));
                 break;
             case MIX_MEMORY:         // the state [head][value column][key coordinate], the normaliser [head][key coordinate], the running maximum
                 off = (off + 3) & ~(size_t)3;
@@ -2664,9 +2807,18 @@ int create(LayeredEngine *e, const nb::ModelDir *dir, uint32_t max_tokens) {
     CK(cudaMemset(e->table, 0, (size_t)e->max_seqs * e->n_pages * 4));
     e->seqs.resize(e->max_seqs);
     for (uint32_t p = e->n_pages; p > 0; p--) e->free_pages.push_back(p - 1);
+    e->page_refs.assign(e->n_pages, 0);
 
     // scratch for one chunk
     const size_t T = e->chunk_cap;
+    if (e->kv4) {
+        size_t row = 0, part = 0;
+        for (const Run &q : e->runs) {
+            const Layer &L = e->layers[q.layer];
+            if (L.type == MIX_GQA || L.type == MIX_ATTN_DELTA) { row = std::max<size_t>(row, L.RL); part = std::max(part, nb::kv4_attn_workspace_most(1, L.G, L.dim, (uint32_t)e->num_sms)); }
+        }
+        DM(e->b_krows, T * row * 4); DM(e->b_kpart, part);
+    }
     uint32_t mC = 0, mZ = 0, mQR = 0, mQ = 0, mHR = 0, mOV = 0, mNE = 0, mTop = 0, mFF = 0, mSFF = 0;
     uint32_t sP = 0, sQK = 0, sXC = 0, sA = 0, sRO = 0, sDBC = 0, sF = 0;
     uint32_t sDP = 0, sDT = 0, sXC2 = 0, sY = 0, sF2 = 0; size_t sSS = 0, diff_smem[4] = {0, 0, 0, 0};      // differential attention, state-space duality, gated feed-forward
@@ -2847,7 +2999,7 @@ extern "C" int nb_family_layered_create(nb200_engine **out, const nb::ModelDir *
     CK(cudaSetDevice(device));
     LayeredEngine *e = new LayeredEngine();
     e->ops = &kLayeredOps;
-    e->device = device; e->f32 = (flags & NB200_FLAG_F32) != 0;
+    e->device = device; e->f32 = (flags & NB200_FLAG_F32) != 0; e->kv4 = (flags & NB200_FLAG_KV4) != 0;
     e->use_pdl = !(flags & NB200_FLAG_NO_PDL) && !env_u32("NB200_NO_PDL", 0);
     e->use_graph = !(flags & NB200_FLAG_NO_GRAPH) && !env_u32("NB200_NO_GRAPH", 0);
     e->branch_streams = !env_u32("NB200_NO_BRANCH_STREAMS", 0);

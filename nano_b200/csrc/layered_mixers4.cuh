@@ -120,6 +120,7 @@ struct GqaArgs {
     float scale, softcap; const float *sink; uint32_t has_gate; float *out;      // softcap 0: none; sink null: none; out [T][H VD]
     uint32_t nsplit; float *part; uint32_t *tickets; uint32_t hb;                // k_gqa_decode: key splits; query heads per block
     uint32_t block, head_norm;
+    uint32_t flat;          // k_qk_norm_rope: row t of `cache` receives token t (a cache of another form is written from there)
 };
 __device__ __forceinline__ uint32_t gqa_first(uint32_t pos, uint32_t block) { return block ? pos - pos % block : 0u; }      // the first key position pos sees
 // coordinate d of one head: normed by r and its gains, turned
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(const GqaArgs a) {
     const float2 *cs = a.tab + (size_t)pos * half;
     // a warp per head; q in place (a lane owns both coordinates of a pair), k into the token's cache row, v beside it
     const uint32_t per = a.D - half, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, nw = blockDim.x >> 5;
-    float *row = a.cache + ((size_t)a.table[pos / kPage] * kPage + pos % kPage) * a.RL;
+    float *row = a.cache + (a.flat ? (size_t)t : (size_t)a.table[pos / kPage] * kPage + pos % kPage) * a.RL;
     for (uint32_t h = warp; h < a.H + a.G; h += nw) {
         const bool isq = h < a.H;
         const uint32_t hh = (isq ? h : h - a.H) * a.D;

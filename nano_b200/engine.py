@@ -18,8 +18,9 @@ f32p = C.POINTER(C.c_float)
 u32p = C.POINTER(C.c_uint32)
 u8p = C.POINTER(C.c_uint8)
 i8p = C.POINTER(C.c_int8)
+i32p = C.POINTER(C.c_int32)
 
-FLAG_EXACT, FLAG_NO_GRAPH, FLAG_NO_PDL, FLAG_NO_STREAM, FLAG_F32 = 0x1, 0x2, 0x4, 0x10, 0x20
+FLAG_EXACT, FLAG_NO_GRAPH, FLAG_NO_PDL, FLAG_NO_STREAM, FLAG_F32, FLAG_KV4 = 0x1, 0x2, 0x4, 0x10, 0x20, 0x40
 ARCH_LAYERED = 16
 F_X, F_XBA, F_HB, F_Q, F_LOGITS, F_KROW, F_VROW, F_ACT_I8, F_ACT_SCALE = 0, 2, 4, 6, 9, 13, 14, 20, 21
 
@@ -33,6 +34,7 @@ EXPORTS = [
     "nb200_lora_load", "nb200_lora_enable", "nb200_lora_unload",
     "nb200_engine_create_tp", "nb200_tp_export", "nb200_tp_attach_ipc", "nb200_tp_attach_local",
     "nb200_engine_create_dir", "nb200_seq_open", "nb200_seq_close", "nb200_step", "nb200_step_timed", "nb200_read_residual",
+    "nb200_seq_fork", "nb200_step_scores", "nb200_read_scores",
     "nb200_dev_token_logprobs", "nb200_dev_pages_copy",
     "nb200_dev_kv4_write", "nb200_dev_kv4_read", "nb200_dev_kv4_attention_workspace", "nb200_dev_kv4_attention",
 ]
@@ -132,6 +134,9 @@ def lib(layered_ok: bool = False):
         L.nb200_step.argtypes = [C.c_void_p, C.c_uint32, u32p, C.c_uint32, u32p, C.c_uint32, f32p]
         L.nb200_step_timed.argtypes = [C.c_void_p, C.c_uint32, u32p, C.c_uint32, C.c_uint32, f32p]
         L.nb200_read_residual.argtypes = [C.c_void_p, C.c_uint32, f32p, C.c_uint32]
+        L.nb200_seq_fork.argtypes = [C.c_void_p, C.c_uint32, u32p]
+        L.nb200_step_scores.argtypes = [C.c_void_p, C.c_uint32, u32p, C.c_uint32, u32p, u32p, C.c_uint32, C.c_uint32, f32p, f32p, f32p, i32p]
+        L.nb200_read_scores.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, f32p, f32p, f32p, i32p]
         L.nb200_dev_token_logprobs.argtypes = [C.c_void_p] * 5 + [C.c_uint32, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]
         L.nb200_dev_pages_copy.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), u32p, C.c_uint32, u32p, u32p, C.c_uint32, C.c_void_p]
         L.nb200_dev_kv4_write.argtypes = L.nb200_dev_kv4_read.argtypes = [C.POINTER(Kv4Rows), C.c_void_p]
@@ -253,6 +258,34 @@ class Engine:
         _check(lib().nb200_step(self.h, int(seq), _p(t, u32p), t.size, _p(w, u32p) if w.size else None, w.size,
                                 _p(out, f32p) if w.size else None))
         return out
+
+    def seq_fork(self, seq: int) -> int:
+        """A sequence that goes on from where `seq` stands: its full pages are shared, the page in progress and the state are copied."""
+        s = C.c_uint32(0)
+        _check(lib().nb200_seq_fork(self.h, int(seq), C.byref(s)))
+        return int(s.value)
+
+    def step_scores(self, seq: int, tokens, want, targets, top: int = 0):
+        """Runs the next tokens of `seq`; returns (logprob [n], entropy [n], top_logprob [n, top], top_id [n, top]) at the places `want` (ascending): the log probability of
+        targets[i] as the token after place want[i], and the `top` (<= 32) most probable ones.  The logits stay on the device."""
+        t = np.ascontiguousarray(tokens, np.uint32); w = np.ascontiguousarray(want, np.uint32); g = np.ascontiguousarray(targets, np.uint32)
+        if w.shape != g.shape or w.ndim != 1:
+            raise NB200Error("a target for every wanted place")
+        both = np.empty((2, w.size), np.float32); tl, ti = self._tops(w.size, top)
+        _check(lib().nb200_step_scores(self.h, int(seq), _p(t, u32p), t.size, _p(w, u32p), _p(g, u32p), w.size, int(top), _p(both[0], f32p), _p(both[1], f32p), _p(tl, f32p), _p(ti, i32p)))
+        return both[0], both[1], tl, ti
+
+    def read_scores(self, target: int, top: int = 0):
+        """(log probability of `target`, entropy, top_logprob [top], top_id [top]) of the logits that logits() would return."""
+        lp, ent = C.c_float(0), C.c_float(0); tl, ti = self._tops(1, top)
+        _check(lib().nb200_read_scores(self.h, int(target), int(top), C.byref(lp), C.byref(ent), _p(tl, f32p), _p(ti, i32p)))
+        return float(lp.value), float(ent.value), tl[0], ti[0]
+
+    @staticmethod
+    def _tops(n: int, top: int):
+        if not 0 <= top <= 32:
+            raise NB200Error(f"{top} alternatives asked for: at most 32")
+        return np.empty((n, top), np.float32), np.empty((n, top), np.int32)
 
     def step_timed(self, seq: int, tokens, reps: int) -> float:
         """Mean device milliseconds of running `tokens` from the sequence's present state (the state is restored between runs)."""
