@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -143,6 +144,7 @@ bool rows_at16(const Kv4Rows &a) {
 // Values that stand for NaN are taken out of the product (0 times NaN would reach columns that do not see them) and make the rows that do see them NaN.
 // ------------------------------------------------------------------------------------------------
 constexpr int kLift = 12;
+constexpr float kLag = 3.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -158,7 +160,9 @@ __device__ __forceinline__ __half2 half2_of(uint32_t v) { return *reinterpret_ca
 // the codes at bits 0-3 and 16-19 (HIGH: 4-7 and 20-23) of w as c s + m
 template <bool HIGH>
 __device__ __forceinline__ uint32_t stand_for(uint32_t w, __half2 s, __half2 m) {
-    const __half2 h = half2_of((w & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+    uint32_t x;          // (one instruction with both constants in registers; written in C++ it became two with immediates)
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "r"(HIGH ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+    const __half2 h = half2_of(x);
     const __half2 c = HIGH ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-64.0f)) : __hsub2(h, __float2half2_rn(1024.0f));
     return bits(__hfma2(c, s, m));
 }
@@ -215,7 +219,7 @@ __device__ __forceinline__ void store_four(const Kv4Attn &a, uint32_t b, uint32_
 }
 
 struct Shape { uint32_t nsplit, tiles, cols; };          // splits of the keys, blocks along the columns of a head, columns of a block
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 template <int NG, int NT, int WK, int W>
 struct Room {
     static constexpr uint32_t block = 1280u * NG, ring = W * kStages * block, merge = WK > 1 ? W * NT * 8u * (32u * NG + 2u) * 4u : 0u,
@@ -224,7 +228,7 @@ struct Room {
 
 // grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
 template <int NG, int NT, int WK, int W>
-__global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shape sh) {
+__global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn(const Kv4Attn a, const Shape sh) {
     pdl_enter4();
     using R = Room<NG, NT, WK, W>;
     constexpr uint32_t D = 32u * NG, COLS = NT * 8u;
@@ -237,6 +241,38 @@ __global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shap
     float *scale_s = reinterpret_cast<float *>(sm + (R::ring > R::merge ? R::ring : R::merge) + R::q) + wr * COLS;
     const uint32_t c0 = tile * sh.cols + wr * COLS;
     const int len = seq_len(a, b);
+
+    // pages that any of this warp's columns sees, and the share of this split
+    const uint32_t c1 = min(c0 + COLS, ncols);
+    const int pos_a = c0 < ncols ? len - (int)a.T + (int)(c0 / rep) : -1, pos_b = c0 < ncols ? len - (int)a.T + (int)((c1 - 1u) / rep) : -1;
+    uint32_t p0 = 0, p1 = 0;
+    int low_b = 0;
+    if (pos_b >= 0) {
+        const uint32_t first = (uint32_t)first_seen(max(pos_a, 0), a.window, a.block) / kKv4Page, np = (uint32_t)pos_b / kKv4Page + 1u - first;
+        p0 = first + (uint32_t)((uint64_t)np * split / sh.nsplit); p1 = first + (uint32_t)((uint64_t)np * (split + 1u) / sh.nsplit);
+        low_b = first_seen(pos_b, a.window, a.block);
+    }
+    const uint32_t count = p0 + wk < p1 ? (p1 - p0 - wk + WK - 1u) / WK : 0u;
+
+    uint32_t ahead = 0;          // page numbers of 32 steps, one to a lane
+    const unsigned char *head = a.pool + (uint64_t)g * R::block;
+    const int32_t *table = a.table + (uint64_t)b * a.table_stride;
+    auto fetch = [&](uint32_t i) {
+        if (i < count) {
+            if ((i & 31u) == 0) { const uint32_t p = p0 + wk + (i + lane) * WK; ahead = p < p1 ? (uint32_t)table[p] : 0u; }
+            const uint32_t page = __shfl_sync(0xffffffffu, ahead, i & 31u), stage = i % kStages;
+            const bool ok = page < a.n_pages;
+            if (lane == 0) known[warp][stage] = ok;
+            if (ok) {
+                const unsigned char *src = head + (uint64_t)page * a.page_stride;
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * R::block);
+#pragma unroll
+                for (uint32_t v = 0; v < (80u * NG + 31u) / 32u; v++) { const uint32_t k = v * 32u + lane; if (80u * NG % 32u == 0 || k < 80u * NG) copy16(dst + k * 16u, src + k * 16u); }
+            }
+        }
+        copy_commit();
+    };
+    for (uint32_t i = 0; i < kStages - 1; i++) fetch(i);
 
     // the queries as the column operand, each row times the power of two that brings its largest number to [1, 2)
     for (uint32_t c = wk; c < COLS; c += WK) {
@@ -264,17 +300,6 @@ __global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shap
     }
     if constexpr (WK > 1) __syncthreads(); else __syncwarp();
 
-    // pages that any of this warp's columns sees, and the share of this split
-    const uint32_t c1 = min(c0 + COLS, ncols);
-    const int pos_a = c0 < ncols ? len - (int)a.T + (int)(c0 / rep) : -1, pos_b = c0 < ncols ? len - (int)a.T + (int)((c1 - 1u) / rep) : -1;
-    uint32_t p0 = 0, p1 = 0;
-    int low_b = 0;
-    if (pos_b >= 0) {
-        const uint32_t first = (uint32_t)first_seen(max(pos_a, 0), a.window, a.block) / kKv4Page, np = (uint32_t)pos_b / kKv4Page + 1u - first;
-        p0 = first + (uint32_t)((uint64_t)np * split / sh.nsplit); p1 = first + (uint32_t)((uint64_t)np * (split + 1u) / sh.nsplit);
-        low_b = first_seen(pos_b, a.window, a.block);
-    }
-    const uint32_t count = p0 + wk < p1 ? (p1 - p0 - wk + WK - 1u) / WK : 0u;
 
     float m[NT][2], l[NT][2], o[2 * NG][NT][4];
 #pragma unroll
@@ -293,25 +318,6 @@ __global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shap
             pos[t][x] = c0 + c < ncols ? len - (int)a.T + (int)((c0 + c) / rep) : -1;
         }
 
-    uint32_t ahead = 0;          // page numbers of 32 steps, one to a lane
-    const unsigned char *head = a.pool + (uint64_t)g * R::block;
-    const int32_t *table = a.table + (uint64_t)b * a.table_stride;
-    auto fetch = [&](uint32_t i) {
-        if (i < count) {
-            if ((i & 31u) == 0) { const uint32_t p = p0 + wk + (i + lane) * WK; ahead = p < p1 ? (uint32_t)table[p] : 0u; }
-            const uint32_t page = __shfl_sync(0xffffffffu, ahead, i & 31u), stage = i % kStages;
-            const bool ok = page < a.n_pages;
-            if (lane == 0) known[warp][stage] = ok;
-            if (ok) {
-                const unsigned char *src = head + (uint64_t)page * a.page_stride;
-                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * R::block);
-#pragma unroll
-                for (uint32_t v = 0; v < (80u * NG + 31u) / 32u; v++) { const uint32_t k = v * 32u + lane; if (80u * NG % 32u == 0 || k < 80u * NG) copy16(dst + k * 16u, src + k * 16u); }
-            }
-        }
-        copy_commit();
-    };
-    for (uint32_t i = 0; i < kStages - 1; i++) fetch(i);
     uint32_t qf[NT == 1 ? 2 * NG : 1][2];
     if constexpr (NT == 1)
 #pragma unroll
@@ -331,9 +337,10 @@ __global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shap
         {
             uint32_t w[NG];
             take<4 * NG>(pg + 1152u * NG + lane * 4u * NG, w);
-            bool odd = false;
+            __half2 zero = __float2half2_rn(0.0f);          // 0 times a pair is 0, or NaN
 #pragma unroll
-            for (int j = 0; j < NG; j++) odd = odd || (w[j] & 0x7c00u) == 0x7c00u || (w[j] & 0x7c000000u) == 0x7c000000u;
+            for (int j = 0; j < NG; j++) zero = __hfma2(half2_of(w[j]), __float2half2_rn(0.0f), zero);
+            const bool odd = !__hbeq2(zero, __float2half2_rn(0.0f));
             bad = __ballot_sync(0xffffffffu, odd);
             if (bad) {
                 if (odd)
@@ -374,46 +381,67 @@ __global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shap
         uint32_t pw[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            float top[2] = {m[t][0], m[t][1]};
+            float top[2] = {-INFINITY, -INFINITY};
+            if (a.softcap > 0.0f) {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) s[k][t][x] = a.softcap * kLog2e * tanhf(s[k][t][x] * f[t][x & 1]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) s[k][t][x] *= f[t][x & 1];
+            }
+            if (!whole) {
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int low = first_seen(max(pos[t][x], 0), a.window, a.block) - key0 - (int)row, high = pos[t][x] - key0 - (int)row;          // of the rows 16 k + 8 r
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) if (k * 16 + r * 8 > high || k * 16 + r * 8 < low) s[k][t][2 * r + x] = -INFINITY;
+                }
+            }
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    float v = s[k][t][x] * f[t][x & 1];
-                    if (a.softcap > 0.0f) v = a.softcap * kLog2e * tanhf(v);
-                    if (!whole) {
-                        const int key = key0 + k * 16 + (x >> 1) * 8 + (int)row;
-                        if (key > pos[t][x & 1] || key < first_seen(max(pos[t][x & 1], 0), a.window, a.block)) v = -INFINITY;
-                    }
-                    s[k][t][x] = v;
-                    top[x & 1] = fmaxf(top[x & 1], v);
+                for (int x = 0; x < 4; x++) top[x & 1] = fmaxf(top[x & 1], s[k][t][x]);
+            // the maximum in use may lag behind by kLag (the weights then reach 2^(kLift + kLag)): most pages leave it, and the values, as they are
+            if (__any_sync(0xffffffffu, top[0] > m[t][0] + kLag || top[1] > m[t][1] + kLag)) {
+                float corr[2];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    top[x] = fmaxf(top[x], m[t][x]);
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], off));
+                    corr[x] = ex2(m[t][x] - (top[x] == -INFINITY ? 0.0f : top[x]));
+                    m[t][x] = top[x];
+                    l[t][x] *= corr[x];
                 }
-            float corr[2], use[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], off));
-                use[x] = top[x] == -INFINITY ? 0.0f : top[x];
-                corr[x] = ex2(m[t][x] - use[x]);
-                m[t][x] = top[x];
-                use[x] -= (float)kLift;
-                l[t][x] *= corr[x];
-            }
-            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f))
 #pragma unroll
                 for (int d = 0; d < 2 * NG; d++) { o[d][t][0] *= corr[0]; o[d][t][1] *= corr[1]; o[d][t][2] *= corr[0]; o[d][t][3] *= corr[1]; }
+            }
+            const float use[2] = {m[t][0] == -INFINITY ? 0.0f : m[t][0] - (float)kLift, m[t][1] == -INFINITY ? 0.0f : m[t][1] - (float)kLift};
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     const float u = ex2(s[k][t][2 * r] - use[0]), v = ex2(s[k][t][2 * r + 1] - use[1]);
                     l[t][0] += u; l[t][1] += v;
-                    if (bad && (bad >> (k * 16 + r * 8 + row) & 1u)) {          // seen, however little it weighs
-                        if (s[k][t][2 * r] != -INFINITY) l[t][0] = NAN;
-                        if (s[k][t][2 * r + 1] != -INFINITY) l[t][1] = NAN;
-                    }
                     pw[t][2 * k + r] = transpose8(bits(__floats2half2_rn(u, v)));
                 }
+        }
+
+        if (bad) {          // values that are no number make the rows that see them NaN, however little they weigh
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (bad >> (k * 8 + row) & 1u) {
+                        if (s[k >> 1][t][2 * (k & 1)] != -INFINITY) l[t][0] = NAN;
+                        if (s[k >> 1][t][2 * (k & 1) + 1] != -INFINITY) l[t][1] = NAN;
+                    }
         }
 
         // weighted values: depth step k takes tokens 16 k + tq + {0, 4, 8, 12}; rows are coordinates 32 j + 4 gq + {0 .. 3}
@@ -511,34 +539,50 @@ __global__ void __launch_bounds__(W * 32) k_kv4_attn(const Kv4Attn a, const Shap
     }
 }
 
-// The parts of a row's splits put together: a warp per row.  grid (ceil(T rep / 8), G, B)
-__global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a, const Shape sh) {
+// The parts of a row's splits put together: a block per row, its warps take every fourth split.  grid (T rep, G, B); shared memory: a weight per split
+constexpr uint32_t kJoinThreads = 128;
+__global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const Kv4Attn a, const Shape sh) {
     pdl_enter4();
-    const uint32_t lane = threadIdx.x & 31u, rep = a.H / a.G, col = blockIdx.x * 8u + (threadIdx.x >> 5), g = blockIdx.y, b = blockIdx.z;
-    if (col >= a.T * rep) return;
-    const uint32_t t = col / rep, h = g * rep + col % rep;
+    extern __shared__ __align__(16) unsigned char sm[];
+    float *w_s = reinterpret_cast<float *>(sm);
+    __shared__ float4 part[kJoinThreads / 32][64];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, rep = a.H / a.G, col = blockIdx.x, g = blockIdx.y, b = blockIdx.z, t = col / rep, h = g * rep + col % rep;
     const uint64_t places = (uint64_t)a.B * a.G * sh.tiles * sh.nsplit * sh.cols, where = ((uint64_t)(b * a.G + g) * sh.tiles + col / sh.cols) * sh.nsplit * sh.cols + col % sh.cols;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + places * a.D);
+    // (every warp finds the row's maximum and sum for itself)
     float top = -INFINITY, sum = 0.0f;
     for (uint32_t s = lane; s < sh.nsplit; s += 32u) top = fmaxf(top, ml[where + (uint64_t)s * sh.cols].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float use = top == -INFINITY ? 0.0f : top;
+    for (uint32_t s = lane; s < sh.nsplit; s += 32u) {
+        const float2 p = ml[where + (uint64_t)s * sh.cols];
+        const float k = ex2(p.x - use);
+        sum = fmaf(p.y, k, sum);
+        if (warp == 0) w_s[s] = k;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
     for (uint32_t d0 = 0; d0 < a.D; d0 += 128u) {
         const uint32_t d = d0 + lane * 4u;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        sum = 0.0f;
-        for (uint32_t s = 0; s < sh.nsplit; s++) {
-            const float2 p = ml[where + (uint64_t)s * sh.cols];
-            const float k = ex2(p.x - use);
-            sum = fmaf(p.y, k, sum);
-            if (d < a.D) {
+        if (d < a.D)
+#pragma unroll 4
+            for (uint32_t s = warp; s < sh.nsplit; s += kJoinThreads / 32u) {
                 const float4 u = *reinterpret_cast<const float4 *>(a.part + (where + (uint64_t)s * sh.cols) * a.D + d);
+                const float k = w_s[s];
                 v.x = fmaf(u.x, k, v.x); v.y = fmaf(u.y, k, v.y); v.z = fmaf(u.z, k, v.z); v.w = fmaf(u.w, k, v.w);
             }
-        }
-        const float k = last_factor(a, t, h, top, sum);
-        if (d < a.D) store_four(a, b, t, h, d, v.x * k, v.y * k, v.z * k, v.w * k);
+        part[warp][d0 / 4u + lane] = v;
+    }
+    __syncthreads();
+    const float k = last_factor(a, t, h, top, sum);
+    for (uint32_t e = threadIdx.x; e < a.D / 4u; e += kJoinThreads) {
+        float4 v = part[0][e];
+#pragma unroll
+        for (uint32_t w = 1; w < kJoinThreads / 32u; w++) { const float4 u = part[w][e]; v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w; }
+        store_four(a, b, t, h, e * 4u, v.x * k, v.y * k, v.z * k, v.w * k);
     }
 }
 
@@ -554,8 +598,9 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 }
 
 // ---- which instance, and how the work is shared out ----
+static uint32_t env_waves() { const char *s = getenv("KV4W"); return s ? atoi(s) : 3; }
 struct Plan { int nt; bool rows; Shape sh; };
-constexpr uint32_t kWarps = 4, kBlocksPerSm = 3;
+constexpr uint32_t kWarps = 4, kBlocksPerSm = 12;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G), most = D > 128 ? 2u : 4u;
     Plan p{};
@@ -566,8 +611,8 @@ Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32
     // pages that a block can have in sight
     const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
     const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
-    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)kBlocksPerSm * sms;
-    const uint32_t least = p.rows ? 8u : 2u * kWarps;          // pages of a split
+    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)(B > 1 ? env_waves() : 1) * 4u * sms;
+    const uint32_t least = p.rows ? 8u : kWarps;          // pages of a split
     p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want / std::max<uint64_t>(1, blocks), std::max(1u, pages / least)));
     return p;
 }
@@ -625,7 +670,7 @@ cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream,
         default: e = attn_launch_nt<8>(a, p, stream, pdl); break;
     }
     if (e == cudaSuccess && p.sh.nsplit > 1)
-        e = launch_on(k_kv4_join, dim3((a.T * (a.H / a.G) + 7u) / 8u, a.G, a.B), 256, 0, stream, true, a, p.sh);
+        e = launch_on(k_kv4_join, dim3(a.T * (a.H / a.G), a.G, a.B), kJoinThreads, p.sh.nsplit * 4u, stream, true, a, p.sh);
     if (launches) *launches = p.sh.nsplit > 1 ? 2 : 1;
     return e;
 }
