@@ -133,18 +133,23 @@ bool rows_at16(const Kv4Rows &a) {
 
 // ------------------------------------------------------------------------------------------------
 // Attention.  A warp multiplies the keys of one page at a time (32, in two tiles of 16 rows) with NT tiles of 8 columns -- column c of key/value head g is
-// query token c / rep, head g rep + c % rep, rep = H / G -- on the matrix instructions: keys and values are the row operand, made in registers from the codes
-// (a code c next to the exponent of 1024 is the fp16 number 1024 + c; minus 1024 and one fp16 multiply-add with the group's pair gives c s + m rounded once), queries
-// and weights the column operand.  Softmax in one pass: per column the running maximum m, the sum l and the weighted values o in fp32; log2 units, weights
-// times 2^kLift so that fp16 keeps small ones.  Rounding to 11 bits: the keys and values (c s + m), the queries (times a power of two per row, so that any
-// magnitude fits) and the weights; each rounding is at most 2^-11 of its number, against the 2^-8 of a bf16 output and the cache's own 1/30 of a group's range.
+// query token c / rep, head g rep + c % rep, rep = H / G -- on the matrix instructions: keys and values are the row operand, made in registers from the codes,
+// queries and weights the column operand, sums in fp32.  A nibble in the lowest bits of an fp16 number is that number: c 2^-24 (or c 2^-20, four bits up), below the
+// smallest normal one and exact.  So:
+//   values   o_d += sum_t c_td (p_t s_t),  one instruction per pair of codes; the pairs' second halves are a product of their own, 16 rows of which the groups take the
+//            first: sum_t m_tg p_t.  c 2^-24 becomes c when o leaves.
+//   keys     NT = 1: the product of the bare codes over one group at a time, s and m times it in fp32 (8 multiply-adds to a group); with more columns that would
+//            cost more than the other way, c s + m in fp16 (1024 + c less 1024, then one fp16 multiply-add): 80 + 112 NT instructions for a page against 270
+// Softmax in one pass: per column a reference r, the sum l and the weighted values o of weights 2^(x - r), x the score in log2 units.  r need not be the maximum: it is
+// renewed when a weight would pass 2^cap, which keeps weights, and weights times s, inside fp16, small ones 2^kSlack below that; most pages leave r and o as they are.
+// Rounding to 11 bits: the queries (times a power of two per row, so that any magnitude fits), the weights, the weights times s, and keys where they are c s + m; each
+// rounding is at most 2^-11 of its number, against the 2^-8 of a bf16 output and the cache's own 1/30 of a group's range.
 // Each warp brings its own pages into its own ring of shared memory (cp.async, one group of copies to a page) and waits for nobody else until the end.
 // WK warps of a block share the columns and take every WK-th page (single tokens: the keys are what there is to share out); with WK = 1 each warp has columns of
 // its own.  The pages of a row are also split over nsplit blocks, whose parts k_kv4_join puts together.
 // Values that stand for NaN are taken out of the product (0 times NaN would reach columns that do not see them) and make the rows that do see them NaN.
 // ------------------------------------------------------------------------------------------------
-constexpr int kLift = 12;
-constexpr float kLag = 3.0f;
+constexpr float kSlack = 3.0f, kCap = 15.0f;          // with s < 2 no weight above 2^15
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -166,6 +171,7 @@ __device__ __forceinline__ uint32_t stand_for(uint32_t w, __half2 s, __half2 m) 
     const __half2 c = HIGH ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-64.0f)) : __hsub2(h, __float2half2_rn(1024.0f));
     return bits(__hfma2(c, s, m));
 }
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;          // the bare codes: c 2^-24 and c 2^-20
 // BYTES (a multiple of 2) bytes of shared memory in words
 template <int BYTES>
 __device__ __forceinline__ void take(const unsigned char *p, uint32_t (&w)[(BYTES + 3) / 4]) {
@@ -196,14 +202,14 @@ __device__ __forceinline__ int seq_len(const Kv4Attn &a, uint32_t b) {
     const long long n = a.lens ? a.lens[b] : (long long)a.pos0 + (a.pos_ptr ? *a.pos_ptr : 0u) + a.T;
     return (int)(n < 0 ? 0 : n < most ? n : most);
 }
-// what is left to do with a column's sums: the sink, the division, the gate.  m in log2 units, l and the values times 2^kLift; returns the values' factor
-__device__ __forceinline__ float last_factor(const Kv4Attn &a, uint32_t t, uint32_t h, float m, float l) {
+// what is left to do with a column's sums: the sink, the division, the gate.  l and the values are in units of 2^r; returns the values' factor
+__device__ __forceinline__ float last_factor(const Kv4Attn &a, uint32_t t, uint32_t h, float r, float l) {
     if (l == 0.0f) return 0.0f;          // no key in sight (a NaN is no zero)
     float f = 1.0f;
     if (a.sink) {
-        const float s = a.sink[h] * kLog2e, top = fmaxf(m, s);
-        f = ex2(m - top);
-        l = fmaf(l, f, ex2(s - top + (float)kLift));
+        const float s = a.sink[h] * kLog2e, top = fmaxf(r, s);
+        f = ex2(r - top);
+        l = fmaf(l, f, ex2(s - top));
     }
     f /= l;
     if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[(uint64_t)t * a.ldg + h]));
@@ -222,8 +228,9 @@ struct Shape { uint32_t nsplit, tiles, cols; };          // splits of the keys, 
 constexpr int kStages = 2;
 template <int NG, int NT, int WK, int W>
 struct Room {
+    static constexpr bool after = NT == 1;          // keys are scaled after the product
     static constexpr uint32_t block = 1280u * NG, ring = W * kStages * block, merge = WK > 1 ? W * NT * 8u * (32u * NG + 2u) * 4u : 0u,
-                              q = (W / WK) * NT * NG * 512u, all = (ring > merge ? ring : merge) + q + (W / WK) * NT * 8u * 4u;
+                              q = (W / WK) * NT * NG * 512u, all = (ring > merge ? ring : merge) + q + (W / WK) * NT * 8u * 4u * (after ? 1u + NG : 1u);
 };
 
 // grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
     const uint32_t split = blockIdx.x % sh.nsplit, tile = blockIdx.x / sh.nsplit, g = blockIdx.y, b = blockIdx.z, rep = a.H / a.G, ncols = a.T * rep;
     unsigned char *ring = sm + warp * kStages * R::block;
     unsigned char *q_s = sm + (R::ring > R::merge ? R::ring : R::merge) + wr * NT * NG * 512u;
-    float *scale_s = reinterpret_cast<float *>(sm + (R::ring > R::merge ? R::ring : R::merge) + R::q) + wr * COLS;
+    float *scale_s = reinterpret_cast<float *>(sm + (R::ring > R::merge ? R::ring : R::merge) + R::q) + wr * COLS * (R::after ? 1u + NG : 1u), *sum_s = scale_s + COLS;          // sum_s (R::after): [column][group] sums of the rounded queries
     const uint32_t c0 = tile * sh.cols + wr * COLS;
     const int len = seq_len(a, b);
 
@@ -294,17 +301,26 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
         // coordinate 32 j + 8 b + i (lane = 8 b + i): step i / 2 % 2 of the group, register i % 2, half i / 4
         const uint32_t bq = lane >> 3, i = lane & 7u;
 #pragma unroll
-        for (int j = 0; j < NG; j++)
-            *reinterpret_cast<__half *>(q_s + (((c >> 3) * NG + j) * 2u + ((i >> 1) & 1u)) * 256u + ((c & 7u) * 4u + bq) * 8u + (i & 1u) * 4u + (i >> 2) * 2u) = __float2half_rn(x[j] * down);
-        if (lane == 0) scale_s[c] = a.scale * __uint_as_float((uint32_t)(127 + e) << 23) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+        for (int j = 0; j < NG; j++) {
+            // (codes at bits 4-7 count sixteen times as much where they are multiplied as they are)
+            const __half y = __float2half_rn(x[j] * down * (R::after && (i & 1u) ? 0.0625f : 1.0f));
+            *reinterpret_cast<__half *>(q_s + (((c >> 3) * NG + j) * 2u + ((i >> 1) & 1u)) * 256u + ((c & 7u) * 4u + bq) * 8u + (i & 1u) * 4u + (i >> 2) * 2u) = y;
+            if constexpr (R::after) {
+                float z = __half2float(y) * (i & 1u ? 16.0f : 1.0f);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+                if (lane == 0) sum_s[c * NG + j] = z * 0x1p-24f;
+            }
+        }
+        if (lane == 0) scale_s[c] = (R::after ? 0x1p24f : 1.0f) * a.scale * __uint_as_float((uint32_t)(127 + e) << 23) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
     }
     if constexpr (WK > 1) __syncthreads(); else __syncwarp();
 
 
-    float m[NT][2], l[NT][2], o[2 * NG][NT][4];
+    float r[NT][2], l[NT][2], o[2 * NG][NT][4], om[NT][4];          // om: row j is the part of the groups' second halves
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        m[t][0] = m[t][1] = -INFINITY; l[t][0] = l[t][1] = 0.0f;
+        r[t][0] = r[t][1] = -INFINITY; l[t][0] = l[t][1] = 0.0f; om[t][0] = om[t][1] = om[t][2] = om[t][3] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2 * NG; i++) { o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.0f; }
     }
@@ -322,6 +338,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
     if constexpr (NT == 1)
 #pragma unroll
         for (int j = 0; j < 2 * NG; j++) { const uint2 v = *reinterpret_cast<const uint2 *>(q_s + j * 256u + lane * 8u); qf[j][0] = v.x; qf[j][1] = v.y; }
+    float qsum[R::after ? NG : 1][2];
+    if constexpr (R::after)
+#pragma unroll
+        for (int j = 0; j < NG; j++) { qsum[j][0] = sum_s[(tq * 2u) * NG + j]; qsum[j][1] = sum_s[(tq * 2u + 1u) * NG + j]; }
+    const uint32_t gm = NG == 8 ? gq : gq % NG;          // the group whose second halves this lane's rows hold
+    float cap = kCap;
+    uint32_t most_s = 0x4000u;          // fp16 bits of the smallest s that cap has no room for
     const uint32_t row = (gq & 1u) * 4u + (gq >> 1);          // row r of eight is token 4 (r % 2) + r / 2 of eight: the transposed weights then pair tokens i and i + 4
     for (uint32_t i = 0; i < count; i++) {
         copy_wait<kStages - 2>();
@@ -332,20 +355,33 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
         unsigned char *pg = ring + stage * R::block;
         const int key0 = (int)((p0 + wk + i * WK) * kKv4Page);
 
-        // values that are no number
+        const bool whole = pos_a >= key0 + (int)kKv4Page - 1 && low_b <= key0;
+        // the values' pairs, one token to a lane: steps that the weights have no room for, pairs that are no numbers (behind a sequence's end lies anything)
         uint32_t bad = 0;
         {
             uint32_t w[NG];
             take<4 * NG>(pg + 1152u * NG + lane * 4u * NG, w);
-            __half2 zero = __float2half2_rn(0.0f);          // 0 times a pair is 0, or NaN
+            __half2 top = half2_of(w[0]);
 #pragma unroll
-            for (int j = 0; j < NG; j++) zero = __hfma2(half2_of(w[j]), __float2half2_rn(0.0f), zero);
-            const bool odd = !__hbeq2(zero, __float2half2_rn(0.0f));
-            bad = __ballot_sync(0xffffffffu, odd);
-            if (bad) {
+            for (int j = 1; j < NG; j++) top = __hmax2_nan(top, half2_of(w[j]));
+            if (__any_sync(0xffffffffu, !whole || (bits(top) & 0xffffu) >= most_s)) {
+                __half2 zero = __float2half2_rn(0.0f);          // 0 times a pair is 0, or NaN
+                float big = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NG; j++) { zero = __hfma2(half2_of(w[j]), __float2half2_rn(0.0f), zero); big = fmaxf(big, fabsf(__low2float(half2_of(w[j])))); }
+                const bool odd = !__hbeq2(zero, __float2half2_rn(0.0f));
+                bad = __ballot_sync(0xffffffffu, odd);
                 if (odd)
 #pragma unroll
                     for (int j = 0; j < NG; j++) reinterpret_cast<uint32_t *>(pg + 1152u * NG + lane * 4u * NG)[j] = 0u;
+                big = odd ? 0.0f : big;
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+                if (big >= 2.0f) {
+                    const int e = (int)(__float_as_uint(big) >> 23) - 127;
+                    cap = fminf(cap, kCap - (float)e);
+                    most_s = max(most_s, (uint32_t)(e + 16) << 10);
+                }
                 __syncwarp();
             }
         }
@@ -362,14 +398,22 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
             take<4 * NG>(pg + 512u * NG + ra * 4u * NG, sa); take<4 * NG>(pg + 512u * NG + rb * 4u * NG, sb);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
+                if constexpr (R::after) {
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const float2 pa = __half22float2(half2_of(sa[j])), pb = __half22float2(half2_of(sb[j]));
+                    mma(c, wa[j] & kLow, wb[j] & kLow, wa[j] & kHigh, wb[j] & kHigh, qf[2 * j][0], qf[2 * j][1]);
+                    mma(c, (wa[j] >> 8) & kLow, (wb[j] >> 8) & kLow, (wa[j] >> 8) & kHigh, (wb[j] >> 8) & kHigh, qf[2 * j + 1][0], qf[2 * j + 1][1]);
+                    s[k][0][0] = fmaf(pa.x, c[0], fmaf(pa.y, qsum[j][0], s[k][0][0])); s[k][0][1] = fmaf(pa.x, c[1], fmaf(pa.y, qsum[j][1], s[k][0][1]));
+                    s[k][0][2] = fmaf(pb.x, c[2], fmaf(pb.y, qsum[j][0], s[k][0][2])); s[k][0][3] = fmaf(pb.x, c[3], fmaf(pb.y, qsum[j][1], s[k][0][3]));
+                    continue;
+                }
                 const __half2 s_a = __low2half2(half2_of(sa[j])), m_a = __high2half2(half2_of(sa[j])), s_b = __low2half2(half2_of(sb[j])), m_b = __high2half2(half2_of(sb[j]));
                 const uint32_t x0 = stand_for<false>(wa[j], s_a, m_a), x1 = stand_for<true>(wa[j], s_a, m_a), x2 = stand_for<false>(wa[j] >> 8, s_a, m_a), x3 = stand_for<true>(wa[j] >> 8, s_a, m_a);
                 const uint32_t y0 = stand_for<false>(wb[j], s_b, m_b), y1 = stand_for<true>(wb[j], s_b, m_b), y2 = stand_for<false>(wb[j] >> 8, s_b, m_b), y3 = stand_for<true>(wb[j] >> 8, s_b, m_b);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     uint2 u, v;
-                    if constexpr (NT == 1) { u = make_uint2(qf[2 * j][0], qf[2 * j][1]); v = make_uint2(qf[2 * j + 1][0], qf[2 * j + 1][1]); }
-                    else { u = *reinterpret_cast<const uint2 *>(q_s + ((t * NG + j) * 2u) * 256u + lane * 8u); v = *reinterpret_cast<const uint2 *>(q_s + ((t * NG + j) * 2u + 1u) * 256u + lane * 8u); }
+                    { u = *reinterpret_cast<const uint2 *>(q_s + ((t * NG + j) * 2u) * 256u + lane * 8u); v = *reinterpret_cast<const uint2 *>(q_s + ((t * NG + j) * 2u + 1u) * 256u + lane * 8u); }
                     mma(s[k][t], x0, y0, x1, y1, u.x, u.y);
                     mma(s[k][t], x2, y2, x3, y3, v.x, v.y);
                 }
@@ -377,7 +421,6 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
         }
 
         // weights, as the column operand of the second product
-        const bool whole = pos_a >= key0 + (int)kKv4Page - 1 && low_b <= key0;
         uint32_t pw[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -396,40 +439,40 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
             if (!whole) {
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const int low = first_seen(max(pos[t][x], 0), a.window, a.block) - key0 - (int)row, high = pos[t][x] - key0 - (int)row;          // of the rows 16 k + 8 r
+                    const int low = first_seen(max(pos[t][x], 0), a.window, a.block) - key0 - (int)row, high = pos[t][x] - key0 - (int)row;          // of the rows 16 k + 8 y
 #pragma unroll
                     for (int k = 0; k < 2; k++)
 #pragma unroll
-                        for (int r = 0; r < 2; r++) if (k * 16 + r * 8 > high || k * 16 + r * 8 < low) s[k][t][2 * r + x] = -INFINITY;
+                        for (int y = 0; y < 2; y++) if (k * 16 + y * 8 > high || k * 16 + y * 8 < low) s[k][t][2 * y + x] = -INFINITY;
                 }
             }
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) top[x & 1] = fmaxf(top[x & 1], s[k][t][x]);
-            // the maximum in use may lag behind by kLag (the weights then reach 2^(kLift + kLag)): most pages leave it, and the values, as they are
-            if (__any_sync(0xffffffffu, top[0] > m[t][0] + kLag || top[1] > m[t][1] + kLag)) {
+            if (__any_sync(0xffffffffu, top[0] > r[t][0] + cap || top[1] > r[t][1] + cap)) {
                 float corr[2];
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    top[x] = fmaxf(top[x], m[t][x]);
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], off));
-                    corr[x] = ex2(m[t][x] - (top[x] == -INFINITY ? 0.0f : top[x]));
-                    m[t][x] = top[x];
+                    const float next = fmaxf(top[x] - (cap - kSlack), r[t][x]);
+                    corr[x] = next == -INFINITY ? 1.0f : ex2(r[t][x] - next);
+                    r[t][x] = next;
                     l[t][x] *= corr[x];
                 }
 #pragma unroll
                 for (int d = 0; d < 2 * NG; d++) { o[d][t][0] *= corr[0]; o[d][t][1] *= corr[1]; o[d][t][2] *= corr[0]; o[d][t][3] *= corr[1]; }
+                om[t][0] *= corr[0]; om[t][1] *= corr[1];
             }
-            const float use[2] = {m[t][0] == -INFINITY ? 0.0f : m[t][0] - (float)kLift, m[t][1] == -INFINITY ? 0.0f : m[t][1] - (float)kLift};
+            const float use[2] = {r[t][0] == -INFINITY ? 0.0f : r[t][0], r[t][1] == -INFINITY ? 0.0f : r[t][1]};
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const float u = ex2(s[k][t][2 * r] - use[0]), v = ex2(s[k][t][2 * r + 1] - use[1]);
+                for (int y = 0; y < 2; y++) {
+                    const float u = ex2(s[k][t][2 * y] - use[0]), v = ex2(s[k][t][2 * y + 1] - use[1]);
                     l[t][0] += u; l[t][1] += v;
-                    pw[t][2 * k + r] = transpose8(bits(__floats2half2_rn(u, v)));
+                    pw[t][2 * k + y] = transpose8(bits(__floats2half2_rn(u, v)));
                 }
         }
 
@@ -447,25 +490,27 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
         // weighted values: depth step k takes tokens 16 k + tq + {0, 4, 8, 12}; rows are coordinates 32 j + 4 gq + {0 .. 3}
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            uint32_t w[4][(NG + 1) / 2], sp[4][NG];
+            uint32_t w[4][(NG + 1) / 2], sp[4][NG], mw[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                const uint32_t r = k * 16u + tq + 4u * x;
-                take<2 * NG>(pg + 640u * NG + r * 16u * NG + gq * 2u * NG, w[x]);
-                take<4 * NG>(pg + 1152u * NG + r * 4u * NG, sp[x]);
+                const uint32_t at = k * 16u + tq + 4u * x;
+                take<2 * NG>(pg + 640u * NG + at * 16u * NG + gq * 2u * NG, w[x]);
+                take<4 * NG>(pg + 1152u * NG + at * 4u * NG, sp[x]);
+                mw[x] = *reinterpret_cast<const uint32_t *>(pg + 1152u * NG + at * 4u * NG + gm * 4u);
             }
+            const uint32_t m_ab = __byte_perm(mw[0], mw[1], 0x7632u), m_cd = __byte_perm(mw[2], mw[3], 0x7632u);
+#pragma unroll
+            for (int t = 0; t < NT; t++) mma(om[t], m_ab, 0u, m_cd, 0u, pw[t][2 * k], pw[t][2 * k + 1]);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
                 const uint32_t ab = __byte_perm(w[0][j / 2], w[1][j / 2], sel), cd = __byte_perm(w[2][j / 2], w[3][j / 2], sel);
-                const __half2 s_ab = half2_of(__byte_perm(sp[0][j], sp[1][j], 0x5410u)), m_ab = half2_of(__byte_perm(sp[0][j], sp[1][j], 0x7632u));
-                const __half2 s_cd = half2_of(__byte_perm(sp[2][j], sp[3][j], 0x5410u)), m_cd = half2_of(__byte_perm(sp[2][j], sp[3][j], 0x7632u));
-                const uint32_t x0 = stand_for<false>(ab, s_ab, m_ab), x1 = stand_for<true>(ab, s_ab, m_ab), x2 = stand_for<false>(ab >> 8, s_ab, m_ab), x3 = stand_for<true>(ab >> 8, s_ab, m_ab);
-                const uint32_t y0 = stand_for<false>(cd, s_cd, m_cd), y1 = stand_for<true>(cd, s_cd, m_cd), y2 = stand_for<false>(cd >> 8, s_cd, m_cd), y3 = stand_for<true>(cd >> 8, s_cd, m_cd);
+                const __half2 s_ab = half2_of(__byte_perm(sp[0][j], sp[1][j], 0x5410u)), s_cd = half2_of(__byte_perm(sp[2][j], sp[3][j], 0x5410u));
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    mma(o[2 * j][t], x0, x1, y0, y1, pw[t][2 * k], pw[t][2 * k + 1]);
-                    mma(o[2 * j + 1][t], x2, x3, y2, y3, pw[t][2 * k], pw[t][2 * k + 1]);
+                    const uint32_t u = bits(__hmul2(half2_of(pw[t][2 * k]), s_ab)), v = bits(__hmul2(half2_of(pw[t][2 * k + 1]), s_cd));
+                    mma(o[2 * j][t], ab & kLow, ab & kHigh, cd & kLow, cd & kHigh, u, v);
+                    mma(o[2 * j + 1][t], (ab >> 8) & kLow, (ab >> 8) & kHigh, (cd >> 8) & kLow, (cd >> 8) & kHigh, u, v);
                 }
             }
         }
@@ -478,6 +523,11 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], off);
 
+    // coordinates 32 j + 4 gq + {0, 1, 2, 3} of column x
+    auto four = [&](int t, int x, int j, float k) {
+        const float mj = __shfl_sync(0xffffffffu, om[t][x], (j << 2) | tq);
+        return make_float4(fmaf(o[2 * j][t][x], 0x1p24f, mj) * k, fmaf(o[2 * j][t][2 + x], 0x1p20f, mj) * k, fmaf(o[2 * j + 1][t][x], 0x1p24f, mj) * k, fmaf(o[2 * j + 1][t][2 + x], 0x1p20f, mj) * k);
+    };
     const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols, places = (uint64_t)a.B * a.G * sh.tiles * sh.nsplit * sh.cols;
     float2 *ml = reinterpret_cast<float2 *>(a.part + places * D);
     if constexpr (WK > 1) {
@@ -490,8 +540,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
                 const uint32_t c = warp * COLS + t * 8u + tq * 2u + x;
 #pragma unroll
                 for (int j = 0; j < NG; j++)
-                    *reinterpret_cast<float4 *>(mo + c * D + j * 32u + gq * 4u) = make_float4(o[2 * j][t][x], o[2 * j][t][2 + x], o[2 * j + 1][t][x], o[2 * j + 1][t][2 + x]);
-                if (gq == 0) { mm[2 * c] = m[t][x]; mm[2 * c + 1] = l[t][x]; }
+                    *reinterpret_cast<float4 *>(mo + c * D + j * 32u + gq * 4u) = four(t, x, j, 1.0f);
+                if (gq == 0) { mm[2 * c] = r[t][x]; mm[2 * c + 1] = l[t][x]; }
             }
         __syncthreads();
         for (uint32_t e = tid; e < COLS * D / 4u; e += W * 32u) {
@@ -525,16 +575,17 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 const uint32_t c = wr * COLS + t * 8u + tq * 2u + x, col = tile * sh.cols + c;
-                if (col >= ncols) continue;
+                const bool mine = col < ncols;
                 const uint32_t tt = col / rep, h = g * rep + col % rep;
-                const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, tt, h, m[t][x], l[t][x]);
+                const float k = !mine || sh.nsplit > 1 ? 1.0f : last_factor(a, tt, h, r[t][x], l[t][x]);
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
-                    const float v0 = o[2 * j][t][x] * k, v1 = o[2 * j][t][2 + x] * k, v2 = o[2 * j + 1][t][x] * k, v3 = o[2 * j + 1][t][2 + x] * k;
-                    if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + (where + c) * D + j * 32u + gq * 4u) = make_float4(v0, v1, v2, v3);
-                    else store_four(a, b, tt, h, j * 32u + gq * 4u, v0, v1, v2, v3);
+                    const float4 v = four(t, x, j, k);
+                    if (!mine) continue;
+                    if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + (where + c) * D + j * 32u + gq * 4u) = v;
+                    else store_four(a, b, tt, h, j * 32u + gq * 4u, v.x, v.y, v.z, v.w);
                 }
-                if (sh.nsplit > 1 && gq == 0) ml[where + c] = make_float2(m[t][x], l[t][x]);
+                if (mine && sh.nsplit > 1 && gq == 0) ml[where + c] = make_float2(r[t][x], l[t][x]);
             }
     }
 }
