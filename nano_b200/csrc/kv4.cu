@@ -235,7 +235,7 @@ struct Room {
 
 // grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
 template <int NG, int NT, int WK, int W>
-__global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1) k_kv4_attn(const Kv4Attn a, const Shape sh) {
+__global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1 /*B*/) k_kv4_attn(const Kv4Attn a, const Shape sh) {
     pdl_enter4();
     using R = Room<NG, NT, WK, W>;
     constexpr uint32_t D = 32u * NG, COLS = NT * 8u;
@@ -651,7 +651,7 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 // ---- which instance, and how the work is shared out ----
 static uint32_t env_waves() { const char *s = getenv("KV4W"); return s ? atoi(s) : 3; }
 struct Plan { int nt; bool rows; Shape sh; };
-constexpr uint32_t kWarps = 4, kBlocksPerSm = 12;
+constexpr uint32_t kWarps = 4, kBlocksPerSm = 15, kRes = 4;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G), most = D > 128 ? 2u : 4u;
     Plan p{};
@@ -662,7 +662,7 @@ Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32
     // pages that a block can have in sight
     const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
     const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
-    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)(B > 1 ? env_waves() : 1) * 4u * sms;
+    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)(B > 1 ? env_waves() : 1) * kRes * sms;
     const uint32_t least = p.rows ? 8u : kWarps;          // pages of a split
     p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want / std::max<uint64_t>(1, blocks), std::max(1u, pages / least)));
     return p;

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <float.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 #include <vector>
@@ -17,15 +18,17 @@ namespace {
 // ------------------------------------------------------------------------------------------------
 // Log probabilities.  For a row x of V logits with maximum M, Z = sum exp(x_i - M):
 //     log p_t = (x_t - M) - log Z,    H = log Z + (1/Z) sum exp(x_i - M) (M - x_i),    alternatives in the order (x descending, index ascending).
-// One pass: every thread keeps (m, z, s) of what it has seen -- z = sum exp(x - m), s = sum exp(x - m) (x - m) -- and rescales them when m grows; two such
-// triples join as  z = z1 f1 + z2 f2,  s = f1 (s1 + z1 (m1 - m)) + f2 (...),  f = exp(m_i - m).  Sums are fp32.
-// The alternatives ride on the same pass: each warp keeps its 32 best in registers (lane i the i-th), as 64-bit keys (ordered bits of x, complement of the index),
-// and looks at a vector of logits one by one only when its largest reaches the k-th best that any warp of the block has.
+// One pass over the row, bound by its bytes: every thread keeps m, z = sum exp(x - m) and s = sum exp(x - m) (x - m) of what it has seen, in log2 units and on
+// pairs of numbers (fma.f32x2: some five instructions to a number, where eleven are what bf16 rows at the full rate of HBM leave), and rescales them when m grows.  Two
+// such triples join as  z = z1 f1 + z2 f2,  s = f1 (s1 + z1 (m1 - m)) + f2 (...),  f = exp(m_i - m).  Sums are fp32.
+// Alternatives: the k-th largest of the threads' maxima is a floor below which no alternative of the block lies, and only threads whose maximum reaches it have any: about
+// k of them, whose vectors are read once more and looked at one by one (a warp keeps its 32 best in registers, lane i the i-th, as 64-bit keys: ordered bits of x,
+// complement of the index).  Lists kept during the pass instead cost 3 to 5 times the pass.
 // A row belongs to a cluster of C blocks, whose parts are joined over distributed shared memory: one launch, no workspace, no order of arrival in the result.
 // -inf (a masked token) adds nothing; a row of nothing else has log probabilities -inf and entropy 0; NaN or +inf anywhere makes a row's numbers NaN (its order
 // of alternatives counts NaN as -inf).
 // ------------------------------------------------------------------------------------------------
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpMaxCluster = 16;
+constexpr int kLpMaxCluster = 16;
 constexpr int kLpUnroll = 4;          // 16-byte vectors in flight per thread
 
 template <typename T> struct Elem;
@@ -124,6 +127,64 @@ __device__ __forceinline__ Sums shfl(const Sums &a, int step) {
     return Sums{__shfl_xor_sync(0xffffffffu, a.m, step), __shfl_xor_sync(0xffffffffu, a.z, step), __shfl_xor_sync(0xffffffffu, a.s, step)};
 }
 
+// two fp32 numbers at once
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t pair(float a, float b) { pair_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void unpair(pair_t p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) { pair_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) { pair_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// What a thread has seen: m, and z, s in units of 2^u, u = m log2 e as it was rounded while m is small (d = x log2 e - u is then one multiply-add), and exact where m is
+// not (m - x first: nothing overflows, and the rounding of a large product does not count)
+constexpr float kSmallLogit = 4096.0f;
+struct Running {
+    float m = -FLT_MAX; pair_t z = 0, s = 0;          // (z and s: partial sums of the even and of the odd places)
+    static __device__ __forceinline__ float off(float m) { return fabsf(m) < kSmallLogit ? fmaf(m, kLog2e, -__fmul_rn(m, kLog2e)) : 0.0f; }          // m log2 e - u
+    __device__ __forceinline__ void rescale(float next, float d) {          // d: the old u less the new one
+        const float f = ex2(d);
+        const pair_t ff = pair(f, f), none = pair(0.0f, 0.0f);
+        s = f > 0.0f ? fma2(fma2(z, pair(d, d), s), ff, none) : none;
+        z = fma2(z, ff, none);
+        m = next;
+    }
+    template <int N> __device__ __forceinline__ void see(const float (&x)[N]) {
+        float top = x[0], low = x[0];
+#pragma unroll
+        for (int i = 1; i < N; i++) { top = fmaxf(top, x[i]); low = fminf(low, x[i]); }
+        if (low > -1e37f && fabsf(fmaxf(top, m)) < kSmallLogit) {          // (NaN is no obstacle: it makes z NaN)
+            if (top > m) rescale(top, __fsub_rn(__fmul_rn(fmaxf(m, -1e37f), kLog2e), __fmul_rn(top, kLog2e)));
+            const float c = __fmul_rn(m, kLog2e);
+            const pair_t L = pair(kLog2e, kLog2e), cc = pair(-c, -c);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const pair_t d = fma2(pair(x[i], x[i + 1]), L, cc);
+                float a, b;
+                unpair(d, a, b);
+                const pair_t p = pair(ex2(a), ex2(b));
+                z = add2(z, p);
+                s = fma2(p, d, s);
+            }
+        } else {          // masked and outsize logits; what weighs nothing is left out of s (0 times -inf)
+            if (top > m) rescale(top, (m - top) * kLog2e - off(m) + off(top));
+            float za, zb, sa, sb;
+            unpair(z, za, zb); unpair(s, sa, sb);
+            const float o = off(m);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float d = fmaf(x[i] - m, kLog2e, o), p = ex2(d);
+                if (i & 1) { zb += p; sb = fmaf(p, fmaxf(d, -1e4f), sb); } else { za += p; sa = fmaf(p, fmaxf(d, -1e4f), sa); }
+            }
+            z = pair(za, zb); s = pair(sa, sb);
+        }
+    }
+    __device__ __forceinline__ Sums done() const {
+        float za, zb, sa, sb;
+        unpair(z, za, zb); unpair(s, sa, sb);
+        const float o = off(m), f = ex2(-o), zz = za + zb;
+        return Sums{m, zz * f, fmaf(-o, zz, sa + sb) * f * 0.69314718055994531f};
+    }
+};
+
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
 template <typename W>
@@ -136,16 +197,57 @@ __device__ __forceinline__ W peer_word(const W *mine, uint32_t rank) {          
     return v;
 }
 
+// a 16-byte vector of a row as numbers; places outside the row (or past v1) hold -inf.  Whole vectors have been loaded into raw already
+template <typename T>
+__device__ __forceinline__ bool whole_vector(uint32_t v, uint32_t v1, uint32_t nv, uint32_t head, uint32_t vocab) {
+    return v < v1 && (v > 0 || head == 0) && (v + 1u < nv || (head + vocab) % Elem<T>::N == 0);
+}
+template <typename T>
+__device__ __forceinline__ void edge_vector(const T *row, uint32_t v, uint32_t v1, uint32_t head, uint32_t vocab, float *x) {
+    if (v >= v1) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::N; e++) x[e] = -INFINITY;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < Elem<T>::N; e++) {
+        const uint32_t i = v * Elem<T>::N + e - head;          // wraps below the row's start
+        x[e] = i < vocab ? Elem<T>::one(row + i) : -INFINITY;
+    }
+}
+
+// 32 lanes' numbers into descending order, and the 32 largest of two such lists
+__device__ __forceinline__ float sort32(float v) {
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (uint32_t size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (uint32_t step = size >> 1; step > 0; step >>= 1) {
+            const float o = __shfl_xor_sync(0xffffffffu, v, step);
+            v = ((lane & size) == 0) == ((lane & step) == 0) ? fmaxf(v, o) : fminf(v, o);
+        }
+    return v;
+}
+__device__ __forceinline__ float merge32(float a, float b) {
+    const uint32_t lane = threadIdx.x & 31u;
+    float v = fmaxf(a, __shfl_xor_sync(0xffffffffu, b, 31u));
+#pragma unroll
+    for (uint32_t step = 16; step > 0; step >>= 1) {
+        const float o = __shfl_xor_sync(0xffffffffu, v, step);
+        v = (lane & step) == 0 ? fmaxf(v, o) : fminf(v, o);
+    }
+    return v;
+}
+
 // grid (C, rows), clusters of C blocks
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 2) k_logprobs(const LogprobArgs a, const uint32_t C) {
-    constexpr int N = Elem<T>::N;
-    __shared__ unsigned long long lists[kLpWarps][32];
-    __shared__ float red[3][kLpWarps], part[3];
-    __shared__ float floor_s;          // no alternative lies below it: the largest k-th best of the block's warps
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const LogprobArgs a, const uint32_t C) {
+    constexpr int N = Elem<T>::N, WARPS = THREADS / 32;
+    __shared__ unsigned long long lists[WARPS > kLpMaxCluster ? WARPS : kLpMaxCluster][32];
+    __shared__ float tops[WARPS][32], red[3][WARPS], part[3];
+    __shared__ uint32_t flagged[THREADS], flags;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = C > 1 ? cluster_rank() : 0u;
     const T *row = static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.row_stride;
-    if (TOP) { if (tid == 0) floor_s = -INFINITY; __syncthreads(); }
 
     long long token = -1;
     float xt = NAN;
@@ -158,96 +260,87 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_logprobs(const LogprobArgs a,
     const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T)), nv = (head + a.vocab + N - 1u) / N, each = (nv + C - 1u) / C;
     const uint32_t v0 = min(nv, rank * each), v1 = min(nv, v0 + each);
     const uint4 *vecs = reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15u);
-    Sums t{-FLT_MAX, 0.0f, 0.0f};
-    TopList best;
-    best.top = a.top;
-    // (every warp walks as many steps as its first lane has vectors: the list is a warp's work)
-    for (uint32_t vb = v0 + warp * 32u; vb < v1; vb += kLpThreads * kLpUnroll) {
+    Running run;
+    for (uint32_t vb = v0 + tid; vb < v1; vb += THREADS * kLpUnroll) {
         uint4 raw[kLpUnroll] = {};
-        float x[kLpUnroll][N], vm[kLpUnroll];
 #pragma unroll
-        for (int j = 0; j < kLpUnroll; j++) {          // all loads of the step are in flight at once; the row's first and last vector are read by the element
-            const uint32_t v = vb + j * kLpThreads + lane;
-            if (v > 0 && v + 1u < nv && v < v1) raw[j] = __ldg(vecs + v);
-        }
+        for (int j = 0; j < kLpUnroll; j++) if (whole_vector<T>(vb + j * THREADS, v1, nv, head, a.vocab)) raw[j] = __ldg(vecs + vb + j * THREADS);          // all in flight at once
+        float x[kLpUnroll * N];
 #pragma unroll
         for (int j = 0; j < kLpUnroll; j++) {
-            const uint32_t v = vb + j * kLpThreads + lane;
-            Elem<T>::widen(raw[j], x[j]);
-            if (!(v > 0 && v + 1u < nv && v < v1)) {
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const uint32_t i = v * N + e - head;          // wraps below the row's start
-                    x[j][e] = v < v1 && i < a.vocab ? Elem<T>::one(row + i) : -INFINITY;
-                }
-            }
+            if (whole_vector<T>(vb + j * THREADS, v1, nv, head, a.vocab)) Elem<T>::widen(raw[j], x + j * N);
+            else edge_vector<T>(row, vb + j * THREADS, v1, head, a.vocab, x + j * N);
         }
-        float bm = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kLpUnroll; j++) {
-            vm[j] = x[j][0];
-#pragma unroll
-            for (int e = 1; e < N; e++) vm[j] = fmaxf(vm[j], x[j][e]);
-            bm = fmaxf(bm, vm[j]);
-        }
-        if (bm > t.m) {
-            const float d = t.m - bm, f = ex2(d * kLog2e);
-            t.s = f > 0.0f ? f * fmaf(t.z, d, t.s) : 0.0f; t.z *= f; t.m = bm;
-        }
-#pragma unroll
-        for (int j = 0; j < kLpUnroll; j++)
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float d = x[j][e] - t.m, p = ex2(d * kLog2e);
-                t.z += p;
-                t.s = fmaf(p, fmaxf(d, -1e4f), t.s);          // (p is 0 below -104; -inf would make 0 * -inf of it)
-            }
-        if constexpr (TOP) {
-            const float low = *(volatile float *)&floor_s;
-#pragma unroll
-            for (int j = 0; j < kLpUnroll; j++) {
-                if (!__any_sync(0xffffffffu, !(vm[j] < low))) continue;
-                const uint32_t first = (vb + j * kLpThreads + lane) * N - head;
-                const bool mine = vb + j * kLpThreads + lane < v1;
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const bool in = mine && first + e < a.vocab && !(x[j][e] < low);
-                    if (__any_sync(0xffffffffu, in)) best.take(in ? top_key(x[j][e], first + e) : 0ull);
-                }
-                if (best.kth && lane == 0) {          // (racing warps may leave the smaller of two floors, which is one too)
-                    const float f = key_value(best.kth);
-                    if (f > *(volatile float *)&floor_s) *(volatile float *)&floor_s = f;
-                }
-            }
-        }
+        run.see(x);
     }
+    Sums t = run.done();
+    [[maybe_unused]] const float mine = t.z == 0.0f ? -INFINITY : t.m;          // this thread's largest logit
 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = join(t, shfl(t, o));
     if (lane == 0) { red[0][warp] = t.m; red[1][warp] = t.z; red[2][warp] = t.s; }
-    if (TOP) lists[warp][lane] = best.list;
+    if constexpr (TOP) { tops[warp][lane] = sort32(mine); if (tid == 0) flags = 0; }
     __syncthreads();
+    bool nan = false;
     if constexpr (TOP) {
 #pragma unroll
-        for (uint32_t half = kLpWarps / 2; half > 0; half >>= 1) {
+        for (uint32_t half = WARPS / 2; half > 0; half >>= 1) {
+            if (warp < half) tops[warp][lane] = merge32(tops[warp][lane], tops[warp + half][lane]);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) nan = nan || red[1][w] != red[1][w];
+        const float low = nan ? -INFINITY : tops[0][a.top - 1u];
+        // the threads that have alternatives, their vectors dealt out one to a lane
+        const uint32_t own = min(v1, v0 + THREADS) - v0;          // threads that have a vector
+        const bool flag = tid < own && (nan || !(mine < low));
+        const uint32_t votes = __ballot_sync(0xffffffffu, flag);
+        uint32_t at = 0;
+        if (lane == 0 && votes) at = atomicAdd(&flags, __popc(votes));
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (flag) flagged[at + __popc(votes & ((1u << lane) - 1u))] = tid;
+        __syncthreads();
+        TopList best;
+        best.top = a.top;
+        const uint32_t per = (v1 - v0 + THREADS - 1u) / THREADS, total = flags * per;          // (at most all vectors, rounded up: below 2^32)
+        for (uint32_t q0 = warp * 32u; q0 < total; q0 += THREADS) {
+            const uint32_t q = q0 + lane, v = q < total ? v0 + flagged[q / per] + (q % per) * THREADS : v1;
+            float x[N];
+            if (whole_vector<T>(v, v1, nv, head, a.vocab)) Elem<T>::widen(__ldg(vecs + v), x);
+            else edge_vector<T>(row, v, v1, head, a.vocab, x);
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
+            if (!__any_sync(0xffffffffu, v < v1 && !(top < low))) continue;
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const bool in = v < v1 && v * N + e - head < a.vocab && !(x[e] < low);
+                if (__any_sync(0xffffffffu, in)) best.take(in ? top_key(x[e], v * N + e - head) : 0ull);
+            }
+        }
+        lists[warp][lane] = best.list;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t half = WARPS / 2; half > 0; half >>= 1) {
             if (warp < half) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + half][lane]);
             __syncthreads();
         }
     }
     if (warp == 0) {
-        t = Sums{lane < kLpWarps ? red[0][lane] : -FLT_MAX, lane < kLpWarps ? red[1][lane] : 0.0f, lane < kLpWarps ? red[2][lane] : 0.0f};
+        t = Sums{lane < WARPS ? red[0][lane] : -FLT_MAX, lane < WARPS ? red[1][lane] : 0.0f, lane < WARPS ? red[2][lane] : 0.0f};
 #pragma unroll
-        for (int o = kLpWarps / 2; o > 0; o >>= 1) t = join(t, shfl(t, o));
+        for (int o = WARPS / 2; o > 0; o >>= 1) t = join(t, shfl(t, o));
         if (lane == 0) { part[0] = t.m; part[1] = t.z; part[2] = t.s; }
     }
     if (C > 1) {
         cluster_sync();
         if (rank == 0) {
-            if (TOP && warp < C && warp > 0) {          // (the block's own list stays where it is)
-                const unsigned long long k = peer_word(&lists[0][lane], warp);
-                __syncwarp();
-                lists[warp][lane] = k;
-            }
+            if constexpr (TOP)
+                for (uint32_t peer = warp ? warp : WARPS; peer < C; peer += WARPS) {          // (the block's own list stays where it is)
+                    const unsigned long long k = peer_word(&lists[0][lane], peer);
+                    __syncwarp();
+                    lists[peer][lane] = k;
+                }
             if (warp == 0) {
                 t = Sums{lane < C ? peer_word(&part[0], lane) : -FLT_MAX, lane < C ? peer_word(&part[1], lane) : 0.0f, lane < C ? peer_word(&part[2], lane) : 0.0f};
 #pragma unroll
@@ -279,14 +372,15 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_logprobs(const LogprobArgs a,
     }
 }
 
-template <typename T, bool TOP>
+static uint32_t env_(const char *n, uint32_t d) { const char *s = getenv(n); return s ? atoi(s) : d; }
+template <typename T, bool TOP, int THREADS>
 cudaError_t logprobs_launch_t(const LogprobArgs &a, cudaStream_t stream) {
     const uint32_t nv = (a.vocab + Elem<T>::N - 1u) / Elem<T>::N;
     // blocks to a row: as long as each thread keeps a vector of it and the device is not full of them
     uint32_t C = 1;
-    while (C < kLpMaxCluster && nv >= 2u * C * kLpThreads && (uint64_t)a.rows * C < 148u * 4u) C *= 2;
+    while (C < kLpMaxCluster && nv >= env_("LPV", 2) * C * THREADS && (uint64_t)a.rows * C < env_("LPB", 592)) C *= 2;
     if (C > 8) {          // more than eight blocks to a cluster are to be asked for, on every device that runs them
-        cudaError_t e = cudaFuncSetAttribute(k_logprobs<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaError_t e = cudaFuncSetAttribute(k_logprobs<T, TOP, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
     for (uint32_t r0 = 0; r0 < a.rows; r0 += 65535u) {          // (the grid's second dimension)
@@ -299,12 +393,12 @@ cudaError_t logprobs_launch_t(const LogprobArgs &a, cudaStream_t stream) {
         if (a.top_logprob) b.top_logprob += (uint64_t)r0 * a.top;
         if (a.top_id) b.top_id += (uint64_t)r0 * a.top;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(C, b.rows); cfg.blockDim = dim3(kLpThreads); cfg.stream = stream;
+        cfg.gridDim = dim3(C, b.rows); cfg.blockDim = dim3(THREADS); cfg.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr; cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_logprobs<T, TOP>, b, C);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_logprobs<T, TOP, THREADS>, b, C);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -348,11 +442,10 @@ cudaError_t pages_launch(const PagePool *pools, uint32_t n_pools, const uint32_t
 
 cudaError_t logprobs_launch(const LogprobArgs &a, cudaStream_t stream) {
     if (!a.rows) return cudaSuccess;
-    switch (a.type) {
-        case T_F32: return a.top ? logprobs_launch_t<float, true>(a, stream) : logprobs_launch_t<float, false>(a, stream);
-        case T_BF16: return a.top ? logprobs_launch_t<__nv_bfloat16, true>(a, stream) : logprobs_launch_t<__nv_bfloat16, false>(a, stream);
-        default: return a.top ? logprobs_launch_t<__half, true>(a, stream) : logprobs_launch_t<__half, false>(a, stream);
-    }
+#define LP(T) (env_("LPT", 256) == 256 ? (a.top ? logprobs_launch_t<T, true, 256>(a, stream) : logprobs_launch_t<T, false, 256>(a, stream)) \
+                                       : (a.top ? logprobs_launch_t<T, true, 512>(a, stream) : logprobs_launch_t<T, false, 512>(a, stream)))
+    return a.type == T_F32 ? LP(float) : a.type == T_BF16 ? LP(__nv_bfloat16) : LP(__half);
+#undef LP
 }
 
 cudaError_t pages_copy_launch(const PagePool *pools, uint32_t n_pools, const uint32_t *src, const uint32_t *dst, uint32_t n, cudaStream_t stream, uint32_t *launches) {
