@@ -4,7 +4,6 @@
 #include <cuda_runtime.h>
 #include <float.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include <algorithm>
 #include <vector>
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
     constexpr int N = Elem<T>::N, WARPS = THREADS / 32;
     __shared__ unsigned long long lists[WARPS > kLpMaxCluster ? WARPS : kLpMaxCluster][32];
     __shared__ float tops[WARPS][32], red[3][WARPS], part[3];
-    __shared__ uint32_t flagged[THREADS], flags;
+    __shared__ uint32_t flagged[THREADS], flags, found;          // found: numbers that reach the floor
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = C > 1 ? cluster_rank() : 0u;
     const T *row = static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.row_stride;
 
@@ -279,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = join(t, shfl(t, o));
     if (lane == 0) { red[0][warp] = t.m; red[1][warp] = t.z; red[2][warp] = t.s; }
-    if constexpr (TOP) { tops[warp][lane] = sort32(mine); if (tid == 0) flags = 0; }
+    if constexpr (TOP) { tops[warp][lane] = sort32(mine); if (tid == 0) flags = found = 0; }
     __syncthreads();
     bool nan = false;
     if constexpr (TOP) {
@@ -300,30 +299,76 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
         at = __shfl_sync(0xffffffffu, at, 0);
         if (flag) flagged[at + __popc(votes & ((1u << lane) - 1u))] = tid;
         __syncthreads();
-        TopList best;
-        best.top = a.top;
         const uint32_t per = (v1 - v0 + THREADS - 1u) / THREADS, total = flags * per;          // (at most all vectors, rounded up: below 2^32)
-        for (uint32_t q0 = warp * 32u; q0 < total; q0 += THREADS) {
-            const uint32_t q = q0 + lane, v = q < total ? v0 + flagged[q / per] + (q % per) * THREADS : v1;
-            float x[N];
+        auto fetch = [&](uint32_t q, float (&x)[N]) {
+            const uint32_t v = q < total ? v0 + flagged[q / per] + (q % per) * THREADS : v1;
             if (whole_vector<T>(v, v1, nv, head, a.vocab)) Elem<T>::widen(__ldg(vecs + v), x);
             else edge_vector<T>(row, v, v1, head, a.vocab, x);
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
-            if (!__any_sync(0xffffffffu, v < v1 && !(top < low))) continue;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const bool in = v < v1 && v * N + e - head < a.vocab && !(x[e] < low);
-                if (__any_sync(0xffffffffu, in)) best.take(in ? top_key(x[e], v * N + e - head) : 0ull);
-            }
-        }
-        lists[warp][lane] = best.list;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t half = WARPS / 2; half > 0; half >>= 1) {
-            if (warp < half) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + half][lane]);
+            return v;
+        };
+        bool few = flags <= THREADS / 4u;
+        if (tops[0][0] == -INFINITY && !nan) {          // nothing but masked tokens: the first ones
+            const uint32_t i = (v0 ? v0 * N - head : 0u) + lane;
+            if (warp == 0) lists[0][lane] = v0 < v1 && i < min(v1 * N - head, a.vocab) ? top_key(-INFINITY, i) : 0ull;
             __syncthreads();
+        } else {
+            if (few) {          // whatever reaches the floor, in any order; sorted afterwards
+                for (uint32_t q0 = warp * 32u; q0 < total; q0 += THREADS * 2u) {
+                    float x[2][N];
+                    uint32_t v[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) v[u] = fetch(q0 + u * THREADS + lane, x[u]);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        float top = x[u][0];
+#pragma unroll
+                        for (int e = 1; e < N; e++) top = fmaxf(top, x[u][e]);
+                        if (v[u] >= v1 || top < low) continue;
+#pragma unroll
+                        for (int e = 0; e < N; e++)
+                            if (!(x[u][e] < low) && v[u] * N + e - head < a.vocab) {
+                                const uint32_t at = atomicAdd(&found, 1u);
+                                if (at < WARPS * 32u) (&lists[0][0])[at] = top_key(x[u][e], v[u] * N + e - head);
+                            }
+                    }
+                }
+                __syncthreads();
+                const uint32_t n = found;
+                few = n <= WARPS * 32u;
+                if (few) {
+                    if (warp * 32u < n || warp == 0) lists[warp][lane] = warp_sort(warp * 32u + lane < n ? lists[warp][lane] : 0ull);
+                    for (uint32_t w = 1; w * 32u < n; w <<= 1) {          // (as many lists as there are, by pairs)
+                        __syncthreads();
+                        if (warp % (2u * w) == 0 && (warp + w) * 32u < n) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + w][lane]);
+                    }
+                }
+                __syncthreads();
+            }
+            if (!few) {          // rows full of equal numbers: a list to a warp, which only a better key enters
+                TopList best;
+                best.top = a.top;
+                for (uint32_t q0 = warp * 32u; q0 < total; q0 += THREADS) {
+                    float x[N];
+                    const uint32_t v = fetch(q0 + lane, x), first = v * N - head;
+                    float top = x[0];
+#pragma unroll
+                    for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
+                    // (no key of the vector is above that of its largest number at its first place)
+                    if (!__any_sync(0xffffffffu, v < v1 && !(top < low) && top_key(top, v ? first : 0u) > best.kth)) continue;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const bool in = v < v1 && first + e < a.vocab && !(x[e] < low);
+                        if (__any_sync(0xffffffffu, in)) best.take(in ? top_key(x[e], first + e) : 0ull);
+                    }
+                }
+                lists[warp][lane] = best.list;
+                __syncthreads();
+#pragma unroll
+                for (uint32_t half = WARPS / 2; half > 0; half >>= 1) {
+                    if (warp < half) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + half][lane]);
+                    __syncthreads();
+                }
+            }
         }
     }
     if (warp == 0) {
@@ -372,13 +417,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
     }
 }
 
-static uint32_t env_(const char *n, uint32_t d) { const char *s = getenv(n); return s ? atoi(s) : d; }
-template <typename T, bool TOP, int THREADS>
+constexpr int kLpThreads = 256;
+template <typename T, bool TOP, int THREADS = kLpThreads>
 cudaError_t logprobs_launch_t(const LogprobArgs &a, cudaStream_t stream) {
     const uint32_t nv = (a.vocab + Elem<T>::N - 1u) / Elem<T>::N;
-    // blocks to a row: as long as each thread keeps a vector of it and the device is not full of them
+    // blocks to a row: until there is one for each SM, as long as a thread keeps a step's vectors.  us at 1 / 2 / 4 / 8 / 16 blocks, with eight alternatives: one row of 151936
+    // fp32 numbers 24 / 17 / 12 / 9 / 8, 64 of 32000 8.6 / 7.5 / 7.5 / 8.3, 256 bf16 rows of 32000 9.1 / 11.4 / 16.5, 1024 of 151936 77 / 89 / 111
     uint32_t C = 1;
-    while (C < kLpMaxCluster && nv >= env_("LPV", 2) * C * THREADS && (uint64_t)a.rows * C < env_("LPB", 592)) C *= 2;
+    while (C < kLpMaxCluster && nv >= (uint32_t)kLpUnroll * C * THREADS && (uint64_t)a.rows * C < 148u) C *= 2;
     if (C > 8) {          // more than eight blocks to a cluster are to be asked for, on every device that runs them
         cudaError_t e = cudaFuncSetAttribute(k_logprobs<T, TOP, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
@@ -442,10 +488,9 @@ cudaError_t pages_launch(const PagePool *pools, uint32_t n_pools, const uint32_t
 
 cudaError_t logprobs_launch(const LogprobArgs &a, cudaStream_t stream) {
     if (!a.rows) return cudaSuccess;
-#define LP(T) (env_("LPT", 256) == 256 ? (a.top ? logprobs_launch_t<T, true, 256>(a, stream) : logprobs_launch_t<T, false, 256>(a, stream)) \
-                                       : (a.top ? logprobs_launch_t<T, true, 512>(a, stream) : logprobs_launch_t<T, false, 512>(a, stream)))
-    return a.type == T_F32 ? LP(float) : a.type == T_BF16 ? LP(__nv_bfloat16) : LP(__half);
-#undef LP
+    return a.type == T_F32 ? (a.top ? logprobs_launch_t<float, true>(a, stream) : logprobs_launch_t<float, false>(a, stream))
+         : a.type == T_BF16 ? (a.top ? logprobs_launch_t<__nv_bfloat16, true>(a, stream) : logprobs_launch_t<__nv_bfloat16, false>(a, stream))
+                            : (a.top ? logprobs_launch_t<__half, true>(a, stream) : logprobs_launch_t<__half, false>(a, stream));
 }
 
 cudaError_t pages_copy_launch(const PagePool *pools, uint32_t n_pools, const uint32_t *src, const uint32_t *dst, uint32_t n, cudaStream_t stream, uint32_t *launches) {
