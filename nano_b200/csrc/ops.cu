@@ -131,6 +131,7 @@ typedef unsigned long long pair_t;
 __device__ __forceinline__ pair_t pair(float a, float b) { pair_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ void unpair(pair_t p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
 __device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) { pair_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ pair_t add2(pair_t a, pair_t b) { pair_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 // What a thread has seen: m, and z, s in units of 2^u, u = m log2 e as it was rounded while m is small (d = x log2 e - u is then one multiply-add), and exact where m is
@@ -146,35 +147,48 @@ struct Running {
         z = fma2(z, ff, none);
         m = next;
     }
-    template <int N> __device__ __forceinline__ void see(const float (&x)[N]) {
-        float top = x[0], low = x[0];
+    // false, and only m renewed, where a number is masked or outsize: -inf log2 e makes s NaN and z not
+    template <int N> __device__ __forceinline__ bool see(const float (&x)[N]) {
+        float top = x[0];
 #pragma unroll
-        for (int i = 1; i < N; i++) { top = fmaxf(top, x[i]); low = fminf(low, x[i]); }
-        if (low > -1e37f && fabsf(fmaxf(top, m)) < kSmallLogit) {          // (NaN is no obstacle: it makes z NaN)
-            if (top > m) rescale(top, __fsub_rn(__fmul_rn(fmaxf(m, -1e37f), kLog2e), __fmul_rn(top, kLog2e)));
-            const float c = __fmul_rn(m, kLog2e);
-            const pair_t L = pair(kLog2e, kLog2e), cc = pair(-c, -c);
+        for (int i = 1; i + 1 < N; i += 2) top = max3(top, x[i], x[i + 1]);
+        if constexpr (N % 2 == 0) top = fmaxf(top, x[N - 1]);
+        if (!(fabsf(fmaxf(top, m)) < kSmallLogit)) return false;
+        if (top > m) rescale(top, __fsub_rn(__fmul_rn(fmaxf(m, -1e37f), kLog2e), __fmul_rn(top, kLog2e)));
+        const float c = __fmul_rn(m, kLog2e);
+        const pair_t L = pair(kLog2e, kLog2e), cc = pair(-c, -c);
+        pair_t zn = z, sn = s;
 #pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                const pair_t d = fma2(pair(x[i], x[i + 1]), L, cc);
-                float a, b;
-                unpair(d, a, b);
-                const pair_t p = pair(ex2(a), ex2(b));
-                z = add2(z, p);
-                s = fma2(p, d, s);
-            }
-        } else {          // masked and outsize logits; what weighs nothing is left out of s (0 times -inf)
-            if (top > m) rescale(top, (m - top) * kLog2e - off(m) + off(top));
-            float za, zb, sa, sb;
-            unpair(z, za, zb); unpair(s, sa, sb);
-            const float o = off(m);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float d = fmaf(x[i] - m, kLog2e, o), p = ex2(d);
-                if (i & 1) { zb += p; sb = fmaf(p, fmaxf(d, -1e4f), sb); } else { za += p; sa = fmaf(p, fmaxf(d, -1e4f), sa); }
-            }
-            z = pair(za, zb); s = pair(sa, sb);
+        for (int i = 0; i < N; i += 2) {
+            const pair_t d = fma2(pair(x[i], x[i + 1]), L, cc);
+            float a, b;
+            unpair(d, a, b);
+            const pair_t p = pair(ex2(a), ex2(b));
+            zn = add2(zn, p);
+            sn = fma2(p, d, sn);
         }
+        float za, zb, sa, sb;
+        unpair(zn, za, zb); unpair(sn, sa, sb);
+        const float sum = sa + sb, all = za + zb;
+        if (sum != sum && all == all) return false;
+        z = zn; s = sn;
+        return true;
+    }
+    // any numbers; what weighs nothing is left out of s (0 times -inf)
+    template <int N> __device__ __forceinline__ void see_any(const float (&x)[N]) {
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
+        if (top > m) rescale(top, (m - top) * kLog2e - off(m) + off(top));
+        float za, zb, sa, sb;
+        unpair(z, za, zb); unpair(s, sa, sb);
+        const float o = off(m);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float d = fmaf(x[i] - m, kLog2e, o), p = ex2(d);
+            if (i & 1) { zb += p; sb = fmaf(p, fmaxf(d, -1e4f), sb); } else { za += p; sa = fmaf(p, fmaxf(d, -1e4f), sa); }
+        }
+        z = pair(za, zb); s = pair(sa, sb);
     }
     __device__ __forceinline__ Sums done() const {
         float za, zb, sa, sb;
@@ -196,24 +210,27 @@ __device__ __forceinline__ W peer_word(const W *mine, uint32_t rank) {          
     return v;
 }
 
-// a 16-byte vector of a row as numbers; places outside the row (or past v1) hold -inf.  Whole vectors have been loaded into raw already
+// The row as 16-byte vectors of memory: vector v holds the places [v N - head, v N - head + N), the first and the last vector possibly in part; [whole0, whole1) are whole
 template <typename T>
-__device__ __forceinline__ bool whole_vector(uint32_t v, uint32_t v1, uint32_t nv, uint32_t head, uint32_t vocab) {
-    return v < v1 && (v > 0 || head == 0) && (v + 1u < nv || (head + vocab) % Elem<T>::N == 0);
-}
-template <typename T>
-__device__ __forceinline__ void edge_vector(const T *row, uint32_t v, uint32_t v1, uint32_t head, uint32_t vocab, float *x) {
-    if (v >= v1) {
-#pragma unroll
-        for (int e = 0; e < Elem<T>::N; e++) x[e] = -INFINITY;
-        return;
+struct RowVectors {
+    const T *row; const uint4 *vecs; uint32_t head, vocab, nv, whole0, whole1;
+    __device__ __forceinline__ RowVectors(const T *r, uint32_t V) : row(r), vocab(V) {
+        constexpr uint32_t N = Elem<T>::N;
+        vecs = reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(r) & ~(uintptr_t)15u);
+        head = (uint32_t)((reinterpret_cast<uintptr_t>(r) & 15u) / sizeof(T));
+        nv = (head + V + N - 1u) / N; whole0 = head ? 1u : 0u; whole1 = (head + V) / N;
     }
+    __device__ __forceinline__ bool whole(uint32_t v) const { return v >= whole0 && v < whole1; }
+    // one of the others, number by number; `none` in the places outside the row
+    __device__ __forceinline__ void edge(uint32_t v, float none, float *x) const {
 #pragma unroll
-    for (int e = 0; e < Elem<T>::N; e++) {
-        const uint32_t i = v * Elem<T>::N + e - head;          // wraps below the row's start
-        x[e] = i < vocab ? Elem<T>::one(row + i) : -INFINITY;
+        for (int e = 0; e < Elem<T>::N; e++) {
+            const uint32_t i = v * Elem<T>::N + e - head;          // wraps below the row's start
+            x[e] = i < vocab ? Elem<T>::one(row + i) : none;
+        }
     }
-}
+    __device__ __forceinline__ uint32_t first(uint32_t v) const { return v ? v * Elem<T>::N - head : 0u; }
+};
 
 // 32 lanes' numbers into descending order, and the 32 largest of two such lists
 __device__ __forceinline__ float sort32(float v) {
@@ -255,22 +272,57 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
         if (token >= 0 && token < (long long)a.vocab) xt = Elem<T>::one(row + token);
     }
 
-    // the row as 16-byte vectors of memory: vector v holds the elements [v N - head, v N - head + N), the first and the last possibly in part
-    const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T)), nv = (head + a.vocab + N - 1u) / N, each = (nv + C - 1u) / C;
+    const RowVectors<T> rv(row, a.vocab);
+    const uint32_t nv = rv.nv, head = rv.head, each = (nv + C - 1u) / C;
     const uint32_t v0 = min(nv, rank * each), v1 = min(nv, v0 + each);
-    const uint4 *vecs = reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15u);
     Running run;
-    for (uint32_t vb = v0 + tid; vb < v1; vb += THREADS * kLpUnroll) {
-        uint4 raw[kLpUnroll] = {};
+    // whole vectors [w0, w1): steps of kLpUnroll vectors to a thread without a test, a step's vectors worked on while the next step's are on their way; the rest one by one
+    const uint32_t w0 = min(max(v0, rv.whole0), v1), w1 = max(min(v1, rv.whole1), w0), steps = (w1 - w0) / (THREADS * kLpUnroll);
+    bool masked = false;          // rows with masked tokens have many
+    auto see = [&](const auto &x) {
+        if (!masked && run.see(x)) return;
+        masked = true;
+        run.see_any(x);
+    };
+    uint4 ahead[kLpUnroll];
+    const uint4 *next = rv.vecs + w0 + tid;
+    if (steps)
 #pragma unroll
-        for (int j = 0; j < kLpUnroll; j++) if (whole_vector<T>(vb + j * THREADS, v1, nv, head, a.vocab)) raw[j] = __ldg(vecs + vb + j * THREADS);          // all in flight at once
-        float x[kLpUnroll * N];
+        for (int j = 0; j < kLpUnroll; j++) ahead[j] = __ldg(next + j * THREADS);
+    for (uint32_t step = 0; step < steps; step++) {
+        uint4 raw[kLpUnroll];
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++) raw[j] = ahead[j];
+        next += THREADS * kLpUnroll;
+        if (step + 1u < steps)
+#pragma unroll
+            for (int j = 0; j < kLpUnroll; j++) ahead[j] = __ldg(next + j * THREADS);
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j += 2) {
+            float x[2 * N];
+            Elem<T>::widen(raw[j], x);
+            Elem<T>::widen(raw[j + 1], x + N);
+            see(x);
+        }
+    }
+    {
+        const uint32_t left = w0 + steps * THREADS * kLpUnroll + tid;
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++) if (left + j * THREADS < w1) ahead[j] = __ldg(next + j * THREADS);
 #pragma unroll
         for (int j = 0; j < kLpUnroll; j++) {
-            if (whole_vector<T>(vb + j * THREADS, v1, nv, head, a.vocab)) Elem<T>::widen(raw[j], x + j * N);
-            else edge_vector<T>(row, vb + j * THREADS, v1, head, a.vocab, x + j * N);
+            if (left + j * THREADS >= w1) break;
+            float x[N];
+            Elem<T>::widen(ahead[j], x);
+            see(x);
         }
-        run.see(x);
+        // the row's first and last vector, if they are not whole
+        const uint32_t v = tid == 0 ? 0u : nv - 1u;
+        if (tid < 2 && v >= v0 && v < v1 && !rv.whole(v) && (tid == 0 || nv > 1u)) {
+            float x[N];
+            rv.edge(v, -INFINITY, x);
+            run.see_any(x);
+        }
     }
     Sums t = run.done();
     [[maybe_unused]] const float mine = t.z == 0.0f ? -INFINITY : t.m;          // this thread's largest logit
@@ -291,24 +343,29 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
         for (int w = 0; w < WARPS; w++) nan = nan || red[1][w] != red[1][w];
         const float low = nan ? -INFINITY : tops[0][a.top - 1u];
         // the threads that have alternatives, their vectors dealt out one to a lane
-        const uint32_t own = min(v1, v0 + THREADS) - v0;          // threads that have a vector
-        const bool flag = tid < own && (nan || !(mine < low));
+        const bool flag = w0 + tid < w1 && (nan || !(mine < low));
         const uint32_t votes = __ballot_sync(0xffffffffu, flag);
         uint32_t at = 0;
         if (lane == 0 && votes) at = atomicAdd(&flags, __popc(votes));
         at = __shfl_sync(0xffffffffu, at, 0);
         if (flag) flagged[at + __popc(votes & ((1u << lane) - 1u))] = tid;
         __syncthreads();
-        const uint32_t per = (v1 - v0 + THREADS - 1u) / THREADS, total = flags * per;          // (at most all vectors, rounded up: below 2^32)
+        // (and the two vectors that are not whole, whoever took them; at most all vectors, rounded up: below 2^32)
+        const uint32_t per = (w1 - w0 + THREADS - 1u) / THREADS, total = 2u + flags * per;
         auto fetch = [&](uint32_t q, float (&x)[N]) {
-            const uint32_t v = q < total ? v0 + flagged[q / per] + (q % per) * THREADS : v1;
-            if (whole_vector<T>(v, v1, nv, head, a.vocab)) Elem<T>::widen(__ldg(vecs + v), x);
-            else edge_vector<T>(row, v, v1, head, a.vocab, x);
+            uint32_t v = v1;
+            if (q >= 2u && q < total) { v = w0 + flagged[(q - 2u) / per] + ((q - 2u) % per) * THREADS; v = v < w1 ? v : v1; }
+            else if (q < 2u && (q == 0 ? rv.whole0 != 0 || rv.whole1 == 0 : nv > 1u && rv.whole1 < nv)) { v = q ? nv - 1u : 0u; v = v >= v0 && v < v1 ? v : v1; }
+            if (v < v1 && rv.whole(v)) Elem<T>::widen(__ldg(rv.vecs + v), x);
+            else if (v < v1) rv.edge(v, -INFINITY, x);
+            else
+#pragma unroll
+                for (int e = 0; e < N; e++) x[e] = -INFINITY;
             return v;
         };
         bool few = flags <= THREADS / 4u;
         if (tops[0][0] == -INFINITY && !nan) {          // nothing but masked tokens: the first ones
-            const uint32_t i = (v0 ? v0 * N - head : 0u) + lane;
+            const uint32_t i = rv.first(v0) + lane;
             if (warp == 0) lists[0][lane] = v0 < v1 && i < min(v1 * N - head, a.vocab) ? top_key(-INFINITY, i) : 0ull;
             __syncthreads();
         } else {
@@ -354,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
 #pragma unroll
                     for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
                     // (no key of the vector is above that of its largest number at its first place)
-                    if (!__any_sync(0xffffffffu, v < v1 && !(top < low) && top_key(top, v ? first : 0u) > best.kth)) continue;
+                    if (!__any_sync(0xffffffffu, v < v1 && !(top < low) && top_key(top, rv.first(v)) > best.kth)) continue;
 #pragma unroll
                     for (int e = 0; e < N; e++) {
                         const bool in = v < v1 && first + e < a.vocab && !(x[e] < low);
