@@ -20,15 +20,16 @@ namespace {
 // One pass over the row, bound by its bytes: every thread keeps m, z = sum exp(x - m) and s = sum exp(x - m) (x - m) of what it has seen, in log2 units and on
 // pairs of numbers (fma.f32x2: some five instructions to a number, where eleven are what bf16 rows at the full rate of HBM leave), and rescales them when m grows.  Two
 // such triples join as  z = z1 f1 + z2 f2,  s = f1 (s1 + z1 (m1 - m)) + f2 (...),  f = exp(m_i - m).  Sums are fp32.
-// Alternatives: the k-th largest of the threads' maxima is a floor below which no alternative of the block lies, and only threads whose maximum reaches it have any: about
-// k of them, whose vectors are read once more and looked at one by one (a warp keeps its 32 best in registers, lane i the i-th, as 64-bit keys: ordered bits of x,
-// complement of the index).  Lists kept during the pass instead cost 3 to 5 times the pass.
+// Alternatives: the k-th largest of the threads' maxima is a floor below which no alternative of the block lies.  Of every thread's steps the maxima of eight segments are
+// kept, and only segments that reach the floor, about k, are read once more (1024 rows of 151936: whole threads instead were 15 us of fetches from HBM); what reaches it is
+// sorted as 64-bit keys, ordered bits of x and complement of the index.  Lists kept during the pass instead cost 3 to 5 times the pass.
 // A row belongs to a cluster of C blocks, whose parts are joined over distributed shared memory: one launch, no workspace, no order of arrival in the result.
 // -inf (a masked token) adds nothing; a row of nothing else has log probabilities -inf and entropy 0; NaN or +inf anywhere makes a row's numbers NaN (its order
 // of alternatives counts NaN as -inf).
 // ------------------------------------------------------------------------------------------------
 constexpr int kLpMaxCluster = 16;
 constexpr int kLpUnroll = 4;          // 16-byte vectors in flight per thread
+constexpr uint32_t kLpSegs = 8;       // segments of a thread's steps whose maxima are kept
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -138,7 +139,7 @@ __device__ __forceinline__ pair_t add2(pair_t a, pair_t b) { pair_t r; asm("add.
 // not (m - x first: nothing overflows, and the rounding of a large product does not count)
 constexpr float kSmallLogit = 4096.0f;
 struct Running {
-    float m = -FLT_MAX; pair_t z = 0, s = 0;          // (z and s: partial sums of the even and of the odd places)
+    float m = -FLT_MAX, seg = -INFINITY; pair_t z = 0, s = 0;          // seg: largest number of the present segment; z and s: partial sums of the even and of the odd places
     static __device__ __forceinline__ float off(float m) { return fabsf(m) < kSmallLogit ? fmaf(m, kLog2e, -__fmul_rn(m, kLog2e)) : 0.0f; }          // m log2 e - u
     __device__ __forceinline__ void rescale(float next, float d) {          // d: the old u less the new one
         const float f = ex2(d);
@@ -153,6 +154,7 @@ struct Running {
 #pragma unroll
         for (int i = 1; i + 1 < N; i += 2) top = max3(top, x[i], x[i + 1]);
         if constexpr (N % 2 == 0) top = fmaxf(top, x[N - 1]);
+        seg = fmaxf(seg, top);
         if (!(fabsf(fmaxf(top, m)) < kSmallLogit)) return false;
         if (top > m) rescale(top, __fsub_rn(__fmul_rn(fmaxf(m, -1e37f), kLog2e), __fmul_rn(top, kLog2e)));
         const float c = __fmul_rn(m, kLog2e);
@@ -179,6 +181,7 @@ struct Running {
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
+        seg = fmaxf(seg, top);
         if (top > m) rescale(top, (m - top) * kLog2e - off(m) + off(top));
         float za, zb, sa, sb;
         unpair(z, za, zb); unpair(s, sa, sb);
@@ -261,7 +264,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
     constexpr int N = Elem<T>::N, WARPS = THREADS / 32;
     __shared__ unsigned long long lists[WARPS > kLpMaxCluster ? WARPS : kLpMaxCluster][32];
     __shared__ float tops[WARPS][32], red[3][WARPS], part[3];
-    __shared__ uint32_t flagged[THREADS], flags, found;          // found: numbers that reach the floor
+    __shared__ float segs[TOP ? kLpSegs : 1][THREADS];
+    __shared__ uint32_t flagged[TOP ? kLpSegs * THREADS : 1], flags, found;          // found: numbers that reach the floor
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = C > 1 ? cluster_rank() : 0u;
     const T *row = static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.row_stride;
 
@@ -284,6 +288,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
         masked = true;
         run.see_any(x);
     };
+    const uint32_t seg_steps = (steps + kLpSegs) / kLpSegs;          // (the rest is one more step)
     uint4 ahead[kLpUnroll];
     const uint4 *next = rv.vecs + w0 + tid;
     if (steps)
@@ -304,6 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
             Elem<T>::widen(raw[j + 1], x + N);
             see(x);
         }
+        if (TOP && (step + 1u) % seg_steps == 0) { segs[step / seg_steps][tid] = run.seg; run.seg = -INFINITY; }
     }
     {
         const uint32_t left = w0 + steps * THREADS * kLpUnroll + tid;
@@ -316,6 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
             Elem<T>::widen(ahead[j], x);
             see(x);
         }
+        if (TOP) segs[steps / seg_steps][tid] = run.seg;
         // the row's first and last vector, if they are not whole
         const uint32_t v = tid == 0 ? 0u : nv - 1u;
         if (tid < 2 && v >= v0 && v < v1 && !rv.whole(v) && (tid == 0 || nv > 1u)) {
@@ -343,18 +350,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const Logp
         for (int w = 0; w < WARPS; w++) nan = nan || red[1][w] != red[1][w];
         const float low = nan ? -INFINITY : tops[0][a.top - 1u];
         // the threads that have alternatives, their vectors dealt out one to a lane
-        const bool flag = w0 + tid < w1 && (nan || !(mine < low));
-        const uint32_t votes = __ballot_sync(0xffffffffu, flag);
-        uint32_t at = 0;
-        if (lane == 0 && votes) at = atomicAdd(&flags, __popc(votes));
-        at = __shfl_sync(0xffffffffu, at, 0);
-        if (flag) flagged[at + __popc(votes & ((1u << lane) - 1u))] = tid;
+        if (w0 + tid < w1 && (nan || !(mine < low)))
+            for (uint32_t g = 0; g <= steps / seg_steps; g++) if (nan || !(segs[g][tid] < low)) flagged[atomicAdd(&flags, 1u)] = g * THREADS + tid;
         __syncthreads();
         // (and the two vectors that are not whole, whoever took them; at most all vectors, rounded up: below 2^32)
-        const uint32_t per = (w1 - w0 + THREADS - 1u) / THREADS, total = 2u + flags * per;
+        const uint32_t per = seg_steps * kLpUnroll, total = 2u + flags * per;
         auto fetch = [&](uint32_t q, float (&x)[N]) {
             uint32_t v = v1;
-            if (q >= 2u && q < total) { v = w0 + flagged[(q - 2u) / per] + ((q - 2u) % per) * THREADS; v = v < w1 ? v : v1; }
+            if (q >= 2u && q < total) { const uint32_t f = flagged[(q - 2u) / per]; v = w0 + f % THREADS + (f / THREADS * per + (q - 2u) % per) * THREADS; v = v < w1 ? v : v1; }
             else if (q < 2u && (q == 0 ? rv.whole0 != 0 || rv.whole1 == 0 : nv > 1u && rv.whole1 < nv)) { v = q ? nv - 1u : 0u; v = v >= v0 && v < v1 ? v : v1; }
             if (v < v1 && rv.whole(v)) Elem<T>::widen(__ldg(rv.vecs + v), x);
             else if (v < v1) rv.edge(v, -INFINITY, x);
