@@ -6,6 +6,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "family.h"
 #include "kv4.h"
@@ -672,7 +673,13 @@ template <int NG, int NT, int WK>
 cudaError_t attn_launch(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, bool pdl) {
     constexpr int smem = (int)Room<NG, NT, WK, kWarps>::all;
     const auto k = k_kv4_attn<NG, NT, WK, kWarps>;
-    const cudaError_t e = smem_at_least(reinterpret_cast<const void *>(k), smem);
+    static std::atomic<uint64_t> asked{0};          // devices (of the first 64) whose limit has been raised: asking costs a microsecond
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev > 63 || !(asked.load(std::memory_order_acquire) >> dev & 1u))) {
+        e = smem_at_least(reinterpret_cast<const void *>(k), smem);
+        if (e == cudaSuccess && dev <= 63) asked.fetch_or(1ull << dev, std::memory_order_release);
+    }
     return e != cudaSuccess ? e : launch_on(k, dim3(sh.nsplit * sh.tiles, a.G, a.B), kWarps * 32, smem, stream, pdl, a, sh);
 }
 template <int NG>

@@ -138,10 +138,10 @@ def lib(layered_ok: bool = False):
         L.nb200_step_scores.argtypes = [C.c_void_p, C.c_uint32, u32p, C.c_uint32, u32p, u32p, C.c_uint32, C.c_uint32, f32p, f32p, f32p, i32p]
         L.nb200_read_scores.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, f32p, f32p, f32p, i32p]
         L.nb200_dev_token_logprobs.argtypes = [C.c_void_p] * 5 + [C.c_uint32, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]
-        L.nb200_dev_pages_copy.argtypes = [C.POINTER(C.c_void_p), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), u32p, C.c_uint32, u32p, u32p, C.c_uint32, C.c_void_p]
-        L.nb200_dev_kv4_write.argtypes = L.nb200_dev_kv4_read.argtypes = [C.POINTER(Kv4Rows), C.c_void_p]
-        L.nb200_dev_kv4_attention_workspace.argtypes = [C.POINTER(Kv4Attention), C.POINTER(C.c_uint64)]
-        L.nb200_dev_kv4_attention.argtypes = [C.POINTER(Kv4Attention), C.c_void_p, C.c_uint64, C.c_void_p]
+        L.nb200_dev_pages_copy.argtypes = [C.c_void_p] * 4 + [C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]          # (host arrays; argument blocks as bytes)
+        L.nb200_dev_kv4_write.argtypes = L.nb200_dev_kv4_read.argtypes = [C.c_void_p, C.c_void_p]
+        L.nb200_dev_kv4_attention_workspace.argtypes = [C.c_void_p, C.POINTER(C.c_uint64)]
+        L.nb200_dev_kv4_attention.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
         L.nb200_lora_load.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64]
         L.nb200_lora_enable.argtypes = [C.c_void_p, C.c_int]
         L.nb200_lora_unload.argtypes = [C.c_void_p]

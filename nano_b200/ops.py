@@ -13,6 +13,7 @@ does not take are refused with NB200Error before anything is queued; there is no
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -21,39 +22,34 @@ from . import engine as E
 from .engine import NB200Error, lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# the argument blocks nb200_kv4_rows and nb200_kv4_attention as bytes: a ctypes.Structure of as many fields takes four times as long to fill
+_ROWS, _ATTENTION = struct.Struct("@QQIIIIIQQQQQQQ").pack, struct.Struct("@QQQQQQQQQQIIIIIIIIQQQQffII").pack
+assert len(_ROWS(*[0] * 14)) == C.sizeof(E.Kv4Rows) and len(_ATTENTION(*[0] * 26)) == C.sizeof(E.Kv4Attention)
+_stream_of, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice          # (torch.cuda's functions of that purpose cost two microseconds a call)
 
 
-def _need(ok, text, *args):
-    if not ok:
-        raise NB200Error(text % args if args else text)
+def _no(text, *args):
+    raise NB200Error(text % args if args else text)
 
 
-class _on:
-    """The device of `t` made current for a call (it is already, nearly always)."""
-
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _cuda(name, t, device=None):
+    """The device of a CUDA tensor, which is to be `device`."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _no("%s is to be a CUDA tensor", name)
+    d = t.get_device()
+    if device is not None and d != device:
+        _no("%s is on another device", name)
+    return d
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _cuda(name, t, like=None):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, "%s is to be a CUDA tensor", name)
-    _need(like is None or t.device == like.device, "%s is on another device", name)
-
-
-def _check(rc):
-    if rc != 0:
+def _call(device, f, *args):
+    """f(*args, stream) on the device and its current stream."""
+    if device == _device_now():
+        rc = f(*args, _stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args, _stream_of(device))
+    if rc:
         E._check(rc)
 
 
@@ -63,105 +59,139 @@ def token_logprobs(logits, tokens, top=0):
 
     Alternatives are ordered by logit, equal ones by id.  -inf masks a token; a row of nothing but -inf has log probabilities -inf and entropy 0, one with NaN or
     +inf has NaN; a token outside the vocabulary has log probability NaN."""
-    _cuda("logits", logits)
-    _cuda("tokens", tokens, logits)
-    _need(logits.dim() == 2 and logits.dtype in _TYPES, "logits are [rows, vocab] of float32, bfloat16 or float16")
+    device = _cuda("logits", logits)
+    _cuda("tokens", tokens, device)
+    kind = _TYPES.get(logits.dtype)
+    if logits.dim() != 2 or kind is None:
+        _no("logits are [rows, vocab] of float32, bfloat16 or float16")
     rows, vocab = logits.shape
-    _need(vocab > 0 or rows == 0, "the vocabulary is empty")
-    _need(tokens.shape == (rows,) and tokens.dtype in (torch.int32, torch.int64), "tokens are [rows] of int32 or int64")
-    _need(0 <= top <= 32 and (top <= vocab or rows == 0), "%d alternatives asked for: at most 32, and no more than the vocabulary has", top)
-    if rows and vocab > 1 and logits.stride(1) != 1 or logits.stride(0) < 0:
+    if rows and not vocab:
+        _no("the vocabulary is empty")
+    if tokens.dim() != 1 or tokens.shape[0] != rows or tokens.dtype not in (torch.int64, torch.int32):
+        _no("tokens are [rows] of int32 or int64")
+    if not 0 <= top <= 32 or (top > vocab and rows):
+        _no("%d alternatives asked for: at most 32, and no more than the vocabulary has", top)
+    stride, step = logits.stride()
+    if (step != 1 and vocab > 1) or stride < 0:
         logits = logits.contiguous()
-    tokens = tokens.contiguous()
-    both = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
-    top_logprob = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    top_id = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        stride = vocab
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    where = logits.device
+    logprob, entropy = torch.empty(rows, dtype=torch.float32, device=where), torch.empty(rows, dtype=torch.float32, device=where)
+    top_logprob, top_id = torch.empty((rows, top), dtype=torch.float32, device=where), torch.empty((rows, top), dtype=torch.int32, device=where)
     if rows:
-        with _on(logits):
-            at = both.data_ptr()
-            _check(lib(True).nb200_dev_token_logprobs(at, at + 4 * rows, top_logprob.data_ptr() or None, top_id.data_ptr() or None, logits.data_ptr(), _TYPES[logits.dtype],
-                                                      logits.stride(0), rows, vocab, tokens.data_ptr(), tokens.element_size(), top, _stream(logits)))
-    return both[0], both[1], top_logprob, top_id
+        _call(device, lib(True).nb200_dev_token_logprobs, logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr() or None, top_id.data_ptr() or None, logits.data_ptr(), kind,
+              stride, rows, vocab, tokens.data_ptr(), tokens.element_size(), top)
+    return logprob, entropy, top_logprob, top_id
 
 
 def pages_copy(pools, src, dst):
     """Page src[i] is copied over page dst[i] in every pool, in place.  pools: tensors [pages, ...] of any type, each page contiguous; src, dst: numbers on the host.
     A source may appear many times; a destination that is a source too or appears twice is refused."""
     pools = list(pools)
-    src, dst = np.ascontiguousarray(src, np.int64), np.ascontiguousarray(dst, np.int64)
-    _need(src.ndim == 1 and src.shape == dst.shape, "src and dst are lists of the same length")
-    n = len(pools)
-    if n == 0:
+    try:
+        both = np.array([src, dst], np.int64)
+    except (ValueError, TypeError):
+        both = np.empty(0)
+    if both.ndim != 2:
+        _no("src and dst are lists of the same length")
+    if not pools:
         return
-    base, size, stride, pages = (C.c_void_p * n)(), (C.c_uint64 * n)(), (C.c_uint64 * n)(), (C.c_uint32 * n)()
-    first = pools[0]
+    device = _cuda("pool 0", pools[0])
+    base, size, stride, pages = [], [], [], []
     for i, p in enumerate(pools):
-        _cuda("pool %d" % i, p, first)
-        _need(p.dim() >= 1 and (p.shape[0] == 0 or p[0].is_contiguous()), "pool %d: a page is to be contiguous", i)
-        e = p.element_size()
-        pages[i] = p.shape[0]
-        size[i] = p[0].numel() * e if p.shape[0] else 0
-        stride[i] = p.stride(0) * e if p.shape[0] > 1 else size[i]
-        base[i] = p.data_ptr()
-    most = min(pages)
-    _need(src.size == 0 or (min(src.min(), dst.min()) >= 0 and max(src.max(), dst.max()) < most), "a page outside the smallest pool's %d", most)
-    src, dst = src.astype(np.uint32), dst.astype(np.uint32)
-    with _on(first):
-        _check(lib(True).nb200_dev_pages_copy(base, size, stride, pages, n, E._p(src, E.u32p), E._p(dst, E.u32p), src.size, _stream(first)))
+        if not isinstance(p, torch.Tensor) or p.get_device() != device or not p.dim():
+            _cuda("pool %d" % i, p, device)
+            _no("pool %d has no pages", i)
+        count = p.size(0)
+        if p.is_contiguous():
+            one = p.nbytes // count if count else 0
+            stride.append(one)
+        else:
+            if not p[0].is_contiguous() or p.stride(0) < 0:
+                _no("pool %d: a page is to be contiguous", i)
+            one = p[0].nbytes
+            stride.append(p.stride(0) * p.element_size() if count > 1 else one)
+        base.append(p.data_ptr())
+        size.append(one)
+        pages.append(count)
+    n, most = len(pools), min(pages)
+    if both.size and (both.min() < 0 or both.max() >= most):
+        _no("a page outside the smallest pool's %d", most)
+    both = both.astype(np.uint32)
+    at, count = both.ctypes.data, both.shape[1]
+    _call(device, lib(True).nb200_dev_pages_copy, (C.c_uint64 * n)(*base), (C.c_uint64 * n)(*size), (C.c_uint64 * n)(*stride), (C.c_uint32 * n)(*pages), n, at, at + 4 * count, count)
 
 
 def kv4_cache(pages, kv_heads, head_dim, device="cuda"):
     """A pool of zeros: uint8 [pages, kv_heads, 40 * head_dim], pages of 32 tokens.  head_dim: a multiple of 32 up to 256."""
-    _need(head_dim > 0 and head_dim % 32 == 0 and head_dim <= 256, "head_dim %d: a cache in 4 bits holds multiples of 32 up to 256", head_dim)
+    if not 0 < head_dim <= 256 or head_dim % 32:
+        _no("head_dim %d: a cache in 4 bits holds multiples of 32 up to 256", head_dim)
     return torch.zeros((pages, kv_heads, 40 * head_dim), dtype=torch.uint8, device=device)
 
 
 def _pool(pool):
-    _cuda("the pool", pool)
-    _need(pool.dim() == 3 and pool.dtype == torch.uint8 and pool.shape[2] % 1280 == 0 and pool.shape[2] > 0, "a pool is uint8 [pages, kv_heads, 40 * head_dim]")
-    _need(pool.stride(2) == 1 and (pool.stride(1) == pool.shape[2] or pool.shape[1] == 1), "a pool's pages are to be contiguous")
-    return pool.shape[0], pool.shape[1], pool.shape[2] // 40
+    """(device, pages, kv_heads, head_dim, bytes from page to page)"""
+    device = _cuda("the pool", pool)
+    if pool.dim() != 3 or pool.dtype != torch.uint8 or pool.shape[2] % 1280 or not pool.shape[2]:
+        _no("a pool is uint8 [pages, kv_heads, 40 * head_dim]")
+    pages, heads, block = pool.shape
+    if not pool.is_contiguous() and (pool.stride(2) != 1 or (pool.stride(1) != block and heads != 1)):
+        _no("a pool's pages are to be contiguous")
+    return device, pages, heads, block // 40, pool.stride(0)
 
 
-def _rows(call, pool, k, v, slots):
-    pages, heads, dim = _pool(pool)
-    r = E.Kv4Rows(pool.data_ptr(), pool.stride(0), pages, heads, dim, _TYPES[k.dtype], k.shape[0], slots.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with _on(pool):
-        _check(call(C.byref(r), _stream(pool)))
-
-
-def _slots(slots, pool):
-    _cuda("slots", slots, pool)
-    _need(slots.dim() == 1 and slots.dtype == torch.int32, "slots are [tokens] of int32")
+def _slots(slots, device):
+    _cuda("slots", slots, device)
+    if slots.dim() != 1 or slots.dtype != torch.int32:
+        _no("slots are [tokens] of int32")
     return slots.contiguous()
+
+
+def _row_strides(x):
+    """x with neighbouring coordinates, and its strides of rows and heads"""
+    t, h, c = x.stride()
+    if c != 1 or t < 0 or h < 0:
+        x = x.contiguous()
+        t, h, c = x.stride()
+    return x, t, h
 
 
 def kv4_write(pool, k, v, slots):
     """Row t of k and v ([tokens, kv_heads, head_dim], float32, bfloat16 or float16, any strides of rows and heads) goes to place slots[t] = page * 32 + place in the
     page of the pool, in place.  Rows whose slot lies outside the pool (-1: padding) are skipped; no slot may be given twice."""
-    pages, heads, dim = _pool(pool)
+    device, pages, heads, dim, stride = _pool(pool)
     for name, x in (("k", k), ("v", v)):
-        _cuda(name, x, pool)
-        _need(x.dim() == 3 and tuple(x.shape[1:]) == (heads, dim) and x.dtype in _TYPES, "%s is [tokens, %d, %d] of float32, bfloat16 or float16", name, heads, dim)
-    _need(k.shape == v.shape and k.dtype == v.dtype, "k and v are of one shape and type")
-    slots = _slots(slots, pool)
-    _need(slots.shape[0] == k.shape[0], "a slot for each row")
-    if not k.shape[0]:
+        _cuda(name, x, device)
+        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim or x.dtype not in _TYPES:
+            _no("%s is [tokens, %d, %d] of float32, bfloat16 or float16", name, heads, dim)
+    tokens = k.shape[0]
+    if v.shape[0] != tokens or k.dtype != v.dtype:
+        _no("k and v are of one shape and type")
+    slots = _slots(slots, device)
+    if slots.shape[0] != tokens:
+        _no("a slot for each row")
+    if not tokens:
         return
-    k, v = (x if x.stride(2) == 1 and x.stride(0) >= 0 and x.stride(1) >= 0 else x.contiguous() for x in (k, v))
-    _rows(lib(True).nb200_dev_kv4_write, pool, k, v, slots)
+    k, kt, kh = _row_strides(k)
+    v, vt, vh = _row_strides(v)
+    rows = _ROWS(pool.data_ptr(), stride, pages, heads, dim, _TYPES[k.dtype], tokens, slots.data_ptr(), k.data_ptr(), v.data_ptr(), kt, kh, vt, vh)
+    _call(device, lib(True).nb200_dev_kv4_write, rows)
 
 
 def kv4_read(pool, slots, dtype=torch.float32):
     """What the places `slots` stand for: (k, v), [tokens, kv_heads, head_dim] each; zeros where a slot lies outside the pool."""
-    pages, heads, dim = _pool(pool)
-    slots = _slots(slots, pool)
-    _need(dtype in _TYPES, "rows are float32, bfloat16 or float16")
-    both = torch.empty((2, slots.shape[0], heads, dim), dtype=dtype, device=pool.device)
-    k, v = both[0], both[1]
-    if slots.shape[0]:
-        _rows(lib(True).nb200_dev_kv4_read, pool, k, v, slots)
+    device, pages, heads, dim, stride = _pool(pool)
+    slots = _slots(slots, device)
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        _no("rows are float32, bfloat16 or float16")
+    tokens = slots.shape[0]
+    k, v = torch.empty((tokens, heads, dim), dtype=dtype, device=pool.device), torch.empty((tokens, heads, dim), dtype=dtype, device=pool.device)
+    if tokens:
+        rows = _ROWS(pool.data_ptr(), stride, pages, heads, dim, kind, tokens, slots.data_ptr(), k.data_ptr(), v.data_ptr(), heads * dim, dim, heads * dim, dim)
+        _call(device, lib(True).nb200_dev_kv4_read, rows)
     return k, v
 
 
@@ -173,31 +203,43 @@ def kv4_attention(q, pool, table, lens, scale=None, window=0, block=0, softcap=0
     `window` (0: all) and those in its own block of `block` positions (0: all).  scale: 1 / sqrt(head_dim) unless given; softcap > 0: softcap * tanh(score / softcap);
     sinks [heads] (float32): one more term exp(sink) in a head's denominator.  A query at a negative position or without a key in sight has zeros.  head_dim 32, 64, 96, 128
     or 256.  Products take 11-bit operands and sum in 32 bits, whichever type q has."""
-    pages, heads, dim = _pool(pool)
-    _cuda("q", q, pool)
-    _cuda("table", table, pool)
-    _cuda("lens", lens, pool)
-    _need(q.dim() == 4 and q.dtype in (torch.float32, torch.bfloat16) and q.shape[3] == dim, "q is [batch, tokens, heads, %d] of bfloat16 or float32", dim)
+    device, pages, heads, dim, stride = _pool(pool)
+    _cuda("q", q, device)
+    _cuda("table", table, device)
+    _cuda("lens", lens, device)
+    kind = _TYPES.get(q.dtype, 2)
+    if q.dim() != 4 or kind == 2 or q.shape[3] != dim:
+        _no("q is [batch, tokens, heads, %d] of bfloat16 or float32", dim)
     B, T, H, _ = q.shape
-    _need(table.dim() == 2 and table.shape[0] == B and table.dtype == torch.int32, "table is [batch, width] of int32")
-    _need(lens.shape == (B,) and lens.dtype == torch.int32, "lens is [batch] of int32")
-    _need(window >= 0 and block >= 0, "window and block are not negative")
+    if table.dim() != 2 or table.shape[0] != B or table.dtype != torch.int32:
+        _no("table is [batch, width] of int32")
+    if lens.dim() != 1 or lens.shape[0] != B or lens.dtype != torch.int32:
+        _no("lens is [batch] of int32")
+    if window < 0 or block < 0:
+        _no("window and block are not negative")
     if sinks is not None:
-        _cuda("sinks", sinks, pool)
-        _need(sinks.shape == (H,) and sinks.dtype == torch.float32, "sinks are [heads] of float32")
+        _cuda("sinks", sinks, device)
+        if sinks.dim() != 1 or sinks.shape[0] != H or sinks.dtype != torch.float32:
+            _no("sinks are [heads] of float32")
         sinks = sinks.contiguous()
-    lens = lens.contiguous()
-    if table.stride(1) != 1 and table.shape[1] > 1 or table.stride(0) < 0:
+    if not lens.is_contiguous():
+        lens = lens.contiguous()
+    if (table.stride(1) != 1 and table.shape[1] > 1) or table.stride(0) < 0:
         table = table.contiguous()
-    if q.stride(3) != 1 or min(q.stride()) < 0:
+    qb, qt, qh, qd = q.stride()
+    if qd != 1 or qb < 0 or qt < 0 or qh < 0:
         q = q.contiguous()
-    out = torch.empty((B, T, H, dim), dtype=q.dtype, device=q.device)
-    p = E.Kv4Attention(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), q.stride(2), T * H * dim, H * dim, dim, pool.data_ptr(), pool.stride(0), pages, heads, dim,
-                       _TYPES[q.dtype], B, T, H, table.shape[1], table.stride(0), table.data_ptr() or None, lens.data_ptr(), None if sinks is None else sinks.data_ptr(),
-                       dim ** -0.5 if scale is None else scale, softcap, window, block)
-    L, need = lib(True), C.c_uint64(0)
-    with _on(pool):
-        _check(L.nb200_dev_kv4_attention_workspace(C.byref(p), C.byref(need)))
-        room = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        _check(L.nb200_dev_kv4_attention(C.byref(p), None if room is None else room.data_ptr(), need.value, _stream(pool)))
+        qb, qt, qh, qd = q.stride()
+    where = q.device
+    out = torch.empty((B, T, H, dim), dtype=q.dtype, device=where)
+    p = _ATTENTION(q.data_ptr(), out.data_ptr(), qb, qt, qh, T * H * dim, H * dim, dim, pool.data_ptr(), stride, pages, heads, dim, kind, B, T, H, table.shape[1], table.stride(0),
+                   table.data_ptr(), lens.data_ptr(), 0 if sinks is None else sinks.data_ptr(), dim ** -0.5 if scale is None else scale, softcap, window, block)
+    L, need = lib(True), C.c_uint64()
+    _call(device, _workspace, L, p, need)
+    room = torch.empty(need.value, dtype=torch.uint8, device=where) if need.value else None
+    _call(device, L.nb200_dev_kv4_attention, p, None if room is None else room.data_ptr(), need.value)
     return out
+
+
+def _workspace(L, p, need, stream):
+    return L.nb200_dev_kv4_attention_workspace(p, C.byref(need))
