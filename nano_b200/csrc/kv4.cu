@@ -192,6 +192,13 @@ __device__ __forceinline__ void take(const unsigned char *p, uint32_t (&w)[(BYTE
     }
 }
 
+// tanh for the soft cap: its series where |x| < 1/2 (off by at most 21844/6081075 x^13 = 4.4e-7), where the special function unit would be the bound; else 1 - 2 / (1 + e^2x)
+__device__ __forceinline__ float tanh_near(float x) {
+    const float y = x * x;
+    return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1382.0f / 155925.0f, 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
+}
+__device__ __forceinline__ float tanh_any(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * x)); }
+
 __device__ __forceinline__ int first_seen(int pos, uint32_t window, uint32_t block) {
     int f = 0;
     if (window && pos >= (int)window) f = pos - (int)window + 1;
@@ -234,9 +241,12 @@ struct Room {
                               q = (W / WK) * NT * NG * 512u, all = (ring > merge ? ring : merge) + q + (W / WK) * NT * 8u * 4u * (after ? 1u + NG : 1u);
 };
 
+// blocks that an SM holds at once: registers allow no more without spills
+__host__ __device__ constexpr int kv4_blocks(int NG, int NT) { return NG <= 2 || (NG <= 4 && NT == 1) ? 4 : NG <= 4 ? 3 : 2; }
+
 // grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
 template <int NG, int NT, int WK, int W>
-__global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1 /*B*/) k_kv4_attn(const Kv4Attn a, const Shape sh) {
+__global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT)) k_kv4_attn(const Kv4Attn a, const Shape sh) {
     pdl_enter4();
     using R = Room<NG, NT, WK, W>;
     constexpr uint32_t D = 32u * NG, COLS = NT * 8u;
@@ -430,7 +440,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 && NG <= 4 ? 4 : 1 /*B*/) k_kv
 #pragma unroll
                 for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int x = 0; x < 4; x++) s[k][t][x] = a.softcap * kLog2e * tanhf(s[k][t][x] * f[t][x & 1]);
+                    for (int x = 0; x < 4; x++) { s[k][t][x] *= f[t][x & 1]; top[0] = fmaxf(top[0], fabsf(s[k][t][x])); }
+                const bool near = __all_sync(0xffffffffu, top[0] < 0.5f);          // (a NaN goes through either)
+                top[0] = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) s[k][t][x] = a.softcap * kLog2e * (near ? tanh_near(s[k][t][x]) : tanh_any(s[k][t][x]));
             } else {
 #pragma unroll
                 for (int k = 0; k < 2; k++)
@@ -654,10 +670,10 @@ static uint32_t env_waves() { const char *s = getenv("KV4W"); return s ? atoi(s)
 struct Plan { int nt; bool rows; Shape sh; };
 constexpr uint32_t kWarps = 4, kBlocksPerSm = 15, kRes = 4;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
-    const uint32_t ncols = T * (H / G), most = D > 128 ? 2u : 4u;
+    const uint32_t ncols = T * (H / G);
     Plan p{};
-    p.nt = ncols <= 8 ? 1 : ncols <= 16 || most == 2 ? 2 : 4;
-    p.rows = ncols > (uint32_t)p.nt * 8u;
+    p.nt = ncols <= 8 ? 1 : 2;
+    p.rows = ncols > 16;
     p.sh.cols = (uint32_t)p.nt * 8u * (p.rows ? kWarps : 1u);
     p.sh.tiles = (ncols + p.sh.cols - 1u) / p.sh.cols;
     // pages that a block can have in sight
@@ -684,11 +700,8 @@ cudaError_t attn_launch(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, 
 }
 template <int NG>
 cudaError_t attn_launch_nt(const Kv4Attn &a, const Plan &p, cudaStream_t stream, bool pdl) {
-    constexpr int most = NG > 4 ? 2 : 4;
-    if (p.rows) return attn_launch<NG, most, 1>(a, p.sh, stream, pdl);
-    if (p.nt == 1) return attn_launch<NG, 1, kWarps>(a, p.sh, stream, pdl);
-    if (p.nt == 2) return attn_launch<NG, 2, kWarps>(a, p.sh, stream, pdl);
-    return attn_launch<NG, most, kWarps>(a, p.sh, stream, pdl);
+    if (p.rows) return attn_launch<NG, 2, 1>(a, p.sh, stream, pdl);
+    return p.nt == 1 ? attn_launch<NG, 1, kWarps>(a, p.sh, stream, pdl) : attn_launch<NG, 2, kWarps>(a, p.sh, stream, pdl);
 }
 
 template <bool WRITE>
