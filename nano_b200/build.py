@@ -46,14 +46,15 @@ UNITS = {
     "engine.cu": ["prefill.h", "attn_tc.h", "kernels.cuh", "expf_ref.cuh", "stream_args.h", "stream_count.h", "stream_groups.h", "stream_host.h", "ops.h", "sample_host.h", "family.h", "../../include/nano_b200.h"],
     "stream.cu": ["kernels.cuh", "expf_ref.cuh", "stream_args.h", "stream_host.h", "stream.cuh"],
     "ops.cu": ["ops.h", "family.h", "../../include/nano_b200.h"],
-    "kv4.cu": ["kv4.h", "ops.h", "family.h", "../../include/nano_b200.h"],
+    "kv4.cu": ["kv4.cuh", "kv4.h", "ops.h", "family.h", "../../include/nano_b200.h"],
+    "kv4_tc.cu": ["kv4.cuh", "kv4.h", "ops.h", "tc_ptx.cuh", "family.h"],
     "sample.cu": ["kernels.cuh", "expf_ref.cuh", "sample_host.h"],
 }
 
 
 # the units a model FOLDER (config.json + model.safetensors) needs: registry, folder reader, layered runtime, device sampler, operators.
 # The model-file family (engine.cu, stream.cu: minutes of nvcc) is not among them.
-LAYERED_UNITS = ["api.cu", "modeldir.cu", "layered.cu", "layered_tc.cu", "attn_tc.cu", "sample.cu", "ops.cu", "kv4.cu"]
+LAYERED_UNITS = ["api.cu", "modeldir.cu", "layered.cu", "layered_tc.cu", "attn_tc.cu", "sample.cu", "ops.cu", "kv4.cu", "kv4_tc.cu"]
 LAYERED_SO = os.path.join(LIB, "libnano_b200_layered.so")
 
 

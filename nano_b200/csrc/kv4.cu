@@ -3,21 +3,15 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include <algorithm>
 #include <atomic>
 
 #include "family.h"
-#include "kv4.h"
+#include "kv4.cuh"
 
 namespace nb {
 namespace {
-
-__device__ __forceinline__ void pdl_enter4() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 
 // ------------------------------------------------------------------------------------------------
 // Writing.  Four lanes hold a group, eight coordinates each: the extremes take two shuffles, a lane's codes are one word of a key row (two halves of a
@@ -150,9 +144,6 @@ bool rows_at16(const Kv4Rows &a) {
 // its own.  The pages of a row are also split over nsplit blocks, whose parts k_kv4_join puts together.
 // Values that stand for NaN are taken out of the product (0 times NaN would reach columns that do not see them) and make the rows that do see them NaN.
 // ------------------------------------------------------------------------------------------------
-constexpr float kSlack = 3.0f, kCap = 15.0f;          // with s < 2 no weight above 2^15
-constexpr float kLog2e = 1.4426950408889634f;
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -161,78 +152,7 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 half2_of(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
-// the codes at bits 0-3 and 16-19 (HIGH: 4-7 and 20-23) of w as c s + m
-template <bool HIGH>
-__device__ __forceinline__ uint32_t stand_for(uint32_t w, __half2 s, __half2 m) {
-    uint32_t x;          // (one instruction with both constants in registers; written in C++ it became two with immediates)
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "r"(HIGH ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
-    const __half2 h = half2_of(x);
-    const __half2 c = HIGH ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-64.0f)) : __hsub2(h, __float2half2_rn(1024.0f));
-    return bits(__hfma2(c, s, m));
-}
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;          // the bare codes: c 2^-24 and c 2^-20
-// BYTES (a multiple of 2) bytes of shared memory in words
-template <int BYTES>
-__device__ __forceinline__ void take(const unsigned char *p, uint32_t (&w)[(BYTES + 3) / 4]) {
-    if constexpr (BYTES % 16 == 0) {
-#pragma unroll
-        for (int i = 0; i < BYTES / 16; i++) { const uint4 v = reinterpret_cast<const uint4 *>(p)[i]; w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
-    } else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2 *>(p); w[0] = v.x; w[1] = v.y; }
-    else if constexpr (BYTES % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < BYTES / 4; i++) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < BYTES / 2; i++) {
-            const uint32_t v = reinterpret_cast<const uint16_t *>(p)[i];
-            if (i & 1) w[i / 2] |= v << 16; else w[i / 2] = v;
-        }
-    }
-}
-
-// tanh for the soft cap: its series where |x| < 1/2 (off by at most 21844/6081075 x^13 = 4.4e-7), where the special function unit would be the bound; else 1 - 2 / (1 + e^2x)
-__device__ __forceinline__ float tanh_near(float x) {
-    const float y = x * x;
-    return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1382.0f / 155925.0f, 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
-}
-__device__ __forceinline__ float tanh_any(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * x)); }
-
-__device__ __forceinline__ int first_seen(int pos, uint32_t window, uint32_t block) {
-    int f = 0;
-    if (window && pos >= (int)window) f = pos - (int)window + 1;
-    if (block) f = max(f, pos - (int)((uint32_t)pos % block));
-    return f;
-}
-__device__ __forceinline__ int seq_len(const Kv4Attn &a, uint32_t b) {
-    const long long most = (long long)a.width * kKv4Page;
-    const long long n = a.lens ? a.lens[b] : (long long)a.pos0 + (a.pos_ptr ? *a.pos_ptr : 0u) + a.T;
-    return (int)(n < 0 ? 0 : n < most ? n : most);
-}
-// what is left to do with a column's sums: the sink, the division, the gate.  l and the values are in units of 2^r; returns the values' factor
-__device__ __forceinline__ float last_factor(const Kv4Attn &a, uint32_t t, uint32_t h, float r, float l) {
-    if (l == 0.0f) return 0.0f;          // no key in sight (a NaN is no zero)
-    float f = 1.0f;
-    if (a.sink) {
-        const float s = a.sink[h] * kLog2e, top = fmaxf(r, s);
-        f = ex2(r - top);
-        l = fmaf(l, f, ex2(s - top));
-    }
-    f /= l;
-    if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[(uint64_t)t * a.ldg + h]));
-    return f;
-}
-__device__ __forceinline__ void store_four(const Kv4Attn &a, uint32_t b, uint32_t t, uint32_t h, uint32_t d, float x0, float x1, float x2, float x3) {
-    const uint64_t at = b * a.o_batch + t * a.o_token + h * a.o_head + d;
-    if (a.type == T_F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(x0, x1, x2, x3);
-    else {
-        const __nv_bfloat162 u = __floats2bfloat162_rn(x0, x1), v = __floats2bfloat162_rn(x2, x3);
-        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(a.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&u), *reinterpret_cast<const uint32_t *>(&v));
-    }
-}
-
-struct Shape { uint32_t nsplit, tiles, cols; };          // splits of the keys, blocks along the columns of a head, columns of a block
 constexpr int kStages = 2;
 template <int NG, int NT, int WK, int W>
 struct Room {
@@ -666,21 +586,24 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 }
 
 // ---- which instance, and how the work is shared out ----
-static uint32_t env_waves() { const char *s = getenv("KV4W"); return s ? atoi(s) : 3; }
-struct Plan { int nt; bool rows; Shape sh; };
-constexpr uint32_t kWarps = 4, kBlocksPerSm = 15, kRes = 4;
+struct Plan { int nt; bool rows, tc; Shape sh; };
+constexpr uint32_t kWarps = 4, kWaves = 3, kTcCols = 17;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G);
     Plan p{};
     p.nt = ncols <= 8 ? 1 : 2;
     p.rows = ncols > 16;
-    p.sh.cols = (uint32_t)p.nt * 8u * (p.rows ? kWarps : 1u);
+    p.tc = D <= 128 && ncols >= kTcCols;
+    p.sh.cols = p.tc ? kKv4TcRows : (uint32_t)p.nt * 8u * (p.rows ? kWarps : 1u);
     p.sh.tiles = (ncols + p.sh.cols - 1u) / p.sh.cols;
     // pages that a block can have in sight
     const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
     const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
-    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)(B > 1 ? env_waves() : 1) * kRes * sms;
-    const uint32_t least = p.rows ? 8u : kWarps;          // pages of a split
+    // a block for every place that the device has; of several sequences, whose lengths may differ, three times as many (32 of up to 8190 tokens: 90 us with one, 73 with two, 69
+    // with three, 75 with six)
+    const uint32_t at_once = p.tc ? 1u : (uint32_t)kv4_blocks((int)D / 32, p.nt);
+    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)(B > 1 ? kWaves : 1u) * at_once * sms;
+    const uint32_t least = p.tc ? 16u : p.rows ? 8u : kWarps;          // pages of a split
     p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want / std::max<uint64_t>(1, blocks), std::max(1u, pages / least)));
     return p;
 }
@@ -727,13 +650,14 @@ size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32
     return p.sh.nsplit == 1 ? 0 : (size_t)B * G * p.sh.tiles * p.sh.nsplit * p.sh.cols * (D + 2u) * 4u;
 }
 
-// (keys are split only while blocks times splits stays within kBlocksPerSm blocks to an SM)
-size_t kv4_attn_workspace_most(uint32_t B, uint32_t G, uint32_t D, uint32_t sms) { return (size_t)std::max(B * G, kBlocksPerSm * sms) * kWarps * 32u * (D + 2u) * 4u; }
+// (keys are split only while blocks times splits stay within kWaves times the four that an SM holds)
+size_t kv4_attn_workspace_most(uint32_t B, uint32_t G, uint32_t D, uint32_t sms) { return (size_t)std::max(B * G, kWaves * 4u * sms) * kKv4TcRows * (D + 2u) * 4u; }
 
 cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, uint32_t *launches) {
     const Plan p = plan_for(a.B, a.T, a.H, a.G, a.D, a.width, a.window, a.block, sms);
     cudaError_t e;
-    switch (a.D / 32u) {
+    if (p.tc) e = kv4_tc_launch(a, p.sh.nsplit, p.sh.tiles, stream, pdl);
+    else switch (a.D / 32u) {
         case 1: e = attn_launch_nt<1>(a, p, stream, pdl); break;
         case 2: e = attn_launch_nt<2>(a, p, stream, pdl); break;
         case 3: e = attn_launch_nt<3>(a, p, stream, pdl); break;

@@ -1,0 +1,368 @@
+// kv4_tc.cu -- attention of long portions over a cache held in 4 bits, on the fifth-generation tensor cores (formulas: kv4.h).
+//
+// A block owns 128 rows (query token, query head) of one key/value head and walks its keys in tiles of 128, four pages.  Four warps make a tile's operands from the
+// codes, a page each: a word of eight key codes is one 16-byte piece of a row of the swizzled key operand (the queries are laid out in the nibbles' order, so that nothing is
+// shuffled), eight tokens' codes of a coordinate one piece of a row of the value operand, both as c s + m in fp16, rounded once.  One thread issues tcgen05.mma: scores
+// into tensor memory, two buffers, and weights (fp16, back in tensor memory where the scores were) times values.  Eight warps do the softmax, two threads to a row with
+// 64 keys of a tile and half of the values each, as one chain over the row's lanes.  Everything is double buffered: a tile's operands are made, and its
+// scores multiplied, under the softmax of the tile before.
+// Every wait has a limit; a block in which one runs out leaves with NaN in its rows (nothing but its own products is ever in flight).
+// Softmax as in k_kv4_attn: log2 units, weights times 2^kLift, a reference that is renewed when it lags kSlack behind the maximum.
+#include <algorithm>
+#include <atomic>
+
+#include "family.h"
+#include "kv4.cuh"
+#include "tc_ptx.cuh"
+
+namespace nb {
+namespace {
+
+constexpr uint32_t kTile = 128, kThreads = 416, kProducers = 4;
+constexpr float kLift = 12.0f;
+// byte of the 16-byte piece c8 (8 fp16) of row r in an operand of 64-wide blocks of `rows` rows, 128-byte swizzle
+__device__ __forceinline__ uint32_t op_byte(uint32_t rows, uint32_t r, uint32_t c8) { return (c8 >> 3) * rows * 128u + r * 128u + (((c8 & 7u) ^ (r & 7u)) << 4); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <int NG> struct Sizes {
+    static constexpr uint32_t D = 32u * NG, DP = NG <= 2 ? 64u : 128u;          // coordinates; those that an operand of queries or keys has room for
+    static constexpr uint32_t qk = kTile * DP * 2u, v = kTile * D * 2u, all = 3u * qk + 2u * v + 1024u;
+};
+
+// grid (nsplit x tiles, G, B)
+template <int NG>
+__global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, const Shape sh) {
+    using Z = Sizes<NG>;
+    constexpr uint32_t D = Z::D;
+    extern __shared__ uint8_t tc_raw[];
+    enum { KFULL = 0, KFREE = 2, VFULL = 4, VFREE = 6, SFULL = 8, PREADY = 10, OREADY, NBAR };          // (pairs: one for each buffer)
+    __shared__ __align__(8) uint64_t bars[NBAR];
+    __shared__ uint32_t tmem_s;
+    __shared__ uint32_t hide_s[4][kProducers], odd_s[4][kProducers];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys or values that are no number
+    __shared__ float scale_s[kTile], top_s[2][2][kTile], sum_s[2][kTile];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t qs = (smem_u32(tc_raw) + 1023u) & ~1023u, ks = qs + Z::qk, vs = ks + 2u * Z::qk;
+    unsigned char *base = tc_raw + (qs - smem_u32(tc_raw));
+    const uint32_t b0 = smem_u32(bars);
+    auto bar = [&](uint32_t i) { return b0 + i * 8u; };
+    if (tid == 0) {
+        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i == PREADY ? 8u : i < KFREE || (i >= VFULL && i < VFREE) ? kProducers : 1u);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) { tc_alloc(smem_u32(&tmem_s), 512); tc_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Only now may the next kernel's blocks come: one that waits for this grid while it holds tensor memory must not be in the way of an allocation here
+    asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
+    const uint32_t tmem = tmem_s;
+    const uint32_t split = blockIdx.x % sh.nsplit, tile = sh.tiles - 1u - blockIdx.x / sh.nsplit, g = blockIdx.y, b = blockIdx.z;          // the longest rows first
+    const uint32_t rep = a.H / a.G, rows = a.T * rep, r0 = tile * kTile, last = min(rows, r0 + kTile) - 1u;
+    const int len = seq_len(a, b), first_pos = len - (int)a.T + (int)(r0 / rep), last_pos = len - (int)a.T + (int)(last / rep);
+    uint32_t lo = 0, n = 0;
+    if (last_pos >= 0) {
+        const uint32_t first = (uint32_t)first_seen(max(first_pos, 0), a.window, a.block) / kTile, all = (uint32_t)last_pos / kTile + 1u - first;
+        lo = first + (uint32_t)((uint64_t)all * split / sh.nsplit);
+        n = first + (uint32_t)((uint64_t)all * (split + 1u) / sh.nsplit) - lo;
+    }
+
+    // queries as the row operand, each row times the power of two that brings its largest number to [1, 2); a piece's eight coordinates in the order 0 4 1 5 2 6 3 7
+    {
+        constexpr uint32_t pieces = 4u * NG, wide = NG == 1 ? 4u : NG == 2 ? 8u : 16u, per = 32u / wide;          // lanes to a row, rows to a warp
+        const uint32_t c = lane % wide;
+        for (uint32_t r = warp * per + lane / wide; r < (kTile + per - 1u) / per * per; r += kThreads / 32u * per) {
+            const uint32_t rr = r0 + r, t = rr / rep, h = g * rep + rr % rep;
+            float x[8] = {}, most = 0.0f;
+            if (r < kTile && rr <= last && c < pieces) {
+                const uint64_t at = b * a.q_batch + t * a.q_token + h * a.q_head + c * 8u;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[i] = a.type == T_F32 ? static_cast<const float *>(a.q)[at + i] : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at + i]);
+                    most = fmaxf(most, fabsf(x[i]));
+                }
+            }
+#pragma unroll
+            for (uint32_t o = wide / 2u; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int e = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126) : 0;
+            float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (a.scale < 0.0f) down = -down;          // the largest product is to be the largest score
+            if (r < kTile && c < pieces) {
+                const uint4 v = make_uint4(bits(__floats2half2_rn(x[0] * down, x[4] * down)), bits(__floats2half2_rn(x[1] * down, x[5] * down)), bits(__floats2half2_rn(x[2] * down, x[6] * down)),
+                                           bits(__floats2half2_rn(x[3] * down, x[7] * down)));
+                *reinterpret_cast<uint4 *>(base + op_byte(kTile, r, c)) = v;
+                if (c == 0) scale_s[r] = fabsf(a.scale) * __uint_as_float((uint32_t)(127 + e) << 23) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+            }
+        }
+        async_fence();
+        __syncthreads();
+    }
+
+    // tensor memory: scores (two buffers of 128 columns), where a tile's weights take the place of its scores (of 32 columns the first 16), and a tile's weighted values
+    constexpr uint32_t OCOL = 256;
+    if (warp == 0) {
+        if (lane == 0 && n) {
+            constexpr uint32_t id_s = (1u << 4) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24), id_o = (1u << 4) | ((D >> 3) << 17) | ((kTile >> 4) << 24);      // fp32 += f16 x f16
+            auto scores = [&](uint32_t i) {
+                const uint32_t s = i & 1u;
+                if (!mbar_wait(bar(KFULL + s), (i >> 1) & 1u)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < 2u * NG; k++) {
+                    const uint32_t off = (k >> 2) * kTile * 128u + (k & 3u) * 32u;
+                    tc_mma_ss(tmem + s * kTile, tc_desc(qs + off), tc_desc(ks + s * Z::qk + off), id_s, k > 0);
+                }
+                tc_commit(bar(KFREE + s)); tc_commit(bar(SFULL + s));
+                return true;
+            };
+            bool ok = scores(0) && (n < 2u || scores(1));
+            for (uint32_t i = 0; i < n && ok; i++) {
+                const uint32_t s = i & 1u;
+                ok = mbar_wait(bar(PREADY), s) && mbar_wait(bar(VFULL + s), (i >> 1) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < kTile / 16u; k++)
+                    tc_mma_ts(tmem + OCOL, tmem + s * kTile + (k >> 1) * 32u + (k & 1u) * 8u, tc_desc(vs + s * Z::v + (k >> 2) * D * 128u + (k & 3u) * 32u), id_o, k > 0);
+                tc_commit(bar(VFREE + s)); tc_commit(bar(OREADY));
+                if (i + 2u < n) ok = mbar_wait(bar(OREADY), s) && scores(i + 2u);          // they overwrite the weights that the products before read
+            }
+        }
+    } else if (warp <= kProducers) {
+        const uint32_t pw = warp - 1u, eight = lane >> 3, bv = lane & 7u;
+        const int32_t *table = a.table + (uint64_t)b * a.table_stride;
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t s = i & 1u, p = (lo + i) * kProducers + pw;
+            uint32_t page = 0xffffffffu;
+            if ((int)(p * kKv4Page) <= last_pos) page = (uint32_t)table[p];          // (a length is no more than the table's width allows)
+            const bool ok = page < a.n_pages;
+            const unsigned char *block = a.pool + (uint64_t)(ok ? page : 0u) * a.page_stride + (uint64_t)g * kv4_block_bytes(D);
+            uint32_t kw[4 * NG], kp[NG], vp[8][NG], vw[8][(NG + 1) / 2], odd = 0;
+            if (ok) {
+                take<16 * NG>(block + lane * 16u * NG, kw);
+                take<4 * NG>(block + 512u * NG + lane * 4u * NG, kp);
+                uint32_t own[NG];
+                take<4 * NG>(block + 1152u * NG + lane * 4u * NG, own);
+                bool bad = false;
+#pragma unroll
+                for (int j = 0; j < NG; j++) bad = bad || (own[j] & 0x7c00u) == 0x7c00u || (own[j] & 0x7c000000u) == 0x7c000000u;
+                odd = __ballot_sync(0xffffffffu, bad);
+#pragma unroll
+                for (uint32_t t = 0; t < 8; t++) {
+                    take<2 * NG>(block + 640u * NG + (eight * 8u + t) * 16u * NG + bv * 2u * NG, vw[t]);
+                    take<4 * NG>(block + 1152u * NG + (eight * 8u + t) * 4u * NG, vp[t]);
+                }
+                if (odd)          // values that are no number would spoil rows that do not see them
+#pragma unroll
+                    for (uint32_t t = 0; t < 8; t++) if (odd >> (eight * 8u + t) & 1u)
+#pragma unroll
+                        for (int j = 0; j < NG; j++) vp[t][j] = 0u;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NG; j++) kp[j] = 0u;
+#pragma unroll
+                for (int j = 0; j < 4 * NG; j++) kw[j] = 0u;
+#pragma unroll
+                for (uint32_t t = 0; t < 8; t++) {
+#pragma unroll
+                    for (int j = 0; j < NG; j++) vp[t][j] = 0u;
+#pragma unroll
+                    for (int j = 0; j < (NG + 1) / 2; j++) vw[t][j] = 0u;
+                }
+            }
+            if (lane == 0) { hide_s[i & 3u][pw] = ok ? 0u : 0xffffffffu; odd_s[i & 3u][pw] = odd; }
+            if (i >= 2u && !mbar_wait_warp(bar(KFREE + s), ((i >> 1) - 1u) & 1u)) break;
+            unsigned char *k_s = base + Z::qk + s * Z::qk, *v_s = base + 3u * Z::qk + s * Z::v;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const __half2 st = __low2half2(half2_of(kp[j])), mn = __high2half2(half2_of(kp[j]));
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t w = kw[q * NG + j];
+                    *reinterpret_cast<uint4 *>(k_s + op_byte(kTile, pw * 32u + lane, 4u * j + q)) =
+                        make_uint4(stand_for<false>(w, st, mn), stand_for<true>(w, st, mn), stand_for<false>(w >> 8, st, mn), stand_for<true>(w >> 8, st, mn));
+                }
+            }
+            async_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(KFULL + s));
+            if (i >= 2u && !mbar_wait_warp(bar(VFREE + s), ((i >> 1) - 1u) & 1u)) break;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                uint32_t y[4][4];          // [coordinate][pair of tokens]
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t w = __byte_perm(vw[2 * q][j / 2], vw[2 * q + 1][j / 2], (j & 1) ? 0x7632u : 0x5410u);
+                    const __half2 st = half2_of(__byte_perm(vp[2 * q][j], vp[2 * q + 1][j], 0x5410u)), mn = half2_of(__byte_perm(vp[2 * q][j], vp[2 * q + 1][j], 0x7632u));
+                    y[0][q] = stand_for<false>(w, st, mn); y[1][q] = stand_for<true>(w, st, mn); y[2][q] = stand_for<false>(w >> 8, st, mn); y[3][q] = stand_for<true>(w >> 8, st, mn);
+                }
+#pragma unroll
+                for (uint32_t d = 0; d < 4; d++) *reinterpret_cast<uint4 *>(v_s + op_byte(D, 32u * j + 4u * bv + d, pw * 4u + eight)) = make_uint4(y[d][0], y[d][1], y[d][2], y[d][3]);
+            }
+            async_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(VFULL + s));
+        }
+    } else {
+        const uint32_t quad = warp & 3u, r = quad * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep;
+        const int pos = len - (int)a.T + (int)t, low = first_seen(max(pos, 0), a.window, a.block), low_last = first_seen(max(last_pos, 0), a.window, a.block);
+        const uint32_t lane_base = (quad * 32u) << 16;
+        // a row belongs to two threads, of warps that reach the same lanes of tensor memory: each has 64 keys of a tile and half of the values.  They share the row's
+        // maximum once a tile (the barrier of their two warps, which also says whether both go on) and their sums at the end.
+        constexpr int VH = (int)D / 2, CH = VH % 32 == 0 ? 32 : 16;
+        const uint32_t half = (warp - 1u - kProducers) >> 2, c_lo = half * (kTile / 2u), v_lo = half * (uint32_t)VH;
+        const float kc = scale_s[r];
+        float m = -INFINITY, l = 0.0f, o[VH];
+#pragma unroll
+        for (int d = 0; d < VH; d++) o[d] = 0.0f;
+        bool ok = true;
+        // the values of the tile before join the sum, which then moves to the new reference
+        auto collect = [&](uint32_t i, float corr) {
+            ok = mbar_wait_warp(bar(OREADY), i & 1u);
+            if (!ok) return;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < VH; c += CH) {
+                uint32_t w[CH];
+                if constexpr (CH == 32) tc_ld32(tmem + lane_base + OCOL + v_lo + c, w); else tc_ld16(tmem + lane_base + OCOL + v_lo + c, w);
+#pragma unroll
+                for (int j = 0; j < CH; j++) o[c + j] = (o[c + j] + __uint_as_float(w[j])) * corr;
+            }
+        };
+        for (uint32_t i = 0; i < n; i++) {
+            const int key0 = (int)((lo + i) * kTile);
+            const uint32_t s_at = tmem + lane_base + (i & 1u) * kTile;
+            ok = ok && mbar_wait_warp(bar(SFULL + (i & 1u)), (i >> 1) & 1u);
+            tc_fence_after();
+            // the keys that this row sees of this thread's 64, two words
+            uint32_t sees[2] = {0xffffffffu, 0xffffffffu}, odd[2];
+            const uint32_t hide = hide_s[i & 3u][2u * half] | hide_s[i & 3u][2u * half + 1u];
+            odd[0] = odd_s[i & 3u][2u * half]; odd[1] = odd_s[i & 3u][2u * half + 1u];
+            const bool whole = key0 + (int)kTile - 1 <= first_pos && key0 >= low_last && hide == 0;          // every row of the block sees every key
+            if (!whole)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int at = key0 + (int)c_lo + 32 * u, from = low - at, to = pos - at;          // places [from, to]
+                    uint32_t w = to < 0 || from > 31 ? 0u : 0xffffffffu;
+                    if (to >= 0 && to < 31) w &= (2u << to) - 1u;
+                    if (from > 0 && from <= 31) w &= 0xffffffffu << from;
+                    sees[u] = w & ~hide_s[i & 3u][2u * half + u];
+                }
+            float top = -INFINITY;
+            if (ok)
+#pragma unroll 1
+            for (uint32_t u = 0; u < 2; u++) {
+                uint32_t w[32];
+                tc_ld32(s_at + c_lo + u * 32u, w);
+                if (whole) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(w[j]));
+                } else {
+                    const uint32_t see = u ? sees[1] : sees[0];
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j++) top = see >> j & 1u ? fmaxf(top, __uint_as_float(w[j])) : top;
+                }
+            }
+            top_s[i & 1u][half][r] = top;
+            if (bar_any(1u + quad, 64u, !ok)) { ok = false; break; }
+            top = fmaxf(top, top_s[i & 1u][half ^ 1u][r]);
+            if (top != -INFINITY) { top *= kc; if (a.softcap > 0.0f) top = a.softcap * kLog2e * tanh_any(top); }
+            const float next = top > m + kSlack ? top : m, corr = next == m ? 1.0f : ex2(m - next);          // (m = -inf: top is taken, if there is one)
+            if (i) collect(i - 1u, corr);
+            if (!ok) continue;          // both warps leave at the next barrier, or after the last tile
+            l *= corr;
+            m = next;
+            const float use = m == -INFINITY ? 0.0f : m - kLift;
+            float sum = 0.0f;
+#pragma unroll 1          // (a tile's whole code does not fit the instruction cache)
+            for (uint32_t u = 0; u < 2; u++) {
+                uint32_t w[32], wh[16];
+                tc_ld32(s_at + c_lo + u * 32u, w);
+                float p[32];
+                if (a.softcap > 0.0f) {
+                    float far = 0.0f;
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j++) { p[j] = __uint_as_float(w[j]) * kc; far = fmaxf(far, fabsf(p[j])); }
+                    if (__all_sync(0xffffffffu, far < 0.5f)) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 32; j++) p[j] = ex2(fmaf(a.softcap * kLog2e, tanh_near(p[j]), -use));
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 32; j++) p[j] = ex2(fmaf(a.softcap * kLog2e, tanh_any(p[j]), -use));
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j++) p[j] = ex2(fmaf(__uint_as_float(w[j]), kc, -use));
+                }
+                if (!whole) {
+                    const uint32_t see = u ? sees[1] : sees[0];
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j++) p[j] = see >> j & 1u ? p[j] : 0.0f;
+                }
+                float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t j = 0; j < 32; j++) s4[j & 3u] += p[j];
+                sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+#pragma unroll
+                for (uint32_t j = 0; j < 16; j++) wh[j] = bits(__floats2half2_rn(p[2 * j], p[2 * j + 1]));
+                tc_st16(s_at + c_lo + u * 32u, wh);
+            }
+            l += sum;
+            if ((odd[0] & sees[0]) | (odd[1] & sees[1])) l = NAN;          // values that are no number make the rows that see them NaN, however little they weigh
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(PREADY));
+        }
+        if (ok && n) collect(n - 1u, 1.0f);
+        sum_s[half][r] = l;
+        ok = !bar_any(1u + quad, 64u, !ok);
+        if (r0 + r <= last) {
+            const float ref = m - kLift, both = ok ? sum_s[0][r] + sum_s[1][r] : NAN;          // a wait that ran out shows as NaN
+            const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols + r;
+            const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, t, h, ref, both);
+#pragma unroll
+            for (int d = 0; d < VH; d += 4) {
+                if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + where * D + v_lo + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+                else store_four(a, b, t, h, v_lo + d, o[d] * k, o[d + 1] * k, o[d + 2] * k, o[d + 3] * k);
+            }
+            if (sh.nsplit > 1 && half == 0) reinterpret_cast<float2 *>(a.part + part_places(a, sh) * D)[where] = make_float2(ref, both);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tc_dealloc(tmem, 512);
+}
+
+template <int NG>
+cudaError_t launch_ng(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, bool pdl) {
+    static std::atomic<uint64_t> asked{0};          // devices (of the first 64) whose shared-memory limit has been raised
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev > 63 || !(asked.load(std::memory_order_acquire) >> dev & 1u))) {
+        e = smem_at_least(reinterpret_cast<const void *>(k_kv4_attn_tc<NG>), (int)Sizes<NG>::all);
+        if (e == cudaSuccess && dev <= 63) asked.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sh.nsplit * sh.tiles, a.G, a.B); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Sizes<NG>::all; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k_kv4_attn_tc<NG>, a, sh);
+}
+
+}  // namespace
+
+cudaError_t kv4_tc_launch(const Kv4Attn &a, uint32_t nsplit, uint32_t tiles, cudaStream_t stream, bool pdl) {
+    const Shape sh{nsplit, tiles, kKv4TcRows};
+    switch (a.D / 32u) {
+        case 1: return launch_ng<1>(a, sh, stream, pdl);
+        case 2: return launch_ng<2>(a, sh, stream, pdl);
+        case 3: return launch_ng<3>(a, sh, stream, pdl);
+        default: return launch_ng<4>(a, sh, stream, pdl);
+    }
+}
+
+}  // namespace nb
