@@ -1,7 +1,7 @@
 // kv4_tc.cu -- attention of long portions over a cache held in 4 bits, on the fifth-generation tensor cores (formulas: kv4.h).
 //
 // A block owns 128 rows (query token, query head) of one key/value head and walks its keys in tiles of 128, four pages.  Four warps make a tile's operands from the
-// codes, a page each: a word of eight key codes is one 16-byte piece of a row of the swizzled key operand (the queries are laid out in the nibbles' order, so that nothing is
+// codes, by the page: a word of eight key codes is one 16-byte piece of a row of the swizzled key operand (the queries are laid out in the nibbles' order, so that nothing is
 // shuffled), eight tokens' codes of a coordinate one piece of a row of the value operand, both as c s + m in fp16, rounded once.  One thread issues tcgen05.mma: scores
 // into tensor memory, two buffers, and weights (fp16, back in tensor memory where the scores were) times values.  Eight warps do the softmax, two threads to a row with
 // 64 keys of a tile and half of the values each, as one chain over the row's lanes.  Everything is double buffered: a tile's operands are made, and its
@@ -13,12 +13,13 @@
 
 #include "family.h"
 #include "kv4.cuh"
+#include "pairs.cuh"
 #include "tc_ptx.cuh"
 
 namespace nb {
 namespace {
 
-constexpr uint32_t kTile = 128, kThreads = 416, kProducers = 4;
+constexpr uint32_t kTile = 128, kPages = kTile / kKv4Page, kThreads = 512, kSoftWarps = 8, kMmaWarp = 8, kProducers = 7;          // warps: 0-7, 8, 9-15
 constexpr float kLift = 12.0f;
 // byte of the 16-byte piece c8 (8 fp16) of row r in an operand of 64-wide blocks of `rows` rows, 128-byte swizzle
 __device__ __forceinline__ uint32_t op_byte(uint32_t rows, uint32_t r, uint32_t c8) { return (c8 >> 3) * rows * 128u + r * 128u + (((c8 & 7u) ^ (r & 7u)) << 4); }
@@ -29,6 +30,13 @@ template <int NG> struct Sizes {
     static constexpr uint32_t qk = kTile * DP * 2u, v = kTile * D * 2u, all = 3u * qk + 2u * v + 1024u;
 };
 
+// tanh_near of two numbers
+__device__ __forceinline__ pair_t tanh_near2(pair_t x) {
+    auto both = [](float c) { return pair(c, c); };
+    const pair_t y = mul2(x, x);
+    return fma2(mul2(x, y), fma2(y, fma2(y, fma2(y, fma2(y, both(-1382.0f / 155925.0f), both(62.0f / 2835.0f)), both(-17.0f / 315.0f)), both(2.0f / 15.0f)), both(-1.0f / 3.0f)), x);
+}
+
 // grid (nsplit x tiles, G, B)
 template <int NG>
 __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, const Shape sh) {
@@ -38,7 +46,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     enum { KFULL = 0, KFREE = 2, VFULL = 4, VFREE = 6, SFULL = 8, PREADY = 10, OREADY, NBAR };          // (pairs: one for each buffer)
     __shared__ __align__(8) uint64_t bars[NBAR];
     __shared__ uint32_t tmem_s;
-    __shared__ uint32_t hide_s[4][kProducers], odd_s[4][kProducers];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys or values that are no number
+    __shared__ uint32_t hide_s[4][kPages], odd_s[4][kPages];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys or values that are no number
     __shared__ float scale_s[kTile], top_s[2][2][kTile], sum_s[2][kTile];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t qs = (smem_u32(tc_raw) + 1023u) & ~1023u, ks = qs + Z::qk, vs = ks + 2u * Z::qk;
@@ -46,10 +54,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     const uint32_t b0 = smem_u32(bars);
     auto bar = [&](uint32_t i) { return b0 + i * 8u; };
     if (tid == 0) {
-        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i == PREADY ? 8u : i < KFREE || (i >= VFULL && i < VFREE) ? kProducers : 1u);
+        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i == PREADY ? 8u : i < KFREE || (i >= VFULL && i < VFREE) ? kPages : 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) { tc_alloc(smem_u32(&tmem_s), 512); tc_relinquish(); }
+    if (warp == kMmaWarp) { tc_alloc(smem_u32(&tmem_s), 512); tc_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -99,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
 
     // tensor memory: scores (two buffers of 128 columns), where a tile's weights take the place of its scores (of 32 columns the first 16), and a tile's weighted values
     constexpr uint32_t OCOL = 256;
-    if (warp == 0) {
+    if (warp == kMmaWarp) {
         if (lane == 0 && n) {
             constexpr uint32_t id_s = (1u << 4) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24), id_o = (1u << 4) | ((D >> 3) << 17) | ((kTile >> 4) << 24);      // fp32 += f16 x f16
             auto scores = [&](uint32_t i) {
@@ -127,80 +135,98 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
                 if (i + 2u < n) ok = mbar_wait(bar(OREADY), s) && scores(i + 2u);          // they overwrite the weights that the products before read
             }
         }
-    } else if (warp <= kProducers) {
-        const uint32_t pw = warp - 1u, eight = lane >> 3, bv = lane & 7u;
+    } else if (warp > kMmaWarp) {
+        // operands: a tile is eight pieces of work, the keys and then the values of its four pages, dealt out to seven warps in turn
+        const uint32_t eight = lane >> 3, bv = lane & 7u;
         const int32_t *table = a.table + (uint64_t)b * a.table_stride;
-        for (uint32_t i = 0; i < n; i++) {
-            const uint32_t s = i & 1u, p = (lo + i) * kProducers + pw;
-            uint32_t page = 0xffffffffu;
-            if ((int)(p * kKv4Page) <= last_pos) page = (uint32_t)table[p];          // (a length is no more than the table's width allows)
+        auto number = [&](uint32_t q) {          // the page of piece q (a length is no more than the table's width allows)
+            const uint32_t p = (lo + q / (2u * kPages)) * kPages + q % kPages;
+            return q < n * 2u * kPages && (int)(p * kKv4Page) <= last_pos ? (uint32_t)table[p] : 0xffffffffu;
+        };
+        uint32_t page = number(warp - kMmaWarp - 1u);
+        for (uint32_t q = warp - kMmaWarp - 1u; q < n * 2u * kPages; q += kProducers) {
+            const uint32_t i = q / (2u * kPages), s = i & 1u, pw = q % kPages, next = number(q + kProducers);
             const bool ok = page < a.n_pages;
             const unsigned char *block = a.pool + (uint64_t)(ok ? page : 0u) * a.page_stride + (uint64_t)g * kv4_block_bytes(D);
-            uint32_t kw[4 * NG], kp[NG], vp[8][NG], vw[8][(NG + 1) / 2], odd = 0;
-            if (ok) {
-                take<16 * NG>(block + lane * 16u * NG, kw);
-                take<4 * NG>(block + 512u * NG + lane * 4u * NG, kp);
-                uint32_t own[NG];
-                take<4 * NG>(block + 1152u * NG + lane * 4u * NG, own);
-                bool bad = false;
+            if (q % (2u * kPages) < kPages) {
+                uint32_t kw[4 * NG], kp[NG], odd = 0;          // odd: tokens whose values are no numbers
+                if (ok) {
+                    uint32_t own[NG];
+                    take<16 * NG>(block + lane * 16u * NG, kw);
+                    take<4 * NG>(block + 512u * NG + lane * 4u * NG, kp);
+                    take<4 * NG>(block + 1152u * NG + lane * 4u * NG, own);
+                    __half2 none = __float2half2_rn(0.0f);          // 0 times a pair is 0, or NaN
 #pragma unroll
-                for (int j = 0; j < NG; j++) bad = bad || (own[j] & 0x7c00u) == 0x7c00u || (own[j] & 0x7c000000u) == 0x7c000000u;
-                odd = __ballot_sync(0xffffffffu, bad);
+                    for (int j = 0; j < NG; j++) none = __hfma2(half2_of(own[j]), __float2half2_rn(0.0f), none);
+                    odd = __ballot_sync(0xffffffffu, !__hbeq2(none, __float2half2_rn(0.0f)));
+                } else {
 #pragma unroll
-                for (uint32_t t = 0; t < 8; t++) {
-                    take<2 * NG>(block + 640u * NG + (eight * 8u + t) * 16u * NG + bv * 2u * NG, vw[t]);
-                    take<4 * NG>(block + 1152u * NG + (eight * 8u + t) * 4u * NG, vp[t]);
+                    for (int j = 0; j < NG; j++) kp[j] = 0u;
+#pragma unroll
+                    for (int j = 0; j < 4 * NG; j++) kw[j] = 0u;
                 }
-                if (odd)          // values that are no number would spoil rows that do not see them
+                if (i >= 2u && !mbar_wait_warp(bar(KFREE + s), ((i >> 1) - 1u) & 1u)) break;
+                unsigned char *k_s = base + Z::qk + s * Z::qk;
 #pragma unroll
-                    for (uint32_t t = 0; t < 8; t++) if (odd >> (eight * 8u + t) & 1u)
+                for (int j = 0; j < NG; j++) {
+                    const __half2 st = __low2half2(half2_of(kp[j])), mn = __high2half2(half2_of(kp[j]));
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const uint32_t w = kw[x * NG + j];
+                        *reinterpret_cast<uint4 *>(k_s + op_byte(kTile, pw * 32u + lane, 4u * j + x)) =
+                            make_uint4(stand_for<false>(w, st, mn), stand_for<true>(w, st, mn), stand_for<false>(w >> 8, st, mn), stand_for<true>(w >> 8, st, mn));
+                    }
+                }
+                if (lane == 0) { hide_s[i & 3u][pw] = ok ? 0u : 0xffffffffu; odd_s[i & 3u][pw] = odd; }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(KFULL + s));
+            } else {
+                uint32_t vp[8][NG], vw[8][(NG + 1) / 2];
+                if (ok) {
+#pragma unroll
+                    for (uint32_t t = 0; t < 8; t++) {
+                        take<2 * NG>(block + 640u * NG + (eight * 8u + t) * 16u * NG + bv * 2u * NG, vw[t]);
+                        take<4 * NG>(block + 1152u * NG + (eight * 8u + t) * 4u * NG, vp[t]);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t t = 0; t < 8; t++) {
 #pragma unroll
                         for (int j = 0; j < NG; j++) vp[t][j] = 0u;
-            } else {
 #pragma unroll
-                for (int j = 0; j < NG; j++) kp[j] = 0u;
-#pragma unroll
-                for (int j = 0; j < 4 * NG; j++) kw[j] = 0u;
+                        for (int j = 0; j < (NG + 1) / 2; j++) vw[t][j] = 0u;
+                    }
+                }
+                // tokens whose pairs are no numbers would spoil rows that do not see them
 #pragma unroll
                 for (uint32_t t = 0; t < 8; t++) {
+                    __half2 none = __float2half2_rn(0.0f);
 #pragma unroll
-                    for (int j = 0; j < NG; j++) vp[t][j] = 0u;
+                    for (int j = 0; j < NG; j++) none = __hfma2(half2_of(vp[t][j]), __float2half2_rn(0.0f), none);
+                    if (!__hbeq2(none, __float2half2_rn(0.0f)))
 #pragma unroll
-                    for (int j = 0; j < (NG + 1) / 2; j++) vw[t][j] = 0u;
+                        for (int j = 0; j < NG; j++) vp[t][j] = 0u;
                 }
-            }
-            if (lane == 0) { hide_s[i & 3u][pw] = ok ? 0u : 0xffffffffu; odd_s[i & 3u][pw] = odd; }
-            if (i >= 2u && !mbar_wait_warp(bar(KFREE + s), ((i >> 1) - 1u) & 1u)) break;
-            unsigned char *k_s = base + Z::qk + s * Z::qk, *v_s = base + 3u * Z::qk + s * Z::v;
+                if (i >= 2u && !mbar_wait_warp(bar(VFREE + s), ((i >> 1) - 1u) & 1u)) break;
+                unsigned char *v_s = base + 3u * Z::qk + s * Z::v;
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const __half2 st = __low2half2(half2_of(kp[j])), mn = __high2half2(half2_of(kp[j]));
+                for (int j = 0; j < NG; j++) {
+                    uint32_t y[4][4];          // [coordinate][pair of tokens]
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint32_t w = kw[q * NG + j];
-                    *reinterpret_cast<uint4 *>(k_s + op_byte(kTile, pw * 32u + lane, 4u * j + q)) =
-                        make_uint4(stand_for<false>(w, st, mn), stand_for<true>(w, st, mn), stand_for<false>(w >> 8, st, mn), stand_for<true>(w >> 8, st, mn));
+                    for (int x = 0; x < 4; x++) {
+                        const uint32_t w = __byte_perm(vw[2 * x][j / 2], vw[2 * x + 1][j / 2], (j & 1) ? 0x7632u : 0x5410u);
+                        const __half2 st = half2_of(__byte_perm(vp[2 * x][j], vp[2 * x + 1][j], 0x5410u)), mn = half2_of(__byte_perm(vp[2 * x][j], vp[2 * x + 1][j], 0x7632u));
+                        y[0][x] = stand_for<false>(w, st, mn); y[1][x] = stand_for<true>(w, st, mn); y[2][x] = stand_for<false>(w >> 8, st, mn); y[3][x] = stand_for<true>(w >> 8, st, mn);
+                    }
+#pragma unroll
+                    for (uint32_t d = 0; d < 4; d++) *reinterpret_cast<uint4 *>(v_s + op_byte(D, 32u * j + 4u * bv + d, pw * 4u + eight)) = make_uint4(y[d][0], y[d][1], y[d][2], y[d][3]);
                 }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(VFULL + s));
             }
-            async_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(KFULL + s));
-            if (i >= 2u && !mbar_wait_warp(bar(VFREE + s), ((i >> 1) - 1u) & 1u)) break;
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                uint32_t y[4][4];          // [coordinate][pair of tokens]
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint32_t w = __byte_perm(vw[2 * q][j / 2], vw[2 * q + 1][j / 2], (j & 1) ? 0x7632u : 0x5410u);
-                    const __half2 st = half2_of(__byte_perm(vp[2 * q][j], vp[2 * q + 1][j], 0x5410u)), mn = half2_of(__byte_perm(vp[2 * q][j], vp[2 * q + 1][j], 0x7632u));
-                    y[0][q] = stand_for<false>(w, st, mn); y[1][q] = stand_for<true>(w, st, mn); y[2][q] = stand_for<false>(w >> 8, st, mn); y[3][q] = stand_for<true>(w >> 8, st, mn);
-                }
-#pragma unroll
-                for (uint32_t d = 0; d < 4; d++) *reinterpret_cast<uint4 *>(v_s + op_byte(D, 32u * j + 4u * bv + d, pw * 4u + eight)) = make_uint4(y[d][0], y[d][1], y[d][2], y[d][3]);
-            }
-            async_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(VFULL + s));
+            page = next;
         }
     } else {
         const uint32_t quad = warp & 3u, r = quad * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep;
@@ -209,11 +235,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
         // a row belongs to two threads, of warps that reach the same lanes of tensor memory: each has 64 keys of a tile and half of the values.  They share the row's
         // maximum once a tile (the barrier of their two warps, which also says whether both go on) and their sums at the end.
         constexpr int VH = (int)D / 2, CH = VH % 32 == 0 ? 32 : 16;
-        const uint32_t half = (warp - 1u - kProducers) >> 2, c_lo = half * (kTile / 2u), v_lo = half * (uint32_t)VH;
+        const uint32_t half = warp >> 2, c_lo = half * (kTile / 2u), v_lo = half * (uint32_t)VH;
         const float kc = scale_s[r];
-        float m = -INFINITY, l = 0.0f, o[VH];
+        float m = -INFINITY, l = 0.0f;
+        pair_t o[VH / 2];
 #pragma unroll
-        for (int d = 0; d < VH; d++) o[d] = 0.0f;
+        for (int d = 0; d < VH / 2; d++) o[d] = pair(0.0f, 0.0f);
         bool ok = true;
         // the values of the tile before join the sum, which then moves to the new reference
         auto collect = [&](uint32_t i, float corr) {
@@ -224,8 +251,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             for (int c = 0; c < VH; c += CH) {
                 uint32_t w[CH];
                 if constexpr (CH == 32) tc_ld32(tmem + lane_base + OCOL + v_lo + c, w); else tc_ld16(tmem + lane_base + OCOL + v_lo + c, w);
+                const pair_t k = pair(corr, corr);
 #pragma unroll
-                for (int j = 0; j < CH; j++) o[c + j] = (o[c + j] + __uint_as_float(w[j])) * corr;
+                for (int j = 0; j < CH / 2; j++) o[c / 2 + j] = add2(o[c / 2 + j], pair(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1])));
+                if (!__all_sync(0xffffffffu, corr == 1.0f))
+#pragma unroll
+                    for (int j = 0; j < CH / 2; j++) o[c / 2 + j] = mul2(o[c / 2 + j], k);
             }
         };
         for (uint32_t i = 0; i < n; i++) {
@@ -253,14 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             for (uint32_t u = 0; u < 2; u++) {
                 uint32_t w[32];
                 tc_ld32(s_at + c_lo + u * 32u, w);
-                if (whole) {
-#pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(w[j]));
-                } else {
+                if (!whole) {
                     const uint32_t see = u ? sees[1] : sees[0];
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) top = see >> j & 1u ? fmaxf(top, __uint_as_float(w[j])) : top;
+                    for (uint32_t j = 0; j < 32; j++) w[j] = see >> j & 1u ? w[j] : 0xff800000u;
                 }
+#pragma unroll
+                for (uint32_t j = 0; j < 32; j += 2) top = max3(top, __uint_as_float(w[j]), __uint_as_float(w[j + 1]));
             }
             top_s[i & 1u][half][r] = top;
             if (bar_any(1u + quad, 64u, !ok)) { ok = false; break; }
@@ -277,33 +307,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             for (uint32_t u = 0; u < 2; u++) {
                 uint32_t w[32], wh[16];
                 tc_ld32(s_at + c_lo + u * 32u, w);
-                float p[32];
-                if (a.softcap > 0.0f) {
-                    float far = 0.0f;
-#pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) { p[j] = __uint_as_float(w[j]) * kc; far = fmaxf(far, fabsf(p[j])); }
-                    if (__all_sync(0xffffffffu, far < 0.5f)) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 32; j++) p[j] = ex2(fmaf(a.softcap * kLog2e, tanh_near(p[j]), -use));
-                    } else {
-#pragma unroll
-                        for (uint32_t j = 0; j < 32; j++) p[j] = ex2(fmaf(a.softcap * kLog2e, tanh_any(p[j]), -use));
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) p[j] = ex2(fmaf(__uint_as_float(w[j]), kc, -use));
-                }
                 if (!whole) {
                     const uint32_t see = u ? sees[1] : sees[0];
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) p[j] = see >> j & 1u ? p[j] : 0.0f;
+                    for (uint32_t j = 0; j < 32; j++) w[j] = see >> j & 1u ? w[j] : 0xff800000u;
                 }
-                float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (a.softcap > 0.0f) {
+                    const pair_t k = pair(kc, kc), cap = pair(a.softcap * kLog2e, a.softcap * kLog2e);
+                    float far = 0.0f;
 #pragma unroll
-                for (uint32_t j = 0; j < 32; j++) s4[j & 3u] += p[j];
-                sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    for (uint32_t j = 0; j < 32; j += 2) far = max3(far, fabsf(__uint_as_float(w[j])), fabsf(__uint_as_float(w[j + 1])));
+                    if (__all_sync(0xffffffffu, far * kc < 0.5f)) {
 #pragma unroll
-                for (uint32_t j = 0; j < 16; j++) wh[j] = bits(__floats2half2_rn(p[2 * j], p[2 * j + 1]));
+                        for (uint32_t j = 0; j < 32; j += 2) {
+                            float x, y;
+                            unpair(mul2(cap, tanh_near2(mul2(pair(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), k))), x, y);
+                            w[j] = __float_as_uint(x); w[j + 1] = __float_as_uint(y);
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 32; j++) w[j] = w[j] == 0xff800000u ? w[j] : __float_as_uint(a.softcap * kLog2e * tanh_any(__uint_as_float(w[j]) * kc));
+                    }
+                }
+                // (masked scores are -inf, whatever the factor: 0 times -inf would be no number)
+                const float by = a.softcap > 0.0f ? 1.0f : whole ? kc : fmaxf(kc, 1e-30f);
+                const pair_t k = pair(by, by), less = pair(-use, -use);
+                pair_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+#pragma unroll
+                for (uint32_t j = 0; j < 16; j++) {
+                    float x, y;
+                    unpair(fma2(pair(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1])), k, less), x, y);
+                    x = ex2(x); y = ex2(y);
+                    s2[j & 1u] = add2(s2[j & 1u], pair(x, y));
+                    wh[j] = bits(__floats2half2_rn(x, y));
+                }
+                float s0, s1;
+                unpair(add2(s2[0], s2[1]), s0, s1);
+                sum += s0 + s1;
                 tc_st16(s_at + c_lo + u * 32u, wh);
             }
             l += sum;
@@ -322,8 +362,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, t, h, ref, both);
 #pragma unroll
             for (int d = 0; d < VH; d += 4) {
-                if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + where * D + v_lo + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-                else store_four(a, b, t, h, v_lo + d, o[d] * k, o[d + 1] * k, o[d + 2] * k, o[d + 3] * k);
+                float4 v;
+                unpair(o[d / 2], v.x, v.y); unpair(o[d / 2 + 1], v.z, v.w);
+                if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + where * D + v_lo + d) = v;
+                else store_four(a, b, t, h, v_lo + d, v.x * k, v.y * k, v.z * k, v.w * k);
             }
             if (sh.nsplit > 1 && half == 0) reinterpret_cast<float2 *>(a.part + part_places(a, sh) * D)[where] = make_float2(ref, both);
         }
@@ -331,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) tc_dealloc(tmem, 512);
+    if (warp == kMmaWarp) tc_dealloc(tmem, 512);
 }
 
 template <int NG>

@@ -10,6 +10,7 @@
 
 #include "family.h"
 #include "ops.h"
+#include "pairs.cuh"
 
 namespace nb {
 namespace {
@@ -126,14 +127,6 @@ __device__ __forceinline__ Sums join(const Sums &a, const Sums &b) {
 __device__ __forceinline__ Sums shfl(const Sums &a, int step) {
     return Sums{__shfl_xor_sync(0xffffffffu, a.m, step), __shfl_xor_sync(0xffffffffu, a.z, step), __shfl_xor_sync(0xffffffffu, a.s, step)};
 }
-
-// two fp32 numbers at once
-typedef unsigned long long pair_t;
-__device__ __forceinline__ pair_t pair(float a, float b) { pair_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ void unpair(pair_t p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
-__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) { pair_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
-__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) { pair_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 // What a thread has seen: m, and z, s in units of 2^u, u = m log2 e as it was rounded while m is small (d = x log2 e - u is then one multiply-add), and exact where m is
 // not (m - x first: nothing overflows, and the rounding of a large product does not count)
