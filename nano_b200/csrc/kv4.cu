@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT)) k_kv4_attn(const K
                 for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int x = 0; x < 4; x++) { s[k][t][x] *= f[t][x & 1]; top[0] = fmaxf(top[0], fabsf(s[k][t][x])); }
-                const bool near = __all_sync(0xffffffffu, top[0] < 0.5f);          // (a NaN goes through either)
+                const bool near = __all_sync(0xffffffffu, top[0] < kTanhNear);          // (a NaN goes through either)
                 top[0] = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < 2; k++)
@@ -650,8 +650,8 @@ size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32
     return p.sh.nsplit == 1 ? 0 : (size_t)B * G * p.sh.tiles * p.sh.nsplit * p.sh.cols * (D + 2u) * 4u;
 }
 
-// (keys are split only while blocks times splits stay within kWaves times the four that an SM holds)
-size_t kv4_attn_workspace_most(uint32_t B, uint32_t G, uint32_t D, uint32_t sms) { return (size_t)std::max(B * G, kWaves * 4u * sms) * kKv4TcRows * (D + 2u) * 4u; }
+// (keys are split only while blocks times splits stay within the waves of what the device holds at once: one block of 128 rows to an SM, or four of at most 64)
+size_t kv4_attn_workspace_most(uint32_t B, uint32_t D, uint32_t sms) { return (size_t)(B > 1 ? kWaves : 1u) * sms * 256u * (D + 2u) * 4u; }
 
 cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, uint32_t *launches) {
     const Plan p = plan_for(a.B, a.T, a.H, a.G, a.D, a.width, a.window, a.block, sms);

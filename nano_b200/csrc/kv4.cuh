@@ -48,10 +48,11 @@ __device__ __forceinline__ void take(const unsigned char *p, uint32_t (&w)[(BYTE
     }
 }
 
-// tanh for the soft cap: its series where |x| < 1/2 (off by at most 21844/6081075 x^13 = 4.4e-7), where the special function unit would be the bound; else 1 - 2 / (1 + e^2x)
+// tanh for the soft cap: its series where |x| < kTanhNear (off by at most 1382/155925 x^11 = 8.6e-8), where the special function unit would be the bound; else 1 - 2 / (1 + e^2x)
+constexpr float kTanhNear = 0.35f;
 __device__ __forceinline__ float tanh_near(float x) {
     const float y = x * x;
-    return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1382.0f / 155925.0f, 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
+    return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
 }
 __device__ __forceinline__ float tanh_any(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * x)); }
 

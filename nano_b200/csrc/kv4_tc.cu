@@ -1,13 +1,13 @@
 // kv4_tc.cu -- attention of long portions over a cache held in 4 bits, on the fifth-generation tensor cores (formulas: kv4.h).
 //
-// A block owns 128 rows (query token, query head) of one key/value head and walks its keys in tiles of 128, four pages.  Four warps make a tile's operands from the
-// codes, by the page: a word of eight key codes is one 16-byte piece of a row of the swizzled key operand (the queries are laid out in the nibbles' order, so that nothing is
-// shuffled), eight tokens' codes of a coordinate one piece of a row of the value operand, both as c s + m in fp16, rounded once.  One thread issues tcgen05.mma: scores
-// into tensor memory, two buffers, and weights (fp16, back in tensor memory where the scores were) times values.  Eight warps do the softmax, two threads to a row with
-// 64 keys of a tile and half of the values each, as one chain over the row's lanes.  Everything is double buffered: a tile's operands are made, and its
-// scores multiplied, under the softmax of the tile before.
+// A block owns 128 rows (query token, query head) of one key/value head and walks their keys in tiles of 128, four pages.  Seven warps make a tile's operands from the codes,
+// by the page: a word of eight key codes is one 16-byte piece of a row of the swizzled key operand (the queries are laid out in the nibbles' order, so that nothing is
+// shuffled), eight tokens' codes of a coordinate one piece of a row of the value operand, both as c s + m in fp16, rounded once; two tiles' operands have room.  One thread
+// issues tcgen05.mma -- scores into tensor memory, two buffers, and weights (fp16, where the scores were) times values onto the running sum there -- and four warps do the
+// softmax, a thread to a row, which holds its 128 scores in registers; their exponentials are the bound (1024 cycles a tile).
 // Every wait has a limit; a block in which one runs out leaves with NaN in its rows (nothing but its own products is ever in flight).
-// Softmax as in k_kv4_attn: log2 units, weights times 2^kLift, a reference that is renewed when it lags kSlack behind the maximum.
+// Softmax as in k_kv4_attn: log2 units, weights times 2^kLift, a reference that is renewed when it lags kSlack behind the maximum, so that the sums in tensor memory
+// are seldom touched.
 #include <algorithm>
 #include <atomic>
 
@@ -19,7 +19,7 @@
 namespace nb {
 namespace {
 
-constexpr uint32_t kTile = 128, kPages = kTile / kKv4Page, kThreads = 512, kSoftWarps = 8, kMmaWarp = 8, kProducers = 7;          // warps: 0-7, 8, 9-15
+constexpr uint32_t kTile = 128, kPages = kTile / kKv4Page, kThreads = 384, kMmaWarp = 4, kMakers = 5, kProducers = 7;          // warps 0-3: softmax, 4: products, 5-11: operands
 constexpr float kLift = 12.0f;
 // byte of the 16-byte piece c8 (8 fp16) of row r in an operand of 64-wide blocks of `rows` rows, 128-byte swizzle
 __device__ __forceinline__ uint32_t op_byte(uint32_t rows, uint32_t r, uint32_t c8) { return (c8 >> 3) * rows * 128u + r * 128u + (((c8 & 7u) ^ (r & 7u)) << 4); }
@@ -34,7 +34,7 @@ template <int NG> struct Sizes {
 __device__ __forceinline__ pair_t tanh_near2(pair_t x) {
     auto both = [](float c) { return pair(c, c); };
     const pair_t y = mul2(x, x);
-    return fma2(mul2(x, y), fma2(y, fma2(y, fma2(y, fma2(y, both(-1382.0f / 155925.0f), both(62.0f / 2835.0f)), both(-17.0f / 315.0f)), both(2.0f / 15.0f)), both(-1.0f / 3.0f)), x);
+    return fma2(mul2(x, y), fma2(y, fma2(y, fma2(y, both(62.0f / 2835.0f), both(-17.0f / 315.0f)), both(2.0f / 15.0f)), both(-1.0f / 3.0f)), x);
 }
 
 // grid (nsplit x tiles, G, B)
@@ -43,18 +43,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     using Z = Sizes<NG>;
     constexpr uint32_t D = Z::D;
     extern __shared__ uint8_t tc_raw[];
-    enum { KFULL = 0, KFREE = 2, VFULL = 4, VFREE = 6, SFULL = 8, PREADY = 10, OREADY, NBAR };          // (pairs: one for each buffer)
+    enum { KFULL = 0, KFREE = 2, VFULL = 4, VFREE = 6, SFULL = 8, PREADY = 10, ODONE = 12, NBAR };          // (two each but the last: one for a buffer.  PREADY too: a warp may be a tile ahead of the others)
     __shared__ __align__(8) uint64_t bars[NBAR];
     __shared__ uint32_t tmem_s;
-    __shared__ uint32_t hide_s[4][kPages], odd_s[4][kPages];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys or values that are no number
-    __shared__ float scale_s[kTile], top_s[2][2][kTile], sum_s[2][kTile];
+    __shared__ uint32_t hide_s[4][kPages], odd_s[4][kPages];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys whose values are no number
+    __shared__ float scale_s[kTile];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t qs = (smem_u32(tc_raw) + 1023u) & ~1023u, ks = qs + Z::qk, vs = ks + 2u * Z::qk;
     unsigned char *base = tc_raw + (qs - smem_u32(tc_raw));
+    const uint32_t split = blockIdx.x % sh.nsplit, tile = sh.tiles - 1u - blockIdx.x / sh.nsplit, g = blockIdx.y, b = blockIdx.z;          // the longest rows first
+    const uint32_t rep = a.H / a.G, rows = a.T * rep, r0 = tile * kKv4TcRows, last = min(rows, r0 + kKv4TcRows) - 1u;
     const uint32_t b0 = smem_u32(bars);
     auto bar = [&](uint32_t i) { return b0 + i * 8u; };
     if (tid == 0) {
-        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i == PREADY ? 8u : i < KFREE || (i >= VFULL && i < VFREE) ? kPages : 1u);
+        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i < KFREE || (i >= VFULL && i < VFREE) ? kPages : i >= PREADY && i < ODONE ? 4u : 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) { tc_alloc(smem_u32(&tmem_s), 512); tc_relinquish(); }
@@ -64,9 +66,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     // Only now may the next kernel's blocks come: one that waits for this grid while it holds tensor memory must not be in the way of an allocation here
     asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
     const uint32_t tmem = tmem_s;
-    const uint32_t split = blockIdx.x % sh.nsplit, tile = sh.tiles - 1u - blockIdx.x / sh.nsplit, g = blockIdx.y, b = blockIdx.z;          // the longest rows first
-    const uint32_t rep = a.H / a.G, rows = a.T * rep, r0 = tile * kTile, last = min(rows, r0 + kTile) - 1u;
-    const int len = seq_len(a, b), first_pos = len - (int)a.T + (int)(r0 / rep), last_pos = len - (int)a.T + (int)(last / rep);
+    const int len = seq_len(a, b), pos_0 = len - (int)a.T;          // position of the first query
+    const int first_pos = pos_0 + (int)(r0 / rep), last_pos = pos_0 + (int)(last / rep);
     uint32_t lo = 0, n = 0;
     if (last_pos >= 0) {
         const uint32_t first = (uint32_t)first_seen(max(first_pos, 0), a.window, a.block) / kTile, all = (uint32_t)last_pos / kTile + 1u - first;
@@ -78,10 +79,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     {
         constexpr uint32_t pieces = 4u * NG, wide = NG == 1 ? 4u : NG == 2 ? 8u : 16u, per = 32u / wide;          // lanes to a row, rows to a warp
         const uint32_t c = lane % wide;
-        for (uint32_t r = warp * per + lane / wide; r < (kTile + per - 1u) / per * per; r += kThreads / 32u * per) {
+        for (uint32_t r = warp * per + lane / wide; r < kTile; r += kThreads / 32u * per) {
             const uint32_t rr = r0 + r, t = rr / rep, h = g * rep + rr % rep;
             float x[8] = {}, most = 0.0f;
-            if (r < kTile && rr <= last && c < pieces) {
+            if (rr <= last && c < pieces) {
                 const uint64_t at = b * a.q_batch + t * a.q_token + h * a.q_head + c * 8u;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             const int e = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126) : 0;
             float down = __uint_as_float((uint32_t)(127 - e) << 23);
             if (a.scale < 0.0f) down = -down;          // the largest product is to be the largest score
-            if (r < kTile && c < pieces) {
+            if (c < pieces) {
                 const uint4 v = make_uint4(bits(__floats2half2_rn(x[0] * down, x[4] * down)), bits(__floats2half2_rn(x[1] * down, x[5] * down)), bits(__floats2half2_rn(x[2] * down, x[6] * down)),
                                            bits(__floats2half2_rn(x[3] * down, x[7] * down)));
                 *reinterpret_cast<uint4 *>(base + op_byte(kTile, r, c)) = v;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
         __syncthreads();
     }
 
-    // tensor memory: scores (two buffers of 128 columns), where a tile's weights take the place of its scores (of 32 columns the first 16), and a tile's weighted values
+    // tensor memory: scores (two buffers of 128 columns), where a tile's weights take the place of its scores (64 columns), and the sums
     constexpr uint32_t OCOL = 256;
     if (warp == kMmaWarp) {
         if (lane == 0 && n) {
@@ -125,17 +126,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             bool ok = scores(0) && (n < 2u || scores(1));
             for (uint32_t i = 0; i < n && ok; i++) {
                 const uint32_t s = i & 1u;
-                ok = mbar_wait(bar(PREADY), s) && mbar_wait(bar(VFULL + s), (i >> 1) & 1u);
+                ok = mbar_wait(bar(VFULL + s), (i >> 1) & 1u) && mbar_wait(bar(PREADY + s), (i >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < kTile / 16u; k++)
-                    tc_mma_ts(tmem + OCOL, tmem + s * kTile + (k >> 1) * 32u + (k & 1u) * 8u, tc_desc(vs + s * Z::v + (k >> 2) * D * 128u + (k & 3u) * 32u), id_o, k > 0);
-                tc_commit(bar(VFREE + s)); tc_commit(bar(OREADY));
-                if (i + 2u < n) ok = mbar_wait(bar(OREADY), s) && scores(i + 2u);          // they overwrite the weights that the products before read
+                    tc_mma_ts(tmem + OCOL, tmem + s * kTile + k * 8u, tc_desc(vs + s * Z::v + (k >> 2) * D * 128u + (k & 3u) * 32u), id_o, i > 0 || k > 0);
+                tc_commit(bar(VFREE + s)); tc_commit(bar(ODONE));
+                if (i + 2u < n) ok = mbar_wait(bar(ODONE), s) && scores(i + 2u);          // they overwrite the weights that the products before read
             }
         }
-    } else if (warp > kMmaWarp) {
+    } else if (warp >= kMakers) {
         // operands: a tile is eight pieces of work, the keys and then the values of its four pages, dealt out to seven warps in turn
         const uint32_t eight = lane >> 3, bv = lane & 7u;
         const int32_t *table = a.table + (uint64_t)b * a.table_stride;
@@ -143,8 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             const uint32_t p = (lo + q / (2u * kPages)) * kPages + q % kPages;
             return q < n * 2u * kPages && (int)(p * kKv4Page) <= last_pos ? (uint32_t)table[p] : 0xffffffffu;
         };
-        uint32_t page = number(warp - kMmaWarp - 1u);
-        for (uint32_t q = warp - kMmaWarp - 1u; q < n * 2u * kPages; q += kProducers) {
+        uint32_t page = number(warp - kMakers);
+        for (uint32_t q = warp - kMakers; q < n * 2u * kPages; q += kProducers) {
             const uint32_t i = q / (2u * kPages), s = i & 1u, pw = q % kPages, next = number(q + kProducers);
             const bool ok = page < a.n_pages;
             const unsigned char *block = a.pool + (uint64_t)(ok ? page : 0u) * a.page_stride + (uint64_t)g * kv4_block_bytes(D);
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
                     for (int j = 0; j < 4 * NG; j++) kw[j] = 0u;
                 }
                 if (i >= 2u && !mbar_wait_warp(bar(KFREE + s), ((i >> 1) - 1u) & 1u)) break;
-                unsigned char *k_s = base + Z::qk + s * Z::qk;
+                unsigned char *k_s = base + (1u + s) * Z::qk;
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
                     const __half2 st = __low2half2(half2_of(kp[j])), mn = __high2half2(half2_of(kp[j]));
@@ -229,146 +230,130 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             page = next;
         }
     } else {
-        const uint32_t quad = warp & 3u, r = quad * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep;
-        const int pos = len - (int)a.T + (int)t, low = first_seen(max(pos, 0), a.window, a.block), low_last = first_seen(max(last_pos, 0), a.window, a.block);
-        const uint32_t lane_base = (quad * 32u) << 16;
-        // a row belongs to two threads, of warps that reach the same lanes of tensor memory: each has 64 keys of a tile and half of the values.  They share the row's
-        // maximum once a tile (the barrier of their two warps, which also says whether both go on) and their sums at the end.
-        constexpr int VH = (int)D / 2, CH = VH % 32 == 0 ? 32 : 16;
-        const uint32_t half = warp >> 2, c_lo = half * (kTile / 2u), v_lo = half * (uint32_t)VH;
+        const uint32_t r = warp * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep;
+        const int pos = pos_0 + (int)t, low = first_seen(max(pos, 0), a.window, a.block), low_last = first_seen(max(last_pos, 0), a.window, a.block);
+        const uint32_t lanes = (warp * 32u) << 16, o_at = tmem + lanes + OCOL;
         const float kc = scale_s[r];
         float m = -INFINITY, l = 0.0f;
-        pair_t o[VH / 2];
-#pragma unroll
-        for (int d = 0; d < VH / 2; d++) o[d] = pair(0.0f, 0.0f);
         bool ok = true;
-        // the values of the tile before join the sum, which then moves to the new reference
-        auto collect = [&](uint32_t i, float corr) {
-            ok = mbar_wait_warp(bar(OREADY), i & 1u);
-            if (!ok) return;
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < VH; c += CH) {
-                uint32_t w[CH];
-                if constexpr (CH == 32) tc_ld32(tmem + lane_base + OCOL + v_lo + c, w); else tc_ld16(tmem + lane_base + OCOL + v_lo + c, w);
-                const pair_t k = pair(corr, corr);
-#pragma unroll
-                for (int j = 0; j < CH / 2; j++) o[c / 2 + j] = add2(o[c / 2 + j], pair(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1])));
-                if (!__all_sync(0xffffffffu, corr == 1.0f))
-#pragma unroll
-                    for (int j = 0; j < CH / 2; j++) o[c / 2 + j] = mul2(o[c / 2 + j], k);
-            }
-        };
         for (uint32_t i = 0; i < n; i++) {
             const int key0 = (int)((lo + i) * kTile);
-            const uint32_t s_at = tmem + lane_base + (i & 1u) * kTile;
-            ok = ok && mbar_wait_warp(bar(SFULL + (i & 1u)), (i >> 1) & 1u);
+            const uint32_t s_at = tmem + lanes + (i & 1u) * kTile;
+            ok = mbar_wait_warp(bar(SFULL + (i & 1u)), (i >> 1) & 1u);
+            if (!ok) break;
             tc_fence_after();
-            // the keys that this row sees of this thread's 64, two words
-            uint32_t sees[2] = {0xffffffffu, 0xffffffffu}, odd[2];
-            const uint32_t hide = hide_s[i & 3u][2u * half] | hide_s[i & 3u][2u * half + 1u];
-            odd[0] = odd_s[i & 3u][2u * half]; odd[1] = odd_s[i & 3u][2u * half + 1u];
+            uint32_t w[kTile];
+            tc_ld128(s_at, w);
+            uint32_t hide = 0, odd = 0;
+#pragma unroll
+            for (int u = 0; u < 4; u++) { hide |= hide_s[i & 3u][u]; odd |= odd_s[i & 3u][u]; }
             const bool whole = key0 + (int)kTile - 1 <= first_pos && key0 >= low_last && hide == 0;          // every row of the block sees every key
+            auto sees = [&](uint32_t u) {          // of 32 keys those that this row sees
+                const int at = key0 + 32 * (int)u, from = low - at, to = pos - at;          // places [from, to]
+                uint32_t v = to < 0 || from > 31 ? 0u : 0xffffffffu;
+                if (to >= 0 && to < 31) v &= (2u << to) - 1u;
+                if (from > 0 && from <= 31) v &= 0xffffffffu << from;
+                return v & ~hide_s[i & 3u][u];
+            };
             if (!whole)
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int at = key0 + (int)c_lo + 32 * u, from = low - at, to = pos - at;          // places [from, to]
-                    uint32_t w = to < 0 || from > 31 ? 0u : 0xffffffffu;
-                    if (to >= 0 && to < 31) w &= (2u << to) - 1u;
-                    if (from > 0 && from <= 31) w &= 0xffffffffu << from;
-                    sees[u] = w & ~hide_s[i & 3u][2u * half + u];
-                }
-            float top = -INFINITY;
-            if (ok)
-#pragma unroll 1
-            for (uint32_t u = 0; u < 2; u++) {
-                uint32_t w[32];
-                tc_ld32(s_at + c_lo + u * 32u, w);
-                if (!whole) {
-                    const uint32_t see = u ? sees[1] : sees[0];
+                for (uint32_t u = 0; u < 4; u++) {
+                    const uint32_t see = sees(u);
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) w[j] = see >> j & 1u ? w[j] : 0xff800000u;
+                    for (uint32_t j = 0; j < 32; j++) w[u * 32u + j] = see >> j & 1u ? w[u * 32u + j] : 0xff800000u;
                 }
+            float top = -INFINITY, far = 0.0f;
 #pragma unroll
-                for (uint32_t j = 0; j < 32; j += 2) top = max3(top, __uint_as_float(w[j]), __uint_as_float(w[j + 1]));
+            for (uint32_t j = 0; j < kTile; j += 2) top = max3(top, __uint_as_float(w[j]), __uint_as_float(w[j + 1]));
+            if (a.softcap > 0.0f) {
+                const pair_t k = pair(kc, kc);
+#pragma unroll
+                for (uint32_t j = 0; j < kTile; j += 2) far = max3(far, fabsf(__uint_as_float(w[j])), fabsf(__uint_as_float(w[j + 1])));
+                if (__all_sync(0xffffffffu, far * kc < kTanhNear)) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kTile; j += 2) {
+                        float y, z;
+                        unpair(tanh_near2(mul2(pair(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), k)), y, z);
+                        w[j] = __float_as_uint(y); w[j + 1] = __float_as_uint(z);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < kTile; j++) w[j] = w[j] == 0xff800000u ? w[j] : __float_as_uint(tanh_any(__uint_as_float(w[j]) * kc));
+                }
             }
-            top_s[i & 1u][half][r] = top;
-            if (bar_any(1u + quad, 64u, !ok)) { ok = false; break; }
-            top = fmaxf(top, top_s[i & 1u][half ^ 1u][r]);
             if (top != -INFINITY) { top *= kc; if (a.softcap > 0.0f) top = a.softcap * kLog2e * tanh_any(top); }
-            const float next = top > m + kSlack ? top : m, corr = next == m ? 1.0f : ex2(m - next);          // (m = -inf: top is taken, if there is one)
-            if (i) collect(i - 1u, corr);
-            if (!ok) continue;          // both warps leave at the next barrier, or after the last tile
-            l *= corr;
-            m = next;
-            const float use = m == -INFINITY ? 0.0f : m - kLift;
-            float sum = 0.0f;
-#pragma unroll 1          // (a tile's whole code does not fit the instruction cache)
-            for (uint32_t u = 0; u < 2; u++) {
-                uint32_t w[32], wh[16];
-                tc_ld32(s_at + c_lo + u * 32u, w);
-                if (!whole) {
-                    const uint32_t see = u ? sees[1] : sees[0];
+            if (__any_sync(0xffffffffu, top > m + kSlack)) {          // (m = -inf: top is taken, if there is one)
+                const float next = top > m + kSlack ? top : m, corr = next == m ? 1.0f : ex2(m - next);
+                l *= corr;
+                m = next;
+                if (i) {          // the sums move to the new reference, once the products before are done
+                    ok = mbar_wait_warp(bar(ODONE), (i - 1u) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const pair_t k = pair(corr, corr);
+#pragma unroll 1
+                    for (uint32_t c = 0; c < D; c += 16u) {
+                        uint32_t v[16];
+                        tc_ld16(o_at + c, v);
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; j++) w[j] = see >> j & 1u ? w[j] : 0xff800000u;
-                }
-                if (a.softcap > 0.0f) {
-                    const pair_t k = pair(kc, kc), cap = pair(a.softcap * kLog2e, a.softcap * kLog2e);
-                    float far = 0.0f;
-#pragma unroll
-                    for (uint32_t j = 0; j < 32; j += 2) far = max3(far, fabsf(__uint_as_float(w[j])), fabsf(__uint_as_float(w[j + 1])));
-                    if (__all_sync(0xffffffffu, far * kc < 0.5f)) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 32; j += 2) {
-                            float x, y;
-                            unpair(mul2(cap, tanh_near2(mul2(pair(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), k))), x, y);
-                            w[j] = __float_as_uint(x); w[j + 1] = __float_as_uint(y);
+                        for (uint32_t j = 0; j < 16; j += 2) {
+                            float y, z;
+                            unpair(mul2(pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), k), y, z);
+                            v[j] = __float_as_uint(y); v[j + 1] = __float_as_uint(z);
                         }
-                    } else {
-#pragma unroll
-                        for (uint32_t j = 0; j < 32; j++) w[j] = w[j] == 0xff800000u ? w[j] : __float_as_uint(a.softcap * kLog2e * tanh_any(__uint_as_float(w[j]) * kc));
+                        tc_st16(o_at + c, v);
                     }
                 }
-                // (masked scores are -inf, whatever the factor: 0 times -inf would be no number)
-                const float by = a.softcap > 0.0f ? 1.0f : whole ? kc : fmaxf(kc, 1e-30f);
-                const pair_t k = pair(by, by), less = pair(-use, -use);
-                pair_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+            }
+            const float use = m == -INFINITY ? 0.0f : m - kLift;
+            // (masked scores are -inf, whatever the factor: 0 times -inf would be no number)
+            const float by = a.softcap > 0.0f ? a.softcap * kLog2e : whole ? kc : fmaxf(kc, 1e-30f);
+            const pair_t k = pair(by, by), less = pair(-use, -use);
+            pair_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) {
+                uint32_t wh[16];
 #pragma unroll
                 for (uint32_t j = 0; j < 16; j++) {
-                    float x, y;
-                    unpair(fma2(pair(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1])), k, less), x, y);
-                    x = ex2(x); y = ex2(y);
-                    s2[j & 1u] = add2(s2[j & 1u], pair(x, y));
-                    wh[j] = bits(__floats2half2_rn(x, y));
+                    float y, z;
+                    unpair(fma2(pair(__uint_as_float(w[u * 32u + 2u * j]), __uint_as_float(w[u * 32u + 2u * j + 1u])), k, less), y, z);
+                    y = ex2(y); z = ex2(z);
+                    s2[j & 1u] = add2(s2[j & 1u], pair(y, z));
+                    wh[j] = bits(__floats2half2_rn(y, z));
                 }
-                float s0, s1;
-                unpair(add2(s2[0], s2[1]), s0, s1);
-                sum += s0 + s1;
-                tc_st16(s_at + c_lo + u * 32u, wh);
+                tc_st16(s_at + u * 16u, wh);
             }
-            l += sum;
-            if ((odd[0] & sees[0]) | (odd[1] & sees[1])) l = NAN;          // values that are no number make the rows that see them NaN, however little they weigh
+            float s0, s1;
+            unpair(add2(s2[0], s2[1]), s0, s1);
+            l += s0 + s1;
+            if (odd)          // values that are no number make the rows that see them NaN, however little they weigh
+#pragma unroll 1
+                for (uint32_t u = 0; u < 4; u++) if (odd_s[i & 3u][u] & sees(u)) l = NAN;
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(PREADY));
+            if (lane == 0) mbar_arrive(bar(PREADY + (i & 1u)));
         }
-        if (ok && n) collect(n - 1u, 1.0f);
-        sum_s[half][r] = l;
-        ok = !bar_any(1u + quad, 64u, !ok);
-        if (r0 + r <= last) {
-            const float ref = m - kLift, both = ok ? sum_s[0][r] + sum_s[1][r] : NAN;          // a wait that ran out shows as NaN
-            const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols + r;
-            const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, t, h, ref, both);
+        // (a tile's scores come after the products of the tile two before it: of the last two products this is known of neither)
+        if (ok && n > 1u) ok = mbar_wait_warp(bar(ODONE), (n - 2u) & 1u);
+        if (ok && n) { ok = mbar_wait_warp(bar(ODONE), (n - 1u) & 1u); tc_fence_after(); }
+        const float ref = m - kLift, sum = ok ? l : NAN;          // a wait that ran out shows as NaN
+        const bool mine = r0 + r <= last;
+        const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols + r;
+        const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, t, h, ref, sum);
+#pragma unroll 1
+        for (uint32_t c = 0; c < D; c += 32u) {
+            uint32_t w[32] = {};
+            if (n && ok) tc_ld32(o_at + c, w);
+            if (mine)
 #pragma unroll
-            for (int d = 0; d < VH; d += 4) {
-                float4 v;
-                unpair(o[d / 2], v.x, v.y); unpair(o[d / 2 + 1], v.z, v.w);
-                if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + where * D + v_lo + d) = v;
-                else store_four(a, b, t, h, v_lo + d, v.x * k, v.y * k, v.z * k, v.w * k);
-            }
-            if (sh.nsplit > 1 && half == 0) reinterpret_cast<float2 *>(a.part + part_places(a, sh) * D)[where] = make_float2(ref, both);
+                for (uint32_t j = 0; j < 32; j += 4) {
+                    const float4 v = make_float4(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), __uint_as_float(w[j + 2]), __uint_as_float(w[j + 3]));
+                    if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + where * D + c + j) = v;
+                    else store_four(a, b, t, h, c + j, v.x * k, v.y * k, v.z * k, v.w * k);
+                }
         }
+        if (mine && sh.nsplit > 1) reinterpret_cast<float2 *>(a.part + part_places(a, sh) * D)[where] = make_float2(ref, sum);
     }
     tc_fence_before();
     __syncthreads();

@@ -2815,7 +2815,7 @@ int create(LayeredEngine *e, const nb::ModelDir *dir, uint32_t max_tokens) {
         size_t row = 0, part = 0;
         for (const Run &q : e->runs) {
             const Layer &L = e->layers[q.layer];
-            if (L.type == MIX_GQA || L.type == MIX_ATTN_DELTA) { row = std::max<size_t>(row, L.RL); part = std::max(part, nb::kv4_attn_workspace_most(1, L.G, L.dim, (uint32_t)e->num_sms)); }
+            if (L.type == MIX_GQA || L.type == MIX_ATTN_DELTA) { row = std::max<size_t>(row, L.RL); part = std::max(part, nb::kv4_attn_workspace_most(1, L.dim, (uint32_t)e->num_sms)); }
         }
         DM(e->b_krows, T * row * 4); DM(e->b_kpart, part);
     }
