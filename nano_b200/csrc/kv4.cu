@@ -15,8 +15,8 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------
 // Writing.  Four lanes hold a group, eight coordinates each: the extremes take two shuffles, a lane's codes are one word of a key row (two halves of a
-// word of a value row).  The code is round_half_even((x - m) / s) of the numbers themselves: the fp32 quotient decides it unless it lies within 1e-4 of a
-// border between two codes (its own error is below 1e-5), where the quotient is taken in 64 bits.
+// word of a value row).  The code is round_half_even((x - m) / s) of the numbers themselves: the fp32 quotient decides it unless it lies within 1e-5 of a
+// border between two codes (its own error is below 3e-6: three roundings of numbers up to 16), where the quotient is taken in 64 bits.
 // ------------------------------------------------------------------------------------------------
 constexpr float kKv4Most = 32768.0f;          // c s + m of a written group stays inside fp16
 constexpr uint32_t kRowThreads = 256;
@@ -35,27 +35,57 @@ __device__ __forceinline__ long long kv4_place(const Kv4Rows &a, uint32_t t) {
     return page < a.n_pages ? (long long)page * kKv4Page + pos % kKv4Page : -1;
 }
 
+// A lane's eight coordinates of a group are 8 b .. 8 b + 7, but of fp32 rows 4 b .. 4 b + 3 and 16 + 4 b .. 16 + 4 b + 3: four lanes' 16-byte accesses then are 64 bytes side by side
+// (with 32 bytes to a lane, half of each sector to an access, 9001 tokens of 8 heads of 128 took 26 us to write and 20 to read; so 22 and 13)
+template <typename T> constexpr bool kHalves = sizeof(T) == 4;
+template <typename T> __device__ __forceinline__ uint32_t second(uint32_t b) { return kHalves<T> ? 16u + 4u * b : 8u * b + 4u; }
+template <typename T> __device__ __forceinline__ uint32_t first(uint32_t b) { return kHalves<T> ? 4u * b : 8u * b; }
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRowThreads) k_kv4_write(const Kv4Rows a) {
-    pdl_enter4();
-    const uint32_t n = a.D / kKv4Group, b = threadIdx.x & 3u;
-    const uint64_t items = (uint64_t)a.T * a.G * n, item = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 2;
-    const bool live = item < items, value = blockIdx.y != 0;
-    const uint32_t t = live ? (uint32_t)(item / (a.G * n)) : 0u, e = live ? (uint32_t)(item % (a.G * n)) : 0u, g = e / n, j = e % n;
-    const long long place = live ? kv4_place(a, t) : -1;
-    float x[8] = {};
-    if (place >= 0) {
-        const T *src = static_cast<const T *>(value ? a.v : a.k) + (value ? t * a.v_token + g * a.v_head : t * a.k_token + g * a.k_head) + j * kKv4Group + b * 8u;
-        if constexpr (VEC) {
-            __align__(16) T raw[8];
+__device__ __forceinline__ void load_eight(const T *group, uint32_t b, float (&x)[8]) {
+    if constexpr (VEC && kHalves<T>) {
+        const float4 u = __ldcs(reinterpret_cast<const float4 *>(group + first<T>(b))), v = __ldcs(reinterpret_cast<const float4 *>(group + second<T>(b)));
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    } else if constexpr (VEC) {
+        __align__(16) T raw[8];
+        *reinterpret_cast<uint4 *>(raw) = __ldcs(reinterpret_cast<const uint4 *>(group + first<T>(b)));
 #pragma unroll
-            for (uint32_t i = 0; i < sizeof raw / 16; i++) reinterpret_cast<uint4 *>(raw)[i] = reinterpret_cast<const uint4 *>(src)[i];
+        for (int i = 0; i < 8; i++) x[i] = widen(raw[i]);
+    } else
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = widen(raw[i]);
-        } else
+        for (int i = 0; i < 4; i++) { x[i] = widen(group[first<T>(b) + i]); x[4 + i] = widen(group[second<T>(b) + i]); }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_eight(T *group, uint32_t b, const float (&x)[8]) {
+    if constexpr (VEC && kHalves<T>) {
+        __stcs(reinterpret_cast<float4 *>(group + first<T>(b)), make_float4(x[0], x[1], x[2], x[3]));
+        __stcs(reinterpret_cast<float4 *>(group + second<T>(b)), make_float4(x[4], x[5], x[6], x[7]));
+    } else if constexpr (VEC) {
+        __align__(16) T y[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = widen(src[i]);
-    }
+        for (int i = 0; i < 8; i++) y[i] = (T)x[i];
+        __stcs(reinterpret_cast<uint4 *>(group + first<T>(b)), *reinterpret_cast<const uint4 *>(y));
+    } else
+#pragma unroll
+        for (int i = 0; i < 4; i++) { group[first<T>(b) + i] = (T)x[i]; group[second<T>(b) + i] = (T)x[4 + i]; }
+}
+// a thread's place in its call: token t, head g, group j of n, its eight coordinates b of the group's 32 (thread 4 k + b of the groups in order); 32-bit numbers (the
+// launch sees to that: divisions of 64-bit ones were a third of the kernels)
+struct Eighth { uint32_t t, g, j, b, n; bool live; };
+__device__ __forceinline__ Eighth kv4_eighth(const Kv4Rows &a) {
+    Eighth e;
+    e.n = a.D / kKv4Group; e.b = threadIdx.x & 3u;
+    const uint32_t item = blockIdx.x * (kRowThreads / 4u) + (threadIdx.x >> 2), per = a.G * e.n;
+    e.t = item / per;
+    const uint32_t rest = item - e.t * per;
+    e.g = rest / e.n; e.j = rest - e.g * e.n;
+    e.live = e.t < a.T;
+    return e;
+}
+__device__ __forceinline__ unsigned char *kv4_block(const Kv4Rows &a, long long place, uint32_t g) {
+    return a.pool + (uint64_t)(place / kKv4Page) * a.page_stride + (uint64_t)g * kv4_block_bytes(a.D);
+}
+// the group that four lanes hold eight coordinates of each: its pair, and this lane's codes
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], __half2 &sm) {
     float lo = x[0], hi = x[0];
     bool fine = true;
 #pragma unroll
@@ -65,60 +95,74 @@ __global__ void __launch_bounds__(kRowThreads) k_kv4_write(const Kv4Rows a) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         fine = __shfl_xor_sync(0xffffffffu, (int)fine, o) && fine;
     }
-    if (place < 0) return;
     __half m = __float2half_rn(lo), s = __float2half_rn((hi - lo) * (1.0f / 15.0f));
     uint32_t word = 0;
     if (!fine) m = s = __ushort_as_half(0x7fff);
     else if (__half2float(s) > 0.0f) {
         const float mf = __half2float(m), sf = __half2float(s), inv = 1.0f / sf;
+        float q[8], r[8], border = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float q = (x[i] - mf) * inv;
-            float r = rintf(q);
-            if (fabsf(q - r) > 0.4999f) r = (float)rint(((double)x[i] - (double)mf) / (double)sf);
-            word |= (uint32_t)fminf(fmaxf(r, 0.0f), 15.0f) << (4 * i);
-        }
+        for (int i = 0; i < 8; i++) { q[i] = (x[i] - mf) * inv; r[i] = rintf(q[i]); border = fmaxf(border, fabsf(q[i] - r[i])); }
+        if (border > 0.49999f)          // (some one in two hundred warps)
+#pragma unroll
+            for (int i = 0; i < 8; i++) r[i] = (float)rint(((double)x[i] - (double)mf) / (double)sf);
+#pragma unroll
+        for (int i = 0; i < 8; i++) word |= (uint32_t)fminf(fmaxf(r[i], 0.0f), 15.0f) << (4 * i);
     }
-    unsigned char *block = a.pool + (uint64_t)(place / kKv4Page) * a.page_stride + (uint64_t)g * kv4_block_bytes(a.D) + (value ? 640u * n : 0u);
-    const uint32_t at = (uint32_t)(place % kKv4Page);
-    unsigned char *codes = block + at * 16u * n;
-    if (value) {
-        reinterpret_cast<uint16_t *>(codes)[2u * b * n + j] = (uint16_t)word;
-        reinterpret_cast<uint16_t *>(codes)[(2u * b + 1u) * n + j] = (uint16_t)(word >> 16);
-    } else reinterpret_cast<uint32_t *>(codes)[b * n + j] = word;
-    if (b == 0) reinterpret_cast<__half2 *>(block + 512u * n)[at * n + j] = __halves2half2(s, m);
+    sm = __halves2half2(s, m);
+    return word;
 }
 
-// Reading back: a thread per eight neighbouring coordinates.  c s is exact in fp32, so one rounding is left
+// a thread: the same eight coordinates of a key and of the value beside it, both on their way at once
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) k_kv4_write(const Kv4Rows a) {
+    pdl_enter4();
+    const Eighth e = kv4_eighth(a);
+    const long long place = e.live ? kv4_place(a, e.t) : -1;
+    float k[8] = {}, v[8] = {};
+    if (place >= 0) {
+        load_eight<T, VEC>(static_cast<const T *>(a.k) + e.t * a.k_token + e.g * a.k_head + e.j * kKv4Group, e.b, k);
+        load_eight<T, VEC>(static_cast<const T *>(a.v) + e.t * a.v_token + e.g * a.v_head + e.j * kKv4Group, e.b, v);
+    }
+    __half2 ks, vs;
+    uint32_t kw = kv4_codes(k, ks);
+    const uint32_t vw = kv4_codes(v, vs);
+    if constexpr (kHalves<T>) {          // a word's eight codes lie with two lanes
+        const uint32_t from = (threadIdx.x & 28u) + 2u * (e.b & 1u), u = __shfl_sync(0xffffffffu, kw, from), w = __shfl_sync(0xffffffffu, kw, from + 1u);
+        kw = __byte_perm(u, w, e.b < 2u ? 0x5410u : 0x7632u);
+    }
+    if (place < 0) return;
+    unsigned char *block = kv4_block(a, place, e.g);
+    const uint32_t at = (uint32_t)(place % kKv4Page), n = e.n;
+    reinterpret_cast<uint32_t *>(block + at * 16u * n)[e.b * n + e.j] = kw;
+    uint16_t *codes = reinterpret_cast<uint16_t *>(block + 640u * n + at * 16u * n);
+    codes[first<T>(e.b) / 4u * n + e.j] = (uint16_t)vw;
+    codes[second<T>(e.b) / 4u * n + e.j] = (uint16_t)(vw >> 16);
+    if (e.b == 0) {
+        reinterpret_cast<__half2 *>(block + 512u * n)[at * n + e.j] = ks;
+        reinterpret_cast<__half2 *>(block + 1152u * n)[at * n + e.j] = vs;
+    }
+}
+
+// Reading back: c s is exact in fp32, so one rounding is left
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) k_kv4_read(const Kv4Rows a) {
-    const uint32_t n = a.D / kKv4Group, b = threadIdx.x & 3u;
-    const uint64_t items = (uint64_t)a.T * a.G * n, item = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 2;
-    if (item >= items) return;
-    const bool value = blockIdx.y != 0;
-    const uint32_t t = (uint32_t)(item / (a.G * n)), e = (uint32_t)(item % (a.G * n)), g = e / n, j = e % n;
-    const long long place = kv4_place(a, t);
-    float x[8] = {};
+    const Eighth e = kv4_eighth(a);
+    if (!e.live) return;
+    const long long place = kv4_place(a, e.t);
+    float k[8] = {}, v[8] = {};
     if (place >= 0) {
-        const unsigned char *block = a.pool + (uint64_t)(place / kKv4Page) * a.page_stride + (uint64_t)g * kv4_block_bytes(a.D) + (value ? 640u * n : 0u);
-        const uint32_t at = (uint32_t)(place % kKv4Page);
-        const unsigned char *codes = block + at * 16u * n;
-        const uint32_t word = value ? reinterpret_cast<const uint16_t *>(codes)[2u * b * n + j] | (uint32_t)reinterpret_cast<const uint16_t *>(codes)[(2u * b + 1u) * n + j] << 16
-                                    : reinterpret_cast<const uint32_t *>(codes)[b * n + j];
-        const float2 sm = __half22float2(reinterpret_cast<const __half2 *>(block + 512u * n)[at * n + j]);
+        const unsigned char *block = kv4_block(a, place, e.g);
+        const uint32_t at = (uint32_t)(place % kKv4Page), n = e.n;
+        const uint16_t *kc = reinterpret_cast<const uint16_t *>(block + at * 16u * n), *vc = reinterpret_cast<const uint16_t *>(block + 640u * n + at * 16u * n);
+        const uint32_t u = first<T>(e.b) / 4u, w = second<T>(e.b) / 4u;          // fours of coordinates; of a key two to a word
+        const uint32_t kw = kc[(u / 2u * n + e.j) * 2u + (u & 1u)] | (uint32_t)kc[(w / 2u * n + e.j) * 2u + (w & 1u)] << 16, vw = vc[u * n + e.j] | (uint32_t)vc[w * n + e.j] << 16;
+        const float2 ks = __half22float2(reinterpret_cast<const __half2 *>(block + 512u * n)[at * n + e.j]), vs = __half22float2(reinterpret_cast<const __half2 *>(block + 1152u * n)[at * n + e.j]);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = fmaf((float)((word >> (4 * i)) & 15u), sm.x, sm.y);
+        for (int i = 0; i < 8; i++) { k[i] = fmaf((float)((kw >> (4 * i)) & 15u), ks.x, ks.y); v[i] = fmaf((float)((vw >> (4 * i)) & 15u), vs.x, vs.y); }
     }
-    T *dst = static_cast<T *>(value ? a.v : a.k) + (value ? t * a.v_token + g * a.v_head : t * a.k_token + g * a.k_head) + j * kKv4Group + b * 8u;
-    __align__(16) T y[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = (T)x[i];
-    if constexpr (VEC) {
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof y / 16; i++) reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(y)[i];
-    } else
-#pragma unroll
-        for (int i = 0; i < 8; i++) dst[i] = y[i];
+    store_eight<T, VEC>(static_cast<T *>(a.k) + e.t * a.k_token + e.g * a.k_head + e.j * kKv4Group, e.b, k);
+    store_eight<T, VEC>(static_cast<T *>(a.v) + e.t * a.v_token + e.g * a.v_head + e.j * kKv4Group, e.b, v);
 }
 
 bool rows_at16(const Kv4Rows &a) {
@@ -628,16 +672,23 @@ cudaError_t attn_launch_nt(const Kv4Attn &a, const Plan &p, cudaStream_t stream,
 }
 
 template <bool WRITE>
-cudaError_t rows_launch(const Kv4Rows &a, cudaStream_t stream, bool pdl) {
-    const uint64_t items = (uint64_t)a.T * a.G * (a.D / kKv4Group);
-    if (!items) return cudaSuccess;
-    const dim3 grid((uint32_t)((items * 4u + kRowThreads - 1u) / kRowThreads), 2);
-    const bool vec = rows_at16(a);
+cudaError_t rows_launch(const Kv4Rows &all, cudaStream_t stream, bool pdl) {
+    const uint32_t per = all.G * (all.D / kKv4Group), most = (1u << 30) / per;          // tokens of a launch
+    const bool vec = rows_at16(all);
+    for (uint32_t t0 = 0; t0 < all.T; t0 += most) {
+        Kv4Rows a = all;
+        a.T = std::min(most, all.T - t0);
+        a.k = static_cast<char *>(all.k) + t0 * all.k_token * elem_size(all.type); a.v = static_cast<char *>(all.v) + t0 * all.v_token * elem_size(all.type);
+        if (all.slots) a.slots += t0; else a.pos0 += t0;
+        const dim3 grid((a.T * per + kRowThreads / 4u - 1u) / (kRowThreads / 4u));
 #define KV4_ROWS(TYPE)                                                                                                                          \
     (WRITE ? (vec ? launch_on(k_kv4_write<TYPE, true>, grid, kRowThreads, 0, stream, pdl, a) : launch_on(k_kv4_write<TYPE, false>, grid, kRowThreads, 0, stream, pdl, a)) \
            : (vec ? launch_on(k_kv4_read<TYPE, true>, grid, kRowThreads, 0, stream, false, a) : launch_on(k_kv4_read<TYPE, false>, grid, kRowThreads, 0, stream, false, a)))
-    return a.type == T_F32 ? KV4_ROWS(float) : a.type == T_BF16 ? KV4_ROWS(__nv_bfloat16) : KV4_ROWS(__half);
+        const cudaError_t e = a.type == T_F32 ? KV4_ROWS(float) : a.type == T_BF16 ? KV4_ROWS(__nv_bfloat16) : KV4_ROWS(__half);
 #undef KV4_ROWS
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
