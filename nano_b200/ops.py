@@ -7,15 +7,15 @@
     kv4_attention    attention of queries over the pages of their sequences
     pages_copy       pages of a paged cache copied (forked, moved) in many pools at once
 
-Calls run on the current stream of the tensors' device, wait for nothing and may be captured into a CUDA graph.  Outputs are new tensors.  Arguments that an operator
-does not take are refused with NB200Error before anything is queued; there is no CPU fallback.
+Calls run on the current stream of the tensors' device, wait for nothing and may be captured into a CUDA graph.  Outputs are new tensors, which carry no gradients.
+Arguments that an operator does not take are refused with NB200Error before anything is queued; there is no CPU fallback.
 """
 from __future__ import annotations
 
 import ctypes as C
 import struct
+from array import array
 
-import numpy as np
 import torch
 
 from . import engine as E
@@ -77,9 +77,9 @@ def token_logprobs(logits, tokens, top=0):
         stride = vocab
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    where = logits.device
-    logprob, entropy = torch.empty(rows, dtype=torch.float32, device=where), torch.empty(rows, dtype=torch.float32, device=where)
-    top_logprob, top_id = torch.empty((rows, top), dtype=torch.float32, device=where), torch.empty((rows, top), dtype=torch.int32, device=where)
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)          # (sizes as a tuple cost a microsecond more each)
+    entropy, top_logprob = torch.empty_like(logprob), logprob.new_empty(rows, top)
+    top_id = torch.empty_like(top_logprob, dtype=torch.int32)
     if rows:
         _call(device, lib(True).nb200_dev_token_logprobs, logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr() or None, top_id.data_ptr() or None, logits.data_ptr(), kind,
               stride, rows, vocab, tokens.data_ptr(), tokens.element_size(), top)
@@ -91,10 +91,12 @@ def pages_copy(pools, src, dst):
     A source may appear many times; a destination that is a source too or appears twice is refused."""
     pools = list(pools)
     try:
-        both = np.array([src, dst], np.int64)
-    except (ValueError, TypeError):
-        both = np.empty(0)
-    if both.ndim != 2:
+        src, dst = array("I", src), array("I", dst)
+    except OverflowError:
+        _no("a page outside the pools")
+    except (TypeError, ValueError):
+        _no("src and dst are lists of page numbers")
+    if len(src) != len(dst):
         _no("src and dst are lists of the same length")
     if not pools:
         return
@@ -104,24 +106,24 @@ def pages_copy(pools, src, dst):
         if not isinstance(p, torch.Tensor) or p.get_device() != device or not p.dim():
             _cuda("pool %d" % i, p, device)
             _no("pool %d has no pages", i)
-        count = p.size(0)
+        count = p.shape[0]
         if p.is_contiguous():
-            one = p.nbytes // count if count else 0
-            stride.append(one)
+            one = step = p.nbytes // count if count else 0
         else:
             if not p[0].is_contiguous() or p.stride(0) < 0:
                 _no("pool %d: a page is to be contiguous", i)
             one = p[0].nbytes
-            stride.append(p.stride(0) * p.element_size() if count > 1 else one)
+            step = p.stride(0) * p.element_size() if count > 1 else one
         base.append(p.data_ptr())
         size.append(one)
+        stride.append(step)
         pages.append(count)
     n, most = len(pools), min(pages)
-    if both.size and (both.min() < 0 or both.max() >= most):
+    if src and (max(src) >= most or max(dst) >= most):
         _no("a page outside the smallest pool's %d", most)
-    both = both.astype(np.uint32)
-    at, count = both.ctypes.data, both.shape[1]
-    _call(device, lib(True).nb200_dev_pages_copy, (C.c_uint64 * n)(*base), (C.c_uint64 * n)(*size), (C.c_uint64 * n)(*stride), (C.c_uint32 * n)(*pages), n, at, at + 4 * count, count)
+    numbers = array("Q", base + size + stride)
+    at, counts = numbers.buffer_info()[0], array("I", pages)
+    _call(device, lib(True).nb200_dev_pages_copy, at, at + 8 * n, at + 16 * n, counts.buffer_info()[0], n, src.buffer_info()[0], dst.buffer_info()[0], len(src))
 
 
 def kv4_cache(pages, kv_heads, head_dim, device="cuda"):
@@ -188,7 +190,8 @@ def kv4_read(pool, slots, dtype=torch.float32):
     if kind is None:
         _no("rows are float32, bfloat16 or float16")
     tokens = slots.shape[0]
-    k, v = torch.empty((tokens, heads, dim), dtype=dtype, device=pool.device), torch.empty((tokens, heads, dim), dtype=dtype, device=pool.device)
+    k = pool.new_empty(tokens, heads, dim, dtype=dtype)
+    v = torch.empty_like(k)
     if tokens:
         rows = _ROWS(pool.data_ptr(), stride, pages, heads, dim, kind, tokens, slots.data_ptr(), k.data_ptr(), v.data_ptr(), heads * dim, dim, heads * dim, dim)
         _call(device, lib(True).nb200_dev_kv4_read, rows)
@@ -230,13 +233,15 @@ def kv4_attention(q, pool, table, lens, scale=None, window=0, block=0, softcap=0
     if qd != 1 or qb < 0 or qt < 0 or qh < 0:
         q = q.contiguous()
         qb, qt, qh, qd = q.stride()
-    where = q.device
-    out = torch.empty((B, T, H, dim), dtype=q.dtype, device=where)
-    p = _ATTENTION(q.data_ptr(), out.data_ptr(), qb, qt, qh, T * H * dim, H * dim, dim, pool.data_ptr(), stride, pages, heads, dim, kind, B, T, H, table.shape[1], table.stride(0),
-                   table.data_ptr(), lens.data_ptr(), 0 if sinks is None else sinks.data_ptr(), dim ** -0.5 if scale is None else scale, softcap, window, block)
+    out = q.new_empty(B, T, H, dim)
+    try:
+        p = _ATTENTION(q.data_ptr(), out.data_ptr(), qb, qt, qh, T * H * dim, H * dim, dim, pool.data_ptr(), stride, pages, heads, dim, kind, B, T, H, table.shape[1], table.stride(0),
+                       table.data_ptr(), lens.data_ptr(), 0 if sinks is None else sinks.data_ptr(), dim ** -0.5 if scale is None else scale, softcap, window, block)
+    except (struct.error, OverflowError):
+        _no("scale and softcap are numbers of 32 bits, window and block whole ones")
     L, need = lib(True), C.c_uint64()
     _call(device, _workspace, L, p, need)
-    room = torch.empty(need.value, dtype=torch.uint8, device=where) if need.value else None
+    room = pool.new_empty(need.value) if need.value else None
     _call(device, L.nb200_dev_kv4_attention, p, None if room is None else room.data_ptr(), need.value)
     return out
 

@@ -176,7 +176,8 @@ def test_pages_copy_beyond_32_bits():
 
 def test_pages_copy_refusals():
     pool = torch.zeros(6, 32, device="cuda")
-    for src, dst, text in [([0], [0], "read"), ([0, 1], [2, 2], "twice"), ([0, 2], [2, 3], "read"), ([6], [0], "outside"), ([-1], [0], "outside"), ([0, 1], [2], "same length")]:
+    for src, dst, text in [([0], [0], "read"), ([0, 1], [2, 2], "twice"), ([0, 2], [2, 3], "read"), ([6], [0], "outside"), ([-1], [0], "outside"), ([0, 1], [2], "same length"),
+                           ([1 << 32], [0], "outside"), (np.array([(1 << 32) + 1]), [0], "outside"), ([0.5], [1], "page numbers"), ([[0, 1]], [[2, 3]], "page numbers"), (3, 4, "page numbers")]:
         with pytest.raises(NB200Error, match=text):
             ops.pages_copy([pool], src, dst)
     with pytest.raises(NB200Error, match="outside"):
@@ -496,7 +497,8 @@ def test_kv4_attention_strides_and_refusals():
     for args, kw, text in [((q[..., :32], pool, table, lens), {}, "q is"), ((q.half(), pool, table, lens), {}, "q is"), ((q[:, :, :3], pool, table, lens), {}, "evenly"),
                            ((q, pool, table.long(), lens), {}, "table"), ((q, pool, table[:1], lens), {}, "table"), ((q, pool, table, lens.long()), {}, "lens"),
                            ((q, pool, table, lens), dict(window=-1), "window"), ((q, pool, table, lens), dict(softcap=-1.0), "softcap"), ((q, pool, table, lens), dict(sinks=torch.zeros(3, device="cuda")), "sinks"),
-                           ((q, pool, table, lens), dict(scale=math.nan), "scale"), ((q, pool.cpu(), table, lens), {}, "CUDA"), ((q, pool, table, lens.cpu()), {}, "CUDA")]:
+                           ((q, pool, table, lens), dict(scale=math.nan), "scale"), ((q, pool, table, lens), dict(scale=1e60), "scale"), ((q, pool, table, lens), dict(window=1 << 40), "window"),
+                           ((q, pool, table, lens), dict(block=1.5), "block"), ((q, pool.cpu(), table, lens), {}, "CUDA"), ((q, pool, table, lens.cpu()), {}, "CUDA")]:
         with pytest.raises(NB200Error, match=text):
             ops.kv4_attention(*args, **kw)
     wide = ops.kv4_cache(2, 1, 160)
