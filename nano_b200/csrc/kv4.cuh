@@ -48,11 +48,12 @@ __device__ __forceinline__ void take(const unsigned char *p, uint32_t (&w)[(BYTE
     }
 }
 
-// tanh for the soft cap: its series where |x| < kTanhNear (off by at most 1382/155925 x^11 = 8.6e-8), where the special function unit would be the bound; else 1 - 2 / (1 + e^2x)
-constexpr float kTanhNear = 0.35f;
+// tanh for the soft cap: where |x| < kTanhNear, x times the polynomial of x^2 whose largest relative error there is least (5.5e-7; the special function unit would be the bound);
+// else 1 - 2 / (1 + e^2x)
+constexpr float kTanhNear = 0.5f, kTanh0 = 0.99999946f, kTanh1 = -0.33326318f, kTanh2 = 0.13190297f, kTanh3 = -0.044402226f;
 __device__ __forceinline__ float tanh_near(float x) {
     const float y = x * x;
-    return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
+    return x * fmaf(y, fmaf(y, fmaf(y, kTanh3, kTanh2), kTanh1), kTanh0);
 }
 __device__ __forceinline__ float tanh_any(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * x)); }
 

@@ -10,6 +10,7 @@
 // are seldom touched.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "family.h"
 #include "kv4.cuh"
@@ -29,13 +30,6 @@ template <int NG> struct Sizes {
     static constexpr uint32_t D = 32u * NG, DP = NG <= 2 ? 64u : 128u;          // coordinates; those that an operand of queries or keys has room for
     static constexpr uint32_t qk = kTile * DP * 2u, v = kTile * D * 2u, all = 3u * qk + 2u * v + 1024u;
 };
-
-// tanh_near of two numbers
-__device__ __forceinline__ pair_t tanh_near2(pair_t x) {
-    auto both = [](float c) { return pair(c, c); };
-    const pair_t y = mul2(x, x);
-    return fma2(mul2(x, y), fma2(y, fma2(y, fma2(y, both(62.0f / 2835.0f), both(-17.0f / 315.0f)), both(2.0f / 15.0f)), both(-1.0f / 3.0f)), x);
-}
 
 // grid (nsplit x tiles, G, B)
 template <int NG>
@@ -233,7 +227,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
         const uint32_t r = warp * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep;
         const int pos = pos_0 + (int)t, low = first_seen(max(pos, 0), a.window, a.block), low_last = first_seen(max(last_pos, 0), a.window, a.block);
         const uint32_t lanes = (warp * 32u) << 16, o_at = tmem + lanes + OCOL;
-        const float kc = scale_s[r];
+        const float kc = scale_s[r], cap = a.softcap * kLog2e, kk = kc * kc;
+        // the soft cap of a score x near 0 is x (c0 + c1 x^2 + c2 x^4 + c3 x^6); factors whose powers leave fp32 take the other way
+        const float c0 = cap * kTanh0 * kc, c1 = cap * kTanh1 * kc * kk, c2 = cap * kTanh2 * kc * kk * kk, c3 = cap * kTanh3 * kc * kk * kk * kk, limit = kc > 1e-4f && kc < 1e4f ? kTanhNear / kc : 0.0f;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         for (uint32_t i = 0; i < n; i++) {
@@ -265,23 +261,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             float top = -INFINITY, far = 0.0f;
 #pragma unroll
             for (uint32_t j = 0; j < kTile; j += 2) top = max3(top, __uint_as_float(w[j]), __uint_as_float(w[j + 1]));
+            bool near = false;          // scores whose soft cap is a polynomial, taken where the weights are made
             if (a.softcap > 0.0f) {
-                const pair_t k = pair(kc, kc);
 #pragma unroll
                 for (uint32_t j = 0; j < kTile; j += 2) far = max3(far, fabsf(__uint_as_float(w[j])), fabsf(__uint_as_float(w[j + 1])));
-                if (__all_sync(0xffffffffu, far * kc < kTanhNear)) {
-#pragma unroll
-                    for (uint32_t j = 0; j < kTile; j += 2) {
-                        float y, z;
-                        unpair(tanh_near2(mul2(pair(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), k)), y, z);
-                        w[j] = __float_as_uint(y); w[j + 1] = __float_as_uint(z);
-                    }
-                } else {
+                near = __all_sync(0xffffffffu, far < limit);
+                if (!near)
 #pragma unroll
                     for (uint32_t j = 0; j < kTile; j++) w[j] = w[j] == 0xff800000u ? w[j] : __float_as_uint(tanh_any(__uint_as_float(w[j]) * kc));
-                }
             }
-            if (top != -INFINITY) { top *= kc; if (a.softcap > 0.0f) top = a.softcap * kLog2e * tanh_any(top); }
+            if (top != -INFINITY) { top *= kc; if (a.softcap > 0.0f) top = cap * tanh_any(top); }
             if (__any_sync(0xffffffffu, top > m + kSlack)) {          // (m = -inf: top is taken, if there is one)
                 const float next = top > m + kSlack ? top : m, corr = next == m ? 1.0f : ex2(m - next);
                 l *= corr;
@@ -307,22 +296,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             }
             const float use = m == -INFINITY ? 0.0f : m - kLift;
             // (masked scores are -inf, whatever the factor: 0 times -inf would be no number)
-            const float by = a.softcap > 0.0f ? a.softcap * kLog2e : whole ? kc : fmaxf(kc, 1e-30f);
+            const float by = a.softcap > 0.0f ? cap : whole ? kc : fmaxf(kc, 1e-30f);
             const pair_t k = pair(by, by), less = pair(-use, -use);
             pair_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+            auto weights = [&](auto capped) {
 #pragma unroll
-            for (uint32_t u = 0; u < 4; u++) {
-                uint32_t wh[16];
+                for (uint32_t u = 0; u < 4; u++) {
+                    uint32_t wh[16];
 #pragma unroll
-                for (uint32_t j = 0; j < 16; j++) {
-                    float y, z;
-                    unpair(fma2(pair(__uint_as_float(w[u * 32u + 2u * j]), __uint_as_float(w[u * 32u + 2u * j + 1u])), k, less), y, z);
-                    y = ex2(y); z = ex2(z);
-                    s2[j & 1u] = add2(s2[j & 1u], pair(y, z));
-                    wh[j] = bits(__floats2half2_rn(y, z));
+                    for (uint32_t j = 0; j < 16; j++) {
+                        float y, z;
+                        const pair_t x = pair(__uint_as_float(w[u * 32u + 2u * j]), __uint_as_float(w[u * 32u + 2u * j + 1u]));
+                        if constexpr (capped.value) {
+                            const pair_t xx = mul2(x, x);
+                            unpair(fma2(x, fma2(xx, fma2(xx, fma2(xx, pair(c3, c3), pair(c2, c2)), pair(c1, c1)), pair(c0, c0)), less), y, z);
+                        } else unpair(fma2(x, k, less), y, z);
+                        y = ex2(y); z = ex2(z);
+                        s2[j & 1u] = add2(s2[j & 1u], pair(y, z));
+                        wh[j] = bits(__floats2half2_rn(y, z));
+                    }
+                    tc_st16(s_at + u * 16u, wh);
                 }
-                tc_st16(s_at + u * 16u, wh);
-            }
+            };
+            if (near) weights(std::true_type{}); else weights(std::false_type{});
             float s0, s1;
             unpair(add2(s2[0], s2[1]), s0, s1);
             l += s0 + s1;
