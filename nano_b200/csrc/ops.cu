@@ -606,7 +606,7 @@ int nb200_dev_pages_copy(void *const *pools, const uint64_t *page_bytes, const u
         if (!n_pools || !n) return 0;
         std::vector<bool> used(pages, false);
         for (uint32_t i = 0; i < n; i++) {
-            if (src[i] >= pages || dst[i] >= pages) return fail(NB200_EINVAL, "pair %u copies page %u to %u: the smallest pool has %u", i, src[i], dst[i], pages);
+            if (src[i] >= pages || dst[i] >= pages) return fail(NB200_EINVAL, "pair %u copies page %u to %u, one outside: the smallest pool has %u", i, src[i], dst[i], pages);
             used[src[i]] = true;
         }
         for (uint32_t i = 0; i < n; i++) {

@@ -86,16 +86,23 @@ def token_logprobs(logits, tokens, top=0):
     return logprob, entropy, top_logprob, top_id
 
 
-def pages_copy(pools, src, dst):
-    """Page src[i] is copied over page dst[i] in every pool, in place.  pools: tensors [pages, ...] of any type, each page contiguous; src, dst: numbers on the host.
-    A source may appear many times; a destination that is a source too or appears twice is refused."""
-    pools = list(pools)
+def _numbers(pages):
+    """Page numbers on the host as 32-bit numbers."""
+    if getattr(pages, "is_cuda", False):
+        _no("src and dst are lists of page numbers on the host")
     try:
-        src, dst = array("I", src), array("I", dst)
+        return array("I", pages.tolist() if hasattr(pages, "tolist") else pages)
     except OverflowError:
         _no("a page outside the pools")
     except (TypeError, ValueError):
         _no("src and dst are lists of page numbers")
+
+
+def pages_copy(pools, src, dst):
+    """Page src[i] is copied over page dst[i] in every pool, in place.  pools: tensors [pages, ...] of any type, each page contiguous; src, dst: numbers on the host.
+    A source may appear many times; a destination that is a source too or appears twice is refused."""
+    pools = list(pools)
+    src, dst = _numbers(src), _numbers(dst)
     if len(src) != len(dst):
         _no("src and dst are lists of the same length")
     if not pools:
@@ -118,9 +125,7 @@ def pages_copy(pools, src, dst):
         size.append(one)
         stride.append(step)
         pages.append(count)
-    n, most = len(pools), min(pages)
-    if src and (max(src) >= most or max(dst) >= most):
-        _no("a page outside the smallest pool's %d", most)
+    n = len(pools)
     numbers = array("Q", base + size + stride)
     at, counts = numbers.buffer_info()[0], array("I", pages)
     _call(device, lib(True).nb200_dev_pages_copy, at, at + 8 * n, at + 16 * n, counts.buffer_info()[0], n, src.buffer_info()[0], dst.buffer_info()[0], len(src))

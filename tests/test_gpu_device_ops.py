@@ -177,7 +177,7 @@ def test_pages_copy_beyond_32_bits():
 def test_pages_copy_refusals():
     pool = torch.zeros(6, 32, device="cuda")
     for src, dst, text in [([0], [0], "read"), ([0, 1], [2, 2], "twice"), ([0, 2], [2, 3], "read"), ([6], [0], "outside"), ([-1], [0], "outside"), ([0, 1], [2], "same length"),
-                           ([1 << 32], [0], "outside"), (np.array([(1 << 32) + 1]), [0], "outside"), ([0.5], [1], "page numbers"), ([[0, 1]], [[2, 3]], "page numbers"), (3, 4, "page numbers")]:
+                           ([1 << 32], [0], "outside"), (np.array([(1 << 32) + 1]), [0], "outside"), ([0.5], [1], "page numbers"), ([[0, 1]], [[2, 3]], "page numbers"), (3, 4, "page numbers"), (torch.tensor([0], device="cuda"), [1], "on the host"), ("ab", [1, 2], "page numbers")]:
         with pytest.raises(NB200Error, match=text):
             ops.pages_copy([pool], src, dst)
     with pytest.raises(NB200Error, match="outside"):
