@@ -208,6 +208,27 @@ struct Room {
 // blocks that an SM holds at once: registers allow no more without spills
 __host__ __device__ constexpr int kv4_blocks(int NG, int NT) { return NG <= 2 || (NG <= 4 && NT == 1) ? 4 : NG <= 4 ? 3 : 2; }
 
+// The sequence that `before` others come before when they are ordered by pages, then by number; up to 32 N of them.  By votes, whose results are known to be the same in all
+// lanes: read back from shared memory the number cost the kernel spills and a tenth of its speed
+template <int N>
+__device__ __forceinline__ uint32_t longest(const Kv4Attn &a, uint32_t before) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t own[N], count[N], b = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) { const uint32_t at = i * 32u + lane; count[i] = 0; own[i] = at < a.B ? (uint32_t)max(a.lens[at], 0) / kKv4Page * 64u + 63u - at : 0u; }
+#pragma unroll 8
+    for (uint32_t l = 0; l < 32; l++)
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const uint32_t other = __shfl_sync(0xffffffffu, own[j], l);
+#pragma unroll
+            for (int i = 0; i < N; i++) count[i] += other > own[i] ? 1u : 0u;
+        }
+#pragma unroll
+    for (int i = 0; i < N; i++) { const uint32_t v = __ballot_sync(0xffffffffu, i * 32u + lane < a.B && count[i] == before); if (v) b = i * 32u + __ffs(v) - 1u; }
+    return b;
+}
+
 // grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
 template <int NG, int NT, int WK, int W>
 __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT)) k_kv4_attn(const Kv4Attn a, const Shape sh) {
@@ -217,7 +238,9 @@ __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT)) k_kv4_attn(const K
     extern __shared__ __align__(16) unsigned char sm[];
     __shared__ uint32_t known[W][kStages];          // whether the page in a stage is one of the pool's
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, wr = warp / WK, wk = warp % WK, gq = lane >> 2, tq = lane & 3u;
-    const uint32_t split = blockIdx.x % sh.nsplit, tile = blockIdx.x / sh.nsplit, g = blockIdx.y, b = blockIdx.z, rep = a.H / a.G, ncols = a.T * rep;
+    const uint32_t split = blockIdx.x % sh.nsplit, tile = blockIdx.x / sh.nsplit, g = blockIdx.y, rep = a.H / a.G, ncols = a.T * rep;
+    uint32_t b = blockIdx.z;
+    if (sh.sorted) b = a.B <= 32u ? longest<1>(a, b) : longest<2>(a, b);
     unsigned char *ring = sm + warp * kStages * R::block;
     unsigned char *q_s = sm + (R::ring > R::merge ? R::ring : R::merge) + wr * NT * NG * 512u;
     float *scale_s = reinterpret_cast<float *>(sm + (R::ring > R::merge ? R::ring : R::merge) + R::q) + wr * COLS * (R::after ? 1u + NG : 1u), *sum_s = scale_s + COLS;          // sum_s (R::after): [column][group] sums of the rounded queries
@@ -631,7 +654,7 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 
 // ---- which instance, and how the work is shared out ----
 struct Plan { int nt; bool rows, tc; Shape sh; };
-constexpr uint32_t kWarps = 4, kWaves = 3, kTcCols = 17;
+constexpr uint32_t kWarps = 4, kWaves = 3, kMost = 64, kTcCols = 17;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G);
     Plan p{};
@@ -643,12 +666,18 @@ Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32
     // pages that a block can have in sight
     const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
     const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
-    // a block for every place that the device has; of several sequences, whose lengths may differ, three times as many (32 of up to 8190 tokens: 90 us with one, 73 with two, 69
-    // with three, 75 with six)
+    // A block for every place that the device has.  Of several sequences, whose lengths may differ, blocks of no more than kMost pages, but at most three times as many blocks as
+    // places: with one, two and three blocks to a place 32 sequences of up to 8190 tokens take 67, 56 and 57 us, of 8190 each 77, 74 and 79, but 8 of them 20, 24 and 29, 3 of up to
+    // 30000 26, 33 and 36 (a block costs some 2 us beside its pages)
     const uint32_t at_once = p.tc ? 1u : (uint32_t)kv4_blocks((int)D / 32, p.nt);
-    const uint64_t blocks = (uint64_t)B * G * p.sh.tiles, want = (uint64_t)(B > 1 ? kWaves : 1u) * at_once * sms;
+    const uint64_t blocks = std::max<uint64_t>(1, (uint64_t)B * G * p.sh.tiles), places = (uint64_t)at_once * sms;
     const uint32_t least = p.tc ? 16u : p.rows ? 8u : kWarps;          // pages of a split
-    p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want / std::max<uint64_t>(1, blocks), std::max(1u, pages / least)));
+    uint64_t n = places / blocks;
+    if (B > 1) n = std::max(n, std::min<uint64_t>((pages + kMost - 1u) / kMost, kWaves * places / blocks));
+    p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(n, std::max(1u, pages / least)));
+    // Of up to 64 sequences the longest first, so that the SMs get long and short ones alike and what is left when others end is short (32 of up to 8190 tokens: 50 us, in the given
+    // order 56; 64 of up to 4000, 4 heads of 64: 25 and 28).  It costs some 0.9 us of a block's start: not for blocks of less than 16 pages (48 of up to 1000: 10.6 us, sorted 11.5)
+    p.sh.sorted = !p.tc && B > 1 && B <= 64 && pages >= 16u * p.sh.nsplit ? 1u : 0u;
     return p;
 }
 

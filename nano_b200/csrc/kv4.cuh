@@ -90,7 +90,7 @@ __device__ __forceinline__ void store_four(const Kv4Attn &a, uint32_t b, uint32_
     }
 }
 
-struct Shape { uint32_t nsplit, tiles, cols; };          // splits of the keys, blocks along the columns of a head, columns of a block
+struct Shape { uint32_t nsplit, tiles, cols, sorted; };          // splits of the keys, blocks along the columns of a head, columns of a block; whether blocks take the longest sequences first
 
 // the sums of a row's splits: values [B][G][tiles][nsplit][columns of a block][D], then (r, l) of each
 __device__ __forceinline__ uint64_t part_places(const Kv4Attn &a, const Shape &sh) { return (uint64_t)a.B * a.G * sh.tiles * sh.nsplit * sh.cols; }

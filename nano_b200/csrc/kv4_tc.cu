@@ -379,7 +379,7 @@ cudaError_t launch_ng(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, bo
 }  // namespace
 
 cudaError_t kv4_tc_launch(const Kv4Attn &a, uint32_t nsplit, uint32_t tiles, cudaStream_t stream, bool pdl) {
-    const Shape sh{nsplit, tiles, kKv4TcRows};
+    const Shape sh{nsplit, tiles, kKv4TcRows, 0};
     switch (a.D / 32u) {
         case 1: return launch_ng<1>(a, sh, stream, pdl);
         case 2: return launch_ng<2>(a, sh, stream, pdl);

@@ -372,6 +372,20 @@ def test_kv4_attention_of_single_tokens(kind, dim, heads, kv_heads):
     check_attention(q, pool, table, lens)
 
 
+@pytest.mark.parametrize("batch,width,tokens", [(20, 60, 1), (32, 40, 1), (33, 40, 2), (64, 20, 1), (65, 20, 1)])
+def test_kv4_attention_of_many_sequences(batch, width, tokens):
+    """Lengths of all kinds, equal ones, none at all, below zero and beyond the table among them, whatever order their blocks run in."""
+    g = gen(batch)
+    pool = filled(g, 100, 8, 32)
+    table = torch.randint(0, 100, (batch, width), device="cuda", generator=g).int()          # (sequences may share pages)
+    lens = torch.randint(1, 32 * width + 1, (batch,), device="cuda", generator=g).int()
+    lens[1:batch:5] = 32 * width
+    lens[2:batch:7] = lens[0]
+    lens[3], lens[4], lens[7], lens[batch - 1] = 0, -3, 32 * width + 100, 2 ** 31 - 1
+    q = torch.randn(batch, tokens, 16, 32, device="cuda", generator=g).bfloat16()
+    check_attention(q, pool, table, lens)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("dim,heads,kv_heads,tokens,context", [(128, 8, 8, 2, 50), (128, 16, 4, 3, 700), (64, 16, 4, 40, 40), (64, 4, 2, 129, 1500), (256, 4, 1, 70, 300), (32, 5, 1, 77, 99), (96, 8, 2, 33, 65), (128, 8, 2, 200, 201)])
 def test_kv4_attention_of_portions(kind, dim, heads, kv_heads, tokens, context):
