@@ -1,9 +1,12 @@
 """CPU tests of the operators on device memory: what their C entry points refuse, before any device is looked for, and that there is no CPU fallback."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
 
+from conftest import ROOT
 from nano_b200 import engine as E
 
 EINVAL, ENODEV = -1, -3
@@ -109,6 +112,26 @@ def test_attention_refusals():
         refused(f(attention(o_head=126)), "multiples of four")
         assert f(attention(batch=0)) == 0 and f(attention(tokens=0)) == 0
     refused(L.nb200_dev_kv4_attention_workspace(attention(), None), "null")
+
+
+def test_a_cache_in_4_bits_is_refused_for_model_files():
+    image, h = np.zeros(400, np.uint8), C.c_void_p()
+    refused(E.lib().nb200_engine_create(C.byref(h), image.ctypes.data, image.size, 16, 0, E.FLAG_KV4), "model folders")
+    assert not h.value
+
+
+def test_waits_of_the_portion_kernel_end_for_a_warp_as_a_whole():
+    """What a block of k_kv4_attn_tc does when a wait runs out is read from the source: whole warps get one verdict, leave their loop with it, and show it in their rows."""
+    text = re.sub(r"//.*", "", open(os.path.join(ROOT, "nano_b200", "csrc", "kv4_tc.cu")).read())
+    body = text[text.index("} else if (warp >= kMakers) {"):text.index("tc_dealloc")]
+    loops = body[:body.index("const float ref = m - kLift")]
+    waits = re.findall(r"mbar_wait\w*\(", loops)
+    assert len(waits) == 6 and set(waits) == {"mbar_wait_warp("}, "a wait without one verdict for the warp"
+    assert len(re.findall(r"!mbar_wait_warp\([^;]*\)\) break;", loops)) == 2 and len(re.findall(r"ok = mbar_wait_warp\([^;]*\);\s*if \(!ok\) break;", loops)) == 2
+    assert "__syncthreads" not in loops and "bar.sync" not in loops
+    assert "sum = ok ? l : NAN" in body and "if (n && ok) tc_ld32" in body
+    one = text[text.index("auto scores = [&](uint32_t i)"):text.index("} else if (warp >= kMakers) {")]          # the thread that issues the products
+    assert len(re.findall(r"mbar_wait\(", one)) == 4 and "mbar_wait_warp" not in one and "if (!ok) break;" in one and "i < n && ok" in one
 
 
 @pytest.mark.skipif(E.device_count() > 0, reason="box has a GPU")
