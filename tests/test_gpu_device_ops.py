@@ -66,7 +66,7 @@ def check_logprobs(x, tokens, top):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("vocab,rows,top", [(1, 3, 1), (2, 1, 0), (31, 5, 31), (33, 7, 32), (100, 700, 5), (4097, 3, 20), (8191, 2, 32), (32000, 64, 0), (50257, 9, 8), (151936, 1, 5), (151936, 150, 20)])
+@pytest.mark.parametrize("vocab,rows,top", [(1, 3, 1), (2, 1, 0), (31, 5, 31), (33, 7, 32), (100, 700, 5), (4097, 3, 20), (8191, 2, 32), (32000, 64, 0), (50257, 9, 8), (151936, 1, 5), (151936, 150, 20), (4097, 593, 32), (16383, 592, 20), (20000, 600, 8)])
 def test_logprobs(kind, vocab, rows, top):
     g = gen(vocab + rows)
     x = (torch.randn(rows, vocab, device="cuda", generator=g) * 3).to(DT[kind])          # 16-bit rows are full of equal numbers
@@ -77,8 +77,9 @@ def test_logprobs(kind, vocab, rows, top):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("offset,pad", [(1, 0), (3, 5), (0, 1), (7, 8)])
-def test_logprobs_of_rows_anywhere(kind, offset, pad):
-    rows, vocab = 6, 5003
+@pytest.mark.parametrize("rows", [6, 700])
+def test_logprobs_of_rows_anywhere(kind, offset, pad, rows):
+    vocab = 5003
     x = (torch.randn(rows, vocab + pad + offset, device="cuda", generator=gen(5)) * 2).to(DT[kind])
     x[:, :offset] = math.nan          # what lies beside the rows is not looked at
     x[:, offset + vocab:] = math.nan
@@ -86,7 +87,8 @@ def test_logprobs_of_rows_anywhere(kind, offset, pad):
     check_logprobs(x.t().contiguous().t()[:, offset:offset + vocab], torch.arange(rows, device="cuda"), 4)
 
 
-def test_logprobs_of_special_rows():
+@pytest.mark.parametrize("times", [1, 40])
+def test_logprobs_of_special_rows(times):
     V, low = 3000, torch.finfo(torch.float32).min
     x = torch.randn(16, V, device="cuda", generator=gen(1))
     x[0] = 0.5                                            # all equal: the first ids, log p = -log V
@@ -108,6 +110,7 @@ def test_logprobs_of_special_rows():
     x[14, 5] = 1000.0                                     # all but certain
     x[15] = math.nan
     tokens = torch.tensor([0, 5, 0, 2, 3, 4, 9, 200, 1, 2999, 0, 7, 3, 11, 5, 1], device="cuda")
+    x, tokens = x.repeat(times, 1), tokens.repeat(times)
     check_logprobs(x, tokens, 20)
     lp, h, tl, ids = ops.token_logprobs(x, tokens, top=3)
     assert lp[0].item() == pytest.approx(-math.log(V), abs=1e-6) and ids[0].tolist() == [0, 1, 2]
