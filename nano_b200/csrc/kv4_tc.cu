@@ -3,8 +3,9 @@
 // A block owns 128 rows (query token, query head) of one key/value head and walks their keys in tiles of 128, four pages.  Seven warps make a tile's operands from the codes,
 // by the page: a word of eight key codes is one 16-byte piece of a row of the swizzled key operand (the queries are laid out in the nibbles' order, so that nothing is
 // shuffled), eight tokens' codes of a coordinate one piece of a row of the value operand, both as c s + m in fp16, rounded once; two tiles' operands have room.  One thread
-// issues tcgen05.mma -- scores into tensor memory, two buffers, and weights (fp16, where the scores were) times values onto the running sum there -- and four warps do the
-// softmax, a thread to a row, which holds its 128 scores in registers; their exponentials are the bound (1024 cycles a tile).
+// issues tcgen05.mma -- scores into tensor memory, two buffers, and weights (fp16, where the scores were) times values onto the running sum there -- and eight warps do the
+// softmax, two threads to a row with 64 of its scores in registers each (one thread to a row: 46 us instead of 41 for 1000 tokens of 16 heads of 64 over 4 behind 3100 and a window of 2500,
+// 58 instead of 51 with a soft cap).
 // Every wait has a limit; a block in which one runs out leaves with NaN in its rows (nothing but its own products is ever in flight).
 // Softmax as in k_kv4_attn: log2 units, weights times 2^kLift, a reference that is renewed when it lags kSlack behind the maximum, so that the sums in tensor memory
 // are seldom touched.
@@ -20,11 +21,16 @@
 namespace nb {
 namespace {
 
-constexpr uint32_t kTile = 128, kPages = kTile / kKv4Page, kThreads = 384, kMmaWarp = 4, kMakers = 5, kProducers = 7;          // warps 0-3: softmax, 4: products, 5-11: operands
+constexpr uint32_t kTile = 128, kPages = kTile / kKv4Page, kThreads = 512, kSoft = 8, kMmaWarp = 8, kMakers = 9, kProducers = 7;          // warps 0-7: softmax, 8: products, 9-15: operands
+constexpr uint32_t kKeys = kTile / 2;          // of a tile, to a thread of the softmax
 constexpr float kLift = 12.0f;
 // byte of the 16-byte piece c8 (8 fp16) of row r in an operand of 64-wide blocks of `rows` rows, 128-byte swizzle
 __device__ __forceinline__ uint32_t op_byte(uint32_t rows, uint32_t r, uint32_t c8) { return (c8 >> 3) * rows * 128u + r * 128u + (((c8 & 7u) ^ (r & 7u)) << 4); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// waits that mostly find what they wait for there: the first try without the clock
+__device__ __forceinline__ bool soon(uint32_t bar, uint32_t parity) { return mbar_try(bar, parity) || mbar_wait(bar, parity); }
+__device__ __forceinline__ bool soon_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, soon(bar, parity)); }
 
 template <int NG> struct Sizes {
     static constexpr uint32_t D = 32u * NG, DP = NG <= 2 ? 64u : 128u;          // coordinates; those that an operand of queries or keys has room for
@@ -41,7 +47,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     __shared__ __align__(8) uint64_t bars[NBAR];
     __shared__ uint32_t tmem_s;
     __shared__ uint32_t hide_s[4][kPages], odd_s[4][kPages];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys whose values are no number
-    __shared__ float scale_s[kTile];
+    __shared__ float scale_s[kTile], top_s[2][kTile], sum_s[2][kTile];          // (what two warps that share rows tell each other)
+    __shared__ uint32_t ok_s[2][kSoft];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t qs = (smem_u32(tc_raw) + 1023u) & ~1023u, ks = qs + Z::qk, vs = ks + 2u * Z::qk;
     unsigned char *base = tc_raw + (qs - smem_u32(tc_raw));
@@ -50,7 +57,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     const uint32_t b0 = smem_u32(bars);
     auto bar = [&](uint32_t i) { return b0 + i * 8u; };
     if (tid == 0) {
-        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i < KFREE || (i >= VFULL && i < VFREE) ? kPages : i >= PREADY && i < ODONE ? 4u : 1u);
+        for (uint32_t i = 0; i < NBAR; i++) mbar_init(bar(i), i < KFREE || (i >= VFULL && i < VFREE) ? kPages : i >= PREADY && i < ODONE ? kSoft : 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) { tc_alloc(smem_u32(&tmem_s), 512); tc_relinquish(); }
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             constexpr uint32_t id_s = (1u << 4) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24), id_o = (1u << 4) | ((D >> 3) << 17) | ((kTile >> 4) << 24);      // fp32 += f16 x f16
             auto scores = [&](uint32_t i) {
                 const uint32_t s = i & 1u;
-                if (!mbar_wait(bar(KFULL + s), (i >> 1) & 1u)) return false;
+                if (!soon(bar(KFULL + s), (i >> 1) & 1u)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < 2u * NG; k++) {
@@ -120,14 +127,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             bool ok = scores(0) && (n < 2u || scores(1));
             for (uint32_t i = 0; i < n && ok; i++) {
                 const uint32_t s = i & 1u;
-                ok = mbar_wait(bar(VFULL + s), (i >> 1) & 1u) && mbar_wait(bar(PREADY + s), (i >> 1) & 1u);
+                ok = soon(bar(VFULL + s), (i >> 1) & 1u) && soon(bar(PREADY + s), (i >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < kTile / 16u; k++)
                     tc_mma_ts(tmem + OCOL, tmem + s * kTile + k * 8u, tc_desc(vs + s * Z::v + (k >> 2) * D * 128u + (k & 3u) * 32u), id_o, i > 0 || k > 0);
                 tc_commit(bar(VFREE + s)); tc_commit(bar(ODONE));
-                if (i + 2u < n) ok = mbar_wait(bar(ODONE), s) && scores(i + 2u);          // they overwrite the weights that the products before read
+                if (i + 2u < n) ok = soon(bar(ODONE), s) && scores(i + 2u);          // they overwrite the weights that the products before read
             }
         }
     } else if (warp >= kMakers) {
@@ -160,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
 #pragma unroll
                     for (int j = 0; j < 4 * NG; j++) kw[j] = 0u;
                 }
-                if (i >= 2u && !mbar_wait_warp(bar(KFREE + s), ((i >> 1) - 1u) & 1u)) break;
+                if (i >= 2u && !soon_warp(bar(KFREE + s), ((i >> 1) - 1u) & 1u)) break;
                 unsigned char *k_s = base + (1u + s) * Z::qk;
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
@@ -203,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
 #pragma unroll
                         for (int j = 0; j < NG; j++) vp[t][j] = 0u;
                 }
-                if (i >= 2u && !mbar_wait_warp(bar(VFREE + s), ((i >> 1) - 1u) & 1u)) break;
+                if (i >= 2u && !soon_warp(bar(VFREE + s), ((i >> 1) - 1u) & 1u)) break;
                 unsigned char *v_s = base + 3u * Z::qk + s * Z::v;
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
@@ -224,9 +231,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             page = next;
         }
     } else {
-        const uint32_t r = warp * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep;
+        // Two threads to a row: warps w and w + 4 share 32 rows, keys 0-63 and 64-127 of a tile.  They meet once a tile, when both hold their scores and the weights may take their
+        // place, and tell each other more only where the reference moves or a wait ran out
+        const uint32_t half = warp >> 2, r = (warp & 3u) * 32u + lane, rr = min(r0 + r, last), t = rr / rep, h = g * rep + rr % rep, id = 1u + (warp & 3u);
         const int pos = pos_0 + (int)t, low = first_seen(max(pos, 0), a.window, a.block), low_last = first_seen(max(last_pos, 0), a.window, a.block);
-        const uint32_t lanes = (warp * 32u) << 16, o_at = tmem + lanes + OCOL;
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16, o_at = tmem + lanes + OCOL;
         const float kc = scale_s[r], cap = a.softcap * kLog2e, kk = kc * kc;
         // the soft cap of a score x near 0 is x (c0 + c1 x^2 + c2 x^4 + c3 x^6); factors whose powers leave fp32 take the other way
         const float c0 = cap * kTanh0 * kc, c1 = cap * kTanh1 * kc * kk, c2 = cap * kTanh2 * kc * kk * kk, c3 = cap * kTanh3 * kc * kk * kk * kk, limit = kc > 1e-4f && kc < 1e4f ? kTanhNear / kc : 0.0f;
@@ -235,53 +244,59 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
         for (uint32_t i = 0; i < n; i++) {
             const int key0 = (int)((lo + i) * kTile);
             const uint32_t s_at = tmem + lanes + (i & 1u) * kTile;
-            ok = mbar_wait_warp(bar(SFULL + (i & 1u)), (i >> 1) & 1u);
-            if (!ok) break;
+            ok = ok && soon_warp(bar(SFULL + (i & 1u)), (i >> 1) & 1u);
             tc_fence_after();
-            uint32_t w[kTile];
-            tc_ld128(s_at, w);
+            uint32_t w[kKeys];
+            tc_ld64(s_at + half * kKeys, w);
             uint32_t hide = 0, odd = 0;
 #pragma unroll
-            for (int u = 0; u < 4; u++) { hide |= hide_s[i & 3u][u]; odd |= odd_s[i & 3u][u]; }
+            for (uint32_t u = 0; u < kPages; u++) hide |= hide_s[i & 3u][u];
+#pragma unroll
+            for (uint32_t u = 0; u < 2; u++) odd |= odd_s[i & 3u][half * 2u + u];
             const bool whole = key0 + (int)kTile - 1 <= first_pos && key0 >= low_last && hide == 0;          // every row of the block sees every key
             auto sees = [&](uint32_t u) {          // of 32 keys those that this row sees
-                const int at = key0 + 32 * (int)u, from = low - at, to = pos - at;          // places [from, to]
+                const int at = key0 + 32 * (int)(half * 2u + u), from = low - at, to = pos - at;          // places [from, to]
                 uint32_t v = to < 0 || from > 31 ? 0u : 0xffffffffu;
                 if (to >= 0 && to < 31) v &= (2u << to) - 1u;
                 if (from > 0 && from <= 31) v &= 0xffffffffu << from;
-                return v & ~hide_s[i & 3u][u];
+                return v & ~hide_s[i & 3u][half * 2u + u];
             };
             if (!whole)
 #pragma unroll
-                for (uint32_t u = 0; u < 4; u++) {
+                for (uint32_t u = 0; u < 2; u++) {
                     const uint32_t see = sees(u);
 #pragma unroll
                     for (uint32_t j = 0; j < 32; j++) w[u * 32u + j] = see >> j & 1u ? w[u * 32u + j] : 0xff800000u;
                 }
-            float top = -INFINITY, far = 0.0f;
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, fars[4] = {};          // (four at a time: one after the other, each would wait for the one before)
 #pragma unroll
-            for (uint32_t j = 0; j < kTile; j += 2) top = max3(top, __uint_as_float(w[j]), __uint_as_float(w[j + 1]));
+            for (uint32_t j = 0; j < kKeys; j += 2) tops[j / 2 & 3u] = max3(tops[j / 2 & 3u], __uint_as_float(w[j]), __uint_as_float(w[j + 1]));
+            float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
             bool near = false;          // scores whose soft cap is a polynomial, taken where the weights are made
             if (a.softcap > 0.0f) {
 #pragma unroll
-                for (uint32_t j = 0; j < kTile; j += 2) far = max3(far, fabsf(__uint_as_float(w[j])), fabsf(__uint_as_float(w[j + 1])));
-                near = __all_sync(0xffffffffu, far < limit);
+                for (uint32_t j = 0; j < kKeys; j += 2) fars[j / 2 & 3u] = max3(fars[j / 2 & 3u], fabsf(__uint_as_float(w[j])), fabsf(__uint_as_float(w[j + 1])));
+                near = __all_sync(0xffffffffu, fmaxf(max3(fars[0], fars[1], fars[2]), fars[3]) < limit);
                 if (!near)
 #pragma unroll
-                    for (uint32_t j = 0; j < kTile; j++) w[j] = w[j] == 0xff800000u ? w[j] : __float_as_uint(tanh_any(__uint_as_float(w[j]) * kc));
+                    for (uint32_t j = 0; j < kKeys; j++) w[j] = w[j] == 0xff800000u ? w[j] : __float_as_uint(tanh_any(__uint_as_float(w[j]) * kc));
             }
             if (top != -INFINITY) { top *= kc; if (a.softcap > 0.0f) top = cap * tanh_any(top); }
-            if (__any_sync(0xffffffffu, top > m + kSlack)) {          // (m = -inf: top is taken, if there is one)
+            if (bar_any(id, 64u, !ok || top > m + kSlack)) {          // (m = -inf: top is taken, if there is one)
+                top_s[half][r] = top;
+                if (lane == 0) ok_s[0][warp] = ok;
+                bar_any(id, 64u, false);
+                if (!(ok = ok && ok_s[0][warp ^ 4u])) break;          // both leave
+                top = fmaxf(top, top_s[half ^ 1u][r]);
                 const float next = top > m + kSlack ? top : m, corr = next == m ? 1.0f : ex2(m - next);
                 l *= corr;
                 m = next;
-                if (i) {          // the sums move to the new reference, once the products before are done
-                    ok = mbar_wait_warp(bar(ODONE), (i - 1u) & 1u);
-                    if (!ok) break;
+                if (i) {          // the sums move to the new reference, once the products before are done; half of the columns each
+                    ok = soon_warp(bar(ODONE), (i - 1u) & 1u);
                     tc_fence_after();
                     const pair_t k = pair(corr, corr);
 #pragma unroll 1
-                    for (uint32_t c = 0; c < D; c += 16u) {
+                    for (uint32_t c = half * (D / 2u); ok && c < (half + 1u) * (D / 2u); c += 16u) {
                         uint32_t v[16];
                         tc_ld16(o_at + c, v);
 #pragma unroll
@@ -301,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             pair_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
             auto weights = [&](auto capped) {
 #pragma unroll
-                for (uint32_t u = 0; u < 4; u++) {
+                for (uint32_t u = 0; u < 2; u++) {
                     uint32_t wh[16];
 #pragma unroll
                     for (uint32_t j = 0; j < 16; j++) {
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
                         s2[j & 1u] = add2(s2[j & 1u], pair(y, z));
                         wh[j] = bits(__floats2half2_rn(y, z));
                     }
-                    tc_st16(s_at + u * 16u, wh);
+                    tc_st16(s_at + half * (kKeys / 2u) + u * 16u, wh);
                 }
             };
             if (near) weights(std::true_type{}); else weights(std::false_type{});
@@ -324,32 +339,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             l += s0 + s1;
             if (odd)          // values that are no number make the rows that see them NaN, however little they weigh
 #pragma unroll 1
-                for (uint32_t u = 0; u < 4; u++) if (odd_s[i & 3u][u] & sees(u)) l = NAN;
+                for (uint32_t u = 0; u < 2; u++) if (odd_s[i & 3u][half * 2u + u] & sees(u)) l = NAN;
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(PREADY + (i & 1u)));
         }
         // (a tile's scores come after the products of the tile two before it: of the last two products this is known of neither)
-        if (ok && n > 1u) ok = mbar_wait_warp(bar(ODONE), (n - 2u) & 1u);
-        if (ok && n) { ok = mbar_wait_warp(bar(ODONE), (n - 1u) & 1u); tc_fence_after(); }
-        const float ref = m - kLift, sum = ok ? l : NAN;          // a wait that ran out shows as NaN
+        if (ok && n > 1u) ok = soon_warp(bar(ODONE), (n - 2u) & 1u);
+        if (ok && n) { ok = soon_warp(bar(ODONE), (n - 1u) & 1u); tc_fence_after(); }
+        sum_s[half][r] = l;
+        if (lane == 0) ok_s[1][warp] = ok;
+        bar_any(id, 64u, false);
+        ok = ok && ok_s[1][warp ^ 4u];
+        const float ref = m - kLift, sum = ok ? l + sum_s[half ^ 1u][r] : NAN;          // a wait that ran out shows as NaN
         const bool mine = r0 + r <= last;
         const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols + r;
         const float k = sh.nsplit > 1 ? 1.0f : last_factor(a, t, h, ref, sum);
 #pragma unroll 1
-        for (uint32_t c = 0; c < D; c += 32u) {
-            uint32_t w[32] = {};
-            if (n && ok) tc_ld32(o_at + c, w);
+        for (uint32_t c = half * (D / 2u); c < (half + 1u) * (D / 2u); c += 16u) {
+            uint32_t w[16] = {};
+            if (n && ok) tc_ld16(o_at + c, w);
             if (mine)
 #pragma unroll
-                for (uint32_t j = 0; j < 32; j += 4) {
+                for (uint32_t j = 0; j < 16; j += 4) {
                     const float4 v = make_float4(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), __uint_as_float(w[j + 2]), __uint_as_float(w[j + 3]));
                     if (sh.nsplit > 1) *reinterpret_cast<float4 *>(a.part + where * D + c + j) = v;
                     else store_four(a, b, t, h, c + j, v.x * k, v.y * k, v.z * k, v.w * k);
                 }
         }
-        if (mine && sh.nsplit > 1) reinterpret_cast<float2 *>(a.part + part_places(a, sh) * D)[where] = make_float2(ref, sum);
+        if (half == 0 && mine && sh.nsplit > 1) reinterpret_cast<float2 *>(a.part + part_places(a, sh) * D)[where] = make_float2(ref, sum);
     }
     tc_fence_before();
     __syncthreads();

@@ -121,17 +121,21 @@ def test_a_cache_in_4_bits_is_refused_for_model_files():
 
 
 def test_waits_of_the_portion_kernel_end_for_a_warp_as_a_whole():
-    """What a block of k_kv4_attn_tc does when a wait runs out is read from the source: whole warps get one verdict, leave their loop with it, and show it in their rows."""
+    """What a block of k_kv4_attn_tc does when a wait runs out is read from the source: whole warps get one verdict, two warps that meet at a barrier leave by what both know there, and it shows in
+    their rows."""
     text = re.sub(r"//.*", "", open(os.path.join(ROOT, "nano_b200", "csrc", "kv4_tc.cu")).read())
     body = text[text.index("} else if (warp >= kMakers) {"):text.index("tc_dealloc")]
-    loops = body[:body.index("const float ref = m - kLift")]
-    waits = re.findall(r"mbar_wait\w*\(", loops)
-    assert len(waits) == 6 and set(waits) == {"mbar_wait_warp("}, "a wait without one verdict for the warp"
-    assert len(re.findall(r"!mbar_wait_warp\([^;]*\)\) break;", loops)) == 2 and len(re.findall(r"ok = mbar_wait_warp\([^;]*\);\s*if \(!ok\) break;", loops)) == 2
-    assert "__syncthreads" not in loops and "bar.sync" not in loops
-    assert "sum = ok ? l : NAN" in body and "if (n && ok) tc_ld32" in body
+    makers, softmax = body.split("const uint32_t half = warp >> 2", 1)
+    loop, end = softmax.split("sum_s[half][r] = l;", 1)
+    waits = re.findall(r"(?:mbar_wait|soon)\w*\(", makers)
+    assert len(waits) == 2 and set(waits) == {"soon_warp("} and len(re.findall(r"!soon_warp\([^;]*\)\) break;", makers)) == 2
+    waits = re.findall(r"(?:mbar_wait|soon)\w*\(", loop)
+    assert len(waits) == 4 and set(waits) == {"soon_warp("}, "a wait without one verdict for the warp"
+    assert "__syncthreads" not in body and "bar.sync" not in body and loop.count("break;") == 1
+    assert "if (!(ok = ok && ok_s[0][warp ^ 4u])) break;" in loop and "bar_any(id, 64u, !ok || top > m + kSlack)" in loop, "warps that part over a barrier"
+    assert "ok = ok && ok_s[1][warp ^ 4u];" in end and "NAN;" in end and "if (n && ok) tc_ld16" in end
     one = text[text.index("auto scores = [&](uint32_t i)"):text.index("} else if (warp >= kMakers) {")]          # the thread that issues the products
-    assert len(re.findall(r"mbar_wait\(", one)) == 4 and "mbar_wait_warp" not in one and "if (!ok) break;" in one and "i < n && ok" in one
+    assert len(re.findall(r"soon\(", one)) == 4 and "soon_warp" not in one and "if (!ok) break;" in one and "i < n && ok" in one
 
 
 @pytest.mark.skipif(E.device_count() > 0, reason="box has a GPU")
