@@ -131,7 +131,7 @@ def test_waits_of_the_portion_kernel_end_for_a_warp_as_a_whole():
     assert len(waits) == 2 and set(waits) == {"soon_warp("} and len(re.findall(r"!soon_warp\([^;]*\)\) break;", makers)) == 2
     waits = re.findall(r"(?:mbar_wait|soon)\w*\(", loop)
     assert len(waits) == 4 and set(waits) == {"soon_warp("}, "a wait without one verdict for the warp"
-    assert "__syncthreads" not in body and "bar.sync" not in body and loop.count("break;") == 1
+    assert "__syncthreads" not in makers + loop and "bar.sync" not in body and loop.count("break;") == 1
     assert "if (!(ok = ok && ok_s[0][warp ^ 4u])) break;" in loop and "bar_any(id, 64u, !ok || top > m + kSlack)" in loop, "warps that part over a barrier"
     assert "ok = ok && ok_s[1][warp ^ 4u];" in end and "NAN;" in end and "if (n && ok) tc_ld16" in end
     one = text[text.index("auto scores = [&](uint32_t i)"):text.index("} else if (warp >= kMakers) {")]          # the thread that issues the products
