@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
     using Z = Sizes<NG>;
     constexpr uint32_t D = Z::D;
     extern __shared__ uint8_t tc_raw[];
-    enum { KFULL = 0, KFREE = 2, VFULL = 4, VFREE = 6, SFULL = 8, PREADY = 10, ODONE = 12, NBAR };          // (two each but the last: one for a buffer.  PREADY too: a warp may be a tile ahead of the others)
+    enum { KFULL = 0, KFREE = 2, VFULL = 4, VFREE = 6, SFULL = 8, PREADY = 10, ODONE = 12, NBAR = 14 };          // two each, tiles in turn.  (PREADY: a warp may be a tile ahead of the others; ODONE: nobody need have seen the tile before last's)
     __shared__ __align__(8) uint64_t bars[NBAR];
     __shared__ uint32_t tmem_s;
     __shared__ uint32_t hide_s[4][kPages], odd_s[4][kPages];          // of a tile's pages (four tiles in turn): keys that nobody sees, keys whose values are no number
@@ -133,8 +133,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
 #pragma unroll
                 for (uint32_t k = 0; k < kTile / 16u; k++)
                     tc_mma_ts(tmem + OCOL, tmem + s * kTile + k * 8u, tc_desc(vs + s * Z::v + (k >> 2) * D * 128u + (k & 3u) * 32u), id_o, i > 0 || k > 0);
-                tc_commit(bar(VFREE + s)); tc_commit(bar(ODONE));
-                if (i + 2u < n) ok = soon(bar(ODONE), s) && scores(i + 2u);          // they overwrite the weights that the products before read
+                tc_commit(bar(VFREE + s)); tc_commit(bar(ODONE + s));
+                if (i + 2u < n) ok = soon(bar(ODONE + s), (i >> 1) & 1u) && scores(i + 2u);          // they overwrite the weights that the products before read
             }
         }
     } else if (warp >= kMakers) {
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
                 l *= corr;
                 m = next;
                 if (i) {          // the sums move to the new reference, once the products before are done; half of the columns each
-                    ok = soon_warp(bar(ODONE), (i - 1u) & 1u);
+                    ok = soon_warp(bar(ODONE + ((i - 1u) & 1u)), ((i - 1u) >> 1) & 1u);
                     tc_fence_after();
                     const pair_t k = pair(corr, corr);
 #pragma unroll 1
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
             if (lane == 0) mbar_arrive(bar(PREADY + (i & 1u)));
         }
         // (a tile's scores come after the products of the tile two before it: of the last two products this is known of neither)
-        if (ok && n > 1u) ok = soon_warp(bar(ODONE), (n - 2u) & 1u);
-        if (ok && n) { ok = soon_warp(bar(ODONE), (n - 1u) & 1u); tc_fence_after(); }
+        if (ok && n > 1u) ok = soon_warp(bar(ODONE + (n & 1u)), ((n - 2u) >> 1) & 1u);
+        if (ok && n) { ok = soon_warp(bar(ODONE + ((n - 1u) & 1u)), ((n - 1u) >> 1) & 1u); tc_fence_after(); }
         sum_s[half][r] = l;
         if (lane == 0) ok_s[1][warp] = ok;
         bar_any(id, 64u, false);
