@@ -5,6 +5,9 @@ terms one after the other (at most 2^-24 each), two dozen joins and the exponent
 A cache in 4 bits is exact: its codes, pairs and values are fixed numbers.  Attention rounds keys, values, queries and weights to 11 significant bits (half a step
 2^-11 each) and the output to its type."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -591,3 +594,45 @@ def test_on_two_streams_at_once():
     torch.cuda.synchronize()
     for x, y in zip(got, want):
         assert all(torch.equal(p.view(torch.uint8), r.view(torch.uint8)) for p, r in zip(x, y))
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from nano_b200 import ops
+import test_gpu_device_ops as t
+g = t.gen(7)
+pool = ops.kv4_cache(40, 2, 64)
+table = torch.arange(40, dtype=torch.int32, device="cuda").view(1, 40)
+k, v = (torch.randn(1280, 2, 64, device="cuda", generator=g) for _ in "kv")
+slots = torch.arange(1280, dtype=torch.int32, device="cuda")
+q = torch.randn(1, 300, 8, 64, device="cuda", generator=g).bfloat16()
+lens = torch.tensor([1275], dtype=torch.int32, device="cuda")
+w = torch.randn(512, 40001, device="cuda", generator=g).bfloat16()
+x, tokens = torch.zeros(1, 40001, device="cuda"), torch.tensor([5], device="cuda")
+
+def run():
+    ops.kv4_write(pool, k, v, slots)
+    one = ops.kv4_attention(q[:, -1:], pool, table, lens)
+    many = ops.kv4_attention(q, pool, table, lens)
+    ops.pages_copy([pool], [0], [39])
+    return one, many, *ops.token_logprobs(x, tokens, top=5), *ops.token_logprobs(x.bfloat16(), tokens), *ops.kv4_read(pool, slots[:64])
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+got = [y.clone() for y in got]
+pool.zero_()
+assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, run()))
+print("the same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=os.path.dirname(here), tests=here)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
