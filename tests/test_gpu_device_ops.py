@@ -1,7 +1,7 @@
 """Operators on device memory (nano_b200.ops) against their definitions in 64 bits, at the sizes, masks, strides and values where they can go wrong.
 
-Tolerances.  log p = (x - M) - log Z: the fp32 result rounds x - M and the difference once each, log Z carries the relative error of Z.  A thread adds k = vocab / threads
-terms one after the other (at most 2^-24 each), two dozen joins and the exponential (2^-22, and 2 |d| 2^-24 for its argument d = x - M, weighted by exp d) add the rest.
+Tolerances.  log p = (x - M) - log Z: the fp32 result rounds x - M and the difference once each, log Z carries the relative error of Z.  A thread adds k = vocab / 512
+terms one after the other (256 threads, pairs of numbers; with 128 threads, only below 32768 numbers, vocab / 256, which is at most 64 more) (at most 2^-24 each), two dozen joins and the exponential (2^-22, and 2 |d| 2^-24 for its argument d = x - M, weighted by exp d) add the rest.
 A cache in 4 bits is exact: its codes, pairs and values are fixed numbers.  Attention rounds keys, values, queries and weights to 11 significant bits (half a step
 2^-11 each) and the output to its type."""
 import math
