@@ -233,7 +233,7 @@ __device__ __forceinline__ uint32_t longest(const Kv4Attn &a, uint32_t before) {
 
 // grid (nsplit x tiles, G, B); part: values [B][G][tiles][nsplit][columns of a block][D], then (m, l) of each
 template <int NG, int NT, int WK, int W>
-__global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT)) k_kv4_attn(const Kv4Attn a, const Shape sh) {
+__global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT) * 4 / W > 1 ? kv4_blocks(NG, NT) * 4 / W : 1) k_kv4_attn(const Kv4Attn a, const Shape sh) {
     pdl_enter4();
     using R = Room<NG, NT, WK, W>;
     constexpr uint32_t D = 32u * NG, COLS = NT * 8u;
@@ -655,8 +655,8 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 }
 
 // ---- which instance, and how the work is shared out ----
-struct Plan { int nt; bool rows, tc; Shape sh; };
-constexpr uint32_t kWarps = 4, kWaves = 3, kMost = 64, kTcCols = 17;
+struct Plan { int nt; bool rows, tc, wide; Shape sh; };
+constexpr uint32_t kWarps = 4, kWide = 8, kShort = 32, kWaves = 3, kMost = 64, kTcCols = 17;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G);
     Plan p{};
@@ -677,16 +677,21 @@ Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32
     uint64_t n = places / blocks;
     if (B > 1) n = std::max(n, std::min<uint64_t>((pages + kMost - 1u) / kMost, kWaves * places / blocks));
     p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(n, std::max(1u, pages / least)));
+    // Few blocks with few pages each: twice the warps and no parts to be joined.  One token of 16 heads of 128 over 8 behind 400: 7.6 us instead of 8.9, behind 777 10.3 instead of 8.9, but one launch
+    // and no workspace: calls in a row take 12.2 us instead of 16.8.  (Sixteen warps: 7.8 and 9.7, behind 60 tokens 6.5 instead of 5.6.)  Heads of 256 behind 400 11.2 instead of 11.3, behind 777
+    // 15.5 instead of 11.5
+    p.wide = !p.tc && !p.rows && pages <= (D > 128u ? kShort / 2u : kShort) && blocks <= sms;
+    if (p.wide) p.sh.nsplit = 1;
     // Of up to 64 sequences the longest first, so that the SMs get long and short ones alike and what is left when others end is short (32 of up to 8190 tokens: 50 us, in the given
     // order 56; 64 of up to 4000, 4 heads of 64: 25 and 28).  It costs some 0.9 us of a block's start: not for blocks of less than 16 pages (48 of up to 1000: 10.6 us, sorted 11.5)
     p.sh.sorted = !p.tc && B > 1 && B <= 64 && pages >= 16u * p.sh.nsplit ? 1u : 0u;
     return p;
 }
 
-template <int NG, int NT, int WK>
+template <int NG, int NT, int WK, int W = kWarps>
 cudaError_t attn_launch(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, bool pdl) {
-    constexpr int smem = (int)Room<NG, NT, WK, kWarps>::all;
-    const auto k = k_kv4_attn<NG, NT, WK, kWarps>;
+    constexpr int smem = (int)Room<NG, NT, WK, W>::all;
+    const auto k = k_kv4_attn<NG, NT, WK, W>;
     static std::atomic<uint64_t> asked{0};          // devices (of the first 64) whose limit has been raised: asking costs a microsecond
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -694,11 +699,12 @@ cudaError_t attn_launch(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, 
         e = smem_at_least(reinterpret_cast<const void *>(k), smem);
         if (e == cudaSuccess && dev <= 63) asked.fetch_or(1ull << dev, std::memory_order_release);
     }
-    return e != cudaSuccess ? e : launch_on(k, dim3(sh.nsplit * sh.tiles, a.G, a.B), kWarps * 32, smem, stream, pdl, a, sh);
+    return e != cudaSuccess ? e : launch_on(k, dim3(sh.nsplit * sh.tiles, a.G, a.B), W * 32, smem, stream, pdl, a, sh);
 }
 template <int NG>
 cudaError_t attn_launch_nt(const Kv4Attn &a, const Plan &p, cudaStream_t stream, bool pdl) {
     if (p.rows) return attn_launch<NG, 2, 1>(a, p.sh, stream, pdl);
+    if (p.wide) return p.nt == 1 ? attn_launch<NG, 1, kWide, kWide>(a, p.sh, stream, pdl) : attn_launch<NG, 2, kWide, kWide>(a, p.sh, stream, pdl);
     return p.nt == 1 ? attn_launch<NG, 1, kWarps>(a, p.sh, stream, pdl) : attn_launch<NG, 2, kWarps>(a, p.sh, stream, pdl);
 }
 

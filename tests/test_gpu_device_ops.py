@@ -378,7 +378,21 @@ def test_kv4_attention_of_single_tokens(kind, dim, heads, kv_heads):
     check_attention(q, pool, table, lens)
 
 
-@pytest.mark.parametrize("batch,width,tokens", [(20, 60, 1), (32, 40, 1), (33, 40, 2), (64, 20, 1), (65, 20, 1)])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("heads,tokens", [(4, 1), (4, 2), (16, 1), (5, 3)])
+@pytest.mark.parametrize("width", [1, 5, 14])
+def test_kv4_attention_of_short_contexts(dim, heads, tokens, width):
+    g = gen(dim + width)
+    pool = filled(g, 3 * width, 1, dim)
+    table = torch.randperm(3 * width, device="cuda", generator=g).view(3, width).int()
+    table[1, width // 2] = 3 * width + 5          # (a page that is none of the pool's)
+    lens = torch.tensor([32 * width, 32 * width - 7, 1], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, tokens, heads, dim, device="cuda", generator=g).bfloat16()
+    check_attention(q, pool, table, lens)
+    check_attention(q, pool, table, lens, window=50, softcap=9.0, sinks=torch.randn(heads, device="cuda", generator=g))
+
+
+@pytest.mark.parametrize("batch,width,tokens", [(9, 24, 1), (17, 31, 1), (20, 60, 1), (32, 40, 1), (33, 40, 2), (64, 20, 1), (65, 20, 1)])
 def test_kv4_attention_of_many_sequences(batch, width, tokens):
     """Lengths of all kinds, equal ones, none at all, below zero and beyond the table among them, whatever order their blocks run in."""
     g = gen(batch)
