@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
         // operands: a tile is eight pieces of work, the keys and then the values of its four pages, dealt out to seven warps in turn
         const uint32_t eight = lane >> 3, bv = lane & 7u;
         const int32_t *table = a.table + (uint64_t)b * a.table_stride;
+        const int low_first = first_seen(max(first_pos, 0), a.window, a.block);          // the block's rows see the keys from here to last_pos, each at least one of them
         auto number = [&](uint32_t q) {          // the page of piece q (a length is no more than the table's width allows)
             const uint32_t p = (lo + q / (2u * kPages)) * kPages + q % kPages;
             return q < n * 2u * kPages && (int)(p * kKv4Page) <= last_pos ? (uint32_t)table[p] : 0xffffffffu;
@@ -200,6 +201,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
                         for (int j = 0; j < (NG + 1) / 2; j++) vw[t][j] = 0u;
                     }
                 }
+                // Tokens that no row sees hold any bytes: their weights are 0, but c s + m may be beyond fp16, and 0 times infinity is no number
+                const int key = (int)((lo + i) * kTile + pw * kKv4Page + eight * 8u);
+                if (key + 7 > last_pos || key < low_first)
+#pragma unroll
+                    for (uint32_t t = 0; t < 8; t++)
+                        if (key + (int)t > last_pos || key + (int)t < low_first)
+#pragma unroll
+                            for (int j = 0; j < NG; j++) vp[t][j] = 0u;
                 // tokens whose pairs are no numbers would spoil rows that do not see them
 #pragma unroll
                 for (uint32_t t = 0; t < 8; t++) {
