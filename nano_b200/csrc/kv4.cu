@@ -371,10 +371,13 @@ __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT) * 4 / W > 1 ? kv4_b
                 for (int j = 0; j < NG; j++) { zero = __hfma2(half2_of(w[j]), __float2half2_rn(0.0f), zero); big = fmaxf(big, fabsf(__low2float(half2_of(w[j])))); }
                 const bool odd = !__hbeq2(zero, __float2half2_rn(0.0f));
                 bad = __ballot_sync(0xffffffffu, odd);
+                // (a token that no column sees weighs nothing, whatever its step: the room, and with it the roundings, does not follow from it)
+                const int at = key0 + (int)lane;
+                const bool seen = whole || (at <= pos_b && at >= first_seen(max(pos_a, 0), a.window, a.block));
                 if (odd)
 #pragma unroll
                     for (int j = 0; j < NG; j++) reinterpret_cast<uint32_t *>(pg + 1152u * NG + lane * 4u * NG)[j] = 0u;
-                big = odd ? 0.0f : big;
+                big = odd || !seen ? 0.0f : big;
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
                 if (big >= 2.0f) {
@@ -425,33 +428,34 @@ __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT) * 4 / W > 1 ? kv4_b
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float top[2] = {-INFINITY, -INFINITY};
-            if (a.softcap > 0.0f) {
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) { s[k][t][x] *= f[t][x & 1]; top[0] = fmaxf(top[0], fabsf(s[k][t][x])); }
-                const bool near = __all_sync(0xffffffffu, top[0] < kTanhNear);          // (a NaN goes through either)
-                top[0] = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) s[k][t][x] = a.softcap * kLog2e * (near ? tanh_near(s[k][t][x]) : tanh_any(s[k][t][x]));
-            } else {
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) s[k][t][x] *= f[t][x & 1];
-            }
-            if (!whole) {
+            auto hide = [&](float as) {          // the scores of keys that a column does not see
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     const int low = first_seen(max(pos[t][x], 0), a.window, a.block) - key0 - (int)row, high = pos[t][x] - key0 - (int)row;          // of the rows 16 k + 8 y
 #pragma unroll
                     for (int k = 0; k < 2; k++)
 #pragma unroll
-                        for (int y = 0; y < 2; y++) if (k * 16 + y * 8 > high || k * 16 + y * 8 < low) s[k][t][2 * y + x] = -INFINITY;
+                        for (int y = 0; y < 2; y++) if (k * 16 + y * 8 > high || k * 16 + y * 8 < low) s[k][t][2 * y + x] = as;
                 }
+            };
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) s[k][t][x] *= f[t][x & 1];
+            if (a.softcap > 0.0f) {
+                if (!whole) hide(0.0f);          // (which form tanh takes does not follow from them)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) top[0] = fmaxf(top[0], fabsf(s[k][t][x]));
+                const bool near = __all_sync(0xffffffffu, top[0] < kTanhNear);          // (a NaN goes through either)
+                top[0] = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) s[k][t][x] = a.softcap * kLog2e * (near ? tanh_near(s[k][t][x]) : tanh_any(s[k][t][x]));
             }
+            if (!whole) hide(-INFINITY);
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll

@@ -48,7 +48,8 @@ def put(pool, dim, places, kind, g):
 
 
 @pytest.mark.parametrize("kind", ["random", "large", "small", "steps", "far", "nan", "inf"])
-@pytest.mark.parametrize("dim,heads,kv_heads,tokens", [(128, 4, 2, 60), (64, 6, 2, 150), (32, 5, 1, 30), (96, 4, 2, 20)])
+@pytest.mark.parametrize("dim,heads,kv_heads,tokens", [(128, 4, 2, 60), (64, 6, 2, 150), (32, 5, 1, 30), (96, 4, 2, 20), (128, 4, 2, 1), (128, 8, 2, 3), (64, 8, 2, 4), (32, 5, 1, 1), (96, 2, 2, 1), (96, 6, 2, 3),
+                                                          (256, 4, 1, 1), (256, 4, 1, 4), (256, 6, 2, 50)])
 def test_bytes_that_nobody_sees(dim, heads, kv_heads, tokens, kind):
     g = gen(dim + tokens)
     pages = 40
