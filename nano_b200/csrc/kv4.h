@@ -43,6 +43,7 @@ struct Kv4Attn {
     uint32_t B, T, H, G, D; float scale, softcap; const float *sink; uint32_t window, block;
     const float *gate; uint32_t ldg;
     float *part;                                                               // kv4_attn_workspace bytes
+    uint32_t *err;                                                             // optional: receives a code where a wait inside a kernel ran out (its rows are NaN either way)
 };
 size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms);
 // the most that any call of B sequences asks for, whatever its tokens and its width

@@ -6,7 +6,7 @@
 // issues tcgen05.mma -- scores into tensor memory, two buffers, and weights (fp16, where the scores were) times values onto the running sum there -- and eight warps do the
 // softmax, two threads to a row with 64 of its scores in registers each (one thread to a row: 46 us instead of 41 for 1000 tokens of 16 heads of 64 over 4 behind 3100 and a window of 2500,
 // 58 instead of 51 with a soft cap).
-// Every wait has a limit; a block in which one runs out leaves with NaN in its rows (nothing but its own products is ever in flight).
+// Every wait has a limit; a block in which one runs out leaves with NaN in its rows (nothing but its own products is ever in flight) and a code in the engine's error word.
 // Softmax as in k_kv4_attn: log2 units, weights times 2^kLift, a reference that is renewed when it lags kSlack behind the maximum, so that the sums in tensor memory
 // are seldom touched.
 #include <algorithm>
@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_attn_tc(const Kv4Attn a, co
         if (lane == 0) ok_s[1][warp] = ok;
         bar_any(id, 64u, false);
         ok = ok && ok_s[1][warp ^ 4u];
+        if (!ok && lane == 0 && a.err) *a.err = 0x300u + warp;          // (whoever's wait it was: without scores and products those of these warps run out too)
         const float ref = m - kLift, sum = ok ? l + sum_s[half ^ 1u][r] : NAN;          // a wait that ran out shows as NaN
         const bool mine = r0 + r <= last;
         const uint64_t where = (((uint64_t)(b * a.G + g) * sh.tiles + tile) * sh.nsplit + split) * sh.cols + r;

@@ -1488,7 +1488,7 @@ int gqa_branch(LayeredEngine *e, const Layer &L, const Run &run, const Ctx &cx, 
         nb::Kv4Attn ka{};      // (queries carry the scale already)
         ka.q = e->b_p; ka.q_token = P; ka.q_head = D; ka.type = nb::T_F32; ka.out = e->b_a; ka.o_token = H * VD; ka.o_head = VD; ka.pool = kr.pool; ka.page_stride = kr.page_stride; ka.n_pages = e->n_pages;
         ka.table = reinterpret_cast<const int32_t *>(cx.table); ka.width = cx.pos_ptr ? e->n_pages : (cx.pos0 + T + kPage - 1u) / kPage; ka.pos0 = cx.pos0; ka.pos_ptr = cx.pos_ptr;
-        ka.B = 1; ka.T = T; ka.H = H; ka.G = G; ka.D = D; ka.scale = 1.0f; ka.softcap = L.softcap; ka.sink = L.sink; ka.block = L.block_size; ka.part = e->b_kpart;
+        ka.B = 1; ka.T = T; ka.H = H; ka.G = G; ka.D = D; ka.scale = 1.0f; ka.softcap = L.softcap; ka.sink = L.sink; ka.block = L.block_size; ka.part = e->b_kpart; ka.err = e->tc.err_dev;
         if (L.has_gate) { ka.gate = e->b_p + L.c_hg; ka.ldg = P; }
         uint32_t launches = 0;
         CK(nb::kv4_attn_launch(ka, (uint32_t)e->num_sms, e->cur, e->use_pdl, &launches));
@@ -2202,13 +2202,13 @@ int step_any(LayeredEngine *e, uint32_t seq, const uint32_t *tokens, uint32_t n,
             s.len += 1;
             CK(cudaStreamSynchronize(e->stream));
             memcpy(logits, e->stage_logits, (size_t)e->V * 4);
-            return 0;
+            return tc_check(&e->tc);
         }
         if ((r = set_step(e, s.len, tokens[0])) || (r = decode_step(e, seq))) return r;
         s.len += 1;
-        if (n_want) return score ? score_rows(e, 1, 0, *score) : fetch_logits(e, 1, logits);
+        if (n_want && (r = score ? score_rows(e, 1, 0, *score) : fetch_logits(e, 1, logits))) return r;
         CK(cudaStreamSynchronize(e->stream));
-        return 0;
+        return tc_check(&e->tc);
     }
     std::vector<uint32_t> done;
     for (uint32_t c0 = 0; c0 < n; c0 += e->max_tokens) {          // the staging buffer holds max_tokens ids
@@ -2988,6 +2988,7 @@ int create(LayeredEngine *e, const nb::ModelDir *dir, uint32_t max_tokens) {
         size_t w = std::max<size_t>(E, mTop * E);
         for (uint32_t v : {2 * mC, mZ, mQR, mQ, mHR, mOV, sP, sQK, sXC, sA, sRO, sDBC, sF, sF2, sXC2, sY, dV, dSp, dGt, mMO, mFF, mFF2, mSFF, mSFF2}) w = std::max<size_t>(w, v);
         if ((r = portion_memory(e, ld, std::max<size_t>(T, kWantBatch) * ((w + 7u) & ~(size_t)7u)))) return r;
+        if (e->kv4 && (r = tc_error_word(&e->tc))) return r;          // (its attention has bounded waits, whether or not there was room for the products')
     }
     CK(cudaDeviceSynchronize());
     return 0;

@@ -344,6 +344,13 @@ template <int TN, bool RAW>
 int optin() { NB_CK(nb::smem_at_least((const void *)k_gemm_tc<TN, RAW>, (int)tc_smem(TN))); return 0; }
 }  // namespace
 
+int tc_error_word(TcState *t) {
+    if (t->err_host) return 0;
+    NB_CK(cudaHostAlloc(&t->err_host, 64, cudaHostAllocMapped));
+    *t->err_host = 0;
+    NB_CK(cudaHostGetDevicePointer(&t->err_dev, t->err_host, 0));
+    return 0;
+}
 int tc_setup(TcState *t, size_t elems, uint32_t sms) {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult got;
@@ -353,11 +360,8 @@ int tc_setup(TcState *t, size_t elems, uint32_t sms) {
     t->sms = sms;
     for (auto &p : t->rows) if (cudaMalloc(&p, elems * 2) != cudaSuccess) { p = nullptr; return fail(NB200_ENOMEM, "cudaMalloc(%zu) failed", elems * 2); }
     t->elems = elems;
-    NB_CK(cudaHostAlloc(&t->err_host, 64, cudaHostAllocMapped));
-    *t->err_host = 0;
-    NB_CK(cudaHostGetDevicePointer(&t->err_dev, t->err_host, 0));
     int r;
-    if ((r = optin<32, true>()) || (r = optin<64, true>()) || (r = optin<32, false>()) || (r = optin<64, false>()) || (r = optin<128, false>())) return r;
+    if ((r = tc_error_word(t)) || (r = optin<32, true>()) || (r = optin<64, true>()) || (r = optin<32, false>()) || (r = optin<64, false>()) || (r = optin<128, false>())) return r;
     return 0;
 }
 void tc_free(TcState *t) {

@@ -18,6 +18,7 @@ struct TcState {
     __nv_bfloat16 *planes = nullptr; size_t plane_elems = 0;      // tc_gemm_split's rows in three parts
 };
 int tc_setup(TcState *t, size_t elems, uint32_t sms);
+int tc_error_word(TcState *t);          // that word alone (tc_setup makes it too)
 void tc_free(TcState *t);
 // after a synchronisation: did a bounded wait of a kernel run out
 int tc_check(TcState *t);
