@@ -45,8 +45,8 @@ UNITS = {
     "prefill.cu": ["prefill.h", "prompt_split.h", "attn_tc.h", "tc_ptx.cuh", "kernels.cuh", "expf_ref.cuh", "family.h"],
     "engine.cu": ["prefill.h", "attn_tc.h", "kernels.cuh", "expf_ref.cuh", "stream_args.h", "stream_count.h", "stream_groups.h", "stream_host.h", "ops.h", "sample_host.h", "family.h", "../../include/nano_b200.h"],
     "stream.cu": ["kernels.cuh", "expf_ref.cuh", "stream_args.h", "stream_host.h", "stream.cuh"],
-    "ops.cu": ["ops.h", "pairs.cuh", "family.h", "../../include/nano_b200.h"],
-    "kv4.cu": ["kv4.cuh", "kv4.h", "ops.h", "family.h", "../../include/nano_b200.h"],
+    "ops.cu": ["ops.h", "pairs.cuh", "portions.h", "family.h", "../../include/nano_b200.h"],
+    "kv4.cu": ["kv4.cuh", "kv4.h", "ops.h", "portions.h", "family.h", "../../include/nano_b200.h"],
     "kv4_tc.cu": ["kv4.cuh", "kv4.h", "ops.h", "pairs.cuh", "tc_ptx.cuh", "family.h"],
     "sample.cu": ["kernels.cuh", "expf_ref.cuh", "sample_host.h"],
 }

@@ -9,6 +9,7 @@
 
 #include "family.h"
 #include "kv4.cuh"
+#include "portions.h"
 
 namespace nb {
 namespace {
@@ -716,20 +717,18 @@ template <bool WRITE>
 cudaError_t rows_launch(const Kv4Rows &all, cudaStream_t stream, bool pdl) {
     const uint32_t per = all.G * (all.D / kKv4Group), most = (1u << 30) / per;          // tokens of a launch
     const bool vec = rows_at16(all);
-    for (uint32_t t0 = 0; t0 < all.T; t0 += most) {
+    return in_portions(all.T, most, [&](uint32_t t0, uint32_t n) {
         Kv4Rows a = all;
-        a.T = std::min(most, all.T - t0);
+        a.T = n;
         a.k = static_cast<char *>(all.k) + t0 * all.k_token * elem_size(all.type); a.v = static_cast<char *>(all.v) + t0 * all.v_token * elem_size(all.type);
         if (all.slots) a.slots += t0; else a.pos0 += t0;
         const dim3 grid((a.T * per + kRowThreads / 4u - 1u) / (kRowThreads / 4u));
 #define KV4_ROWS(TYPE)                                                                                                                          \
     (WRITE ? (vec ? launch_on(k_kv4_write<TYPE, true>, grid, kRowThreads, 0, stream, pdl, a) : launch_on(k_kv4_write<TYPE, false>, grid, kRowThreads, 0, stream, pdl, a)) \
            : (vec ? launch_on(k_kv4_read<TYPE, true>, grid, kRowThreads, 0, stream, false, a) : launch_on(k_kv4_read<TYPE, false>, grid, kRowThreads, 0, stream, false, a)))
-        const cudaError_t e = a.type == T_F32 ? KV4_ROWS(float) : a.type == T_BF16 ? KV4_ROWS(__nv_bfloat16) : KV4_ROWS(__half);
+        return a.type == T_F32 ? KV4_ROWS(float) : a.type == T_BF16 ? KV4_ROWS(__nv_bfloat16) : KV4_ROWS(__half);
 #undef KV4_ROWS
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+    });
 }
 
 }  // namespace

@@ -11,6 +11,7 @@
 #include "family.h"
 #include "ops.h"
 #include "pairs.cuh"
+#include "portions.h"
 
 namespace nb {
 namespace {
@@ -483,9 +484,9 @@ cudaError_t logprobs_launch_of(const LogprobArgs &a, cudaStream_t stream) {
         cudaError_t e = cudaFuncSetAttribute(k_logprobs<T, TOP, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
-    for (uint32_t r0 = 0; r0 < a.rows; r0 += 65535u) {          // (the grid's second dimension)
+    return in_portions(a.rows, 65535u, [&](uint32_t r0, uint32_t n) {          // (the grid's second dimension)
         LogprobArgs b = a;
-        b.rows = std::min(65535u, a.rows - r0);
+        b.rows = n;
         b.logits = static_cast<const char *>(a.logits) + (uint64_t)r0 * a.row_stride * sizeof(T);
         if (a.tokens) b.tokens = static_cast<const char *>(a.tokens) + (uint64_t)r0 * a.token_bytes;
         if (a.logprob) b.logprob += r0;
@@ -498,10 +499,8 @@ cudaError_t logprobs_launch_of(const LogprobArgs &a, cudaStream_t stream) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr; cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_logprobs<T, TOP, THREADS>, b, C);
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+        return cudaLaunchKernelEx(&cfg, k_logprobs<T, TOP, THREADS>, b, C);
+    });
 }
 
 // Blocks of 256 threads; of 128 where there are more rows than blocks of 256 run at once (four to an SM) and a row is short, so that what follows a row's pass has more
@@ -556,8 +555,7 @@ cudaError_t logprobs_launch(const LogprobArgs &a, cudaStream_t stream) {
 }
 
 cudaError_t pages_copy_launch(const PagePool *pools, uint32_t n_pools, const uint32_t *src, const uint32_t *dst, uint32_t n, cudaStream_t stream, uint32_t *launches) {
-    for (uint32_t p0 = 0; p0 < n_pools; p0 += kPagePools) {
-        const uint32_t np = std::min(kPagePools, n_pools - p0);
+    return in_portions(n_pools, kPagePools, [&](uint32_t p0, uint32_t np) -> cudaError_t {
         uint64_t bytes = 0;
         bool vec = true;
         for (uint32_t i = 0; i < np; i++) {
@@ -565,17 +563,15 @@ cudaError_t pages_copy_launch(const PagePool *pools, uint32_t n_pools, const uin
             bytes = std::max(bytes, p.page_bytes);
             vec = vec && ((reinterpret_cast<uintptr_t>(p.base) | p.page_bytes | p.page_stride) & 15u) == 0;
         }
-        if (!bytes) continue;
-        for (uint32_t i = 0; i < n; i += kPagePairs) {
-            const uint32_t m = std::min(kPagePairs, n - i);
+        if (!bytes) return cudaSuccess;
+        return in_portions(n, kPagePairs, [&](uint32_t i, uint32_t m) {
             cudaError_t e;
             if (m <= 64u) e = vec ? pages_launch<64, true>(pools + p0, np, src + i, dst + i, m, bytes, stream) : pages_launch<64, false>(pools + p0, np, src + i, dst + i, m, bytes, stream);
             else e = vec ? pages_launch<kPagePairs, true>(pools + p0, np, src + i, dst + i, m, bytes, stream) : pages_launch<kPagePairs, false>(pools + p0, np, src + i, dst + i, m, bytes, stream);
-            if (e != cudaSuccess) return e;
-            if (launches) ++*launches;
-        }
-    }
-    return cudaSuccess;
+            if (e == cudaSuccess && launches) ++*launches;
+            return e;
+        });
+    });
 }
 
 }  // namespace nb
