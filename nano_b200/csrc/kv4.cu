@@ -185,8 +185,8 @@ bool rows_at16(const Kv4Rows &a) {
 // Rounding to 11 bits: the queries (times a power of two per row, so that any magnitude fits), the weights, the weights times s, and keys where they are c s + m; each
 // rounding is at most 2^-11 of its number, against the 2^-8 of a bf16 output and the cache's own 1/30 of a group's range.
 // Each warp brings its own pages into its own ring of shared memory (cp.async, one group of copies to a page) and waits for nobody else until the end.
-// WK warps of a block share the columns and take every WK-th page (single tokens: the keys are what there is to share out); with WK = 1 each warp has columns of
-// its own.  The pages of a row are also split over nsplit blocks, whose parts k_kv4_join puts together.
+// WK warps of a block share the columns and take every WK-th page (single tokens: the keys are what there is to share out); with WK = 1 (heads of 256,
+// more than 16 columns) each warp has columns of its own.  The pages of a row are also split over nsplit blocks, whose parts k_kv4_join puts together.
 // Measured: 32 heads over 8 of 128 behind 131000 tokens 44 us, with k_kv4_join (3.8 TB/s of the cache's bytes); bound by the chain of a warp's page -- 632 instructions, a scheduler issues in 54 % of its
 // cycles -- not by mma.sync (34 to a page, one every 8.5 cycles of 1170).
 // Values that stand for NaN are taken out of the product (0 times NaN would reach columns that do not see them) and make the rows that do see them NaN.
@@ -661,13 +661,13 @@ cudaError_t launch_on(K k, dim3 grid, uint32_t threads, size_t smem, cudaStream_
 
 // ---- which instance, and how the work is shared out ----
 struct Plan { int nt; bool rows, tc, wide; Shape sh; };
-constexpr uint32_t kWarps = 4, kWide = 8, kShort = 32, kWaves = 3, kMost = 64, kTcCols = 17;
+constexpr uint32_t kWarps = 4, kWide = 8, kShort = 32, kWaves = 3, kMost = 64;
 Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms) {
     const uint32_t ncols = T * (H / G);
     Plan p{};
     p.nt = ncols <= 8 ? 1 : 2;
     p.rows = ncols > 16;
-    p.tc = D <= 128 && ncols >= kTcCols;
+    p.tc = p.rows && D <= 128;
     p.sh.cols = p.tc ? kKv4TcRows : (uint32_t)p.nt * 8u * (p.rows ? kWarps : 1u);
     p.sh.tiles = (ncols + p.sh.cols - 1u) / p.sh.cols;
     // pages that a block can have in sight
@@ -708,7 +708,7 @@ cudaError_t attn_launch(const Kv4Attn &a, const Shape &sh, cudaStream_t stream, 
 }
 template <int NG>
 cudaError_t attn_launch_nt(const Kv4Attn &a, const Plan &p, cudaStream_t stream, bool pdl) {
-    if (p.rows) return attn_launch<NG, 2, 1>(a, p.sh, stream, pdl);
+    if constexpr (NG > 4) { if (p.rows) return attn_launch<NG, 2, 1>(a, p.sh, stream, pdl); }          // (of up to 128 the tensor-memory kernel takes them: plan_for)
     if (p.wide) return p.nt == 1 ? attn_launch<NG, 1, kWide, kWide>(a, p.sh, stream, pdl) : attn_launch<NG, 2, kWide, kWide>(a, p.sh, stream, pdl);
     return p.nt == 1 ? attn_launch<NG, 1, kWarps>(a, p.sh, stream, pdl) : attn_launch<NG, 2, kWarps>(a, p.sh, stream, pdl);
 }
