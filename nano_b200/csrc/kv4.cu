@@ -744,7 +744,7 @@ size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32
 // (keys are split only while blocks times splits stay within the waves of what the device holds at once: one block of 128 rows to an SM, or four of at most 64)
 size_t kv4_attn_workspace_most(uint32_t B, uint32_t D, uint32_t sms) { return (size_t)(B > 1 ? kWaves : 1u) * sms * 256u * (D + 2u) * 4u; }
 
-cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, uint32_t *launches) {
+cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, bool pdl_join, uint32_t *launches) {
     const Plan p = plan_for(a.B, a.T, a.H, a.G, a.D, a.width, a.window, a.block, sms);
     cudaError_t e;
     if (p.tc) e = kv4_tc_launch(a, p.sh.nsplit, p.sh.tiles, stream, pdl);
@@ -756,7 +756,7 @@ cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream,
         default: e = attn_launch_nt<8>(a, p, stream, pdl); break;
     }
     if (e == cudaSuccess && p.sh.nsplit > 1)
-        e = launch_on(k_kv4_join, dim3(a.T * (a.H / a.G), a.G, a.B), kJoinThreads, p.sh.nsplit * 4u, stream, true, a, p.sh);
+        e = launch_on(k_kv4_join, dim3(a.T * (a.H / a.G), a.G, a.B), kJoinThreads, p.sh.nsplit * 4u, stream, pdl_join, a, p.sh);
     if (launches) *launches = p.sh.nsplit > 1 ? 2 : 1;
     return e;
 }
@@ -859,7 +859,7 @@ int nb200_dev_kv4_attention(const nb200_kv4_attention *p, void *workspace, uint6
     const nb::Kv4Attn a{p->q, p->q_batch, p->q_token, p->q_head, p->type, p->out, p->o_batch, p->o_token, p->o_head, static_cast<const unsigned char *>(p->pool), p->page_stride, p->n_pages,
                         p->table, p->table_stride, p->width, p->lens, 0, nullptr, p->batch, p->tokens, p->heads, p->kv_heads, p->head_dim, p->scale, p->softcap, p->sinks, p->window, p->block,
                         nullptr, 0, static_cast<float *>(workspace)};
-    NB_CK(nb::kv4_attn_launch(a, sms, static_cast<cudaStream_t>(stream), false, nullptr));
+    NB_CK(nb::kv4_attn_launch(a, sms, static_cast<cudaStream_t>(stream), false, true, nullptr));          // (whose kernel comes before is not known; before the join it is this call's own)
     return 0;
 }
 

@@ -48,7 +48,8 @@ struct Kv4Attn {
 size_t kv4_attn_workspace(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32_t width, uint32_t window, uint32_t block, uint32_t sms);
 // the most that any call of B sequences asks for, whatever its tokens and its width
 size_t kv4_attn_workspace_most(uint32_t B, uint32_t D, uint32_t sms);
-// one launch, or two (the keys of a row split over several blocks, then joined); *launches says how many
-cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, uint32_t *launches);
+// one launch, or two (the keys of a row split over several blocks, then joined); *launches says how many.  pdl, pdl_join: whether the first and the second may be launched while the
+// kernel before them runs
+cudaError_t kv4_attn_launch(const Kv4Attn &a, uint32_t sms, cudaStream_t stream, bool pdl, bool pdl_join, uint32_t *launches);
 
 }  // namespace nb

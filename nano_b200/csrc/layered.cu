@@ -1491,7 +1491,7 @@ int gqa_branch(LayeredEngine *e, const Layer &L, const Run &run, const Ctx &cx, 
         ka.B = 1; ka.T = T; ka.H = H; ka.G = G; ka.D = D; ka.scale = 1.0f; ka.softcap = L.softcap; ka.sink = L.sink; ka.block = L.block_size; ka.part = e->b_kpart; ka.err = e->tc.err_dev;
         if (L.has_gate) { ka.gate = e->b_p + L.c_hg; ka.ldg = P; }
         uint32_t launches = 0;
-        CK(nb::kv4_attn_launch(ka, (uint32_t)e->num_sms, e->cur, e->use_pdl, &launches));
+        CK(nb::kv4_attn_launch(ka, (uint32_t)e->num_sms, e->cur, e->use_pdl, e->use_pdl, &launches));
         e->launches += 1u + launches;
         return gemm(e, plain(e->b_a, H * VD, L.o, dst, e->E, T), 1, T);
     }
