@@ -234,7 +234,8 @@ int nb200_dev_token_logprobs(float *logprob, float *entropy, float *top_logprob,
 
 /* Copies pages of a cache: page src[i] over page dst[i], i < n, in each of n_pools pools; page p of pool k is the page_bytes[k] bytes at pools[k] + p *
  * page_stride[k], p < n_pages[k].  All arrays are on the host.  A source may appear many times (a prompt's page forked for several continuations); a destination
- * that is a source too or appears twice is refused. */
+ * that is a source too or appears twice is refused, and so are pools that overlap where a page which one of them writes lies over a page which another reads or writes (pages of several
+ * layers side by side in one allocation are not in each other's way). */
 int nb200_dev_pages_copy(void *const *pools, const uint64_t *page_bytes, const uint64_t *page_stride, const uint32_t *n_pages, uint32_t n_pools,
                          const uint32_t *src, const uint32_t *dst, uint32_t n, void *stream);
 

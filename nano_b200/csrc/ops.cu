@@ -6,6 +6,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "family.h"
@@ -578,6 +580,51 @@ cudaError_t pages_copy_launch(const PagePool *pools, uint32_t n_pools, const uin
 
 using nb::fail;
 
+namespace {
+// Pools of one call whose memory meets: pages of several layers may lie side by side in one tensor, but no page that is written may lie over another that is read or written (blocks run in any
+// order).  The pool given twice is taken once.  A walk over the pools where their memory is apart, which is the rule; residues of the stride where their pages are interleaved; else every page that is touched is looked at.
+int pages_apart(std::vector<nb::PagePool> &list, uint32_t pages, const uint32_t *src, const uint32_t *dst, uint32_t n) {
+    typedef unsigned __int128 wide;
+    auto start = [](const nb::PagePool &p) { return (uint64_t)reinterpret_cast<uintptr_t>(p.base); };
+    auto end = [&](const nb::PagePool &p) { return (wide)start(p) + (wide)(pages - 1u) * p.page_stride + p.page_bytes; };
+    list.erase(std::remove_if(list.begin(), list.end(), [](const nb::PagePool &p) { return p.page_bytes == 0; }), list.end());
+    bool apart = true;
+    for (size_t i = 1; i < list.size(); i++) apart = apart && end(list[i - 1]) <= start(list[i]);
+    if (apart) return 0;
+    auto key = [&](const nb::PagePool &p) { return std::make_tuple(start(p), p.page_stride, p.page_bytes); };
+    std::sort(list.begin(), list.end(), [&](const nb::PagePool &a, const nb::PagePool &b) { return key(a) < key(b); });
+    list.erase(std::unique(list.begin(), list.end(), [&](const nb::PagePool &a, const nb::PagePool &b) { return key(a) == key(b); }), list.end());
+    bool even = true;
+    wide last = 0;
+    apart = true;
+    for (const nb::PagePool &p : list) { apart = apart && last <= start(p); last = std::max(last, end(p)); even = even && p.page_stride == list[0].page_stride; }
+    if (apart) return 0;
+    if (even) {
+        const uint64_t step = list[0].page_stride;
+        std::vector<std::pair<uint64_t, uint64_t>> at;          // where in a step a pool's pages lie
+        for (const nb::PagePool &p : list) at.emplace_back((start(p) - start(list[0])) % step, p.page_bytes);
+        std::sort(at.begin(), at.end());
+        bool free = (wide)at.back().first + at.back().second <= (wide)step + at[0].first;
+        for (size_t i = 1; i < at.size(); i++) free = free && at[i - 1].first + at[i - 1].second <= at[i].first;
+        if (free) return 0;
+    }
+    struct Touch { wide from, to; bool write; };
+    std::vector<Touch> touched;
+    touched.reserve(2u * (size_t)n * list.size());
+    for (const nb::PagePool &p : list)
+        for (uint32_t i = 0; i < n; i++)
+            for (const bool write : {false, true}) { const wide from = (wide)start(p) + (wide)(write ? dst[i] : src[i]) * p.page_stride; touched.push_back(Touch{from, from + p.page_bytes, write}); }
+    std::sort(touched.begin(), touched.end(), [](const Touch &a, const Touch &b) { return a.from < b.from; });
+    wide written = 0, any = 0;          // where what lies before ends
+    for (const Touch &t : touched) {
+        if (t.from < written || (t.write && t.from < any)) return fail(NB200_EINVAL, "pools overlap: a page that this call writes in one lies over a page that it reads or writes in another");
+        any = std::max(any, t.to);
+        if (t.write) written = std::max(written, t.to);
+    }
+    return 0;
+}
+}  // namespace
+
 extern "C" {
 
 int nb200_dev_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_id, const void *logits, uint32_t type, uint64_t row_stride,
@@ -618,8 +665,9 @@ int nb200_dev_pages_copy(void *const *pools, const uint64_t *page_bytes, const u
             if (used[dst[i]]) return fail(NB200_EINVAL, "page %u is written and read, or written twice, by one call", dst[i]);
             used[dst[i]] = true;
         }
+        if (const int r = pages_apart(list, pages, src, dst, n)) return r;
         if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
-        NB_CK(nb::pages_copy_launch(list.data(), n_pools, src, dst, n, static_cast<cudaStream_t>(stream), nullptr));
+        NB_CK(nb::pages_copy_launch(list.data(), (uint32_t)list.size(), src, dst, n, static_cast<cudaStream_t>(stream), nullptr));
     } catch (const std::bad_alloc &) { return fail(NB200_ENOMEM, "out of host memory"); }
     return 0;
 }

@@ -100,7 +100,8 @@ def _numbers(pages):
 
 def pages_copy(pools, src, dst):
     """Page src[i] is copied over page dst[i] in every pool, in place.  pools: tensors [pages, ...] of any type, each page contiguous; src, dst: numbers on the host.
-    A source may appear many times; a destination that is a source too or appears twice is refused."""
+    A source may appear many times; a destination that is a source too or appears twice is refused, and so are pools that share memory where a page that is written in one is read or written
+    in another (x[:, 0] and x[:, 1] do not meet; x[:-1] and x[1:] may)."""
     pools = list(pools)
     src, dst = _numbers(src), _numbers(dst)
     if len(src) != len(dst):
