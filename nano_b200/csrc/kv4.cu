@@ -254,9 +254,10 @@ __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT) * 4 / W > 1 ? kv4_b
     const uint32_t c1 = min(c0 + COLS, ncols);
     const int pos_a = c0 < ncols ? len - (int)a.T + (int)(c0 / rep) : -1, pos_b = c0 < ncols ? len - (int)a.T + (int)((c1 - 1u) / rep) : -1;
     uint32_t p0 = 0, p1 = 0;
-    int low_b = 0;
+    int low_a = 0, low_b = 0;          // the first key that a column sees, and the last column's first
     if (pos_b >= 0) {
-        const uint32_t first = (uint32_t)first_seen(max(pos_a, 0), a.window, a.block) / kKv4Page, np = (uint32_t)pos_b / kKv4Page + 1u - first;
+        low_a = first_seen(max(pos_a, 0), a.window, a.block);
+        const uint32_t first = (uint32_t)low_a / kKv4Page, np = (uint32_t)pos_b / kKv4Page + 1u - first;
         p0 = first + (uint32_t)((uint64_t)np * split / sh.nsplit); p1 = first + (uint32_t)((uint64_t)np * (split + 1u) / sh.nsplit);
         low_b = first_seen(pos_b, a.window, a.block);
     }
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(W * 32, kv4_blocks(NG, NT) * 4 / W > 1 ? kv4_b
                 bad = __ballot_sync(0xffffffffu, odd);
                 // (a token that no column sees weighs nothing, whatever its step: the room, and with it the roundings, does not follow from it)
                 const int at = key0 + (int)lane;
-                const bool seen = whole || (at <= pos_b && at >= first_seen(max(pos_a, 0), a.window, a.block));
+                const bool seen = at <= pos_b && at >= low_a;
                 if (odd)
 #pragma unroll
                     for (int j = 0; j < NG; j++) reinterpret_cast<uint32_t *>(pg + 1152u * NG + lane * 4u * NG)[j] = 0u;
