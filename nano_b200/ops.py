@@ -71,6 +71,8 @@ def token_logprobs(logits, tokens, top=0):
         _no("tokens are [rows] of int32 or int64")
     if not 0 <= top <= 32 or (top > vocab and rows):
         _no("%d alternatives asked for: at most 32, and no more than the vocabulary has", top)
+    if rows >> 32 or vocab >> 31:          # (counts are 32-bit numbers in the C calls: ctypes would cut larger ones off; struct refuses them)
+        _no("%d rows of %d logits are too many for one call", rows, vocab)
     stride, step = logits.stride()
     if (step != 1 and vocab > 1) or stride < 0:
         logits = logits.contiguous()
@@ -106,6 +108,8 @@ def pages_copy(pools, src, dst):
     src, dst = _numbers(src), _numbers(dst)
     if len(src) != len(dst):
         _no("src and dst are lists of the same length")
+    if len(src) >> 32:
+        _no("%d pairs are too many for one call", len(src))
     if not pools:
         return
     device = _cuda("pool 0", pools[0])
@@ -128,7 +132,11 @@ def pages_copy(pools, src, dst):
         pages.append(count)
     n = len(pools)
     numbers = array("Q", base + size + stride)
-    at, counts = numbers.buffer_info()[0], array("I", pages)
+    try:
+        counts = array("I", pages)
+    except OverflowError:
+        _no("pools of %d pages are too large", max(pages))
+    at = numbers.buffer_info()[0]
     _call(device, lib(True).nb200_dev_pages_copy, at, at + 8 * n, at + 16 * n, counts.buffer_info()[0], n, src.buffer_info()[0], dst.buffer_info()[0], len(src))
 
 
@@ -147,6 +155,8 @@ def _pool(pool):
     pages, heads, block = pool.shape
     if not pool.is_contiguous() and (pool.stride(2) != 1 or (pool.stride(1) != block and heads != 1)):
         _no("a pool's pages are to be contiguous")
+    if (pages | heads) >> 32:
+        _no("a pool of %d pages of %d heads is too large", pages, heads)
     return device, pages, heads, block // 40, pool.stride(0)
 
 
@@ -154,6 +164,10 @@ def _slots(slots, device):
     _cuda("slots", slots, device)
     if slots.dim() != 1 or slots.dtype != torch.int32:
         _no("slots are [tokens] of int32")
+    if slots.is_contiguous():
+        return slots
+    if slots.shape[0] >> 32:
+        _no("%d tokens are too many for one call", slots.shape[0])
     return slots.contiguous()
 
 
@@ -184,6 +198,8 @@ def kv4_write(pool, k, v, slots):
         return
     k, kt, kh = _row_strides(k)
     v, vt, vh = _row_strides(v)
+    if tokens >> 32:
+        _no("%d tokens are too many for one call", tokens)
     rows = _ROWS(pool.data_ptr(), stride, pages, heads, dim, _TYPES[k.dtype], tokens, slots.data_ptr(), k.data_ptr(), v.data_ptr(), kt, kh, vt, vh)
     _call(device, lib(True).nb200_dev_kv4_write, rows)
 
@@ -224,6 +240,8 @@ def kv4_attention(q, pool, table, lens, scale=None, window=0, block=0, softcap=0
         _no("table is [batch, width] of int32")
     if lens.dim() != 1 or lens.shape[0] != B or lens.dtype != torch.int32:
         _no("lens is [batch] of int32")
+    if (B | T | H) >> 32:
+        _no("%d sequences of %d tokens of %d heads are too many for one call", B, T, H)
     if window < 0 or block < 0:
         _no("window and block are not negative")
     if sinks is not None:
