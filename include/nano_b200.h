@@ -258,7 +258,7 @@ int nb200_dev_kv4_read(const nb200_kv4_rows *rows, void *stream);
  * key/value head h / (heads / kv_heads).  A query sees the keys of positions up to its own, of these only the last `window` (0: all) and those in its own block of `block` positions
  * counted from 0 (0: all); scores are scale q . k, with softcap > 0 softcap tanh(scale q . k / softcap); sinks [heads] (or NULL) join the softmax denominator as exp(sink).
  * A query at a negative position, or one that sees no key, has an output of zeros; a length beyond width * 32 counts as that; the tokens of a page number outside the pool
- * are not seen.  A key or value that stands for NaN makes the rows that see it NaN, and no others.
+ * are not seen.  A key or value that stands for NaN makes the rows that see it NaN, and no others; places that no query of a sequence sees may hold any bytes.
  * type: of q and out, fp32 or bf16.  Either way products take operands of 11 bits (c s + m, queries, softmax weights rounded to fp16 significands) and sum in fp32.
  * Strides are in numbers; out's base and strides are multiples of four numbers.  The workspace's bytes do not depend on what lies in device memory;
  * two calls that may run at the same time need one each. */

@@ -208,7 +208,9 @@ struct Room {
                               q = (W / WK) * NT * NG * 512u, all = (ring > merge ? ring : merge) + q + (W / WK) * NT * 8u * 4u * (after ? 1u + NG : 1u);
 };
 
-// blocks that an SM holds at once: registers allow no more without spills
+// Blocks that an SM holds at once.  Four of heads of 128 leave 128 registers to a thread, and the instances spill up to 80 bytes (two tiles of columns: 56 at three blocks and 168 registers; heads
+// of 64 with two tiles 72 at four and 128); one block less spills nothing.  As it is / one block less, us: one token of 32 heads of 128 over 8 behind 131000 43.6 / 42.7, three tokens 57.4 / 53.4; 32 sequences
+// of up to 8190 42.8 / 45.1, 8 of 8190 26.0 / 26.7, four tokens of 16 heads over 4 in 32 sequences of 4000 37.1 / 36.8, of heads of 64 26.4 / 25.8: many sequences gain by the places
 __host__ __device__ constexpr int kv4_blocks(int NG, int NT) { return NG <= 2 || (NG <= 4 && NT == 1) ? 4 : NG <= 4 ? 3 : 2; }
 
 // The sequence that `before` others come before when they are ordered by pages, then by number; up to 32 N of them.  By votes, whose results are known to be the same in all
@@ -675,17 +677,17 @@ Plan plan_for(uint32_t B, uint32_t T, uint32_t H, uint32_t G, uint32_t D, uint32
     const uint64_t reach = std::min<uint64_t>(window ? window : ~0u, block ? block : ~0u) + (p.sh.cols + H / G - 1u) / (H / G) + kKv4Page;
     const uint32_t pages = (uint32_t)std::min<uint64_t>(width, reach / kKv4Page + 1u);
     // A block for every place that the device has.  Of several sequences, whose lengths may differ, blocks of no more than kMost pages, but at most three times as many blocks as
-    // places: with one, two and three blocks to a place 32 sequences of up to 8190 tokens take 67, 56 and 57 us, of 8190 each 77, 74 and 79, but 8 of them 20, 24 and 29, 3 of up to
-    // 30000 26, 33 and 36 (a block costs some 2 us beside its pages)
+    // places.  In the given order of sequences (measured before the longest came first, below), with one, two and three blocks to a place, 32 sequences of up to 8190 tokens take 67, 56 and 57 us,
+    // of 8190 each 77, 74 and 79, but 8 of them 20, 24 and 29, 3 of up to 30000 26, 33 and 36 (a block costs some 2 us beside its pages)
     const uint32_t at_once = p.tc ? 1u : (uint32_t)kv4_blocks((int)D / 32, p.nt);
     const uint64_t blocks = std::max<uint64_t>(1, (uint64_t)B * G * p.sh.tiles), places = (uint64_t)at_once * sms;
     const uint32_t least = p.tc ? 16u : p.rows ? 8u : kWarps;          // pages of a split
     uint64_t n = places / blocks;
     if (B > 1) n = std::max(n, std::min<uint64_t>((pages + kMost - 1u) / kMost, kWaves * places / blocks));
     p.sh.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(n, std::max(1u, pages / least)));
-    // Few blocks with few pages each: twice the warps and no parts to be joined.  One token of 16 heads of 128 over 8 behind 400: 7.6 us instead of 8.9, behind 777 10.3 instead of 8.9, but one launch
-    // and no workspace: calls in a row take 12.2 us instead of 16.8.  (Sixteen warps: 7.8 and 9.7, behind 60 tokens 6.5 instead of 5.6.)  Heads of 256 behind 400 11.2 instead of 11.3, behind 777
-    // 15.5 instead of 11.5
+    // Few blocks with few pages each: twice the warps and no parts to be joined.  One token of 16 heads of 128 over 8 behind 200, 400, 500, 600, 777 and 1000 tokens takes 5.9, 7.2, 7.6, 8.6, 10.0 and 10.3 us on
+    // the device, with the keys split 6.4, 8.5, 7.7, 8.5, 8.9 and 7.9; but it is one launch without a workspace, and calls in a row, bound by the host, take 12.6 us instead of 17.  So the border lies where
+    // the call gains, beyond the 550 or so where the device does.  (Sixteen warps behind 400: 7.8, 777: 9.7, 60: 6.5 instead of 5.3.)  Heads of 256 behind 200 7.8 instead of 8.3, 400 10.3 as the split, 500 10.8 instead of 9.2
     p.wide = !p.tc && !p.rows && pages <= (D > 128u ? kShort / 2u : kShort) && blocks <= sms;
     if (p.wide) p.sh.nsplit = 1;
     // Of up to 64 sequences the longest first, so that the SMs get long and short ones alike and what is left when others end is short (32 of up to 8190 tokens: 50 us, in the given

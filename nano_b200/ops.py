@@ -226,7 +226,7 @@ def kv4_attention(q, pool, table, lens, scale=None, window=0, block=0, softcap=0
     Query t of sequence b sits at position lens[b] - tokens + t; lens [batch] (int32) counts all tokens of a sequence, the new ones (written before) among them;
     table [batch, width] (int32) names its pages.  Head h reads key/value head h // (heads / kv_heads).  A query sees the keys up to its own position, of these only the last
     `window` (0: all) and those in its own block of `block` positions (0: all).  scale: 1 / sqrt(head_dim) unless given; softcap > 0: softcap * tanh(score / softcap);
-    sinks [heads] (float32): one more term exp(sink) in a head's denominator.  A query at a negative position or without a key in sight has zeros.  head_dim 32, 64, 96, 128
+    sinks [heads] (float32): one more term exp(sink) in a head's denominator.  A query at a negative position or without a key in sight has zeros; places that no query sees may hold any bytes.  head_dim 32, 64, 96, 128
     or 256.  Products take 11-bit operands and sum in 32 bits, whichever type q has."""
     device, pages, heads, dim, stride = _pool(pool)
     _cuda("q", q, device)
