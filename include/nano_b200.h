@@ -271,6 +271,52 @@ typedef struct nb200_kv4_attention {
 int nb200_dev_kv4_attention_workspace(const nb200_kv4_attention *p, uint64_t *bytes);
 int nb200_dev_kv4_attention(const nb200_kv4_attention *p, void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* Rows of numbers in microscaled 4-bit floating point: 32 neighbours of a row share a scale, the last group is filled up with zeros.  A row is 16 bytes of codes for each group, two codes to
+ * a byte, the lower four bits first, and one byte E for each group, its scale 2^(E - 127) (255: NaN).  A code is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (two bits of exponent, one of mantissa).
+ * nb200_dev_mx4_quantize: of a group's largest magnitude a the scale is 2^(floor(log2 a) - 2), between 2^-127 and 2^127 (2^-127 where a = 0); a code is the nearest to x / scale, of two as near the
+ * one with an even number, and what lies beyond 6 becomes 6.  A group with a NaN or an infinity is NaN.  nb200_dev_mx4_read writes what the rows stand for to x, rounded to its type.
+ * codes: base and stride are multiples of 16 bytes.  scales: any.  x: strides in numbers. */
+typedef struct nb200_mx4_rows {
+    void *codes, *scales; uint64_t code_stride, scale_stride;                    /* bytes from row to row */
+    void *x; uint64_t x_stride; uint32_t type, rows, columns;
+} nb200_mx4_rows;
+int nb200_dev_mx4_quantize(const nb200_mx4_rows *rows, void *stream);
+int nb200_dev_mx4_read(const nb200_mx4_rows *rows, void *stream);
+
+/* out[r][n] = sum over k of x[r][k] w[n][k], rows r < rows, n < outputs, k < columns; w in that format, x too (x_type NB200_T_MX4: codes, with x_scales), or numbers that the call
+ * quantises as nb200_dev_mx4_quantize does.  Products are exact, sums are fp32, rounded once to out_type.  A group's sum that leaves the range of fp32 makes the result infinite or NaN.
+ * experts > 0: w holds a matrix for each expert (w_expert, ws_expert: bytes from one to the next), rows offsets[e] .. offsets[e + 1] - 1 (offsets [experts + 1] ascending) are multiplied with
+ * that of expert e, and rows outside of all become zeros.
+ * What fills up a last group does not count, whatever it holds.  Codes: bases and strides are multiples of 16 bytes.  x_stride counts numbers (bytes for codes), out_stride numbers.  The workspace holds x as it was quantised (none for codes); its bytes do not
+ * depend on what lies in device memory; two calls that may run at the same time need one each. */
+#define NB200_T_MX4 3u
+typedef struct nb200_mx4_product {
+    const void *x, *x_scales; uint64_t x_stride, xs_stride;
+    const void *w, *w_scales; uint64_t w_stride, ws_stride, w_expert, ws_expert;
+    void *out; uint64_t out_stride; const int32_t *offsets;
+    uint32_t x_type, out_type, rows, outputs, columns, experts;
+} nb200_mx4_product;
+int nb200_dev_mx4_product_workspace(const nb200_mx4_product *p, uint64_t *bytes);
+int nb200_dev_mx4_product(const nb200_mx4_product *p, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Rows by expert.  ids [n] (32-bit or 64-bit numbers: id_bytes 4 or 8) names an expert for each place of a list; what lies outside [0, experts) names none.  order [n]: the places, sorted by expert
+ * and, within one, ascending, then -1 for those that name none; offsets [experts + 1]: where in it each expert's begin; place [n]: where in order a place stands, -1 if it names none.
+ * At most 1024 experts, 2^30 places. */
+int nb200_dev_experts_sort(int32_t *order, int32_t *offsets, int32_t *place, const void *ids, uint32_t id_bytes, uint32_t n, uint32_t experts, void *stream);
+/* The list's place t * top + j is token t's: out row r is x row order[r] / top, zeros where order[r] is no place of tokens * top.  Rows of row_bytes bytes (any type), strides in bytes. */
+int nb200_dev_experts_gather(void *out, uint64_t out_stride, const void *x, uint64_t x_stride, uint64_t row_bytes, const int32_t *order, uint32_t n, uint32_t top, uint32_t tokens, void *stream);
+/* And back: out row t = sum over j of weights[t * top + j] y[place[t * top + j]], j ascending, in fp32, rounded once; a place outside [0, rows) adds nothing.  weights: fp32, NULL for ones.
+ * y, out: `columns` numbers of `type` a row, strides in numbers. */
+typedef struct nb200_experts_rows {
+    void *out; uint64_t out_stride; const void *y; uint64_t y_stride;
+    const float *weights; const int32_t *place, *order; uint32_t type, tokens, top, rows, columns;
+    const void *grad; uint64_t grad_stride; void *dy; uint64_t dy_stride; float *dweights;         /* of nb200_dev_experts_combine_grad alone */
+} nb200_experts_rows;
+int nb200_dev_experts_combine(const nb200_experts_rows *p, void *stream);
+/* Its gradient.  grad [tokens][columns] is the gradient of out: dy row r = weights[order[r]] grad[order[r] / top], zeros where order[r] is no place (rows <= tokens * top of them);
+ * dweights[i] = the scalar product of grad[i / top] and y[place[i]], fp32, 0 where place[i] is none.  dy or dweights may be NULL; order and place belong together, as nb200_dev_experts_sort leaves them. */
+int nb200_dev_experts_combine_grad(const nb200_experts_rows *p, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,8 @@ EXPORTS = [
     "nb200_seq_fork", "nb200_step_scores", "nb200_read_scores",
     "nb200_dev_token_logprobs", "nb200_dev_pages_copy",
     "nb200_dev_kv4_write", "nb200_dev_kv4_read", "nb200_dev_kv4_attention_workspace", "nb200_dev_kv4_attention",
+    "nb200_dev_mx4_quantize", "nb200_dev_mx4_read", "nb200_dev_mx4_product_workspace", "nb200_dev_mx4_product",
+    "nb200_dev_experts_sort", "nb200_dev_experts_gather", "nb200_dev_experts_combine", "nb200_dev_experts_combine_grad",
 ]
 
 
@@ -57,6 +59,23 @@ class Kv4Attention(C.Structure):
                [("pool", C.c_void_p), ("page_stride", C.c_uint64)] + [(n, C.c_uint32) for n in ("n_pages", "kv_heads", "head_dim", "type", "batch", "tokens", "heads", "width")] + \
                [("table_stride", C.c_uint64), ("table", C.c_void_p), ("lens", C.c_void_p), ("sinks", C.c_void_p), ("scale", C.c_float), ("softcap", C.c_float),
                 ("window", C.c_uint32), ("block", C.c_uint32)]
+
+
+class Mx4Rows(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("code_stride", C.c_uint64), ("scale_stride", C.c_uint64), ("x", C.c_void_p), ("x_stride", C.c_uint64)] + \
+               [(n, C.c_uint32) for n in ("type", "rows", "columns")]
+
+
+class Mx4Product(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_scales", C.c_void_p), ("x_stride", C.c_uint64), ("xs_stride", C.c_uint64), ("w", C.c_void_p), ("w_scales", C.c_void_p)] + \
+               [(n, C.c_uint64) for n in ("w_stride", "ws_stride", "w_expert", "ws_expert")] + [("out", C.c_void_p), ("out_stride", C.c_uint64), ("offsets", C.c_void_p)] + \
+               [(n, C.c_uint32) for n in ("x_type", "out_type", "rows", "outputs", "columns", "experts")]
+
+
+class ExpertsRows(C.Structure):
+    _fields_ = [("out", C.c_void_p), ("out_stride", C.c_uint64), ("y", C.c_void_p), ("y_stride", C.c_uint64), ("weights", C.c_void_p), ("place", C.c_void_p), ("order", C.c_void_p)] + \
+               [(n, C.c_uint32) for n in ("type", "tokens", "top", "rows", "columns")] + \
+               [("grad", C.c_void_p), ("grad_stride", C.c_uint64), ("dy", C.c_void_p), ("dy_stride", C.c_uint64), ("dweights", C.c_void_p)]
 
 
 class NB200Error(RuntimeError):
@@ -142,6 +161,12 @@ def lib(layered_ok: bool = False):
         L.nb200_dev_kv4_write.argtypes = L.nb200_dev_kv4_read.argtypes = [C.c_void_p, C.c_void_p]
         L.nb200_dev_kv4_attention_workspace.argtypes = [C.c_void_p, C.POINTER(C.c_uint64)]
         L.nb200_dev_kv4_attention.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.nb200_dev_mx4_quantize.argtypes = L.nb200_dev_mx4_read.argtypes = [C.c_void_p, C.c_void_p]
+        L.nb200_dev_mx4_product_workspace.argtypes = [C.c_void_p, C.POINTER(C.c_uint64)]
+        L.nb200_dev_mx4_product.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.nb200_dev_experts_sort.argtypes = [C.c_void_p] * 4 + [C.c_uint32] * 3 + [C.c_void_p]
+        L.nb200_dev_experts_gather.argtypes = [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]
+        L.nb200_dev_experts_combine.argtypes = L.nb200_dev_experts_combine_grad.argtypes = [C.c_void_p, C.c_void_p]
         L.nb200_lora_load.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64]
         L.nb200_lora_enable.argtypes = [C.c_void_p, C.c_int]
         L.nb200_lora_unload.argtypes = [C.c_void_p]

@@ -6,8 +6,16 @@
     kv4_read         what rows of a pool stand for
     kv4_attention    attention of queries over the pages of their sequences
     pages_copy       pages of a paged cache copied (forked, moved) in many pools at once
+    mx4_quantize     rows in microscaled 4-bit floating point (Mx4)
+    mx4_read         what such rows stand for
+    mx4_product      rows times a matrix in that format
+    experts_sort     which rows go to which expert (Routing)
+    experts_gather   tokens' rows in the order of their experts
+    experts_product  those rows times their experts' matrices in 4 bits
+    experts_combine  experts' rows back to their tokens, weighted and summed
 
-Calls run on the current stream of the tensors' device, wait for nothing and may be captured into a CUDA graph.  Outputs are new tensors, which carry no gradients.
+Calls run on the current stream of the tensors' device, wait for nothing and may be captured into a CUDA graph.  Outputs are new tensors; only those of experts_gather and experts_combine
+carry gradients.
 Arguments that an operator does not take are refused with NB200Error before anything is queued; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -15,6 +23,7 @@ from __future__ import annotations
 import ctypes as C
 import struct
 from array import array
+from typing import NamedTuple
 
 import torch
 
@@ -24,6 +33,8 @@ from .engine import NB200Error, lib
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # the argument blocks nb200_kv4_rows and nb200_kv4_attention as bytes: a ctypes.Structure of as many fields takes four times as long to fill
 _ROWS, _ATTENTION = struct.Struct("@QQIIIIIQQQQQQQ").pack, struct.Struct("@QQQQQQQQQQIIIIIIIIQQQQffII").pack
+_MX4_ROWS, _MX4_PRODUCT, _EXPERTS_ROWS = struct.Struct("@QQQQQQIII4x").pack, struct.Struct("@QQQQQQQQQQQQQIIIIII").pack, struct.Struct("@QQQQQQQIIIIIQQQQQ").pack
+assert len(_MX4_ROWS(*[0] * 9)) == C.sizeof(E.Mx4Rows) and len(_MX4_PRODUCT(*[0] * 19)) == C.sizeof(E.Mx4Product) and len(_EXPERTS_ROWS(*[0] * 17)) == C.sizeof(E.ExpertsRows)
 assert len(_ROWS(*[0] * 14)) == C.sizeof(E.Kv4Rows) and len(_ATTENTION(*[0] * 26)) == C.sizeof(E.Kv4Attention)
 _stream_of, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice          # (torch.cuda's functions of that purpose cost two microseconds a call)
 
@@ -272,3 +283,282 @@ def kv4_attention(q, pool, table, lens, scale=None, window=0, block=0, softcap=0
 
 def _workspace(L, p, need, stream):
     return L.nb200_dev_kv4_attention_workspace(p, C.byref(need))
+
+
+class Mx4(NamedTuple):
+    """Rows of numbers in microscaled 4-bit floating point: groups of 32 neighbours share a scale, the last group is filled up with zeros.
+
+    codes [..., 16 * groups] (uint8): two to a byte, the lower four bits first; a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  scales [..., groups] (uint8): E stands for 2^(E - 127), 255
+    for NaN.  columns: how many numbers a row has; groups = ceil(columns / 32)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    columns: int
+
+
+class Routing(NamedTuple):
+    """Places of a list of experts' numbers [tokens, top], sorted by expert.  order [tokens * top] (int32): the places t * top + j by expert and, within one, ascending, then -1 for those without an
+    expert; offsets [experts + 1] (int32): where each expert's rows begin in it; place [tokens, top] (int32): where in order a place stands, or -1."""
+    order: torch.Tensor
+    offsets: torch.Tensor
+    place: torch.Tensor
+
+
+def _rows_of(name, x):
+    """A tensor [..., columns] of numbers as (device, tensor of neighbouring numbers, rows, columns, stride from row to row)."""
+    device = _cuda(name, x)
+    if not x.dim():
+        _no("%s is [..., columns]", name)
+    columns = x.shape[-1]
+    if x.dim() == 2:
+        rows, stride = x.shape[0], x.stride(0)
+        if (x.stride(1) != 1 and columns > 1) or stride < 0:
+            x, stride = x.contiguous(), columns
+    else:
+        x, stride = x.contiguous(), columns
+        rows = x.numel() // columns if columns else 0
+    if (rows | columns) >> 31:
+        _no("%s: %d rows of %d are too many for one call", name, rows, columns)
+    return device, x, rows, columns, stride
+
+
+def _mx4(name, m, device=None):
+    """(device, rows, groups, bytes from row to row of codes and of scales) of the last two dimensions"""
+    codes, scales, columns = m
+    device = _cuda(name, codes, device)
+    _cuda(name, scales, device)
+    groups = -(-columns // 32)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.dim() or codes.shape[-1] != 16 * groups or scales.shape[-1:] != (groups,) or codes.shape[:-1] != scales.shape[:-1]:
+        _no("%s has uint8 codes [..., %d] and scales [..., %d] for %d columns", name, 16 * groups, groups, columns)
+    if (codes.stride(-1) != 1 and groups) or (scales.stride(-1) != 1 and groups > 1):
+        _no("%s: a row's bytes are to be neighbours", name)
+    return device, groups
+
+
+def _mx4_rows(name, m):
+    """The rows of an Mx4 as (device, codes [rows, ...], scales [rows, ...])."""
+    device, groups = _mx4(name, m)
+    codes, scales = m.codes, m.scales
+    if codes.dim() != 2:
+        codes, scales = codes.reshape(-1, 16 * groups) if groups else codes.new_empty(0, 0), scales.reshape(-1, groups) if groups else scales.new_empty(0, 0)
+    if codes.stride(0) < 0 or scales.stride(0) < 0:
+        codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.shape[0] >> 31 or m.columns >> 31:
+        _no("%s: %d rows of %d are too many for one call", name, codes.shape[0], m.columns)
+    return device, codes, scales
+
+
+def mx4_quantize(x):
+    """x [..., columns] (float32, bfloat16 or float16; rows of a matrix may lie any stride apart) as an Mx4.  Of a group's largest magnitude a the scale is 2^(floor(log2 a) - 2); a number becomes the
+    nearest code, of two as near the one with an even number, and what lies beyond 6 becomes 6.  A group with a NaN or an infinity is NaN."""
+    device, x2, rows, columns, stride = _rows_of("x", x)
+    kind = _TYPES.get(x.dtype)
+    if kind is None:
+        _no("x is float32, bfloat16 or float16")
+    groups, shape = -(-columns // 32), x.shape[:-1]
+    codes = torch.empty((*shape, 16 * groups), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*shape, groups), dtype=torch.uint8, device=x.device)
+    if rows and columns:
+        _call(device, lib(True).nb200_dev_mx4_quantize, _MX4_ROWS(codes.data_ptr(), scales.data_ptr(), 16 * groups, groups, x2.data_ptr(), stride, kind, rows, columns))
+    return Mx4(codes, scales, columns)
+
+
+def mx4_read(m, dtype=torch.float32):
+    """What an Mx4 stands for: [..., columns]."""
+    device, codes, scales = _mx4_rows("m", m)
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        _no("rows are float32, bfloat16 or float16")
+    out = torch.empty((*m.codes.shape[:-1], m.columns), dtype=dtype, device=codes.device)
+    if out.numel():
+        _call(device, lib(True).nb200_dev_mx4_read, _MX4_ROWS(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0), out.data_ptr(), m.columns, kind, codes.shape[0], m.columns))
+    return out
+
+
+def _product(x, w, offsets, dtype):
+    wc, ws, columns = w
+    device, groups = _mx4("w", w)
+    experts = 0
+    if offsets is None:
+        if wc.dim() != 2:
+            _no("w is an Mx4 of [outputs, columns]")
+        w_expert = ws_expert = 0
+    else:
+        if wc.dim() != 3 or not wc.shape[0]:
+            _no("w is an Mx4 of [experts, outputs, columns]")
+        experts, w_expert, ws_expert = wc.shape[0], wc.stride(0), ws.stride(0)
+        _cuda("offsets", offsets, device)
+        if offsets.dim() != 1 or offsets.shape[0] != experts + 1 or offsets.dtype != torch.int32:
+            _no("offsets are [experts + 1] of int32")
+        offsets = offsets.contiguous()
+    outputs, w_stride, ws_stride = wc.shape[-2], wc.stride(-2), ws.stride(-2)
+    if isinstance(x, Mx4):
+        at, x2, xs = _mx4_rows("x", x)
+        shape, kind, rows, given = x.codes.shape[:-1], 3, x2.shape[0], x.columns
+        x_stride, xs_at, xs_stride = x2.stride(0), xs.data_ptr(), xs.stride(0)
+        dtype = dtype or torch.bfloat16
+    else:
+        at, x2, rows, given, x_stride = _rows_of("x", x)
+        shape, kind, xs_at, xs_stride = x.shape[:-1], _TYPES.get(x.dtype), 0, 0
+        if kind is None:
+            _no("x is float32, bfloat16, float16 or an Mx4")
+        dtype = dtype or x.dtype
+    if at != device:
+        _no("x is on another device")
+    if given != columns:
+        _no("x has %d columns, w %d", given, columns)
+    if offsets is not None and len(shape) != 1:
+        _no("x is [rows, columns]")
+    out_kind = _TYPES.get(dtype)
+    if out_kind is None:
+        _no("results are float32, bfloat16 or float16")
+    out = torch.empty((*shape, outputs), dtype=dtype, device=wc.device)
+    if not out.numel():
+        return out
+    if not columns:
+        return out.zero_()
+    try:
+        p = _MX4_PRODUCT(x2.data_ptr(), xs_at, x_stride, xs_stride, wc.data_ptr(), ws.data_ptr(), w_stride, ws_stride, w_expert, ws_expert, out.data_ptr(), outputs,
+                         0 if offsets is None else offsets.data_ptr(), kind, out_kind, rows, outputs, columns, experts)
+    except struct.error:
+        _no("strides are not negative, counts numbers of 32 bits")
+    need = 0 if kind == 3 else rows * 17 * groups          # (as nb200_dev_mx4_product_workspace says)
+    room = torch.empty(need, dtype=torch.uint8, device=wc.device) if need else None
+    _call(device, lib(True).nb200_dev_mx4_product, p, room.data_ptr() if need else None, need)
+    return out
+
+
+def mx4_product(x, w, dtype=None):
+    """x w^T: x [..., columns], an Mx4 or numbers (float32, bfloat16 or float16) that the call quantises as mx4_quantize does; w an Mx4 of [outputs, columns] -> [..., outputs] of dtype (x's; bfloat16
+    where x is an Mx4).  Products are exact, sums have 32 bits."""
+    return _product(x, w, None, dtype)
+
+
+def experts_product(x, w, offsets, dtype=None):
+    """Rows sorted by expert times their experts' matrices: x [rows, columns] as in mx4_product, w an Mx4 of [experts, outputs, columns], offsets [experts + 1] (int32, Routing.offsets): rows
+    offsets[e] .. offsets[e + 1] - 1 are multiplied with w[e], what lies outside of all becomes zeros -> [rows, outputs].  At most 1024 experts."""
+    if offsets is None:
+        _no("offsets are [experts + 1] of int32")
+    return _product(x, w, offsets, dtype)
+
+
+def experts_sort(ids, experts):
+    """ids [tokens, top] or [tokens] (int32 or int64): the experts of each token, in [0, experts); other numbers name none -> Routing.  At most 1024 experts."""
+    device = _cuda("ids", ids)
+    if ids.dim() not in (1, 2) or ids.dtype not in (torch.int64, torch.int32):
+        _no("ids are [tokens, top] of int32 or int64")
+    if not 0 < experts <= 1024:
+        _no("%d experts: 1 to 1024", experts)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    n = ids.numel()
+    if n >> 31:
+        _no("%d places are too many for one call", n)
+    order = torch.empty(n, dtype=torch.int32, device=ids.device)
+    place = torch.empty_like(ids, dtype=torch.int32)
+    offsets = order.new_empty(experts + 1)
+    _call(device, lib(True).nb200_dev_experts_sort, order.data_ptr(), offsets.data_ptr(), place.data_ptr(), ids.data_ptr(), ids.element_size(), n, experts)
+    return Routing(order, offsets, place)
+
+
+def _routing(routing, device):
+    """(order, place, tokens, top), contiguous"""
+    order, _, place = routing
+    _cuda("order", order, device)
+    _cuda("place", place, device)
+    if order.dim() != 1 or order.dtype != torch.int32 or place.dtype != torch.int32 or place.dim() not in (1, 2) or place.numel() != order.shape[0]:
+        _no("a routing has order [tokens * top] and place [tokens, top] of int32")
+    if order.shape[0] >> 31:
+        _no("%d places are too many for one call", order.shape[0])
+    return order.contiguous(), place.contiguous(), place.shape[0], place.shape[1] if place.dim() == 2 else 1
+
+
+def _gather(x, order, tokens, top):
+    """Rows order[r] / top of x [tokens, columns], any type."""
+    device, x, rows, columns, stride = _rows_of("x", x)
+    if rows != tokens:
+        _no("x has %d rows for %d tokens", rows, tokens)
+    n, size = order.shape[0], x.element_size()
+    out = x.new_empty(n, columns)
+    if out.numel():
+        _call(device, lib(True).nb200_dev_experts_gather, out.data_ptr(), columns * size, x.data_ptr(), stride * size, columns * size, order.data_ptr(), n, top, tokens)
+    return out
+
+
+def _combine(y, place, weights, tokens, top):
+    device, y, rows, columns, stride = _rows_of("y", y)
+    out = y.new_empty(tokens, columns)
+    if out.numel():
+        _call(device, lib(True).nb200_dev_experts_combine, _EXPERTS_ROWS(out.data_ptr(), columns, y.data_ptr(), stride, 0 if weights is None else weights.data_ptr(), place.data_ptr(), 0,
+                                                                         _TYPES[y.dtype], tokens, top, rows, columns, 0, 0, 0, 0, 0))
+    return out
+
+
+class _Gather(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order, place, tokens, top):
+        ctx.save_for_backward(place)
+        ctx.sizes = tokens, top
+        return _gather(x, order, tokens, top)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _combine(grad, ctx.saved_tensors[0], None, *ctx.sizes), None, None, None, None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, order, place, tokens, top):
+        ctx.save_for_backward(y, weights, order, place)
+        ctx.sizes = tokens, top
+        return _combine(y, place, weights, tokens, top)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weights, order, place = ctx.saved_tensors
+        tokens, top = ctx.sizes
+        device, grad, _, columns, grad_stride = _rows_of("the gradient", grad)
+        _, y, rows, _, y_stride = _rows_of("y", y)
+        dy = y.new_empty(rows, columns) if ctx.needs_input_grad[0] else None
+        dw = None if weights is None or not ctx.needs_input_grad[1] else torch.empty_like(weights)
+        _call(device, lib(True).nb200_dev_experts_combine_grad, _EXPERTS_ROWS(0, 0, y.data_ptr(), y_stride, 0 if weights is None else weights.data_ptr(), place.data_ptr(), order.data_ptr(),
+                                                                              _TYPES[y.dtype], tokens, top, rows, columns, grad.data_ptr(), grad_stride, 0 if dy is None else dy.data_ptr(), columns,
+                                                                              0 if dw is None else dw.data_ptr()))
+        return dy, dw, None, None, None, None
+
+
+def experts_gather(x, routing):
+    """Tokens' rows in the order of their experts: x [tokens, columns] (any type, or an Mx4) -> [tokens * top, columns], row r that of token order[r] / top, zeros behind the last place that has an
+    expert.  A token's gradient is the sum, in 32 bits, of those of its rows (float32, bfloat16 and float16)."""
+    if isinstance(x, Mx4):
+        device, _ = _mx4("x", x)
+        order, _, tokens, top = _routing(routing, device)
+        if x.codes.dim() != 2:
+            _no("x is an Mx4 of [tokens, columns]")
+        return Mx4(_gather(x.codes, order, tokens, top), _gather(x.scales, order, tokens, top), x.columns)
+    order, place, tokens, top = _routing(routing, _cuda("x", x))
+    if x.dim() != 2:
+        _no("x is [tokens, columns]")
+    if x.requires_grad and torch.is_grad_enabled():
+        if x.dtype not in _TYPES:
+            _no("rows with gradients are float32, bfloat16 or float16")
+        return _Gather.apply(x, order, place, tokens, top)
+    return _gather(x, order, tokens, top)
+
+
+def experts_combine(y, routing, weights=None):
+    """Experts' rows back to their tokens: y [rows, columns] (float32, bfloat16 or float16), rows as experts_gather gives them, weights [tokens, top] (ones unless given) ->
+    [tokens, columns], sum over j of weights[t, j] y[place[t, j]] in 32 bits, rounded once to y's type; a place without an expert adds nothing.  Gradients go to y and weights."""
+    device = _cuda("y", y)
+    order, place, tokens, top = _routing(routing, device)
+    if y.dim() != 2 or y.shape[0] != order.shape[0] or y.dtype not in _TYPES:
+        _no("y is [%d, columns] of float32, bfloat16 or float16", order.shape[0])
+    if weights is not None:
+        _cuda("weights", weights, device)
+        if weights.shape != routing.place.shape or not weights.is_floating_point():
+            _no("weights are [tokens, top] of numbers")
+        weights = weights.float().contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Combine.apply(y, weights, order, place, tokens, top)
+    return _combine(y, place, weights, tokens, top)
