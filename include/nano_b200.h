@@ -287,7 +287,7 @@ int nb200_dev_mx4_read(const nb200_mx4_rows *rows, void *stream);
  * quantises as nb200_dev_mx4_quantize does.  Products are exact, sums are fp32, rounded once to out_type.  A group's sum that leaves the range of fp32 makes the result infinite or NaN.
  * experts > 0: w holds a matrix for each expert (w_expert, ws_expert: bytes from one to the next), rows offsets[e] .. offsets[e + 1] - 1 (offsets [experts + 1] ascending) are multiplied with
  * that of expert e, and rows outside of all become zeros.
- * What fills up a last group does not count, whatever it holds.  Codes: bases and strides are multiples of 16 bytes.  x_stride counts numbers (bytes for codes), out_stride numbers.  The workspace holds x as it was quantised (none for codes); its bytes do not
+ * What fills up a last group does not count, whatever it holds.  Codes: bases and strides are multiples of 16 bytes.  x_stride counts numbers (bytes for codes), out_stride numbers.  The workspace holds x as it was quantised (none is needed for codes of an even number of columns); its bytes do not
  * depend on what lies in device memory; two calls that may run at the same time need one each. */
 #define NB200_T_MX4 3u
 typedef struct nb200_mx4_product {

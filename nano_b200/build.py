@@ -49,6 +49,7 @@ UNITS = {
     "kv4.cu": ["kv4.cuh", "kv4.h", "ops.h", "portions.h", "family.h", "../../include/nano_b200.h"],
     "kv4_tc.cu": ["kv4.cuh", "kv4.h", "ops.h", "pairs.cuh", "tc_ptx.cuh", "family.h"],
     "mx4.cu": ["mx4.h", "ops.h", "portions.h", "family.h", "../../include/nano_b200.h"],
+    "mx4_tc.cu": ["mx4.h", "ops.h", "tc_ptx.cuh", "family.h"],
     "experts.cu": ["ops.h", "portions.h", "family.h", "../../include/nano_b200.h"],
     "sample.cu": ["kernels.cuh", "expf_ref.cuh", "sample_host.h"],
 }
@@ -56,7 +57,7 @@ UNITS = {
 
 # the units a model FOLDER (config.json + model.safetensors) needs: registry, folder reader, layered runtime, device sampler, operators.
 # The model-file family (engine.cu, stream.cu: minutes of nvcc) is not among them.
-LAYERED_UNITS = ["api.cu", "modeldir.cu", "layered.cu", "layered_tc.cu", "attn_tc.cu", "sample.cu", "ops.cu", "kv4.cu", "kv4_tc.cu", "mx4.cu", "experts.cu"]
+LAYERED_UNITS = ["api.cu", "modeldir.cu", "layered.cu", "layered_tc.cu", "attn_tc.cu", "sample.cu", "ops.cu", "kv4.cu", "kv4_tc.cu", "mx4.cu", "mx4_tc.cu", "experts.cu"]
 LAYERED_SO = os.path.join(LIB, "libnano_b200_layered.so")
 
 

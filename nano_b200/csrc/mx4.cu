@@ -141,7 +141,7 @@ cudaError_t by_rows(const Mx4Rows &a, uint32_t per_row, F f) {
         Mx4Rows b = a;
         b.rows = n;
         b.codes += (uint64_t)r0 * a.code_stride; b.scales += (uint64_t)r0 * a.scale_stride;
-        b.x = static_cast<char *>(a.x) + (uint64_t)r0 * a.x_stride * elem_size(a.type);
+        if (a.type != T_MX4) b.x = static_cast<char *>(a.x) + (uint64_t)r0 * a.x_stride * elem_size(a.type);
         f(b, n * per_row, (n * per_row + kThreads - 1u) / kThreads);
         return cudaGetLastError();
     });
@@ -159,62 +159,17 @@ cudaError_t read_launch_t(const Mx4Rows &a, cudaStream_t stream) {
     return go(k_mx4_read<T, 1>, 1);
 }
 
-// ------------------------------------------------------------------------------------------------
-// Products, the plainest: a block has 64 outputs of 64 rows of one expert, and brings a group of each at a time to shared memory as fp32.
-// ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void store_out(const Mx4Product &a, uint64_t row, uint32_t n, float v) {
-    const uint64_t at = row * a.out_stride + n;
-    if (a.out_type == T_F32) static_cast<float *>(a.out)[at] = v;
-    else if (a.out_type == T_BF16) static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half *>(a.out)[at] = __float2half_rn(v);
-}
-// grid (outputs / 64, rows / 64, experts + 1): the last one's rows are those of no expert
-__global__ void __launch_bounds__(256) k_mx4_plain(const Mx4Product a, const uint32_t G) {
-    __shared__ float xs[64][33], ws[64][33];
-    const uint32_t e = blockIdx.z, n0 = blockIdx.x * 64u, tid = threadIdx.x, tx = tid % 16u, ty = tid / 16u;
-    uint32_t r0 = 0, r1 = a.rows;
-    if (a.offsets) {
-        const uint32_t first = min((uint32_t)max(a.offsets[0], 0), a.rows);
-        if (e < a.experts) { r0 = min((uint32_t)max(a.offsets[e], 0), a.rows); r1 = min((uint32_t)max(a.offsets[e + 1], 0), a.rows); }
-        else r0 = min((uint32_t)max(a.offsets[a.experts], 0), a.rows);
-        if (e == a.experts && first > 0)
-            for (uint32_t r = blockIdx.y * 64u + ty; r < min(first, blockIdx.y * 64u + 64u); r += 16u) for (uint32_t n = n0 + tx; n < min(a.outputs, n0 + 64u); n += 16u) store_out(a, r, n, 0.0f);
-    }
-    r0 += blockIdx.y * 64u;
-    if (r0 >= r1) return;
-    const bool none = a.offsets && e == a.experts;
-    float acc[4][4] = {};
-    if (!none)
-        for (uint32_t g = 0; g < G; g++) {
-            for (uint32_t i = tid; i < 64u * 16u; i += 256u) {
-                const uint32_t r = i / 16u, b = i % 16u;
-                float2 v = make_float2(0.0f, 0.0f), u = v;
-                if (r0 + r < r1) {
-                    const uint32_t k = g * 32u + 2u * b, byte = k < a.columns ? a.x[(uint64_t)(r0 + r) * a.x_stride + g * 16u + b] : 0u;          // what fills up the last group does not count
-                    v = __half22float2(numbers_of(k + 1u < a.columns ? byte : byte & 15u));
-                    const float s = scale_of(a.xs[(uint64_t)(r0 + r) * a.xs_stride + g]);
-                    v.x *= s; v.y *= s;
-                }
-                if (n0 + r < a.outputs) {
-                    u = __half22float2(numbers_of(a.w[e * a.w_expert + (uint64_t)(n0 + r) * a.w_stride + g * 16u + b]));
-                    const float s = scale_of(a.ws[e * a.ws_expert + (uint64_t)(n0 + r) * a.ws_stride + g]);
-                    u.x *= s; u.y *= s;
-                }
-                xs[r][2 * b] = v.x; xs[r][2 * b + 1] = v.y; ws[r][2 * b] = u.x; ws[r][2 * b + 1] = u.y;
-            }
-            __syncthreads();
-            for (uint32_t k = 0; k < 32u; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][j] = fmaf(xs[ty * 4 + i][k], ws[tx + 16 * j][k], acc[i][j]);
-            __syncthreads();
-        }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (r0 + ty * 4u + i < r1 && n0 + tx + 16u * j < a.outputs) store_out(a, r0 + ty * 4u + i, n0 + tx + 16u * j, acc[i][j]);
+// Rows of codes as a product wants them where a row ends inside a byte: what fills up the last group is zeros.  A group to a thread.
+__global__ void __launch_bounds__(kThreads) k_mx4_clean(const Mx4Rows a, const uint8_t *codes, const uint64_t code_stride, const uint8_t *scales, const uint64_t scale_stride, const uint32_t per_row,
+                                                        const uint32_t items) {
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+    if (i >= items) return;
+    const uint32_t row = i / per_row, g = i % per_row, live = min(kMx4Group, a.columns - g * kMx4Group);
+    uint4 v = __ldg(reinterpret_cast<const uint4 *>(codes + (uint64_t)row * code_stride) + g);
+    auto keep = [&](uint32_t w, uint32_t from) { return live >= from + 8u ? w : live <= from ? 0u : w & ((1u << (4u * (live - from))) - 1u); };
+    v = make_uint4(keep(v.x, 0), keep(v.y, 8), keep(v.z, 16), keep(v.w, 24));
+    reinterpret_cast<uint4 *>(a.codes + (uint64_t)row * a.code_stride)[g] = v;
+    a.scales[(uint64_t)row * a.scale_stride + g] = scales[(uint64_t)row * scale_stride + g];
 }
 
 }  // namespace
@@ -230,10 +185,13 @@ cudaError_t mx4_quantize_launch(const Mx4Rows &a, cudaStream_t stream) {
 cudaError_t mx4_read_launch(const Mx4Rows &a, cudaStream_t stream) {
     return a.type == T_F32 ? read_launch_t<float>(a, stream) : a.type == T_BF16 ? read_launch_t<__nv_bfloat16>(a, stream) : read_launch_t<__half>(a, stream);
 }
-cudaError_t mx4_product_launch(const Mx4Product &a, cudaStream_t stream) {
-    if (!a.rows || !a.outputs) return cudaSuccess;
-    k_mx4_plain<<<dim3((a.outputs + 63u) / 64u, (a.rows + 63u) / 64u, a.offsets ? a.experts + 1u : 1u), 256, 0, stream>>>(a, mx4_groups(a.columns));
-    return cudaGetLastError();
+cudaError_t mx4_clean_launch(const Mx4Rows &a, const uint8_t *codes, uint64_t code_stride, const uint8_t *scales, uint64_t scale_stride, cudaStream_t stream) {
+    const uint32_t per_row = mx4_groups(a.columns);
+    uint32_t r0 = 0;
+    return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
+        k_mx4_clean<<<blocks, kThreads, 0, stream>>>(b, codes + r0 * code_stride, code_stride, scales + r0 * scale_stride, scale_stride, per_row, items);
+        r0 += b.rows;
+    });
 }
 
 }  // namespace nb
@@ -277,7 +235,7 @@ int product_checked(const nb200_mx4_product *p, uint64_t *work) {
     if (reinterpret_cast<uintptr_t>(p->out) % nb::elem_size(p->out_type)) return fail(NB200_EINVAL, "results are not aligned to their type");
     if (p->rows > 1 && p->out_stride < p->outputs) return fail(NB200_EINVAL, "rows of results overlap");
     if (p->experts && reinterpret_cast<uintptr_t>(p->offsets) % 4u) return fail(NB200_EINVAL, "offsets are not aligned to their type");
-    if (!codes) *work = p->rows * (row + groups);
+    if (!codes || p->columns % 2u) *work = p->rows * (row + groups);
     return 0;
 }
 }  // namespace
@@ -316,13 +274,14 @@ int nb200_dev_mx4_product(const nb200_mx4_product *p, void *workspace, uint64_t 
     nb::Mx4Product a{static_cast<const uint8_t *>(p->x), static_cast<const uint8_t *>(p->x_scales), static_cast<const uint8_t *>(p->w), static_cast<const uint8_t *>(p->w_scales),
                      p->x_stride, p->xs_stride, p->w_stride, p->ws_stride, p->w_expert, p->ws_expert, p->out, p->out_stride, p->experts ? p->offsets : nullptr,
                      p->out_type, p->rows, p->outputs, p->columns, p->experts};
-    if (p->x_type != NB200_T_MX4) {
+    if (need) {
         const uint64_t groups = nb::mx4_groups(p->columns);
         uint8_t *codes = static_cast<uint8_t *>(workspace), *scales = codes + p->rows * groups * 16u;
-        NB_CK(nb::mx4_quantize_launch(nb::Mx4Rows{codes, scales, groups * 16u, groups, const_cast<void *>(p->x), p->x_stride, p->x_type, p->rows, p->columns}, s));
+        const nb::Mx4Rows rows{codes, scales, groups * 16u, groups, const_cast<void *>(p->x), p->x_stride, p->x_type, p->rows, p->columns};
+        NB_CK(p->x_type == NB200_T_MX4 ? nb::mx4_clean_launch(rows, a.x, a.x_stride, a.xs, a.xs_stride, s) : nb::mx4_quantize_launch(rows, s));
         a.x = codes; a.xs = scales; a.x_stride = groups * 16u; a.xs_stride = groups;
     }
-    NB_CK(nb::mx4_product_launch(a, s));
+    NB_CK(nb::mx4_tc_launch(a, need != 0, s));
     return 0;
 }
 

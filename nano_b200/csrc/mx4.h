@@ -10,11 +10,13 @@
 
 namespace nb {
 
-constexpr uint32_t T_MX4 = 3, kMx4Group = 32, kMx4GroupBytes = 16;
+constexpr uint32_t T_MX4 = 3, kMx4Group = 32;
 inline uint32_t mx4_groups(uint32_t columns) { return columns / kMx4Group + (columns % kMx4Group != 0); }
 
 struct Mx4Rows { uint8_t *codes, *scales; uint64_t code_stride, scale_stride; void *x; uint64_t x_stride; uint32_t type, rows, columns; };
 cudaError_t mx4_quantize_launch(const Mx4Rows &a, cudaStream_t stream);
+// codes and scales of type T_MX4 with zeros where a row's last group is filled up, to a.codes and a.scales
+cudaError_t mx4_clean_launch(const Mx4Rows &a, const uint8_t *codes, uint64_t code_stride, const uint8_t *scales, uint64_t scale_stride, cudaStream_t stream);
 cudaError_t mx4_read_launch(const Mx4Rows &a, cudaStream_t stream);
 
 // x and w are codes here
@@ -23,6 +25,7 @@ struct Mx4Product {
     void *out; uint64_t out_stride; const int32_t *offsets;          // null: one matrix for all rows
     uint32_t out_type, rows, outputs, columns, experts;
 };
-cudaError_t mx4_product_launch(const Mx4Product &a, cudaStream_t stream);
+// made: the kernel queued before this one made x and xs, and nothing else that this one reads
+cudaError_t mx4_tc_launch(const Mx4Product &a, bool made, cudaStream_t stream);
 
 }  // namespace nb

@@ -421,7 +421,7 @@ def _product(x, w, offsets, dtype):
                          0 if offsets is None else offsets.data_ptr(), kind, out_kind, rows, outputs, columns, experts)
     except struct.error:
         _no("strides are not negative, counts numbers of 32 bits")
-    need = 0 if kind == 3 else rows * 17 * groups          # (as nb200_dev_mx4_product_workspace says)
+    need = rows * 17 * groups if kind != 3 or columns % 2 else 0          # (as nb200_dev_mx4_product_workspace says)
     room = torch.empty(need, dtype=torch.uint8, device=wc.device) if need else None
     _call(device, lib(True).nb200_dev_mx4_product, p, room.data_ptr() if need else None, need)
     return out
