@@ -1,8 +1,8 @@
 // mx4_tc.cu -- products of rows in microscaled 4-bit floating point on the fifth-generation tensor cores, which multiply the codes as they are (format: mx4.h).
 //
-// out^T = W X^T in tiles of 128 rows of W x TN rows of X: tcgen05.mma kind::mxf4 takes 64 columns of both and two scales for each row, which lie in tensor memory (tcgen05.cp brings them there).
-// A stage is 256 columns: codes by cp.async.bulk.tensor into 128-byte-swizzled rows, scales by two warps, which lay 128 rows x 4 scales out as that copy wants them (32 lines of 16 bytes: row r's word
-// is word r / 32 of line r % 32).  A lane of tensor memory is an output column, so a warp's stores of one row are neighbours.
+// out^T = W X^T in tiles of 128 rows of W x TN rows of X: tcgen05.mma kind::mxf4 takes 64 columns of both and two scales for each row, which lie in tensor memory.
+// A stage is 256 columns: codes by cp.async.bulk.tensor into 128-byte-swizzled rows, scales by four warps.  A lane of tensor memory is an output column, so a warp's stores of one row are
+// neighbours.
 // Every wait has a limit; a block in which one runs out leaves with NaN in its results.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -17,17 +17,16 @@
 namespace nb {
 namespace {
 
-constexpr uint32_t kRows = 128, kDepth = 256, kStageGroups = kDepth / kMx4Group;          // rows of W in a tile; columns of a stage
+constexpr uint32_t kRows = 128, kDepth = 256, kStageGroups = kDepth / kMx4Group, kMostExperts = 1024;          // rows of W in a tile; columns of a stage
 template <int TN> struct Tile {
-    static constexpr uint32_t blocks = (TN + 127) / 128;          // of 128 rows, as scales are laid out
-    static constexpr uint32_t x_at = kRows * 128u, ws_at = x_at + TN * 128u, xs_at = ws_at + 1024u, bytes = xs_at + 1024u * blocks;          // of a stage
-    static constexpr uint32_t stages = TN <= 16 ? 5 : TN <= 64 ? 4 : 3;          // up to 104 KB: two blocks to an SM
-    static constexpr uint32_t scale_cols = 8u + 8u * blocks, cols_used = (TN < 32 ? 32u : TN) + stages * scale_cols;
-    static constexpr uint32_t cols = cols_used <= 128 ? 128 : cols_used <= 256 ? 256 : 512;
-    static constexpr uint32_t smem = stages * bytes + 1024u;
+    static constexpr uint32_t blocks = (TN + 127) / 128;          // of 128 rows, as tensor memory holds scales: row r's word in lane r % 32, column r / 32
+    static constexpr uint32_t x_at = kRows * 128u, bytes = x_at + TN * 128u;          // of a stage
+    static constexpr uint32_t scale_cols = 8u + 8u * blocks, sum_cols = TN < 32 ? 32 : TN;          // of tensor memory
+    static constexpr uint32_t staged = (kRows + 128u * blocks) * 8u;          // a stage's scales, eight to a row, on their way
 };
+__host__ __device__ constexpr uint32_t cols_for(uint32_t used) { return used <= 128u ? 128u : used <= 256u ? 256u : 512u; }
 
-struct alignas(64) TcArgs { CUtensorMap wmap, xmap; Mx4Product p; uint32_t groups, steps, ks, wtiles, pairs, w_align, x_align, made; };
+struct alignas(64) TcArgs { CUtensorMap wmap, xmap; Mx4Product p; uint32_t groups, steps, ks, wtiles, pairs, w_unit, x_unit, made; };
 
 __device__ __forceinline__ bool soon(uint32_t bar, uint32_t parity) { return mbar_try(bar, parity) || mbar_wait(bar, parity); }
 __device__ __forceinline__ bool soon_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, soon(bar, parity)); }
@@ -38,75 +37,100 @@ __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint
     asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %6, 0;\ntcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add) : "memory");
 }
-// 32 lines of 16 bytes to four columns of tensor memory, the same in all four quarters of its lanes
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) { asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory"); }
-__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) { return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46); }          // no swizzle, 8 lines every 128 bytes
 // e2m1 x e2m1, scales in 8 bits of exponent, N columns; scales from byte `id` (0 or 2) of their words
 __host__ __device__ constexpr uint32_t idesc_of(uint32_t n, uint32_t id) { return (id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((kRows >> 4) << 24) | (id << 29); }
 
-// eight neighbouring scales of a row, from group g on; zeros behind its last
-__device__ __forceinline__ uint2 scales8(const uint8_t *row, uint32_t g, uint32_t groups, uint32_t align) {
+// Eight neighbouring scales of a row, from group g on; zeros behind its last.  UNIT: bytes that one load may bring, for every row and every g that is a multiple of it
+template <int UNIT>
+__device__ __forceinline__ uint2 scales8(const uint8_t *row, uint32_t g, uint32_t groups) {
+    if constexpr (UNIT == 8) return __ldg(reinterpret_cast<const uint2 *>(row + g));
     uint2 v = make_uint2(0u, 0u);
-    if (g + 8u <= groups && align >= 8u) return __ldg(reinterpret_cast<const uint2 *>(row + g));
-    if (g + 8u <= groups && align >= 4u) return make_uint2(__ldg(reinterpret_cast<const uint32_t *>(row + g)), __ldg(reinterpret_cast<const uint32_t *>(row + g + 4u)));
+    if constexpr (UNIT == 4) {
+        if (g < groups) v.x = __ldg(reinterpret_cast<const uint32_t *>(row + g));
+        if (g + 4u < groups) v.y = __ldg(reinterpret_cast<const uint32_t *>(row + g + 4u));
+    } else
 #pragma unroll
-    for (uint32_t i = 0; i < 8; i++) {
-        const uint32_t b = g + i < groups ? (uint32_t)row[g + i] : 0u;
-        if (i < 4) v.x |= b << (8u * i); else v.y |= b << (8u * (i - 4u));
-    }
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t b = g + i < groups ? (uint32_t)__ldg(row + g + i) : 0u;
+            if (i < 4) v.x |= b << (8u * i); else v.y |= b << (8u * (i - 4u));
+        }
     return v;
 }
 
-// A warp brings the scales of up to 128 * BLOCKS rows, stage after stage: a lane has rows lane, lane + 32, ..., and writes the words of four of them at once
-template <uint32_t BLOCKS>
-struct ScaleWarp {
-    const uint8_t *row[BLOCKS * 4];
-    uint32_t groups, align;
-    // rows [0, live) at `base`; what lies behind them counts for nothing and is read from the first
-    __device__ __forceinline__ void at(const uint8_t *base, uint64_t stride, uint32_t live, uint32_t lane) {
+// Four warps bring the scales of tile after tile to tensor memory: a thread loads those of one row of W and of one or two of X, eight at a time and kAhead stages ahead, the four exchange them
+// through shared memory, and each writes all of them to its quarter of the lanes.  (tcgen05.cp, which replicates by itself, takes its turn with the products, some 55 cycles for each 128 x 4
+// scales, a quarter of a stage of 128 x 256: 8192 x 8192 x 8192 took 266 us with it.)
+constexpr uint32_t kAhead = 4, kScaleThreads = 128, kScaleBar = 1;
+__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+struct ScaleRows { const uint8_t *base; uint64_t stride; uint32_t live; };          // rows [0, live); what lies behind them counts for nothing
+struct ScaleRing { uint32_t staged, tmem, stages, full, empty, groups, w_unit, x_unit; };
+template <int TN, int WU, int XU, typename F>
+__device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t total, uint32_t s0, uint32_t ns, F &next) {
+    using Z = Tile<TN>;
+    constexpr uint32_t XR = Z::blocks;          // rows of X to a thread
+    const uint32_t tid = threadIdx.x & (kScaleThreads - 1u), warp = tid >> 5, lane = tid & 31u;
+    const uint8_t *w_row = nullptr, *x_row[XR] = {};
+    uint2 v[kAhead][1 + XR];
+    uint32_t asked = 0, step = ns;
+    auto ask = [&](uint2 (&to)[1 + XR]) {
+        if (asked == total) return;
+        if (step == ns) {
+            ScaleRows w, x;
+            next(w, x);
+            w_row = w.base + (tid < w.live ? tid : 0u) * w.stride;
 #pragma unroll
-        for (uint32_t i = 0; i < BLOCKS * 4; i++) { const uint32_t r = lane + 32u * i; row[i] = base + (r < live ? r : 0u) * stride; }
-    }
-    __device__ __forceinline__ void load(uint32_t step, uint2 (&v)[BLOCKS * 4]) const {
-#pragma unroll
-        for (uint32_t i = 0; i < BLOCKS * 4; i++) v[i] = scales8(row[i], step * kStageGroups, groups, align);
-    }
-    __device__ __forceinline__ static void store(uint32_t to, const uint2 (&v)[BLOCKS * 4], uint32_t lane) {          // [half of the stage][block][line]
-#pragma unroll
-        for (uint32_t b = 0; b < BLOCKS; b++) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + b * 512u + lane * 16u), "r"(v[4 * b].x), "r"(v[4 * b + 1].x), "r"(v[4 * b + 2].x), "r"(v[4 * b + 3].x) : "memory");
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (BLOCKS + b) * 512u + lane * 16u), "r"(v[4 * b].y), "r"(v[4 * b + 1].y), "r"(v[4 * b + 2].y), "r"(v[4 * b + 3].y) : "memory");
+            for (uint32_t i = 0; i < XR; i++) { const uint32_t q = tid + i * kScaleThreads; x_row[i] = x.base + (q < x.live ? q : 0u) * x.stride; }
+            step = 0;
         }
-    }
-};
-template <uint32_t BLOCKS>
-__device__ __forceinline__ bool bring_scales(const ScaleWarp<BLOCKS> &w, uint32_t s0, uint32_t ns, uint32_t ring, uint32_t bytes, uint32_t off, uint32_t stages, uint32_t full, uint32_t empty, uint32_t lane) {
-    uint2 v[2][BLOCKS * 4];
-    if (ns > 0) w.load(s0, v[0]);
-    if (ns > 1) w.load(s0 + 1u, v[1]);
-#pragma unroll 2
-    for (uint32_t i = 0; i < ns; i++) {
-        const uint32_t st = i % stages;
-        if (i >= stages && !soon_warp(empty + st * 8u, ((i / stages) - 1u) & 1u)) return false;
-        ScaleWarp<BLOCKS>::store(ring + st * bytes + off, v[i & 1u], lane);
-        if (i + 2u < ns) w.load(s0 + i + 2u, v[i & 1u]);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // plain stores, read by the tensor core
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + st * 8u);
-    }
+        to[0] = scales8<WU>(w_row, (s0 + step) * kStageGroups, r.groups);
+#pragma unroll
+        for (uint32_t i = 0; i < XR; i++) to[1 + i] = scales8<XU>(x_row[i], (s0 + step) * kStageGroups, r.groups);
+        step++; asked++;
+    };
+#pragma unroll
+    for (uint32_t d = 0; d < kAhead; d++) ask(v[d]);
+    uint32_t st = 0, turn = 0;
+    for (uint32_t i = 0; i < total; i += kAhead)
+#pragma unroll
+        for (uint32_t d = 0; d < kAhead; d++) {
+            if (i + d >= total) return true;
+            const uint32_t at = r.staged + (d & 1u) * Z::staged;          // (two stages in turn: kAhead is even)
+#pragma unroll
+            for (uint32_t j = 0; j < 1 + XR; j++) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + (j * kScaleThreads + tid) * 8u), "r"(v[d][j].x), "r"(v[d][j].y) : "memory");
+            const bool ok = !turn || soon_warp(r.empty + st * 8u, (turn - 1u) & 1u);
+            if (bar_any(kScaleBar, kScaleThreads, !ok)) return false;          // one verdict for the four warps, which meet here
+            tc_fence_after();
+            ask(v[d]);
+            uint32_t w[8], x[8 * XR];          // [half of the stage][row / 32]
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j]), "=r"(w[4 + j]) : "r"(at + (j * 32u + lane) * 8u) : "memory");
+#pragma unroll
+            for (uint32_t j = 0; j < 4 * XR; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[j]), "=r"(x[4 * XR + j]) : "r"(at + (kRows + j * 32u + lane) * 8u) : "memory");
+            const uint32_t to = r.tmem + ((warp * 32u) << 16) + st * Z::scale_cols;
+            tc_st8(to, w);
+            if constexpr (XR == 1) tc_st8(to + 8u, x); else tc_st16(to + 8u, x);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(r.full + st * 8u);
+            if (++st == r.stages) { st = 0; turn++; }
+        }
     return true;
 }
+// next(w, x) names the rows of the next tile; `total` stages, ns to a tile, the first of them step s0 of its depth
+template <int TN, typename F>
+__device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t total, uint32_t s0, uint32_t ns, F next) {
+    if (r.w_unit == 8u && r.x_unit == 8u) return bring_scales<TN, 8, 8>(r, total, s0, ns, next);
+    if (r.w_unit >= 4u && r.x_unit >= 4u) return bring_scales<TN, 4, 4>(r, total, s0, ns, next);
+    return bring_scales<TN, 1, 1>(r, total, s0, ns, next);
+}
 
-// one stage's products
+// a stage's products
 template <int TN>
 __device__ __forceinline__ void stage_products(uint32_t at, uint32_t d, uint32_t scales, bool first) {
     using Z = Tile<TN>;
-#pragma unroll
-    for (uint32_t h = 0; h < 2; h++) {
-        copy_scales(scales + h * 4u, scale_desc(at + Z::ws_at + h * 512u));
-#pragma unroll
-        for (uint32_t b = 0; b < Z::blocks; b++) copy_scales(scales + 8u + (h * Z::blocks + b) * 4u, scale_desc(at + Z::xs_at + (h * Z::blocks + b) * 512u));
-    }
     const uint64_t wd = tc_desc(at), xd = tc_desc(at + Z::x_at);
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++)
@@ -161,18 +185,26 @@ __device__ __forceinline__ void put_rows(const Mx4Product &p, uint64_t row, uint
     else put_column<J>(static_cast<__half *>(p.out) + at, p.out_stride, live, [&](uint32_t j) { return __float2half_rn(v[j]); });
 }
 
-// grid (tiles of W x (pairs + 1 with experts), 1, ks), clusters of ks blocks that share a tile's depth
+// ------------------------------------------------------------------------------------------------
+// Few tiles: a tile's depth is shared by a cluster of ks blocks, each of which finishes some of its rows.  grid (tiles of W x (pairs + 1 with experts), 1, ks)
+// ------------------------------------------------------------------------------------------------
+template <int TN> struct Few {
+    static constexpr uint32_t stages = TN <= 32 ? 5 : TN <= 64 ? 4 : 3, cols = cols_for(Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols);          // up to 107 KB: two blocks to an SM
+    static constexpr uint32_t smem = stages * Tile<TN>::bytes + 1024u;
+};
 template <int TN>
-__global__ void __launch_bounds__(192) k_mx4_tiles(const __grid_constant__ TcArgs t) {
+__global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs t) {
     using Z = Tile<TN>;
-    constexpr uint32_t ST = Z::stages;
+    constexpr uint32_t ST = Few<TN>::stages;
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 1];
+    __shared__ __align__(8) uint8_t staged[2 * Z::staged];
     __shared__ uint32_t tmem_s, bad_s;
     __shared__ Span span_s;
     const Mx4Product &p = t.p;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, part = blockIdx.z, n0 = blockIdx.x % t.wtiles * kRows, pair = blockIdx.x / t.wtiles;
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u, full = smem_u32(bars), empty = full + ST * 8u, done = full + 2u * ST * 8u;
+    const uint32_t per = (t.steps + t.ks - 1u) / t.ks, s0 = min(t.steps, part * per), ns = min(t.steps, s0 + per) - s0;
     Span span{0u, pair * TN, min(pair * TN + TN, p.rows)};
     if (p.offsets) {
         if (pair == t.pairs) {          // rows of no expert
@@ -187,66 +219,66 @@ __global__ void __launch_bounds__(192) k_mx4_tiles(const __grid_constant__ TcArg
         span = span_s;
         if (span.r0 >= span.r1) { pdl_wait(); return; }          // (all blocks of a cluster)
     }
-    if (threadIdx.x == 0) {
+    auto weights = [&](uint32_t i) {
+        const uint32_t st = i % ST;
+        mbar_expect(full + st * 8u, Z::bytes);
+        tma_3d(ring + st * Z::bytes, &t.wmap, (s0 + i) * (kDepth / 2u), n0, span.e, full + st * 8u);
+    };
+    const uint32_t npre = min(ST, ns);
+    if (threadIdx.x == 128u) {
         bad_s = 0;
-        for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, 3); mbar_init(empty + i * 8u, 1); }
+        for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, 5); mbar_init(empty + i * 8u, 1); }
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (uint32_t i = 0; i < npre; i++) weights(i);          // these do not depend on the kernel before, which quantises the rows
     }
-    if (warp == 1) { tc_alloc(smem_u32(&tmem_s), Z::cols); tc_relinquish(); }
+    if (warp == 5) { tc_alloc(smem_u32(&tmem_s), Few<TN>::cols); tc_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_s, scales_at = tmem + (TN < 32 ? 32u : TN), per = (t.steps + t.ks - 1u) / t.ks, s0 = min(t.steps, part * per), ns = min(t.steps, s0 + per) - s0;
-    if (warp == 0 && lane == 0) {
-        const uint32_t npre = min(ST, ns);
-        auto weights = [&](uint32_t i) {
-            const uint32_t st = i % ST;
-            mbar_expect(full + st * 8u, Z::ws_at);
-            tma_3d(ring + st * Z::bytes, &t.wmap, (s0 + i) * (kDepth / 2u), n0, span.e, full + st * 8u);
-        };
-        for (uint32_t i = 0; i < npre; i++) weights(i);          // these do not depend on the kernel before, which quantises the rows
-        pdl_wait();
-        for (uint32_t i = 0; i < ns; i++) {
-            const uint32_t st = i % ST;
-            if (i >= ST) {
-                if (!soon(empty + st * 8u, ((i / ST) - 1u) & 1u)) { bad_s = 1; break; }
-                weights(i);
+    const uint32_t tmem = tmem_s, scales_at = tmem + Z::sum_cols;
+    if (warp == 4) {
+        if (lane == 0) {
+            pdl_wait();
+            for (uint32_t i = 0; i < ns; i++) {
+                const uint32_t st = i % ST;
+                if (i >= ST) {
+                    if (!soon(empty + st * 8u, ((i / ST) - 1u) & 1u)) { bad_s = 1; break; }
+                    weights(i);
+                }
+                tma_3d(ring + st * Z::bytes + Z::x_at, &t.xmap, (s0 + i) * (kDepth / 2u), span.r0, 0, full + st * 8u);
             }
-            tma_3d(ring + st * Z::bytes + Z::x_at, &t.xmap, (s0 + i) * (kDepth / 2u), span.r0, 0, full + st * 8u);
         }
-    } else if (warp == 1 && lane == 0) {
-        bool ok = true;
-        for (uint32_t i = 0; i < ns; i++) {
-            const uint32_t st = i % ST;
-            ok = soon(full + st * 8u, (i / ST) & 1u);
-            if (!ok) break;
-            tc_fence_after();
-            stage_products<TN>(ring + st * Z::bytes, tmem, scales_at + st * Z::scale_cols, i == 0);
-            tc_commit(empty + st * 8u);
+    } else if (warp == 5) {
+        if (lane == 0) {
+            bool ok = true;
+            for (uint32_t i = 0; i < ns; i++) {
+                const uint32_t st = i % ST;
+                ok = soon(full + st * 8u, (i / ST) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                stage_products<TN>(ring + st * Z::bytes, tmem, scales_at + st * Z::scale_cols, i == 0);
+                tc_commit(empty + st * 8u);
+            }
+            if (ok) tc_commit(done); else bad_s = 1;          // (the waits on it run out too)
         }
-        if (ok) tc_commit(done); else bad_s = 1;          // (the waits on it run out too)
-    } else if (warp == 2) {
-        ScaleWarp<1> w;
-        w.groups = t.groups; w.align = t.w_align;
-        w.at(p.ws + span.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0, lane);
-        if (!bring_scales(w, s0, ns, ring, Z::bytes, Z::ws_at, ST, full, empty, lane)) bad_s = 1;
-    } else if (warp == 3) {
+    } else {
         pdl_wait();
-        ScaleWarp<Z::blocks> w;
-        w.groups = t.groups; w.align = t.x_align;
-        w.at(p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0, lane);
-        if (!bring_scales(w, s0, ns, ring, Z::bytes, Z::xs_at, ST, full, empty, lane)) bad_s = 1;
+        const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_unit, t.x_unit};
+        if (!bring_scales<TN>(r, ns, s0, ns, [&](ScaleRows &w, ScaleRows &x) {
+                w = ScaleRows{p.ws + span.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
+                x = ScaleRows{p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0};
+            })) bad_s = 1;
     }
     __syncwarp();
-    const uint32_t quad = warp & 3u, n = n0 + quad * 32u + lane;
+    const uint32_t quad = warp & 3u, n = n0 + quad * 32u + lane, rows = span.r1 - span.r0;
     bool ok = true;
-    if (warp >= 2) { ok = ns == 0 || soon_warp(done, 0); tc_fence_after(); if (!ok) bad_s = 1; }
+    if (warp < 4) { ok = ns == 0 || soon_warp(done, 0); tc_fence_after(); if (!ok) bad_s = 1; }
     float *mine = reinterpret_cast<float *>(raw + (ring - smem_u32(raw))) + quad * 32u + lane;          // partial tiles, [TN][128], where the stages were
-    if (warp >= 2) {
+    if (warp < 4) {
 #pragma unroll 1
         for (uint32_t c = 0; c < TN; c += 16u) {
-            if (span.r0 + c >= span.r1) break;
+            if (c >= rows) break;
             uint32_t v[16];
             if (ns && ok) tc_ld16(tmem + ((quad * 32u) << 16) + c, v);
             float f[16];
@@ -255,21 +287,24 @@ __global__ void __launch_bounds__(192) k_mx4_tiles(const __grid_constant__ TcArg
             if (t.ks > 1) {
 #pragma unroll
                 for (uint32_t j = 0; j < 16; j++) mine[(c + j) * kRows] = f[j];
-            } else if (n < p.outputs) put_rows<16>(p, span.r0 + c, n, f, span.r1 - span.r0 - c);
+            } else if (n < p.outputs) put_rows<16>(p, span.r0 + c, n, f, rows - c);
         }
     }
-    if (t.ks > 1) {          // every block of the cluster finishes TN / ks rows, its parts added up in the order of the depth
+    if (t.ks > 1) {          // every block of the cluster finishes some of the tile's rows, in turn, its parts added up in the order of the depth
         cluster_sync_all();
-        if (warp >= 2 && n < p.outputs) {
-            const uint32_t each = TN / t.ks, j1 = min((part + 1u) * each, span.r1 - span.r0), at = smem_u32(mine);
-            for (uint32_t j = part * each; j < j1; j++) {
-                float f = 0.0f;
+        if (warp < 4 && n < p.outputs) {
+            const uint32_t at = smem_u32(mine);
+            constexpr uint32_t J = 4;
+            for (uint32_t j = part * J; j < rows; j += t.ks * J) {
+                float f[J] = {};
+#pragma unroll 4
                 for (uint32_t q = 0; q < t.ks; q++) {
                     uint32_t peer;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + j * kRows * 4u), "r"(q));
-                    f += ld_cluster_f32(peer);
+#pragma unroll
+                    for (uint32_t i = 0; i < J; i++) f[i] += ld_cluster_f32(peer + i * kRows * 4u);          // (a part has all TN rows' places)
                 }
-                put(p, span.r0 + j, n, f);
+                put_rows<J>(p, span.r0 + j, n, f, rows - j);
             }
         }
         cluster_sync_all();          // no block leaves while another reads its part
@@ -281,7 +316,186 @@ __global__ void __launch_bounds__(192) k_mx4_tiles(const __grid_constant__ TcArg
         const long long t0 = clock64();
         while (clock64() - t0 < 20000000ll) __nanosleep(1000);
     }
-    if (warp == 1) tc_dealloc(tmem, Z::cols);
+    if (warp == 5) tc_dealloc(tmem, Few<TN>::cols);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many tiles: a block to each SM takes tiles in turn.  Codes and scales run ahead of the products over the tiles' borders, and a tile's results are written while the next one's products run: in
+// another set of columns of tensor memory (tiles of up to 128 rows of X), or, of 256, after the sums have been read out at once, 128 columns to a thread.
+// ------------------------------------------------------------------------------------------------
+template <int TN> struct Many {
+    static constexpr uint32_t stages = TN <= 16 ? 11 : TN <= 32 ? 10 : TN <= 64 ? 8 : TN <= 128 ? 6 : 4, sets = TN <= 128 ? 2 : 1, drain = TN <= 32 ? 4 : 8, columns = TN / (drain / 4);          // (columns of a thread)
+    static constexpr uint32_t tma = 4 + drain, mma = 5 + drain;          // warps 0-3: scales, then those that write results, then one each
+    static constexpr uint32_t cols = cols_for(sets * Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols), threads = 32u * (drain + 6u), smem = stages * Tile<TN>::bytes + 1024u;
+};
+template <int TN>
+__global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_constant__ TcArgs t) {
+    using Z = Tile<TN>;
+    using Y = Many<TN>;
+    constexpr uint32_t ST = Y::stages, SETS = Y::sets;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t bars[2 * ST + 2 * SETS];
+    __shared__ __align__(8) uint8_t staged[2 * Z::staged];
+    __shared__ uint32_t tmem_s, bad_s, pairs_s[kMostExperts + 1];          // of (expert, TN rows): those before an expert's
+    const Mx4Product &p = t.p;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u, full = smem_u32(bars), empty = full + ST * 8u, sums = full + 2u * ST * 8u, room = sums + SETS * 8u;
+    if (threadIdx.x == 0) {
+        bad_s = 0;
+        for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, 5); mbar_init(empty + i * 8u, 1); }
+        for (uint32_t i = 0; i < SETS; i++) { mbar_init(sums + i * 8u, 1); mbar_init(room + i * 8u, Y::drain); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == Y::mma) { tc_alloc(smem_u32(&tmem_s), Y::cols); tc_relinquish(); }
+    if (p.offsets && warp == Y::tma) {
+        uint32_t run = 0;
+        for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
+            const uint32_t e = e0 + lane, a = e < p.experts ? clamp_row(p.offsets[e], p.rows) : 0u, b = e < p.experts ? clamp_row(p.offsets[e + 1u], p.rows) : 0u, tiles = b > a ? (b - a + TN - 1u) / TN : 0u;
+            uint32_t up = tiles;
+#pragma unroll
+            for (uint32_t o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, up, o); up += lane >= o ? x : 0u; }
+            if (e < p.experts) pairs_s[e] = run + up - tiles;
+            run += __shfl_sync(0xffffffffu, up, 31);
+        }
+        if (lane == 0) pairs_s[p.experts] = run;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s, scales_at = tmem + SETS * Z::sum_cols, ns = t.steps;
+    const uint64_t tiles = (uint64_t)t.wtiles * (p.offsets ? pairs_s[p.experts] : t.pairs), mine = tiles > blockIdx.x ? (tiles - 1u - blockIdx.x) / gridDim.x + 1u : 0u;
+    uint32_t e_now = 0;
+    auto span = [&](uint64_t tile) {          // tiles come in ascending order
+        const uint32_t pair = (uint32_t)(tile / t.wtiles);
+        if (!p.offsets) return Span{0u, pair * TN, min(pair * TN + TN, p.rows)};
+        while (pairs_s[e_now + 1u] <= pair) e_now++;
+        const uint32_t r0 = clamp_row(p.offsets[e_now], p.rows) + (pair - pairs_s[e_now]) * TN;
+        return Span{e_now, r0, min(r0 + TN, clamp_row(p.offsets[e_now + 1u], p.rows))};
+    };
+    if (warp == Y::tma) {
+        if (lane == 0) {
+            bool ok = true, waited = false;
+            uint32_t st = 0, turn = 0;
+            for (uint64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                const Span s = span(tile);
+                const uint32_t n0 = (uint32_t)(tile % t.wtiles) * kRows;
+                auto weights = [&](uint32_t i, uint32_t at) {
+                    mbar_expect(full + at * 8u, Z::bytes);
+                    tma_3d(ring + at * Z::bytes, &t.wmap, i * (kDepth / 2u), n0, s.e, full + at * 8u);
+                };
+                uint32_t early = 0;
+                if (!waited) {          // the first tile's weights do not depend on the kernel before, which quantises the rows
+                    for (; early < min(ST, ns); early++) weights(early, early);
+                    pdl_wait();
+                    waited = true;
+                }
+                for (uint32_t i = 0; i < ns; i++) {
+                    ok = !turn || soon(empty + st * 8u, (turn - 1u) & 1u);
+                    if (!ok) { bad_s = 1; break; }
+                    if (i >= early) weights(i, st);
+                    tma_3d(ring + st * Z::bytes + Z::x_at, &t.xmap, i * (kDepth / 2u), s.r0, 0, full + st * 8u);
+                    if (++st == ST) { st = 0; turn++; }
+                }
+            }
+        }
+    } else if (warp == Y::mma) {
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t st = 0, phase = 0, set = 0, turn = 0;
+            for (uint64_t n = 0; n < mine && ok; n++) {
+                ok = !turn || soon(room + set * 8u, (turn - 1u) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                for (uint32_t i = 0; i < ns; i++) {
+                    ok = soon(full + st * 8u, phase);
+                    if (!ok) break;
+                    tc_fence_after();
+                    stage_products<TN>(ring + st * Z::bytes, tmem + set * Z::sum_cols, scales_at + st * Z::scale_cols, i == 0);
+                    tc_commit(empty + st * 8u);
+                    if (++st == ST) { st = 0; phase ^= 1u; }
+                }
+                if (ok) tc_commit(sums + set * 8u);
+                if (++set == SETS) { set = 0; turn++; }
+            }
+            if (!ok) bad_s = 1;
+        }
+    } else if (warp < 4) {
+        pdl_wait();
+        uint64_t tile = blockIdx.x;
+        const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_unit, t.x_unit};
+        if (!bring_scales<TN>(r, (uint32_t)mine * ns, 0, ns, [&](ScaleRows &w, ScaleRows &x) {
+                const Span s = span(tile);
+                const uint32_t n0 = (uint32_t)(tile % t.wtiles) * kRows;
+                w = ScaleRows{p.ws + s.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
+                x = ScaleRows{p.xs + (uint64_t)s.r0 * p.xs_stride, p.xs_stride, s.r1 - s.r0};
+                tile += gridDim.x;
+            })) bad_s = 1;
+    } else {
+        constexpr uint32_t CO = Y::columns, LD = CO < 32 ? 16 : 32, HELD = CO < 64 ? CO : 64;          // sums that a thread reads at once: 64 of fp32, all in 16 bits
+        const uint32_t quad = warp & 3u, c0 = ((warp - 4u) >> 2) * CO;
+        bool ok = true;
+        for (uint64_t i = 0; i < mine; i++) {
+            const uint64_t tile = blockIdx.x + i * gridDim.x;
+            const uint32_t set = (uint32_t)i % SETS, n = (uint32_t)(tile % t.wtiles) * kRows + quad * 32u + lane;
+            const Span s = span(tile);
+            ok = ok && soon_warp(sums + set * 8u, (uint32_t)(i / SETS) & 1u);
+            tc_fence_after();
+            const uint32_t from = tmem + set * Z::sum_cols + ((quad * 32u) << 16) + c0, rows = n < p.outputs && s.r0 + c0 < s.r1 ? s.r1 - s.r0 - c0 : 0u;
+            auto read = [&](uint32_t c, uint32_t (&v)[LD]) {
+                if (!ok) {
+#pragma unroll
+                    for (uint32_t j = 0; j < LD; j++) v[j] = 0x7fc00000u;
+                } else if constexpr (LD == 16) tc_ld16(from + c, v);
+                else tc_ld32(from + c, v);
+            };
+            auto free = [&] { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(room + set * 8u); };
+            if (p.out_type == T_F32) {
+#pragma unroll
+                for (uint32_t h = 0; h < CO; h += HELD) {
+                    float f[HELD];
+#pragma unroll
+                    for (uint32_t c = 0; c < HELD; c += LD) {
+                        uint32_t v[LD];
+                        read(h + c, v);
+#pragma unroll
+                        for (uint32_t j = 0; j < LD; j++) f[c + j] = __uint_as_float(v[j]);
+                    }
+                    if (h + HELD == CO) free();
+                    if (rows > h) put_column<HELD>(static_cast<float *>(p.out) + (uint64_t)(s.r0 + c0 + h) * p.out_stride + n, p.out_stride, rows - h, [&](uint32_t j) { return f[j]; });
+                }
+            } else {
+                uint32_t f[CO / 2];
+#pragma unroll
+                for (uint32_t c = 0; c < CO; c += LD) {
+                    uint32_t v[LD];
+                    read(c, v);
+#pragma unroll
+                    for (uint32_t j = 0; j < LD; j += 2) {
+                        if (p.out_type == T_BF16) { const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); f[(c + j) / 2] = *reinterpret_cast<const uint32_t *>(&y); }
+                        else { const __half2 y = __floats2half2_rn(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); f[(c + j) / 2] = *reinterpret_cast<const uint32_t *>(&y); }
+                    }
+                }
+                free();
+                if (rows) put_column<CO>(static_cast<uint16_t *>(p.out) + (uint64_t)(s.r0 + c0) * p.out_stride + n, p.out_stride, rows, [&](uint32_t j) { return (uint16_t)(f[j / 2] >> (16u * (j & 1u))); });
+            }
+        }
+        if (!ok) bad_s = 1;
+        if (p.offsets) {          // rows of no expert
+            const uint32_t first = clamp_row(p.offsets[0], p.rows), none = first + (p.rows - clamp_row(p.offsets[p.experts], p.rows));
+            for (uint32_t i = blockIdx.x * Y::drain + warp - 4u; i < none; i += gridDim.x * Y::drain)
+                for (uint32_t n = lane; n < p.outputs; n += 32u) put(p, i < first ? i : p.rows - none + i, n, 0.0f);
+        }
+        pdl_wait();          // no block ends before the kernel that quantises
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (bad_s) {          // copies still in flight land in this block's shared memory before it is given back
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20000000ll) __nanosleep(1000);
+    }
+    if (warp == Y::mma) tc_dealloc(tmem, Y::cols);
 }
 
 // ---- host side ----
@@ -308,25 +522,32 @@ bool map_of(CUtensorMap *m, const void *base, uint32_t columns, uint64_t rows, u
     return e && e(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// scales that a load may bring: whole in every row
+uint32_t unit_of(const void *base, uint64_t stride, uint64_t expert, uint32_t groups) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(base) | stride | expert | groups;
+    return at % 8u == 0 ? 8u : at % 4u == 0 ? 4u : 1u;
+}
+constexpr uint32_t kSms = 148;
 
+// ks 0: the kernel for many tiles
 template <int TN>
-cudaError_t launch_tiles(TcArgs &t, uint32_t pairs, cudaStream_t stream) {
-    static std::atomic<uint64_t> asked{0};          // devices (of the first 64) whose shared-memory limit has been raised
+cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
+    static std::atomic<uint64_t> asked[2];          // devices (of the first 64) whose shared-memory limit has been raised
+    const bool many = t.ks == 0;
+    void (*const kernel)(TcArgs) = many ? k_mx4_many<TN> : TN <= 128 ? k_mx4_few<TN <= 128 ? TN : 128> : nullptr;
+    const uint32_t smem = many ? Many<TN>::smem : Few<TN <= 128 ? TN : 128>::smem;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && (dev > 63 || !(asked.load(std::memory_order_acquire) >> dev & 1u))) {
-        e = smem_at_least(reinterpret_cast<const void *>(k_mx4_tiles<TN>), (int)Tile<TN>::smem);
-        if (e == cudaSuccess && dev <= 63) asked.fetch_or(1ull << dev, std::memory_order_release);
+    if (e == cudaSuccess && (dev > 63 || !(asked[many].load(std::memory_order_acquire) >> dev & 1u))) {
+        e = smem_at_least(reinterpret_cast<const void *>(kernel), (int)smem);
+        if (e == cudaSuccess && dev <= 63) asked[many].fetch_or(1ull << dev, std::memory_order_release);
     }
     if (e != cudaSuccess) return e;
     if (!map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, TN) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
         return cudaErrorInvalidValue;
-    t.pairs = pairs;
-    const uint64_t tiles = (uint64_t)t.wtiles * pairs;
-    t.ks = 1;
-    while (t.ks < 8u && tiles * t.ks < 148u && t.steps >= 2u * t.ks) t.ks *= 2u;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((uint32_t)(t.wtiles * (pairs + (t.p.offsets ? 1u : 0u))), 1, t.ks); cfg.blockDim = dim3(192); cfg.dynamicSmemBytes = Tile<TN>::smem; cfg.stream = stream;
+    cfg.blockDim = dim3(many ? Many<TN>::threads : 192u); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = many ? dim3((uint32_t)std::min<uint64_t>(kSms, (uint64_t)t.wtiles * t.pairs)) : dim3(t.wtiles * (t.pairs + (t.p.offsets ? 1u : 0u)), 1, t.ks);
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
     if (t.made) {
@@ -337,11 +558,7 @@ cudaError_t launch_tiles(TcArgs &t, uint32_t pairs, cudaStream_t stream) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
         attr[cfg.numAttrs].val.clusterDim.x = 1; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs++].val.clusterDim.z = t.ks;
     }
-    return cudaLaunchKernelEx(&cfg, k_mx4_tiles<TN>, t);
-}
-uint32_t align_of(const void *base, uint64_t stride, uint64_t expert) {
-    const uint64_t at = reinterpret_cast<uintptr_t>(base) | stride | expert;
-    return at % 8u == 0 ? 8u : at % 4u == 0 ? 4u : 1u;
+    return cudaLaunchKernelEx(&cfg, kernel, t);
 }
 
 }  // namespace
@@ -349,13 +566,24 @@ uint32_t align_of(const void *base, uint64_t stride, uint64_t expert) {
 cudaError_t mx4_tc_launch(const Mx4Product &a, bool made, cudaStream_t stream) {
     TcArgs t{};
     t.p = a; t.groups = mx4_groups(a.columns); t.steps = (t.groups + kStageGroups - 1u) / kStageGroups; t.wtiles = (a.outputs + kRows - 1u) / kRows; t.made = made;
-    t.w_align = align_of(a.ws, a.ws_stride, a.ws_expert); t.x_align = align_of(a.xs, a.xs_stride, 0);
+    t.w_unit = unit_of(a.ws, a.ws_stride, a.ws_expert, t.groups); t.x_unit = unit_of(a.xs, a.xs_stride, 0, t.groups);
     const uint32_t each = a.offsets ? (a.rows + a.experts - 1u) / a.experts : a.rows;          // rows to a matrix, on average
     auto pairs = [&](uint32_t tn) { return a.offsets ? std::min(a.rows, a.rows / tn + std::min(a.rows, a.experts)) : (a.rows + tn - 1u) / tn; };
-    if (each <= 16u) return launch_tiles<16>(t, pairs(16), stream);
-    if (each <= 32u) return launch_tiles<32>(t, pairs(32), stream);
-    if (each <= 64u) return launch_tiles<64>(t, pairs(64), stream);
-    return launch_tiles<128>(t, pairs(128), stream);
+    uint32_t tn = each <= 16u ? 16u : each <= 32u ? 32u : each <= 64u ? 64u : each <= 128u ? 128u : 256u;
+    if (tn == 256 && (uint64_t)t.wtiles * pairs(256) < kSms) tn = 128;
+    t.pairs = pairs(tn);
+    const uint64_t tiles = (uint64_t)t.wtiles * t.pairs;
+    if (tiles < 2u * kSms && tn < 256u) {
+        t.ks = 1;
+        while (t.ks < 8u && tiles * t.ks < kSms && t.steps >= 2u * t.ks) t.ks *= 2u;
+    }
+    switch (tn) {
+        case 16: return launch_of<16>(t, stream);
+        case 32: return launch_of<32>(t, stream);
+        case 64: return launch_of<64>(t, stream);
+        case 128: return launch_of<128>(t, stream);
+        default: return launch_of<256>(t, stream);
+    }
 }
 
 }  // namespace nb
