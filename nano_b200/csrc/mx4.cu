@@ -82,9 +82,13 @@ __device__ __forceinline__ float scale_of(uint32_t e) { return e == 255u ? __uin
 // power of two is exact, so the one rounding is the conversion's.  Bound by memory: a number is read and 17/32 bytes are written, in whole words.
 // ------------------------------------------------------------------------------------------------
 constexpr uint32_t kThreads = 256;
+__device__ __forceinline__ uint8_t *scale_at(const Mx4Rows &a, uint32_t row, uint32_t g) { return a.scales + (uint64_t)row * a.scale_stride + (g >> 4) * a.scale_step + (g & 15u); }
+// in the second order the last sixteen are filled up with zeros
+__device__ __forceinline__ void fill_scales(const Mx4Rows &a, uint32_t row, uint32_t g, uint32_t groups) {
+    if (a.scale_step != 16u && g + 1u == groups) for (uint32_t i = groups; i & 15u; i++) *scale_at(a, row, i) = 0;
+}
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, const uint32_t per_row, const uint32_t items) {
-    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+__device__ __forceinline__ void quantise(const Mx4Rows &a, uint32_t per_row, uint32_t items, uint32_t i) {          // by all threads of a warp
     const bool live = i < items;
     const uint32_t row = live ? i / per_row : 0u, q = live ? i % per_row : 0u, k = q * 8u;
     float x[8] = {};
@@ -104,8 +108,10 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, cons
     for (int j = 0; j < 4; j++) w |= codes_of(x[2 * j] * by, x[2 * j + 1] * by) << (8 * j);
     if (!live) return;
     *reinterpret_cast<uint32_t *>(a.codes + (uint64_t)row * a.code_stride + q * 4u) = e == 255u ? 0u : w;
-    if ((q & 3u) == 0) a.scales[(uint64_t)row * a.scale_stride + (q >> 2)] = (uint8_t)e;
+    if ((q & 3u) == 0) { *scale_at(a, row, q >> 2) = (uint8_t)e; fill_scales(a, row, q >> 2, per_row / 4u); }
 }
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, const uint32_t per_row, const uint32_t items) { quantise<T>(a, per_row, items, blockIdx.x * kThreads + threadIdx.x); }
 
 // And back, V neighbours to a thread: as many as stores of whole vectors allow for every row
 template <typename T, int V>
@@ -141,7 +147,7 @@ cudaError_t by_rows(const Mx4Rows &a, uint32_t per_row, F f) {
         Mx4Rows b = a;
         b.rows = n;
         b.codes += (uint64_t)r0 * a.code_stride; b.scales += (uint64_t)r0 * a.scale_stride;
-        if (a.type != T_MX4) b.x = static_cast<char *>(a.x) + (uint64_t)r0 * a.x_stride * elem_size(a.type);
+        b.x = static_cast<char *>(a.x) + (uint64_t)r0 * a.x_stride * elem_size(a.type);
         f(b, n * per_row, (n * per_row + kThreads - 1u) / kThreads);
         return cudaGetLastError();
     });
@@ -159,17 +165,50 @@ cudaError_t read_launch_t(const Mx4Rows &a, cudaStream_t stream) {
     return go(k_mx4_read<T, 1>, 1);
 }
 
-// Rows of codes as a product wants them where a row ends inside a byte: what fills up the last group is zeros.  A group to a thread.
-__global__ void __launch_bounds__(kThreads) k_mx4_clean(const Mx4Rows a, const uint8_t *codes, const uint64_t code_stride, const uint8_t *scales, const uint64_t scale_stride, const uint32_t per_row,
-                                                        const uint32_t items) {
-    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+// ------------------------------------------------------------------------------------------------
+// What a product wants made before it, in one launch: its rows quantised (or, where codes end inside a byte, what fills up their last group set to zeros), and scales in the second order: blocks
+// [0, first) work on x, the others on the scales of w.
+// ------------------------------------------------------------------------------------------------
+struct Scales { const uint8_t *from; uint64_t stride, expert; uint8_t *to; uint32_t rows, groups, chunks, unit; };          // of `rows` rows of each expert
+__device__ __forceinline__ void second_order(const Scales &a, uint64_t i, uint64_t items) {          // sixteen scales of a row to a thread
     if (i >= items) return;
-    const uint32_t row = i / per_row, g = i % per_row, live = min(kMx4Group, a.columns - g * kMx4Group);
-    uint4 v = __ldg(reinterpret_cast<const uint4 *>(codes + (uint64_t)row * code_stride) + g);
-    auto keep = [&](uint32_t w, uint32_t from) { return live >= from + 8u ? w : live <= from ? 0u : w & ((1u << (4u * (live - from))) - 1u); };
+    const uint32_t row = (uint32_t)(i % a.rows), chunk = (uint32_t)(i / a.rows % a.chunks);
+    const uint8_t *from = a.from + i / a.rows / a.chunks * a.expert + (uint64_t)row * a.stride + chunk * 16u;
+    const uint32_t in = min(16u, a.groups - chunk * 16u);
+    uint32_t w[4] = {};
+    if (a.unit == 16u) { const uint4 v = __ldg(reinterpret_cast<const uint4 *>(from)); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    else if (a.unit >= 4u)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) w[j] = j * 4u < in ? __ldg(reinterpret_cast<const uint32_t *>(from) + j) : 0u;
+    else
+#pragma unroll
+        for (uint32_t j = 0; j < 16; j++) w[j / 4] |= (j < in ? (uint32_t)__ldg(from + j) : 0u) << (8u * (j % 4u));
+    reinterpret_cast<uint4 *>(a.to)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+struct Codes { const uint8_t *codes, *scales; uint64_t code_stride, scale_stride; };
+// a group to a thread
+__device__ __forceinline__ void clean(const Mx4Rows &a, const Codes &from, uint32_t groups, uint32_t items, uint32_t i) {
+    if (i >= items) return;
+    const uint32_t row = i / groups, g = i % groups, live = min(kMx4Group, a.columns - g * kMx4Group);
+    uint4 v = __ldg(reinterpret_cast<const uint4 *>(from.codes + (uint64_t)row * from.code_stride) + g);
+    auto keep = [&](uint32_t w, uint32_t at) { return live >= at + 8u ? w : live <= at ? 0u : w & ((1u << (4u * (live - at))) - 1u); };
     v = make_uint4(keep(v.x, 0), keep(v.y, 8), keep(v.z, 16), keep(v.w, 24));
     reinterpret_cast<uint4 *>(a.codes + (uint64_t)row * a.code_stride)[g] = v;
-    a.scales[(uint64_t)row * a.scale_stride + g] = scales[(uint64_t)row * scale_stride + g];
+    *scale_at(a, row, g) = from.scales[(uint64_t)row * from.scale_stride + g];
+    fill_scales(a, row, g, groups);
+}
+struct Prepare { Mx4Rows rows; Codes codes; Scales xs, ws; uint64_t x_items, w_items; uint32_t per_row, first; };
+enum { kOfF32, kOfBf16, kOfF16, kOfCodes, kOfScales };          // what x is: numbers, codes to be cleaned, codes whose scales are put in order
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) k_mx4_prepare(const __grid_constant__ Prepare a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // the product sets itself up and brings its first weights meanwhile
+    if (blockIdx.x >= a.first) { second_order(a.ws, (uint64_t)(blockIdx.x - a.first) * kThreads + threadIdx.x, a.w_items); return; }
+    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+    if constexpr (KIND == kOfF32) quantise<float>(a.rows, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
+    else if constexpr (KIND == kOfBf16) quantise<__nv_bfloat16>(a.rows, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
+    else if constexpr (KIND == kOfF16) quantise<__half>(a.rows, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
+    else if constexpr (KIND == kOfCodes) clean(a.rows, a.codes, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
+    else second_order(a.xs, i, a.x_items);
 }
 
 }  // namespace
@@ -185,12 +224,38 @@ cudaError_t mx4_quantize_launch(const Mx4Rows &a, cudaStream_t stream) {
 cudaError_t mx4_read_launch(const Mx4Rows &a, cudaStream_t stream) {
     return a.type == T_F32 ? read_launch_t<float>(a, stream) : a.type == T_BF16 ? read_launch_t<__nv_bfloat16>(a, stream) : read_launch_t<__half>(a, stream);
 }
-cudaError_t mx4_clean_launch(const Mx4Rows &a, const uint8_t *codes, uint64_t code_stride, const uint8_t *scales, uint64_t scale_stride, cudaStream_t stream) {
-    const uint32_t per_row = mx4_groups(a.columns);
-    uint32_t r0 = 0;
-    return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
-        k_mx4_clean<<<blocks, kThreads, 0, stream>>>(b, codes + r0 * code_stride, code_stride, scales + r0 * scale_stride, scale_stride, per_row, items);
-        r0 += b.rows;
+cudaError_t mx4_prepare_launch(const Mx4Product &p, const Mx4Plan &plan, uint8_t *workspace, cudaStream_t stream) {
+    const uint32_t groups = mx4_groups(p.columns), chunks = (groups + 15u) / 16u;
+    uint8_t *xs = workspace + plan.x_scales_at;
+    auto unit = [&](const uint8_t *at, uint64_t stride, uint64_t expert) { const uint64_t all = reinterpret_cast<uintptr_t>(at) | stride | expert | groups; return all % 16u == 0 ? 16u : all % 4u == 0 ? 4u : 1u; };
+    Prepare a{};
+    a.ws = Scales{p.ws, p.ws_stride, p.ws_expert, workspace + plan.w_scales_at, p.outputs, groups, chunks, unit(p.ws, p.ws_stride, p.ws_expert)};
+    a.w_items = plan.w_scales ? (uint64_t)std::max(1u, p.experts) * p.outputs * chunks : 0;
+    a.rows = Mx4Rows{workspace, xs, groups * 16ull, plan.x_second ? 16ull : groups, plan.x_second ? p.rows * 16ull : 16ull, const_cast<void *>(p.x), p.x_stride, p.x_type, p.rows, p.columns};
+    a.codes = Codes{static_cast<const uint8_t *>(p.x), p.xs, p.x_stride, p.xs_stride};
+    a.xs = Scales{p.xs, p.xs_stride, 0, xs, p.rows, groups, chunks, p.x_type == T_MX4 ? unit(p.xs, p.xs_stride, 0) : 1u};
+    const uint32_t kind = p.x_type != T_MX4 ? p.x_type : plan.x_codes ? (uint32_t)kOfCodes : (uint32_t)kOfScales;
+    a.per_row = kind < kOfCodes ? groups * 4u : kind == kOfCodes ? groups : chunks;
+    // x in portions whose items are counted in 31 bits, w's scales with the first
+    return in_portions(plan.x_codes || plan.x_scales ? p.rows : 1u, std::max(1u, 0x7fffff00u / a.per_row), [&](uint32_t r0, uint32_t n) {
+        Prepare b = a;
+        if (plan.x_codes || plan.x_scales) b.x_items = kind == kOfScales ? (uint64_t)p.rows * chunks : (uint64_t)n * a.per_row;
+        if (kind == kOfScales && r0) return cudaSuccess;          // (all rows at once: counted in 64 bits)
+        if (r0) b.w_items = 0;
+        b.rows.rows = n;
+        b.rows.codes += r0 * a.rows.code_stride; b.rows.scales += r0 * a.rows.scale_stride;
+        if (kind < kOfCodes) b.rows.x = static_cast<char *>(a.rows.x) + r0 * p.x_stride * elem_size(p.x_type);
+        else { b.codes.codes += r0 * p.x_stride; if (p.xs) b.codes.scales += r0 * p.xs_stride; }
+        b.first = (uint32_t)((b.x_items + kThreads - 1u) / kThreads);
+        const uint32_t blocks = b.first + (uint32_t)((b.w_items + kThreads - 1u) / kThreads);
+        switch (kind) {
+            case kOfF32: k_mx4_prepare<kOfF32><<<blocks, kThreads, 0, stream>>>(b); break;
+            case kOfBf16: k_mx4_prepare<kOfBf16><<<blocks, kThreads, 0, stream>>>(b); break;
+            case kOfF16: k_mx4_prepare<kOfF16><<<blocks, kThreads, 0, stream>>>(b); break;
+            case kOfCodes: k_mx4_prepare<kOfCodes><<<blocks, kThreads, 0, stream>>>(b); break;
+            default: k_mx4_prepare<kOfScales><<<blocks, kThreads, 0, stream>>>(b);
+        }
+        return cudaGetLastError();
     });
 }
 
@@ -210,18 +275,17 @@ int rows_checked(const nb200_mx4_rows *p, nb::Mx4Rows *a) {
     if (reinterpret_cast<uintptr_t>(p->codes) % 16u || p->code_stride % 16u) return fail(NB200_EINVAL, "codes start and go on in multiples of 16 bytes");
     if (reinterpret_cast<uintptr_t>(p->x) % nb::elem_size(p->type)) return fail(NB200_EINVAL, "numbers are not aligned to their type");
     if (p->rows > 1 && (p->code_stride < groups * 16u || p->scale_stride < groups)) return fail(NB200_EINVAL, "rows of codes or scales overlap");
-    *a = nb::Mx4Rows{static_cast<uint8_t *>(p->codes), static_cast<uint8_t *>(p->scales), p->code_stride, p->scale_stride, p->x, p->x_stride, p->type, p->rows, p->columns};
+    *a = nb::Mx4Rows{static_cast<uint8_t *>(p->codes), static_cast<uint8_t *>(p->scales), p->code_stride, p->scale_stride, 16, p->x, p->x_stride, p->type, p->rows, p->columns};
     return 0;
 }
 
-// checks the call; *work: bytes of x as it is quantised
-int product_checked(const nb200_mx4_product *p, uint64_t *work) {
-    if (!p || !work) return fail(NB200_EINVAL, "null argument");
+int product_checked(const nb200_mx4_product *p, nb::Mx4Product *a) {
+    if (!p) return fail(NB200_EINVAL, "null argument");
     if (p->x_type > NB200_T_MX4) return fail(NB200_EINVAL, "rows are fp32, bf16, fp16 or in microscaled 4-bit floating point (type %u)", p->x_type);
     if (p->out_type > nb::T_F16) return fail(NB200_EINVAL, "results are fp32, bf16 or fp16 (type %u)", p->out_type);
     if (p->rows > 1u << 30 || p->outputs > 1u << 30 || p->columns > 1u << 30) return fail(NB200_EINVAL, "a product of %u x %u x %u is too large", p->rows, p->outputs, p->columns);
     if (p->experts > 1024u) return fail(NB200_EINVAL, "%u experts: at most 1024", p->experts);
-    *work = 0;
+    *a = nb::Mx4Product{};
     if (!p->rows || !p->outputs) return 0;
     if (!p->columns) return fail(NB200_EINVAL, "rows of no numbers");
     const bool codes = p->x_type == NB200_T_MX4;
@@ -235,7 +299,8 @@ int product_checked(const nb200_mx4_product *p, uint64_t *work) {
     if (reinterpret_cast<uintptr_t>(p->out) % nb::elem_size(p->out_type)) return fail(NB200_EINVAL, "results are not aligned to their type");
     if (p->rows > 1 && p->out_stride < p->outputs) return fail(NB200_EINVAL, "rows of results overlap");
     if (p->experts && reinterpret_cast<uintptr_t>(p->offsets) % 4u) return fail(NB200_EINVAL, "offsets are not aligned to their type");
-    if (!codes || p->columns % 2u) *work = p->rows * (row + groups);
+    *a = nb::Mx4Product{p->x, static_cast<const uint8_t *>(p->x_scales), static_cast<const uint8_t *>(p->w), static_cast<const uint8_t *>(p->w_scales), p->x_stride, p->xs_stride, p->w_stride,
+                        p->ws_stride, p->w_expert, p->ws_expert, p->out, p->out_stride, p->experts ? p->offsets : nullptr, p->x_type, p->out_type, p->rows, p->outputs, p->columns, p->experts};
     return 0;
 }
 }  // namespace
@@ -261,27 +326,32 @@ int nb200_dev_mx4_read(const nb200_mx4_rows *rows, void *stream) {
     return 0;
 }
 
-int nb200_dev_mx4_product_workspace(const nb200_mx4_product *p, uint64_t *bytes) { return product_checked(p, bytes); }
+int nb200_dev_mx4_product_workspace(const nb200_mx4_product *p, uint64_t *bytes) {
+    nb::Mx4Product a{};
+    if (!bytes) return fail(NB200_EINVAL, "null argument");
+    if (const int r = product_checked(p, &a)) return r;
+    *bytes = a.rows ? nb::mx4_plan(a).bytes : 0;
+    return 0;
+}
 
 int nb200_dev_mx4_product(const nb200_mx4_product *p, void *workspace, uint64_t workspace_bytes, void *stream) {
-    uint64_t need = 0;
-    if (const int r = product_checked(p, &need)) return r;
-    if (!p->rows || !p->outputs) return 0;
-    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16u))
-        return fail(NB200_EINVAL, "the workspace has %llu bytes, 16-byte aligned: %llu are needed", (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);
+    nb::Mx4Product a{};
+    if (const int r = product_checked(p, &a)) return r;
+    if (!a.rows) return 0;
+    const nb::Mx4Plan plan = nb::mx4_plan(a);
+    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || reinterpret_cast<uintptr_t>(workspace) % 16u))
+        return fail(NB200_EINVAL, "the workspace has %llu bytes, 16-byte aligned: %llu are needed", (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)plan.bytes);
     if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    nb::Mx4Product a{static_cast<const uint8_t *>(p->x), static_cast<const uint8_t *>(p->x_scales), static_cast<const uint8_t *>(p->w), static_cast<const uint8_t *>(p->w_scales),
-                     p->x_stride, p->xs_stride, p->w_stride, p->ws_stride, p->w_expert, p->ws_expert, p->out, p->out_stride, p->experts ? p->offsets : nullptr,
-                     p->out_type, p->rows, p->outputs, p->columns, p->experts};
-    if (need) {
-        const uint64_t groups = nb::mx4_groups(p->columns);
-        uint8_t *codes = static_cast<uint8_t *>(workspace), *scales = codes + p->rows * groups * 16u;
-        const nb::Mx4Rows rows{codes, scales, groups * 16u, groups, const_cast<void *>(p->x), p->x_stride, p->x_type, p->rows, p->columns};
-        NB_CK(p->x_type == NB200_T_MX4 ? nb::mx4_clean_launch(rows, a.x, a.x_stride, a.xs, a.xs_stride, s) : nb::mx4_quantize_launch(rows, s));
-        a.x = codes; a.xs = scales; a.x_stride = groups * 16u; a.xs_stride = groups;
+    uint8_t *made = static_cast<uint8_t *>(workspace);
+    uint64_t xs_step = 16, ws_step = 16;
+    if (plan.bytes) {
+        NB_CK(nb::mx4_prepare_launch(a, plan, made, s));
+        if (plan.x_codes) { a.x = made; a.x_stride = nb::mx4_groups(a.columns) * 16ull; }
+        if (plan.x_scales) { a.xs = made + plan.x_scales_at; a.xs_stride = plan.x_second ? 16 : nb::mx4_groups(a.columns); xs_step = plan.x_second ? a.rows * 16ull : 16; }
+        if (plan.w_scales) { a.ws = made + plan.w_scales_at; a.ws_stride = 16; ws_step = a.outputs * 16ull; a.ws_expert = ws_step * ((nb::mx4_groups(a.columns) + 15u) / 16u); }
     }
-    NB_CK(nb::mx4_tc_launch(a, need != 0, s));
+    NB_CK(nb::mx4_tc_launch(a, plan, xs_step, ws_step, plan.bytes != 0, s));
     return 0;
 }
 

@@ -13,19 +13,27 @@ namespace nb {
 constexpr uint32_t T_MX4 = 3, kMx4Group = 32;
 inline uint32_t mx4_groups(uint32_t columns) { return columns / kMx4Group + (columns % kMx4Group != 0); }
 
-struct Mx4Rows { uint8_t *codes, *scales; uint64_t code_stride, scale_stride; void *x; uint64_t x_stride; uint32_t type, rows, columns; };
+// Scales lie row after row (stride bytes apart, sixteen every 16 bytes), or sixteen of every row after the other (16 bytes from row to row, `step` to the next sixteen), which neighbouring threads
+// read as neighbours: scale g of row r is byte r stride + (g / 16) step + g % 16
+struct Mx4Rows { uint8_t *codes, *scales; uint64_t code_stride, scale_stride, scale_step; void *x; uint64_t x_stride; uint32_t type, rows, columns; };
 cudaError_t mx4_quantize_launch(const Mx4Rows &a, cudaStream_t stream);
-// codes and scales of type T_MX4 with zeros where a row's last group is filled up, to a.codes and a.scales
-cudaError_t mx4_clean_launch(const Mx4Rows &a, const uint8_t *codes, uint64_t code_stride, const uint8_t *scales, uint64_t scale_stride, cudaStream_t stream);
 cudaError_t mx4_read_launch(const Mx4Rows &a, cudaStream_t stream);
 
-// x and w are codes here
-struct Mx4Product {
-    const uint8_t *x, *xs, *w, *ws; uint64_t x_stride, xs_stride, w_stride, ws_stride, w_expert, ws_expert;
-    void *out; uint64_t out_stride; const int32_t *offsets;          // null: one matrix for all rows
-    uint32_t out_type, rows, outputs, columns, experts;
+// How a product is run: by sizes, types and alignment alone
+struct Mx4Plan {
+    uint32_t tn, ks, per, pairs;          // rows of X in a tile; blocks that share a tile's depth (0: the kernel for many tiles); steps to each; tiles of rows, over all experts at most
+    bool x_codes, x_scales, w_scales, x_second;          // what a kernel makes before: codes of x, its scales (in the second order?) and those of w in the second order
+    uint64_t x_scales_at, w_scales_at, bytes;          // in the workspace; codes come first
 };
-// made: the kernel queued before this one made x and xs, and nothing else that this one reads
-cudaError_t mx4_tc_launch(const Mx4Product &a, bool made, cudaStream_t stream);
+struct Mx4Product {
+    const void *x; const uint8_t *xs, *w, *ws; uint64_t x_stride, xs_stride, w_stride, ws_stride, w_expert, ws_expert;
+    void *out; uint64_t out_stride; const int32_t *offsets;          // null: one matrix for all rows
+    uint32_t x_type, out_type, rows, outputs, columns, experts;
+};
+Mx4Plan mx4_plan(const Mx4Product &p);
+// the kernel before: to the workspace, what the plan names
+cudaError_t mx4_prepare_launch(const Mx4Product &p, const Mx4Plan &plan, uint8_t *workspace, cudaStream_t stream);
+// the product, of codes; steps: bytes from sixteen scales to the next.  made: the kernel queued before this one made x, its scales and w's, and nothing else that this one reads
+cudaError_t mx4_tc_launch(const Mx4Product &p, const Mx4Plan &plan, uint64_t xs_step, uint64_t ws_step, bool made, cudaStream_t stream);
 
 }  // namespace nb

@@ -22,11 +22,11 @@ template <int TN> struct Tile {
     static constexpr uint32_t blocks = (TN + 127) / 128;          // of 128 rows, as tensor memory holds scales: row r's word in lane r % 32, column r / 32
     static constexpr uint32_t x_at = kRows * 128u, bytes = x_at + TN * 128u;          // of a stage
     static constexpr uint32_t scale_cols = 8u + 8u * blocks, sum_cols = TN < 32 ? 32 : TN;          // of tensor memory
-    static constexpr uint32_t staged = (kRows + 128u * blocks) * 8u;          // a stage's scales, eight to a row, on their way
+    static constexpr uint32_t staged = (kRows + 128u * blocks) * 16u;          // two stages' scales, sixteen to a row, on their way
 };
 __host__ __device__ constexpr uint32_t cols_for(uint32_t used) { return used <= 128u ? 128u : used <= 256u ? 256u : 512u; }
 
-struct alignas(64) TcArgs { CUtensorMap wmap, xmap; Mx4Product p; uint32_t groups, steps, ks, wtiles, pairs, w_unit, x_unit, made; };
+struct alignas(64) TcArgs { CUtensorMap wmap, xmap; Mx4Product p; uint64_t w_step, x_step; uint32_t groups, steps, ks, per, wtiles, pairs, w_unit, x_unit, made; };
 
 __device__ __forceinline__ bool soon(uint32_t bar, uint32_t parity) { return mbar_try(bar, parity) || mbar_wait(bar, parity); }
 __device__ __forceinline__ bool soon_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, soon(bar, parity)); }
@@ -40,91 +40,116 @@ __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint
 // e2m1 x e2m1, scales in 8 bits of exponent, N columns; scales from byte `id` (0 or 2) of their words
 __host__ __device__ constexpr uint32_t idesc_of(uint32_t n, uint32_t id) { return (id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((kRows >> 4) << 24) | (id << 29); }
 
-// Eight neighbouring scales of a row, from group g on; zeros behind its last.  UNIT: bytes that one load may bring, for every row and every g that is a multiple of it
+// Sixteen neighbouring scales of a row, from group g (a multiple of 16, or of 8 for UNIT 8) on; zeros behind its last.  UNIT: bytes that one load may bring, for every row and every g
 template <int UNIT>
-__device__ __forceinline__ uint2 scales8(const uint8_t *row, uint32_t g, uint32_t groups) {
-    if constexpr (UNIT == 8) return __ldg(reinterpret_cast<const uint2 *>(row + g));
-    uint2 v = make_uint2(0u, 0u);
-    if constexpr (UNIT == 4) {
-        if (g < groups) v.x = __ldg(reinterpret_cast<const uint32_t *>(row + g));
-        if (g + 4u < groups) v.y = __ldg(reinterpret_cast<const uint32_t *>(row + g + 4u));
-    } else
+__device__ __forceinline__ uint4 scales16(const uint8_t *at, uint32_t g, uint32_t groups) {
+    if constexpr (UNIT == 16) return __ldg(reinterpret_cast<const uint4 *>(at));
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (UNIT == 8) {
+        uint2 lo = make_uint2(0u, 0u), hi = lo;
+        if (g < groups) lo = __ldg(reinterpret_cast<const uint2 *>(at));
+        if (g + 8u < groups) hi = __ldg(reinterpret_cast<const uint2 *>(at) + 1);
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else if constexpr (UNIT == 4) {
+        if (g < groups) v.x = __ldg(reinterpret_cast<const uint32_t *>(at));
+        if (g + 4u < groups) v.y = __ldg(reinterpret_cast<const uint32_t *>(at) + 1);
+        if (g + 8u < groups) v.z = __ldg(reinterpret_cast<const uint32_t *>(at) + 2);
+        if (g + 12u < groups) v.w = __ldg(reinterpret_cast<const uint32_t *>(at) + 3);
+    } else {
+        uint32_t w[4] = {};
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            const uint32_t b = g + i < groups ? (uint32_t)__ldg(row + g + i) : 0u;
-            if (i < 4) v.x |= b << (8u * i); else v.y |= b << (8u * (i - 4u));
-        }
+        for (uint32_t i = 0; i < 16; i++) w[i / 4] |= (g + i < groups ? (uint32_t)__ldg(at + i) : 0u) << (8u * (i % 4u));
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
     return v;
 }
 
 // Four warps bring the scales of tile after tile to tensor memory: a thread loads those of one row of W and of one or two of X, eight at a time and kAhead stages ahead, the four exchange them
 // through shared memory, and each writes all of them to its quarter of the lanes.  (tcgen05.cp, which replicates by itself, takes its turn with the products, some 55 cycles for each 128 x 4
 // scales, a quarter of a stage of 128 x 256: 8192 x 8192 x 8192 took 266 us with it.)
-constexpr uint32_t kAhead = 4, kScaleThreads = 128, kScaleBar = 1;
+constexpr uint32_t kAhead = 2, kScaleThreads = 128, kScaleBar = 1;
 __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 struct ScaleRows { const uint8_t *base; uint64_t stride; uint32_t live; };          // rows [0, live); what lies behind them counts for nothing
-struct ScaleRing { uint32_t staged, tmem, stages, full, empty, groups, w_unit, x_unit; };
+struct ScaleRing { uint32_t staged, tmem, stages, full, empty, groups; uint64_t w_step, x_step; uint32_t w_unit, x_unit; };
 template <int TN, int WU, int XU, typename F>
-__device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t total, uint32_t s0, uint32_t ns, F &next) {
+__device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles, uint32_t s0, uint32_t ns, F &next) {
     using Z = Tile<TN>;
     constexpr uint32_t XR = Z::blocks;          // rows of X to a thread
-    const uint32_t tid = threadIdx.x & (kScaleThreads - 1u), warp = tid >> 5, lane = tid & 31u;
+    const uint32_t tid = threadIdx.x & (kScaleThreads - 1u), warp = tid >> 5, lane = tid & 31u, pairs = (ns + 1u) / 2u, total = tiles * pairs;          // two stages at a time
     const uint8_t *w_row = nullptr, *x_row[XR] = {};
-    uint2 v[kAhead][1 + XR];
-    uint32_t asked = 0, step = ns;
-    auto ask = [&](uint2 (&to)[1 + XR]) {
+    uint4 v[kAhead][1 + XR];
+    uint32_t asked = 0, pair = pairs;
+    auto ask = [&](uint4 (&to)[1 + XR]) {
         if (asked == total) return;
-        if (step == ns) {
+        if (pair == pairs) {
             ScaleRows w, x;
             next(w, x);
-            w_row = w.base + (tid < w.live ? tid : 0u) * w.stride;
+            w_row = w.base + (tid < w.live ? tid : 0u) * w.stride + (s0 >> 1) * r.w_step + (s0 & 1u) * 8u;
 #pragma unroll
-            for (uint32_t i = 0; i < XR; i++) { const uint32_t q = tid + i * kScaleThreads; x_row[i] = x.base + (q < x.live ? q : 0u) * x.stride; }
-            step = 0;
+            for (uint32_t i = 0; i < XR; i++) { const uint32_t q = tid + i * kScaleThreads; x_row[i] = x.base + (q < x.live ? q : 0u) * x.stride + (s0 >> 1) * r.x_step + (s0 & 1u) * 8u; }
+            pair = 0;
         }
-        to[0] = scales8<WU>(w_row, (s0 + step) * kStageGroups, r.groups);
+        const uint32_t g = (s0 + 2u * pair) * kStageGroups;
+        to[0] = scales16<WU>(w_row, g, r.groups);
+        w_row += r.w_step;
 #pragma unroll
-        for (uint32_t i = 0; i < XR; i++) to[1 + i] = scales8<XU>(x_row[i], (s0 + step) * kStageGroups, r.groups);
-        step++; asked++;
+        for (uint32_t i = 0; i < XR; i++) { to[1 + i] = scales16<XU>(x_row[i], g, r.groups); x_row[i] += r.x_step; }
+        pair++; asked++;
     };
 #pragma unroll
     for (uint32_t d = 0; d < kAhead; d++) ask(v[d]);
-    uint32_t st = 0, turn = 0;
+    uint32_t st = 0, turn = 0, done = 0;
+    bool ok = true;
     for (uint32_t i = 0; i < total; i += kAhead)
 #pragma unroll
         for (uint32_t d = 0; d < kAhead; d++) {
-            if (i + d >= total) return true;
-            const uint32_t at = r.staged + (d & 1u) * Z::staged;          // (two stages in turn: kAhead is even)
+            if (i + d >= total) return ok;
+            const uint32_t at = r.staged + (d & 1u) * Z::staged, count = min(2u, ns - done);          // (two buffers in turn: kAhead is even)
 #pragma unroll
-            for (uint32_t j = 0; j < 1 + XR; j++) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + (j * kScaleThreads + tid) * 8u), "r"(v[d][j].x), "r"(v[d][j].y) : "memory");
-            const bool ok = !turn || soon_warp(r.empty + st * 8u, (turn - 1u) & 1u);
+            for (uint32_t j = 0; j < 1 + XR; j++) {          // the two stages' apart: neighbours, for the loads
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + (j * kScaleThreads + tid) * 8u), "r"(v[d][j].x), "r"(v[d][j].y) : "memory");
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + Z::staged / 2u + (j * kScaleThreads + tid) * 8u), "r"(v[d][j].z), "r"(v[d][j].w) : "memory");
+            }
+            ok = ok && (!turn || soon_warp(r.empty + st * 8u, (turn - 1u) & 1u));
             if (bar_any(kScaleBar, kScaleThreads, !ok)) return false;          // one verdict for the four warps, which meet here
-            tc_fence_after();
             ask(v[d]);
-            uint32_t w[8], x[8 * XR];          // [half of the stage][row / 32]
+            for (uint32_t h = 0; h < count; h++) {
+                if (h && turn) {          // (the others learn of a wait that runs out where they meet again)
+                    ok = soon_warp(r.empty + st * 8u, (turn - 1u) & 1u);
+                    if (!ok) break;
+                }
+                tc_fence_after();
+                uint32_t w[8], x[8 * XR];          // [half of the stage][row / 32]
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j]), "=r"(w[4 + j]) : "r"(at + (j * 32u + lane) * 8u) : "memory");
+                for (uint32_t j = 0; j < 4; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j]), "=r"(w[4 + j]) : "r"(at + h * (Z::staged / 2u) + (j * 32u + lane) * 8u) : "memory");
 #pragma unroll
-            for (uint32_t j = 0; j < 4 * XR; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[j]), "=r"(x[4 * XR + j]) : "r"(at + (kRows + j * 32u + lane) * 8u) : "memory");
-            const uint32_t to = r.tmem + ((warp * 32u) << 16) + st * Z::scale_cols;
-            tc_st8(to, w);
-            if constexpr (XR == 1) tc_st8(to + 8u, x); else tc_st16(to + 8u, x);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(r.full + st * 8u);
-            if (++st == r.stages) { st = 0; turn++; }
+                for (uint32_t j = 0; j < 4 * XR; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[j]), "=r"(x[4 * XR + j]) : "r"(at + h * (Z::staged / 2u) + (kRows + j * 32u + lane) * 8u) : "memory");
+                const uint32_t to = r.tmem + ((warp * 32u) << 16) + st * Z::scale_cols;
+                tc_st8(to, w);
+                if constexpr (XR == 1) tc_st8(to + 8u, x); else tc_st16(to + 8u, x);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(r.full + st * 8u);
+                if (++st == r.stages) { st = 0; turn++; }
+            }
+            done = done + count == ns ? 0u : done + count;
         }
-    return true;
+    return ok;
 }
-// next(w, x) names the rows of the next tile; `total` stages, ns to a tile, the first of them step s0 of its depth
+// next(w, x) names the rows of the next of `tiles` tiles, of which steps [s0, s0 + ns) of the depth are wanted
 template <int TN, typename F>
-__device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t total, uint32_t s0, uint32_t ns, F next) {
-    if (r.w_unit == 8u && r.x_unit == 8u) return bring_scales<TN, 8, 8>(r, total, s0, ns, next);
-    if (r.w_unit >= 4u && r.x_unit >= 4u) return bring_scales<TN, 4, 4>(r, total, s0, ns, next);
-    return bring_scales<TN, 1, 1>(r, total, s0, ns, next);
+__device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles, uint32_t s0, uint32_t ns, F next) {
+    if (r.x_unit == 16u) {
+        if (r.w_unit == 16u) return bring_scales<TN, 16, 16>(r, tiles, s0, ns, next);
+        if (r.w_unit >= 4u) return bring_scales<TN, 4, 16>(r, tiles, s0, ns, next);
+        return bring_scales<TN, 1, 16>(r, tiles, s0, ns, next);
+    }
+    if (r.w_unit >= 8u && r.x_unit >= 8u) return bring_scales<TN, 8, 8>(r, tiles, s0, ns, next);
+    if (r.w_unit >= 4u && r.x_unit >= 4u) return bring_scales<TN, 4, 4>(r, tiles, s0, ns, next);
+    return bring_scales<TN, 1, 1>(r, tiles, s0, ns, next);
 }
 
 // a stage's products
@@ -198,13 +223,13 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     constexpr uint32_t ST = Few<TN>::stages;
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 1];
-    __shared__ __align__(8) uint8_t staged[2 * Z::staged];
+    __shared__ __align__(16) uint8_t staged[2 * Z::staged];
     __shared__ uint32_t tmem_s, bad_s;
     __shared__ Span span_s;
     const Mx4Product &p = t.p;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, part = blockIdx.z, n0 = blockIdx.x % t.wtiles * kRows, pair = blockIdx.x / t.wtiles;
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u, full = smem_u32(bars), empty = full + ST * 8u, done = full + 2u * ST * 8u;
-    const uint32_t per = (t.steps + t.ks - 1u) / t.ks, s0 = min(t.steps, part * per), ns = min(t.steps, s0 + per) - s0;
+    const uint32_t s0 = min(t.steps, part * t.per), ns = min(t.steps, s0 + t.per) - s0;
     Span span{0u, pair * TN, min(pair * TN + TN, p.rows)};
     if (p.offsets) {
         if (pair == t.pairs) {          // rows of no expert
@@ -264,8 +289,8 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
         }
     } else {
         pdl_wait();
-        const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_unit, t.x_unit};
-        if (!bring_scales<TN>(r, ns, s0, ns, [&](ScaleRows &w, ScaleRows &x) {
+        const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_step, t.x_step, t.w_unit, t.x_unit};
+        if (!bring_scales<TN>(r, 1, s0, ns, [&](ScaleRows &w, ScaleRows &x) {
                 w = ScaleRows{p.ws + span.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
                 x = ScaleRows{p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0};
             })) bad_s = 1;
@@ -335,7 +360,7 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
     constexpr uint32_t ST = Y::stages, SETS = Y::sets;
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 2 * SETS];
-    __shared__ __align__(8) uint8_t staged[2 * Z::staged];
+    __shared__ __align__(16) uint8_t staged[2 * Z::staged];
     __shared__ uint32_t tmem_s, bad_s, pairs_s[kMostExperts + 1];          // of (expert, TN rows): those before an expert's
     const Mx4Product &p = t.p;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -422,8 +447,8 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
     } else if (warp < 4) {
         pdl_wait();
         uint64_t tile = blockIdx.x;
-        const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_unit, t.x_unit};
-        if (!bring_scales<TN>(r, (uint32_t)mine * ns, 0, ns, [&](ScaleRows &w, ScaleRows &x) {
+        const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_step, t.x_step, t.w_unit, t.x_unit};
+        if (!bring_scales<TN>(r, (uint32_t)mine, 0, ns, [&](ScaleRows &w, ScaleRows &x) {
                 const Span s = span(tile);
                 const uint32_t n0 = (uint32_t)(tile % t.wtiles) * kRows;
                 w = ScaleRows{p.ws + s.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
@@ -522,10 +547,10 @@ bool map_of(CUtensorMap *m, const void *base, uint32_t columns, uint64_t rows, u
     return e && e(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// scales that a load may bring: whole in every row
-uint32_t unit_of(const void *base, uint64_t stride, uint64_t expert, uint32_t groups) {
-    const uint64_t at = reinterpret_cast<uintptr_t>(base) | stride | expert | groups;
-    return at % 8u == 0 ? 8u : at % 4u == 0 ? 4u : 1u;
+// scales that a load may bring, of every row and every step of the depth (`odd`: that may start at an odd one)
+uint32_t unit_of(const void *base, uint64_t stride, uint64_t expert, uint64_t step, uint32_t groups, bool odd) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(base) | stride | expert | step | (step == 16u ? groups : 0u);          // (the second order is filled up)
+    return at % 16u == 0 && !odd ? 16u : at % 8u == 0 ? 8u : at % 4u == 0 ? 4u : 1u;
 }
 constexpr uint32_t kSms = 148;
 
@@ -563,21 +588,39 @@ cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t mx4_tc_launch(const Mx4Product &a, bool made, cudaStream_t stream) {
+Mx4Plan mx4_plan(const Mx4Product &a) {
+    Mx4Plan r{};
+    const uint32_t groups = mx4_groups(a.columns), steps = (groups + kStageGroups - 1u) / kStageGroups, chunks = (groups + 15u) / 16u, wtiles = (a.outputs + kRows - 1u) / kRows;
+    const uint32_t each = a.experts ? (a.rows + a.experts - 1u) / a.experts : a.rows;          // rows to a matrix, on average
+    auto pairs = [&](uint32_t tn) { return a.experts ? std::min(a.rows, a.rows / tn + std::min(a.rows, a.experts)) : (a.rows + tn - 1u) / tn; };
+    r.tn = each <= 16u ? 16u : each <= 32u ? 32u : each <= 64u ? 64u : each <= 128u ? 128u : 256u;
+    if (r.tn == 256u && (uint64_t)wtiles * pairs(256) < kSms) r.tn = 128;
+    r.pairs = pairs(r.tn);
+    const uint64_t tiles = (uint64_t)wtiles * r.pairs;
+    if (tiles < 2u * kSms && r.tn < 256u) {
+        r.ks = 1;
+        while (r.ks < 8u && tiles * r.ks < kSms && steps >= 2u * r.ks) r.ks *= 2u;
+    }
+    r.per = (steps + std::max(1u, r.ks) - 1u) / std::max(1u, r.ks);
+    r.x_second = r.ks <= 1u || r.per % 2u == 0;          // (two steps of the depth are sixteen scales)
+    const bool codes = a.x_type == T_MX4;
+    r.x_codes = !codes || a.columns % 2u;
+    r.w_scales = r.tn == 256u && (uint64_t)r.pairs >= 4u * (uint64_t)std::max(1u, a.experts);
+    r.x_scales = r.x_codes || (codes && r.tn == 256u);
+    r.x_scales_at = r.x_codes ? (uint64_t)a.rows * groups * 16u : 0;
+    r.w_scales_at = r.x_scales_at + (r.x_scales ? (uint64_t)a.rows * chunks * 16u : 0);
+    r.bytes = r.w_scales_at + (r.w_scales ? (uint64_t)std::max(1u, a.experts) * a.outputs * chunks * 16u : 0);
+    return r;
+}
+
+cudaError_t mx4_tc_launch(const Mx4Product &a, const Mx4Plan &plan, uint64_t xs_step, uint64_t ws_step, bool made, cudaStream_t stream) {
     TcArgs t{};
     t.p = a; t.groups = mx4_groups(a.columns); t.steps = (t.groups + kStageGroups - 1u) / kStageGroups; t.wtiles = (a.outputs + kRows - 1u) / kRows; t.made = made;
-    t.w_unit = unit_of(a.ws, a.ws_stride, a.ws_expert, t.groups); t.x_unit = unit_of(a.xs, a.xs_stride, 0, t.groups);
-    const uint32_t each = a.offsets ? (a.rows + a.experts - 1u) / a.experts : a.rows;          // rows to a matrix, on average
-    auto pairs = [&](uint32_t tn) { return a.offsets ? std::min(a.rows, a.rows / tn + std::min(a.rows, a.experts)) : (a.rows + tn - 1u) / tn; };
-    uint32_t tn = each <= 16u ? 16u : each <= 32u ? 32u : each <= 64u ? 64u : each <= 128u ? 128u : 256u;
-    if (tn == 256 && (uint64_t)t.wtiles * pairs(256) < kSms) tn = 128;
-    t.pairs = pairs(tn);
-    const uint64_t tiles = (uint64_t)t.wtiles * t.pairs;
-    if (tiles < 2u * kSms && tn < 256u) {
-        t.ks = 1;
-        while (t.ks < 8u && tiles * t.ks < kSms && t.steps >= 2u * t.ks) t.ks *= 2u;
-    }
-    switch (tn) {
+    t.pairs = plan.pairs; t.ks = plan.ks; t.per = plan.per;
+    const bool odd = t.ks > 1 && t.per % 2u;
+    t.w_step = ws_step; t.x_step = xs_step;
+    t.w_unit = unit_of(a.ws, a.ws_stride, a.ws_expert, ws_step, t.groups, odd); t.x_unit = unit_of(a.xs, a.xs_stride, 0, xs_step, t.groups, odd);
+    switch (plan.tn) {
         case 16: return launch_of<16>(t, stream);
         case 32: return launch_of<32>(t, stream);
         case 64: return launch_of<64>(t, stream);

@@ -421,10 +421,16 @@ def _product(x, w, offsets, dtype):
                          0 if offsets is None else offsets.data_ptr(), kind, out_kind, rows, outputs, columns, experts)
     except struct.error:
         _no("strides are not negative, counts numbers of 32 bits")
-    need = rows * 17 * groups if kind != 3 or columns % 2 else 0          # (as nb200_dev_mx4_product_workspace says)
-    room = torch.empty(need, dtype=torch.uint8, device=wc.device) if need else None
-    _call(device, lib(True).nb200_dev_mx4_product, p, room.data_ptr() if need else None, need)
+    L, need = lib(True), C.c_uint64()
+    _call(device, _product_room, L, p, need)
+    need = need.value
+    room = wc.new_empty(need, dtype=torch.uint8) if need else None
+    _call(device, L.nb200_dev_mx4_product, p, room.data_ptr() if need else None, need)
     return out
+
+
+def _product_room(L, p, need, stream):
+    return L.nb200_dev_mx4_product_workspace(p, C.byref(need))
 
 
 def mx4_product(x, w, dtype=None):
