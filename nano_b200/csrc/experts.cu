@@ -8,16 +8,18 @@
 #include "family.h"
 #include "ops.h"
 #include "portions.h"
+#include "rows.cuh"
 
 namespace nb {
 namespace {
 
 // ------------------------------------------------------------------------------------------------
 // Sorting places by expert: counts, their running sums, and a second walk that hands out the places in order.  A warp owns a run of neighbouring places and a row of counts in shared memory, a
-// block the runs of its warps, a cluster of up to eight blocks the list: sums run over experts, then blocks, then warps, so the result is the stable one whatever the order of arrival, in one
-// launch without a workspace.  Within 32 places __match_any_sync gives a place its rank.  Bound by the walks' latency: 2 x places / (32 warps) rounds of some 100 cycles.
+// block the runs of its warps, a cluster of up to sixteen blocks the list: sums run over experts, then blocks, then warps, so the result is the stable one whatever the order of arrival, in one
+// launch without a workspace.  Within 32 places a place's rank is counted from ballots over the bits of its expert's number.  Bound by latency: eight loads of a warp are under way at once, and the first eight of its run stay in
+// registers for the second walk.
 // ------------------------------------------------------------------------------------------------
-constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCluster = 8, kMaxExperts = 1024;
+constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCluster = 16, kMaxExperts = 1024, kSortAhead = 8;
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -34,31 +36,51 @@ __global__ void __launch_bounds__(kSortThreads) k_experts_sort(const SortArgs a,
     extern __shared__ uint32_t counts[];          // [warps][experts], then the block's sums [experts] and where its runs begin [experts]
     __shared__ uint32_t sums[kSortWarps];
     const uint32_t E = a.experts, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = C > 1 ? cluster_rank() : 0u;
-    uint32_t *mine = counts + warp * E, *block = counts + kSortWarps * E, *begin = block + E;
-    for (uint32_t i = tid; i < kSortWarps * E; i += kSortThreads) counts[i] = 0;
+    uint32_t *mine = counts + warp * E, *block = counts + (blockDim.x / 32u) * E, *begin = block + E;
+    const uint32_t threads = blockDim.x, warps = threads / 32u;
+    for (uint32_t i = tid; i < warps * E; i += threads) counts[i] = 0;
     // runs of whole 32 places, as even as that allows
-    const uint32_t pieces = (a.n + 31u) / 32u, runs = C * kSortWarps, per = (pieces + runs - 1u) / runs;
-    const uint32_t p0 = min(pieces, (rank * kSortWarps + warp) * per), p1 = min(pieces, p0 + per);
+    const uint32_t pieces = (a.n + 31u) / 32u, runs = C * warps, per = (pieces + runs - 1u) / runs;
+    const uint32_t p0 = min(pieces, (rank * warps + warp) * per), p1 = min(pieces, p0 + per);
     auto expert = [&](uint32_t i) {          // E: none
         if (i >= a.n) return E;
-        const long long id = a.wide ? static_cast<const long long *>(a.ids)[i] : (long long)static_cast<const int *>(a.ids)[i];
+        const long long id = a.wide ? __ldg(static_cast<const long long *>(a.ids) + i) : (long long)__ldg(static_cast<const int *>(a.ids) + i);
         return id >= 0 && id < (long long)E ? (uint32_t)id : E;
     };
+    const uint32_t bits = 32u - __clz(E);          // (of 0 .. E)
+    auto alike = [&](uint32_t e) {          // the lanes with the same number
+        uint32_t same = 0xffffffffu;
+        for (uint32_t b = 0; b < bits; b++) { const bool one = e >> b & 1u; const uint32_t m = __ballot_sync(0xffffffffu, one); same &= one ? m : ~m; }
+        return same;
+    };
+    uint32_t held[kSortAhead];
+    auto load = [&](uint32_t p) {
+#pragma unroll
+        for (uint32_t j = 0; j < kSortAhead; j++) held[j] = p + j < p1 ? expert((p + j) * 32u + lane) : E;
+    };
+    load(p0);
     __syncthreads();
-    for (uint32_t p = p0; p < p1; p++) {
-        const uint32_t e = expert(p * 32u + lane), same = __match_any_sync(0xffffffffu, e);
-        if (e < E && lane == (uint32_t)__ffs(same) - 1u) mine[e] += __popc(same);
-        __syncwarp();
+    for (uint32_t p = p0; p < p1; p += kSortAhead) {
+        if (p != p0) load(p);
+#pragma unroll
+        for (uint32_t j = 0; j < kSortAhead; j++) if (held[j] < E) atomicAdd(mine + held[j], 1u);          // (a count does not depend on the order)
     }
+    if (p1 - p0 > kSortAhead) load(p0);
     __syncthreads();
-    for (uint32_t e = tid; e < E; e += kSortThreads) {
-        uint32_t run = 0;
-        for (uint32_t w = 0; w < kSortWarps; w++) { const uint32_t c = counts[w * E + e]; counts[w * E + e] = run; run += c; }
+    for (uint32_t e = tid; e < E; e += threads) {
+        uint32_t c[kSortWarps], run = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWarps; w++) c[w] = w < warps ? counts[w * E + e] : 0u;
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWarps; w++) { const uint32_t x = c[w]; c[w] = run; run += x; }
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWarps; w++) if (w < warps) counts[w * E + e] = c[w];          // those of the warps before
         block[e] = run;
     }
     if (C > 1) cluster_sync(); else __syncthreads();
     uint32_t all = 0, before = 0;          // of expert tid: in the whole list, in the blocks before this one
     if (tid < E)
+#pragma unroll 8
         for (uint32_t c = 0; c < C; c++) { const uint32_t x = C > 1 ? peer_u32(block + tid, c) : block[tid]; all += x; before += c < rank ? x : 0u; }
     uint32_t up = all;
 #pragma unroll
@@ -66,152 +88,180 @@ __global__ void __launch_bounds__(kSortThreads) k_experts_sort(const SortArgs a,
     if (lane == 31u) sums[warp] = up;
     __syncthreads();
     if (warp == 0) {
-        uint32_t s = sums[lane];
+        uint32_t s = lane < warps ? sums[lane] : 0u;
 #pragma unroll
         for (uint32_t o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, s, o); s += lane >= o ? x : 0u; }
-        sums[lane] = s;
+        sums[lane] = s;          // (all 32)
     }
     __syncthreads();
-    const uint32_t from = up - all + (warp ? sums[warp - 1u] : 0u), known = sums[kSortWarps - 1u];
+    const uint32_t from = up - all + (warp ? sums[warp - 1u] : 0u), known = sums[31];
     if (tid < E) {
         begin[tid] = from + before;
         if (rank == 0) { a.offsets[tid] = (int32_t)from; if (tid == E - 1u) a.offsets[E] = (int32_t)known; }
     }
     __syncthreads();
-    for (uint32_t p = p0; p < p1; p++) {
-        const uint32_t i = p * 32u + lane, e = expert(i), same = __match_any_sync(0xffffffffu, e);
-        uint32_t at = 0;
-        if (e < E) at = begin[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
-        __syncwarp();
-        if (e < E && lane == (uint32_t)__ffs(same) - 1u) mine[e] += __popc(same);
-        __syncwarp();
-        if (i < a.n) a.place[i] = e < E ? (int32_t)at : -1;
-        if (e < E) a.order[at] = (int32_t)i;
+    for (uint32_t i = tid; i < warps * E; i += threads) counts[i] += begin[i % E];          // where a warp's first place of an expert goes
+    __syncthreads();
+    for (uint32_t p = p0; p < p1; p += kSortAhead) {
+        if (p != p0) load(p);
+#pragma unroll
+        for (uint32_t j = 0; j < kSortAhead; j++) {
+            if (p + j >= p1) break;
+            const uint32_t i = (p + j) * 32u + lane, e = held[j], same = alike(e);
+            uint32_t at = 0;
+            if (e < E) at = mine[e];
+            __syncwarp();
+            if (e < E && lane == (uint32_t)__ffs(same) - 1u) mine[e] = at + __popc(same);
+            __syncwarp();
+            at += __popc(same & ((1u << lane) - 1u));
+            if (i < a.n) a.place[i] = e < E ? (int32_t)at : -1;
+            if (e < E) a.order[at] = (int32_t)i;
+        }
     }
-    for (uint64_t r = known + (uint64_t)rank * kSortThreads + tid; r < a.n; r += C * kSortThreads) a.order[r] = -1;
+    for (uint64_t r = known + (uint64_t)rank * threads + tid; r < a.n; r += C * threads) a.order[r] = -1;
     if (C > 1) cluster_sync();          // nobody leaves while its shared memory is read
 }
 
 // ------------------------------------------------------------------------------------------------
-// Rows to their places.  Pure movement, bound by memory: units of U bytes, the widest that every row's start and length allow, two to a thread.
+// Rows to their places.  Pure movement, bound by memory.  Where every row starts on a 16-byte border, pieces of 16 bytes, four to a thread; elsewhere pieces of the result's memory, whose bytes are
+// shifted out of two of the row's.
 // ------------------------------------------------------------------------------------------------
-constexpr uint32_t kMoveThreads = 256, kMoveUnits = 2;
-struct GatherArgs { char *out; const char *x; const int32_t *order; uint64_t out_stride, x_stride; uint32_t units, top, tokens; };
-template <int U> struct Unit;
-template <> struct Unit<16> { typedef uint4 T; };
-template <> struct Unit<8> { typedef uint2 T; };
-template <> struct Unit<4> { typedef uint32_t T; };
-template <> struct Unit<2> { typedef uint16_t T; };
-template <> struct Unit<1> { typedef uint8_t T; };
-
-template <int U>
-__global__ void __launch_bounds__(kMoveThreads) k_experts_gather(const GatherArgs a, const uint32_t items) {
-    typedef typename Unit<U>::T T;
-    T v[kMoveUnits] = {};
+constexpr uint32_t kMoveThreads = 256, kMoveUnits = 4;
+struct GatherArgs { uint8_t *out; const uint8_t *x; const int32_t *order; uint64_t out_stride, x_stride; uint32_t bytes, top, tokens; };
+__device__ __forceinline__ const uint8_t *token_row(const GatherArgs &a, uint32_t r) {          // null: none
+    const int32_t o = __ldg(a.order + r);
+    const uint32_t t = (uint32_t)o / a.top;
+    return o >= 0 && t < a.tokens ? a.x + t * a.x_stride : nullptr;
+}
+__global__ void __launch_bounds__(kMoveThreads) k_experts_gather(const GatherArgs a, const uint32_t per_row, const uint32_t items) {
+    uint4 v[kMoveUnits] = {};
     const uint32_t i0 = blockIdx.x * kMoveThreads * kMoveUnits + threadIdx.x;
 #pragma unroll
     for (uint32_t j = 0; j < kMoveUnits; j++) {
-        const uint32_t i = i0 + j * kMoveThreads;
+        const uint32_t i = i0 + j * kMoveThreads, r = i / per_row;
         if (i >= items) break;
-        const int32_t o = a.order[i / a.units];
-        const uint32_t t = (uint32_t)o / a.top;
-        if (o >= 0 && t < a.tokens) v[j] = __ldg(reinterpret_cast<const T *>(a.x + t * a.x_stride) + i % a.units);
+        if (const uint8_t *row = token_row(a, r)) v[j] = __ldg(reinterpret_cast<const uint4 *>(row) + (i - r * per_row));
     }
 #pragma unroll
     for (uint32_t j = 0; j < kMoveUnits; j++) {
-        const uint32_t i = i0 + j * kMoveThreads;
+        const uint32_t i = i0 + j * kMoveThreads, r = i / per_row;
         if (i >= items) break;
-        reinterpret_cast<T *>(a.out + (uint64_t)(i / a.units) * a.out_stride)[i % a.units] = v[j];
+        reinterpret_cast<uint4 *>(a.out + (uint64_t)r * a.out_stride)[i - r * per_row] = v[j];
     }
+}
+__global__ void __launch_bounds__(kMoveThreads) k_experts_gather_any(const GatherArgs a, const uint32_t per_row, const uint32_t items) {
+    const uint32_t i = blockIdx.x * kMoveThreads + threadIdx.x, r = i / per_row;
+    if (i >= items) return;
+    uint8_t *to = a.out + (uint64_t)r * a.out_stride;
+    const uint8_t *row = token_row(a, r);
+    const int k = piece_at(to, i - r * per_row);
+    if (k >= (int)a.bytes) return;
+    if (k >= 0 && (uint32_t)k + 16u <= a.bytes) {
+        uint32_t w[4] = {};
+        if (row && inside<16, uint8_t>(a.bytes, k)) load_words<4, true>(row + k, w);
+        else if (row)
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j / 4] |= (uint32_t)__ldg(row + k + j) << (8 * (j % 4));
+        *reinterpret_cast<uint4 *>(to + k) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else
+        for (int j = max(k, 0); j < min(k + 16, (int)a.bytes); j++) to[j] = row ? __ldg(row + j) : (uint8_t)0;
 }
 
 // ------------------------------------------------------------------------------------------------
-// And back.  V neighbours of a token's row to a thread, which adds up the rows of its experts in fp32, in the list's order; the gradient by rows of the sorted list, a warp to each, which reads
-// the token's gradient (the other experts of the token find it in L2) and its own row once.  Both bound by memory.
+// And back.  A piece of 16 bytes of a token's row to a thread, which adds up the rows of its experts in fp32, in the list's order; the gradient by rows of the sorted list, which read the token's
+// gradient (the other experts of the token find it in L2) and their own row once.  Both bound by memory.
 // ------------------------------------------------------------------------------------------------
 struct CombineArgs {
     void *out; const void *y; const float *weights; const int32_t *place, *order; uint64_t out_stride, y_stride; uint32_t tokens, top, rows, columns;
     const void *grad; void *dy; float *dweights; uint64_t grad_stride, dy_stride;
 };
-template <typename T> __device__ __forceinline__ float widen(T v);
-template <> __device__ __forceinline__ float widen(float v) { return v; }
-template <> __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
-template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T v[V]; };
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kMoveThreads) k_experts_combine(const CombineArgs a, const uint32_t per_row, const uint32_t items) {
-    const uint32_t i = blockIdx.x * kMoveThreads + threadIdx.x;
-    if (i >= items) return;
-    const uint32_t t = i / per_row, c = i % per_row * V;
-    const uint64_t first = (uint64_t)t * a.top;
-    float sum[V] = {};
+template <typename T, Where WHERE>
+__device__ __forceinline__ void combine_piece(const CombineArgs &a, T *out, uint64_t first, int c) {
+    constexpr int P = 16 / sizeof(T);
+    float sum[P] = {};
 #pragma unroll 4
     for (uint32_t j = 0; j < a.top; j++) {
-        const uint32_t r = (uint32_t)a.place[first + j];          // (-1: beyond all rows)
-        const float w = a.weights ? a.weights[first + j] : 1.0f;
+        const uint32_t r = (uint32_t)__ldg(a.place + first + j);          // (-1: beyond all rows)
+        const float w = a.weights ? __ldg(a.weights + first + j) : 1.0f;
         if (r < a.rows) {
-            const Vec<T, V> y = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(a.y) + r * a.y_stride + c);
+            float y[P];
+            load_row<WHERE>(static_cast<const T *>(a.y) + r * a.y_stride, a.columns, c, y);
 #pragma unroll
-            for (int k = 0; k < V; k++) sum[k] = fmaf(w, widen(y.v[k]), sum[k]);
+            for (int k = 0; k < P; k++) sum[k] = fmaf(w, y[k], sum[k]);
         }
     }
-    Vec<T, V> out;
-#pragma unroll
-    for (int k = 0; k < V; k++) out.v[k] = narrow<T>(sum[k]);
-    *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.out) + t * a.out_stride + c) = out;
+    store_piece<WHERE>(out, a.columns, c, sum);
+}
+// BORDERS: every row starts on a 16-byte border and is whole pieces
+template <typename T, bool BORDERS>
+__global__ void __launch_bounds__(kMoveThreads) k_experts_combine(const CombineArgs a, const uint32_t per_row, const uint32_t items) {
+    constexpr int P = 16 / sizeof(T);
+    const uint32_t i = blockIdx.x * kMoveThreads + threadIdx.x, t = i / per_row;
+    if (i >= items) return;
+    T *out = static_cast<T *>(a.out) + t * a.out_stride;
+    if constexpr (BORDERS) combine_piece<T, EVEN>(a, out, (uint64_t)t * a.top, (int)((i - t * per_row) * P));
+    else {
+        const int c = piece_at(out, i - t * per_row);
+        if (c >= (int)a.columns) return;
+        if (inside<P, T>(a.columns, c)) combine_piece<T, INSIDE>(a, out, (uint64_t)t * a.top, c);
+        else combine_piece<T, ANY>(a, out, (uint64_t)t * a.top, c);
+    }
 }
 
-template <typename T, int V>
+template <typename T> struct GradRow { const T *g, *y; T *dy; bool known, wanted, weigh; float w; uint32_t columns; };
+template <Where WHERE, typename T>
+__device__ __forceinline__ float grad_piece(const GradRow<T> &r, int c) {
+    constexpr int P = 16 / sizeof(T);
+    float d[P] = {}, dot = 0.0f;
+    if (r.known) {
+        load_row<WHERE>(r.g, r.columns, c, d);
+        if (r.weigh) {
+            float v[P];
+            load_row<WHERE>(r.y, r.columns, c, v);
+#pragma unroll
+            for (int k = 0; k < P; k++) dot = fmaf(d[k], v[k], dot);
+        }
+#pragma unroll
+        for (int k = 0; k < P; k++) d[k] *= r.w;
+    }
+    if (r.wanted) store_piece<WHERE>(r.dy, r.columns, c, d);
+    return dot;
+}
+// LANES threads to a row
+template <typename T, int LANES, bool BORDERS>
 __global__ void __launch_bounds__(kMoveThreads) k_experts_combine_grad(const CombineArgs a, const uint32_t n) {
-    const uint32_t r = blockIdx.x * (kMoveThreads / 32u) + threadIdx.x / 32u, lane = threadIdx.x & 31u;
-    if (a.dweights && r < n && lane == 0 && (uint32_t)a.place[r] >= a.rows) a.dweights[r] = 0.0f;          // of place r of the list
-    if (r >= a.rows) return;
-    const uint32_t o = (uint32_t)a.order[r], t = o / a.top;
+    constexpr int P = 16 / sizeof(T);
+    const uint32_t r = blockIdx.x * (kMoveThreads / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    if (a.dweights && r < n && lane == 0 && (uint32_t)__ldg(a.place + r) >= a.rows) a.dweights[r] = 0.0f;          // of place r of the list
+    const uint32_t o = r < a.rows ? (uint32_t)__ldg(a.order + r) : 0xffffffffu, t = o / a.top;
     const bool known = o < n;
-    const float w = known && a.weights ? a.weights[o] : 1.0f;
-    const T *g = static_cast<const T *>(a.grad) + t * a.grad_stride, *y = static_cast<const T *>(a.y) + r * a.y_stride;
-    T *dy = a.dy ? static_cast<T *>(a.dy) + r * a.dy_stride : nullptr;
+    // (dy's address shares the columns out whether it is wanted or not: the same sums)
+    const GradRow<T> row{static_cast<const T *>(a.grad) + t * a.grad_stride, static_cast<const T *>(a.y) + r * a.y_stride, static_cast<T *>(a.dy) + r * a.dy_stride, known, a.dy != nullptr,
+                         a.dweights != nullptr, known && a.weights ? __ldg(a.weights + o) : 1.0f, a.columns};
     float dot = 0.0f;
+    if (r < a.rows) {
+        if constexpr (BORDERS) {
 #pragma unroll 4
-    for (uint32_t c = lane * V; c < a.columns; c += 32u * V) {
-        Vec<T, V> d = {};
-        if (known) {
-            const Vec<T, V> gv = *reinterpret_cast<const Vec<T, V> *>(g + c);
-            if (a.dweights) {
-                const Vec<T, V> yv = *reinterpret_cast<const Vec<T, V> *>(y + c);
-#pragma unroll
-                for (int k = 0; k < V; k++) dot = fmaf(widen(gv.v[k]), widen(yv.v[k]), dot);
-            }
-#pragma unroll
-            for (int k = 0; k < V; k++) d.v[k] = narrow<T>(w * widen(gv.v[k]));
+            for (uint32_t c = lane * P; c < a.columns; c += LANES * P) dot += grad_piece<EVEN>(row, (int)c);
+        } else {
+            // pieces [b0, b1) are inside, whatever borders the other rows have; those before and behind go number by number
+            const uint32_t head = (uint32_t)-piece_at(row.dy, 0), pieces = (a.columns + head + P - 1u) / P, b0 = head ? 2u : 1u, b1 = a.columns + head >= 2u * P ? (a.columns + head - 2u * P) / P + 1u : 0u;
+#pragma unroll 4
+            for (uint32_t b = b0 + lane; b < b1; b += LANES) dot += grad_piece<INSIDE>(row, piece_at(row.dy, b));
+            const uint32_t ends = b1 > b0 ? b0 + (pieces - b1) : pieces;
+            for (uint32_t b = lane; b < ends; b += LANES) dot += grad_piece<ANY>(row, piece_at(row.dy, b1 > b0 && b >= b0 ? b1 + (b - b0) : b));
         }
-        if (dy) *reinterpret_cast<Vec<T, V> *>(dy + c) = d;
     }
-    if (!a.dweights || !known) return;
+    if (!a.dweights) return;
 #pragma unroll
-    for (uint32_t s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-    if (lane == 0) a.dweights[o] = dot;
+    for (uint32_t s = LANES / 2; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+    if (lane == 0 && known) a.dweights[o] = dot;
 }
-
-// neighbours that one load may bring: all that the pointers, strides and the width are multiples of, at most 16 bytes
-template <typename T>
-uint32_t width_of(std::initializer_list<uint64_t> all, uint32_t columns) {
-    uint64_t at = (uint64_t)columns * sizeof(T);
-    for (const uint64_t x : all) at |= x;
-    uint32_t v = 16u / sizeof(T);
-    while (v > 1u && at % (v * sizeof(T))) v /= 2u;
-    return v;
-}
-inline uint64_t bits(const void *p) { return reinterpret_cast<uintptr_t>(p); }
 
 template <typename T>
 cudaError_t combine_launch(const CombineArgs &a, cudaStream_t stream) {
-    const uint32_t v = width_of<T>({bits(a.out), bits(a.y), a.out_stride * sizeof(T), a.y_stride * sizeof(T)}, a.columns), per_row = a.columns / v;
+    const bool out = on_borders<T>(a.out, a.out_stride, a.tokens), all = out && on_borders<T>(a.y, a.y_stride, a.rows) && a.columns * sizeof(T) % 16u == 0;
+    const uint32_t per_row = most_pieces<T>(a.columns, out);
     return in_portions(a.tokens, std::max(1u, 0x7fffff00u / per_row), [&](uint32_t t0, uint32_t nt) {
         CombineArgs b = a;
         b.tokens = nt;
@@ -219,22 +269,20 @@ cudaError_t combine_launch(const CombineArgs &a, cudaStream_t stream) {
         b.place += (uint64_t)t0 * a.top;
         if (a.weights) b.weights += (uint64_t)t0 * a.top;
         const uint32_t items = nt * per_row, blocks = (items + kMoveThreads - 1u) / kMoveThreads;
-        if (v * sizeof(T) == 16) k_experts_combine<T, 16 / sizeof(T)><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
-        else if (v * sizeof(T) == 8) k_experts_combine<T, 8 / sizeof(T)><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
-        else if (v * sizeof(T) == 4) k_experts_combine<T, 4 / sizeof(T)><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
-        else k_experts_combine<T, 1><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
+        if (all) k_experts_combine<T, true><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
+        else k_experts_combine<T, false><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
         return cudaGetLastError();
     });
 }
 template <typename T>
 cudaError_t grad_launch(const CombineArgs &a, cudaStream_t stream) {
-    const uint32_t v = width_of<T>({bits(a.y), bits(a.grad), bits(a.dy), a.y_stride * sizeof(T), a.grad_stride * sizeof(T), a.dy_stride * sizeof(T)}, a.columns), n = a.tokens * a.top;
-    const uint32_t blocks = (std::max(n, a.rows) + kMoveThreads / 32u - 1u) / (kMoveThreads / 32u);
-    if (v * sizeof(T) == 16) k_experts_combine_grad<T, 16 / sizeof(T)><<<blocks, kMoveThreads, 0, stream>>>(a, n);
-    else if (v * sizeof(T) == 8) k_experts_combine_grad<T, 8 / sizeof(T)><<<blocks, kMoveThreads, 0, stream>>>(a, n);
-    else if (v * sizeof(T) == 4) k_experts_combine_grad<T, 4 / sizeof(T)><<<blocks, kMoveThreads, 0, stream>>>(a, n);
-    else k_experts_combine_grad<T, 1><<<blocks, kMoveThreads, 0, stream>>>(a, n);
-    return cudaGetLastError();
+    const bool even = on_borders<T>(a.dy, a.dy_stride, a.rows) && on_borders<T>(a.y, a.y_stride, a.rows) && on_borders<T>(a.grad, a.grad_stride, a.tokens) && a.columns * sizeof(T) % 16u == 0;
+    const uint32_t pieces = (a.columns * (uint32_t)sizeof(T) + 15u) / 16u, n = a.tokens * a.top, all = std::max(n, a.rows);
+    // threads to a row: as many as it has pieces, up to a warp (rows and places are at most 2^30)
+    auto go = [&](auto kernel, uint32_t lanes) { kernel<<<(uint32_t)(((uint64_t)all * lanes + kMoveThreads - 1u) / kMoveThreads), kMoveThreads, 0, stream>>>(a, n); return cudaGetLastError(); };
+    if (pieces <= 4u) return even ? go(k_experts_combine_grad<T, 4, true>, 4) : go(k_experts_combine_grad<T, 4, false>, 4);
+    if (pieces <= 8u) return even ? go(k_experts_combine_grad<T, 8, true>, 8) : go(k_experts_combine_grad<T, 8, false>, 8);
+    return even ? go(k_experts_combine_grad<T, 32, true>, 32) : go(k_experts_combine_grad<T, 32, false>, 32);
 }
 
 }  // namespace
@@ -247,16 +295,21 @@ constexpr uint32_t kMostPlaces = 1u << 30;
 
 cudaError_t sort_launch(const nb::SortArgs &a, cudaStream_t stream) {
     using namespace nb;
-    // blocks: one for each 4096 places, up to the eight that any cluster may have
+    // blocks: one for each 4096 places, up to the sixteen that a cluster may have if it is asked for
     uint32_t C = 1;
     while (C < kSortCluster && a.n > C * 4096u) C *= 2u;
-    const uint32_t smem = (kSortWarps + 2u) * a.experts * 4u;
+    if (C > 8u) {
+        const cudaError_t e = cudaFuncSetAttribute(k_experts_sort, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    // warps: one for each 32 places, up to the block's 32, and threads for all experts
+    const uint32_t warps = std::min(kSortWarps, std::max((a.n + 32u * C - 1u) / (32u * C), (a.experts + 31u) / 32u)), smem = (warps + 2u) * a.experts * 4u;
     if (smem > 40u * 1024u) {
         const cudaError_t e = smem_at_least(reinterpret_cast<const void *>(k_experts_sort), (int)smem);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(C); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = dim3(C); cfg.blockDim = dim3(std::max(1u, warps) * 32u); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -308,21 +361,14 @@ int nb200_dev_experts_gather(void *out, uint64_t out_stride, const void *x, uint
     if (reinterpret_cast<uintptr_t>(order) % 4u) return fail(NB200_EINVAL, "order is not aligned to its type");
     if (n > 1 && out_stride < row_bytes) return fail(NB200_EINVAL, "rows of the result overlap");
     if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
-    const uint64_t at = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(x) | out_stride | x_stride | row_bytes;
-    uint32_t unit = 16;
-    while (at % unit) unit /= 2u;
-    const uint32_t units = (uint32_t)(row_bytes / unit), each = nb::kMoveThreads * nb::kMoveUnits;
+    const bool even = (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(x) | out_stride | x_stride | row_bytes) % 16u == 0;
+    const uint32_t bytes = (uint32_t)row_bytes, per_row = even ? bytes / 16u : nb::most_pieces<uint8_t>(bytes, false);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    NB_CK(nb::in_portions(n, std::max(1u, 0x7fffff00u / units), [&](uint32_t r0, uint32_t rows) {
-        const nb::GatherArgs a{static_cast<char *>(out) + r0 * out_stride, static_cast<const char *>(x), order + r0, out_stride, x_stride, units, top, tokens};
-        const uint32_t items = rows * units, blocks = (items + each - 1u) / each;
-        switch (unit) {
-            case 16: nb::k_experts_gather<16><<<blocks, nb::kMoveThreads, 0, s>>>(a, items); break;
-            case 8: nb::k_experts_gather<8><<<blocks, nb::kMoveThreads, 0, s>>>(a, items); break;
-            case 4: nb::k_experts_gather<4><<<blocks, nb::kMoveThreads, 0, s>>>(a, items); break;
-            case 2: nb::k_experts_gather<2><<<blocks, nb::kMoveThreads, 0, s>>>(a, items); break;
-            default: nb::k_experts_gather<1><<<blocks, nb::kMoveThreads, 0, s>>>(a, items);
-        }
+    NB_CK(nb::in_portions(n, std::max(1u, 0x7fffff00u / per_row), [&](uint32_t r0, uint32_t rows) {
+        const nb::GatherArgs a{static_cast<uint8_t *>(out) + r0 * out_stride, static_cast<const uint8_t *>(x), order + r0, out_stride, x_stride, bytes, top, tokens};
+        const uint32_t items = rows * per_row, each = nb::kMoveThreads * nb::kMoveUnits;
+        if (even) nb::k_experts_gather<<<(items + each - 1u) / each, nb::kMoveThreads, 0, s>>>(a, per_row, items);
+        else nb::k_experts_gather_any<<<(items + nb::kMoveThreads - 1u) / nb::kMoveThreads, nb::kMoveThreads, 0, s>>>(a, per_row, items);
         return cudaGetLastError();
     }));
     return 0;

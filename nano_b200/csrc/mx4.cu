@@ -8,60 +8,10 @@
 #include "family.h"
 #include "mx4.h"
 #include "portions.h"
+#include "rows.cuh"
 
 namespace nb {
 namespace {
-
-template <typename T> struct Num;
-template <> struct Num<float> {
-    static __device__ __forceinline__ float widen(float v) { return v; }
-    static __device__ __forceinline__ float narrow(float v) { return v; }
-};
-template <> struct Num<__nv_bfloat16> {
-    static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
-};
-template <> struct Num<__half> {
-    static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
-};
-
-// Eight neighbours at p as numbers; `in` of them are the row's, the others zero.  Rows start anywhere: the 16-byte pieces of memory that hold the eight are read, and what is wanted is
-// shifted out of them, where all of the pieces lie within the row [first, end); number by number at its ends.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, uint32_t in, const T *first, const T *end, float (&x)[8]) {
-    constexpr uint32_t W = 8 * sizeof(T) / 4;          // words of eight numbers
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p), low = at & ~(uintptr_t)15u;
-    const uint32_t shift = (uint32_t)(at & 15u);
-    uint32_t w[W];
-    if (shift == 0 && in == 8u) {
-#pragma unroll
-        for (uint32_t i = 0; i < W / 4; i++) { const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
-    } else if (in == 8u && low >= reinterpret_cast<uintptr_t>(first) && low + W * 4u + 16u <= reinterpret_cast<uintptr_t>(end)) {
-        uint32_t v[W + 4];
-#pragma unroll
-        for (uint32_t i = 0; i < W / 4 + 1; i++) { const uint4 q = __ldg(reinterpret_cast<const uint4 *>(low) + i); v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w; }
-        if (shift & 8u)
-#pragma unroll
-            for (uint32_t i = 0; i < W + 2; i++) v[i] = v[i + 2];
-        if (shift & 4u)
-#pragma unroll
-            for (uint32_t i = 0; i < W + 1; i++) v[i] = v[i + 1];
-#pragma unroll
-        for (uint32_t i = 0; i < W; i++) w[i] = sizeof(T) == 2 && (shift & 2u) ? __funnelshift_r(v[i], v[i + 1], 16) : v[i];
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) x[i] = i < in ? Num<T>::widen(p[i]) : 0.0f;
-        return;
-    }
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) { const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2))); x[i] = Num<T>::widen(*reinterpret_cast<const T *>(&h)); }
-    }
-}
 
 // two numbers to two codes, the first in the lower four bits: nearest, ties to even, beyond 6 (NaN too) to 6
 __device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
@@ -78,8 +28,9 @@ __device__ __forceinline__ __half2 numbers_of(uint32_t byte) {
 __device__ __forceinline__ float scale_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fc00000u) : e == 0u ? __uint_as_float(1u << 22) : __uint_as_float(e << 23); }
 
 // ------------------------------------------------------------------------------------------------
-// Quantisation.  Four threads to a group, eight numbers each: the largest magnitude's bits by two exchanges; of a number 2^(f - 127) m, 1 <= m < 2, the scale's byte is f - 2, and division by a
-// power of two is exact, so the one rounding is the conversion's.  Bound by memory: a number is read and 17/32 bytes are written, in whole words.
+// Quantisation.  A thread has 32 bytes of a group (a quarter of its fp32 numbers, half of its 16-bit ones): the largest magnitude's bits by one or two exchanges; of a number 2^(f - 127) m,
+// 1 <= m < 2, the scale's byte is f - 2, and division by a power of two is exact, so the one rounding is the conversion's.  Bound by memory: a number is read and 17/32 bytes are written, in
+// whole words.
 // ------------------------------------------------------------------------------------------------
 constexpr uint32_t kThreads = 256;
 __device__ __forceinline__ uint8_t *scale_at(const Mx4Rows &a, uint32_t row, uint32_t g) { return a.scales + (uint64_t)row * a.scale_stride + (g >> 4) * a.scale_step + (g & 15u); }
@@ -87,56 +38,76 @@ __device__ __forceinline__ uint8_t *scale_at(const Mx4Rows &a, uint32_t row, uin
 __device__ __forceinline__ void fill_scales(const Mx4Rows &a, uint32_t row, uint32_t g, uint32_t groups) {
     if (a.scale_step != 16u && g + 1u == groups) for (uint32_t i = groups; i & 15u; i++) *scale_at(a, row, i) = 0;
 }
+template <typename T> constexpr uint32_t kEach = 32u / sizeof(T);          // numbers to a thread
 template <typename T>
 __device__ __forceinline__ void quantise(const Mx4Rows &a, uint32_t per_row, uint32_t items, uint32_t i) {          // by all threads of a warp
+    constexpr uint32_t P = kEach<T>, SHARE = kMx4Group / P;          // threads to a group
     const bool live = i < items;
-    const uint32_t row = live ? i / per_row : 0u, q = live ? i % per_row : 0u, k = q * 8u;
-    float x[8] = {};
-    if (live && k < a.columns) {
+    const uint32_t row = live ? i / per_row : 0u, q = live ? i - row * per_row : 0u;
+    float x[P] = {};
+    if (live) {
         const T *first = static_cast<const T *>(a.x) + (uint64_t)row * a.x_stride;
-        load8(first + k, min(8u, a.columns - k), first, first + a.columns, x);
+        const int k = (int)(q * P);
+        if ((reinterpret_cast<uintptr_t>(first) & 15u) == 0 && q * P + P <= a.columns) load_row<EVEN>(first, a.columns, k, x);
+        else if (inside<P, T>(a.columns, k)) load_row<INSIDE>(first, a.columns, k, x);
+        else load_row<ANY>(first, a.columns, k, x);
     }
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);          // (NaN above infinity above all others)
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    for (uint32_t j = 0; j < P; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);          // (NaN above infinity above all others)
+#pragma unroll
+    for (uint32_t s = 1; s < SHARE; s *= 2u) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
     const uint32_t f = top >> 23, e = f == 255u ? 255u : f > 2u ? f - 2u : 0u;
     const float by = __uint_as_float((254u - min(e, 252u)) << 23);          // 2^(127 - e)
-    uint32_t w = 0;
+    uint32_t w[P / 8] = {};
 #pragma unroll
-    for (int j = 0; j < 4; j++) w |= codes_of(x[2 * j] * by, x[2 * j + 1] * by) << (8 * j);
+    for (uint32_t j = 0; j < P / 2; j++) w[j / 4] |= codes_of(x[2 * j] * by, x[2 * j + 1] * by) << (8u * (j % 4u));
     if (!live) return;
-    *reinterpret_cast<uint32_t *>(a.codes + (uint64_t)row * a.code_stride + q * 4u) = e == 255u ? 0u : w;
-    if ((q & 3u) == 0) { *scale_at(a, row, q >> 2) = (uint8_t)e; fill_scales(a, row, q >> 2, per_row / 4u); }
+    uint8_t *to = a.codes + (uint64_t)row * a.code_stride + q * (P / 2u);
+    if constexpr (P == 8) *reinterpret_cast<uint32_t *>(to) = e == 255u ? 0u : w[0];
+    else *reinterpret_cast<uint2 *>(to) = e == 255u ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
+    if (q % SHARE == 0) { *scale_at(a, row, q / SHARE) = (uint8_t)e; fill_scales(a, row, q / SHARE, per_row / SHARE); }
 }
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, const uint32_t per_row, const uint32_t items) { quantise<T>(a, per_row, items, blockIdx.x * kThreads + threadIdx.x); }
 
-// And back, V neighbours to a thread: as many as stores of whole vectors allow for every row
-template <typename T, int V>
+// And back, by pieces of 16 bytes of the result, 64 bytes to a thread, whose loads are under way at once: the codes of a piece's numbers are nibbles of two neighbouring words, its scales one or two
+// (of one word and one where rows start on borders).  8192 rows of 2560 fp32 numbers FIGURE us
+template <typename T, bool BORDERS>
 __global__ void __launch_bounds__(kThreads) k_mx4_read(const Mx4Rows a, const uint32_t per_row, const uint32_t items) {
-    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-    if (i >= items) return;
-    const uint32_t row = i / per_row, k = i % per_row * V;
-    const uint8_t *codes = a.codes + (uint64_t)row * a.code_stride + k / 2u;
-    const float s = scale_of(a.scales[(uint64_t)row * a.scale_stride + k / kMx4Group]);
-    uint32_t w;
-    if constexpr (V == 8) w = __ldg(reinterpret_cast<const uint32_t *>(codes));
-    else if constexpr (V == 4) w = __ldg(reinterpret_cast<const uint16_t *>(codes));
-    else w = V == 2 || k % 2u == 0 ? *codes : *codes >> 4;
-    struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec { T v[V]; } out;
+    constexpr int P = 16 / sizeof(T), U = 4;
+    const uint32_t groups = (a.columns + kMx4Group - 1u) / kMx4Group, i0 = blockIdx.x * (kThreads * U) + threadIdx.x;
+    uint32_t lo[U], hi[U], e0[U], e1[U];
+    T *first[U];
+    int k[U];
 #pragma unroll
-    for (int j = 0; j < V; j += 2) {
-        const float2 n = __half22float2(numbers_of(w >> (4 * j)));
-        out.v[j] = Num<T>::narrow(n.x * s);
-        if constexpr (V > 1) out.v[j + 1] = Num<T>::narrow(n.y * s);
+    for (int u = 0; u < U; u++) {
+        const uint32_t i = i0 + u * kThreads, row = i < items ? i / per_row : 0u;
+        first[u] = static_cast<T *>(a.x) + (uint64_t)row * a.x_stride;
+        k[u] = i >= items ? 0x7fffffff - P : BORDERS ? (int)((i - row * per_row) * P) : piece_at(first[u], i - row * per_row);
+        const uint32_t from = k[u] >= (int)a.columns ? 0u : (uint32_t)max(k[u], 0), at = from / 8u, g = from / kMx4Group;
+        const uint8_t *scales = a.scales + (uint64_t)row * a.scale_stride;
+        const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.codes + (uint64_t)row * a.code_stride);
+        lo[u] = __ldg(codes + at);
+        e0[u] = scales[g];
+        if (!BORDERS) { hi[u] = __ldg(codes + min(at + 1u, groups * 4u - 1u)); e1[u] = scales[min((from + P - 1u) / kMx4Group, groups - 1u)]; }
     }
-    T *to = static_cast<T *>(a.x) + (uint64_t)row * a.x_stride + k;
-    if (k + V <= a.columns) *reinterpret_cast<Vec *>(to) = out;
-    else
 #pragma unroll
-        for (int j = 0; j < V; j++) if (k + j < a.columns) to[j] = out.v[j];
+    for (int u = 0; u < U; u++) {
+        if (k[u] >= (int)a.columns) continue;
+        const uint32_t from = (uint32_t)max(k[u], 0), border = (from / kMx4Group + 1u) * kMx4Group;
+        uint32_t w = BORDERS ? lo[u] >> (4u * (from % 8u)) : __funnelshift_r(lo[u], hi[u], 4u * (from % 8u));
+        if (!BORDERS && k[u] < 0) w <<= -4 * k[u];          // (the row's first piece: its numbers are the last of it)
+        const float s0 = scale_of(e0[u]), s1 = BORDERS ? s0 : scale_of(e1[u]);
+        float x[P];
+#pragma unroll
+        for (int j = 0; j < P; j += 2) {
+            const float2 n = __half22float2(numbers_of(w >> (4 * j)));
+            x[j] = n.x * (k[u] + j < (int)border ? s0 : s1);
+            x[j + 1] = n.y * (k[u] + j + 1 < (int)border ? s0 : s1);
+        }
+        store_piece<ANY>(first[u], a.columns, k[u], x);
+    }
 }
 
 // rows in portions whose items are counted in 31 bits
@@ -154,15 +125,13 @@ cudaError_t by_rows(const Mx4Rows &a, uint32_t per_row, F f) {
 }
 template <typename T>
 cudaError_t read_launch_t(const Mx4Rows &a, cudaStream_t stream) {
-    const uint64_t at = reinterpret_cast<uintptr_t>(a.x) | a.x_stride * sizeof(T);
-    auto go = [&](auto k, uint32_t v) {
-        const uint32_t per_row = (a.columns + v - 1u) / v;
-        return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) { k<<<blocks, kThreads, 0, stream>>>(b, per_row, items); });
-    };
-    if (at % std::min<uint64_t>(16, 8 * sizeof(T)) == 0) return go(k_mx4_read<T, 8>, 8);
-    if (at % (4 * sizeof(T)) == 0) return go(k_mx4_read<T, 4>, 4);
-    if (at % (2 * sizeof(T)) == 0) return go(k_mx4_read<T, 2>, 2);
-    return go(k_mx4_read<T, 1>, 1);
+    const bool borders = on_borders<T>(a.x, a.x_stride, a.rows);
+    const uint32_t per_row = most_pieces<T>(a.columns, borders);
+    return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
+        blocks = (blocks + 3u) / 4u;
+        if (borders) k_mx4_read<T, true><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
+        else k_mx4_read<T, false><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
+    });
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -214,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) k_mx4_prepare(const __grid_constant_
 }  // namespace
 
 cudaError_t mx4_quantize_launch(const Mx4Rows &a, cudaStream_t stream) {
-    const uint32_t per_row = mx4_groups(a.columns) * 4u;
+    const uint32_t per_row = mx4_groups(a.columns) * (a.type == T_F32 ? 4u : 2u);
     return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
         if (a.type == T_F32) k_mx4_quantize<float><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
         else if (a.type == T_BF16) k_mx4_quantize<__nv_bfloat16><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
@@ -235,7 +204,7 @@ cudaError_t mx4_prepare_launch(const Mx4Product &p, const Mx4Plan &plan, uint8_t
     a.codes = Codes{static_cast<const uint8_t *>(p.x), p.xs, p.x_stride, p.xs_stride};
     a.xs = Scales{p.xs, p.xs_stride, 0, xs, p.rows, groups, chunks, p.x_type == T_MX4 ? unit(p.xs, p.xs_stride, 0) : 1u};
     const uint32_t kind = p.x_type != T_MX4 ? p.x_type : plan.x_codes ? (uint32_t)kOfCodes : (uint32_t)kOfScales;
-    a.per_row = kind < kOfCodes ? groups * 4u : kind == kOfCodes ? groups : chunks;
+    a.per_row = kind == kOfF32 ? groups * 4u : kind < kOfCodes ? groups * 2u : kind == kOfCodes ? groups : chunks;
     // x in portions whose items are counted in 31 bits, w's scales with the first
     return in_portions(plan.x_codes || plan.x_scales ? p.rows : 1u, std::max(1u, 0x7fffff00u / a.per_row), [&](uint32_t r0, uint32_t n) {
         Prepare b = a;
@@ -268,7 +237,7 @@ int rows_checked(const nb200_mx4_rows *p, nb::Mx4Rows *a) {
     if (!p) return fail(NB200_EINVAL, "null argument");
     if (p->type > nb::T_F16) return fail(NB200_EINVAL, "rows are fp32, bf16 or fp16 (type %u)", p->type);
     if (p->rows && !p->columns) return fail(NB200_EINVAL, "rows of no numbers");
-    if (p->columns > 0x7fffffffu) return fail(NB200_EINVAL, "rows of %u numbers are too long", p->columns);
+    if (p->columns > 1u << 30) return fail(NB200_EINVAL, "rows of %u numbers are too long", p->columns);
     if (!p->rows) return 0;
     if (!p->codes || !p->scales || !p->x) return fail(NB200_EINVAL, "null argument");
     const uint64_t groups = nb::mx4_groups(p->columns);

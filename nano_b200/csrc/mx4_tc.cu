@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "family.h"
 #include "mx4.h"
@@ -210,6 +211,26 @@ __device__ __forceinline__ void put_rows(const Mx4Product &p, uint64_t row, uint
     else put_column<J>(static_cast<__half *>(p.out) + at, p.out_stride, live, [&](uint32_t j) { return __float2half_rn(v[j]); });
 }
 
+// Of a tile whose parts lie in the blocks of a cluster, block `part` finishes J rows in every J * ks: the parts added up in the order of the depth.  As many rows at once as there may be: a
+// word of another block is some 200 ns away
+template <int J>
+__device__ __forceinline__ void finish_parts(const Mx4Product &p, uint32_t at, uint32_t part, uint32_t ks, uint32_t r0, uint32_t n, uint32_t rows) {
+    for (uint32_t j = part * J; j < rows; j += ks * J) {
+        float f[J] = {};
+#pragma unroll 2
+        for (uint32_t q = 0; q < ks; q++) {
+            uint32_t peer;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + j * kRows * 4u), "r"(q));
+            float v[J];
+#pragma unroll
+            for (uint32_t i = 0; i < J; i++) v[i] = ld_cluster_f32(peer + i * kRows * 4u);          // (a part has all TN rows' places)
+#pragma unroll
+            for (uint32_t i = 0; i < J; i++) f[i] += v[i];
+        }
+        put_rows<J>(p, r0 + j, n, f, rows - j);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // Few tiles: a tile's depth is shared by a cluster of ks blocks, each of which finishes some of its rows.  grid (tiles of W x (pairs + 1 with experts), 1, ks)
 // ------------------------------------------------------------------------------------------------
@@ -318,19 +339,8 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     if (t.ks > 1) {          // every block of the cluster finishes some of the tile's rows, in turn, its parts added up in the order of the depth
         cluster_sync_all();
         if (warp < 4 && n < p.outputs) {
-            const uint32_t at = smem_u32(mine);
-            constexpr uint32_t J = 4;
-            for (uint32_t j = part * J; j < rows; j += t.ks * J) {
-                float f[J] = {};
-#pragma unroll 4
-                for (uint32_t q = 0; q < t.ks; q++) {
-                    uint32_t peer;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + j * kRows * 4u), "r"(q));
-#pragma unroll
-                    for (uint32_t i = 0; i < J; i++) f[i] += ld_cluster_f32(peer + i * kRows * 4u);          // (a part has all TN rows' places)
-                }
-                put_rows<J>(p, span.r0 + j, n, f, rows - j);
-            }
+            if (TN >= 32 && rows > 4u * t.ks) finish_parts<16>(p, smem_u32(mine), part, t.ks, span.r0, n, rows);
+            else finish_parts<4>(p, smem_u32(mine), part, t.ks, span.r0, n, rows);
         }
         cluster_sync_all();          // no block leaves while another reads its part
     }
@@ -593,14 +603,26 @@ Mx4Plan mx4_plan(const Mx4Product &a) {
     const uint32_t groups = mx4_groups(a.columns), steps = (groups + kStageGroups - 1u) / kStageGroups, chunks = (groups + 15u) / 16u, wtiles = (a.outputs + kRows - 1u) / kRows;
     const uint32_t each = a.experts ? (a.rows + a.experts - 1u) / a.experts : a.rows;          // rows to a matrix, on average
     auto pairs = [&](uint32_t tn) { return a.experts ? std::min(a.rows, a.rows / tn + std::min(a.rows, a.experts)) : (a.rows + tn - 1u) / tn; };
-    r.tn = each <= 16u ? 16u : each <= 32u ? 32u : each <= 64u ? 64u : each <= 128u ? 128u : 256u;
-    if (r.tn == 256u && (uint64_t)wtiles * pairs(256) < kSms) r.tn = 128;
-    r.pairs = pairs(r.tn);
-    const uint64_t tiles = (uint64_t)wtiles * r.pairs;
-    if (tiles < 2u * kSms && r.tn < 256u) {
-        r.ks = 1;
-        while (r.ks < 8u && tiles * r.ks < kSms && steps >= 2u * r.ks) r.ks *= 2u;
+    // Tiles of tn rows of X, ks blocks to one: what takes least by a model of the time in us, fitted to products of 1 to 1024 rows with 1024 x 2048 up to 20000 x 1024 and 2560 x 9728.  A step of the depth
+    // takes `one` in the kernel for few tiles (once more for each 296 blocks, which begin anew, a quarter more where SMs have two), parts of a tile and their exchange some more; in the kernel for many tiles `step`,
+    // a tile `tile`.  us as measured, few / many: 1 x 9728 x 2560 7.8 / 8.4 (16 rows), 128 9.8 / 9.0 (128 rows), 256 11.0 / 12.9; split 1 / 2 / 4 / 8: 1 x 2560 x 9728 17.7 / 11.5 / 8.6 / 8.7,
+    // 1 x 9728 x 2560 7.8 / 7.8 / 10.3 / 15.1; 64 / 128 / 256 rows: 512 x 9728 x 2560 22.3 / 17.8 / 16.6, 128 9.3 / 9.0 / 10.6
+    struct Cost { uint32_t tn; float one, step, tile; };
+    constexpr Cost costs[5] = {{16, 0.40f, 0.33f, 0.40f}, {32, 0.42f, 0.34f, 0.45f}, {64, 0.45f, 0.36f, 0.50f}, {128, 0.60f, 0.34f, 1.1f}, {256, 0.0f, 0.50f, 1.3f}};
+    float best = 3e38f;
+    for (const Cost &c : costs) {
+        if (c.tn > 16u && c.tn >= 4u * each) break;
+        // tiles as they may be expected: half a tile of an expert's rows is empty
+        const double rows = a.experts ? std::min<double>(a.rows, a.rows / (double)c.tn + 0.5 * std::min(a.rows, a.experts)) : pairs(c.tn), tiles = std::max(1.0, rows) * wtiles;
+        auto take = [&](double us, uint32_t ks) { if (us < best) { best = (float)us; r.tn = c.tn; r.ks = ks; } };
+        take(4.0 + std::ceil(tiles / kSms) * (steps * c.step + c.tile), 0);
+        if (c.tn == 256u || (uint64_t)wtiles * pairs(c.tn) > (1u << 24)) continue;
+        for (uint32_t ks = 1; ks <= 8u && (ks == 1u || steps >= ks); ks *= 2u) {
+            const double blocks = tiles * ks, waves = std::ceil(blocks / (2.0 * kSms)), busy = blocks > kSms;
+            take(3.5 + waves * ((steps + ks - 1u) / ks) * c.one * (1.0 + 0.25 * busy) + 2.0 * (waves - 1.0) + (ks > 1u ? 0.5 + 0.02 * std::min(c.tn, each) + busy : 0.0), ks);
+        }
     }
+    r.pairs = pairs(r.tn);
     r.per = (steps + std::max(1u, r.ks) - 1u) / std::max(1u, r.ks);
     r.x_second = r.ks <= 1u || r.per % 2u == 0;          // (two steps of the depth are sixteen scales)
     const bool codes = a.x_type == T_MX4;

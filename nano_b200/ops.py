@@ -36,6 +36,7 @@ _ROWS, _ATTENTION = struct.Struct("@QQIIIIIQQQQQQQ").pack, struct.Struct("@QQQQQ
 _MX4_ROWS, _MX4_PRODUCT, _EXPERTS_ROWS = struct.Struct("@QQQQQQIII4x").pack, struct.Struct("@QQQQQQQQQQQQQIIIIII").pack, struct.Struct("@QQQQQQQIIIIIQQQQQ").pack
 assert len(_MX4_ROWS(*[0] * 9)) == C.sizeof(E.Mx4Rows) and len(_MX4_PRODUCT(*[0] * 19)) == C.sizeof(E.Mx4Product) and len(_EXPERTS_ROWS(*[0] * 17)) == C.sizeof(E.ExpertsRows)
 assert len(_ROWS(*[0] * 14)) == C.sizeof(E.Kv4Rows) and len(_ATTENTION(*[0] * 26)) == C.sizeof(E.Kv4Attention)
+_U8 = torch.uint8
 _stream_of, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice          # (torch.cuda's functions of that purpose cost two microseconds a call)
 
 
@@ -306,14 +307,15 @@ class Routing(NamedTuple):
 def _rows_of(name, x):
     """A tensor [..., columns] of numbers as (device, tensor of neighbouring numbers, rows, columns, stride from row to row)."""
     device = _cuda(name, x)
-    if not x.dim():
-        _no("%s is [..., columns]", name)
-    columns = x.shape[-1]
     if x.dim() == 2:
-        rows, stride = x.shape[0], x.stride(0)
-        if (x.stride(1) != 1 and columns > 1) or stride < 0:
+        rows, columns = x.shape
+        stride, one = x.stride()
+        if (one != 1 and columns > 1) or stride < 0:
             x, stride = x.contiguous(), columns
     else:
+        if not x.dim():
+            _no("%s is [..., columns]", name)
+        columns = x.shape[-1]
         x, stride = x.contiguous(), columns
         rows = x.numel() // columns if columns else 0
     if (rows | columns) >> 31:
@@ -322,12 +324,14 @@ def _rows_of(name, x):
 
 
 def _mx4(name, m, device=None):
-    """(device, rows, groups, bytes from row to row of codes and of scales) of the last two dimensions"""
+    """(device, groups) of an Mx4"""
     codes, scales, columns = m
     device = _cuda(name, codes, device)
     _cuda(name, scales, device)
     groups = -(-columns // 32)
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.dim() or codes.shape[-1] != 16 * groups or scales.shape[-1:] != (groups,) or codes.shape[:-1] != scales.shape[:-1]:
+    shape, scale_shape, n = codes.shape, scales.shape, codes.dim()
+    if codes.dtype is not _U8 or scales.dtype is not _U8 or not n or scales.dim() != n or shape[-1] != 16 * groups or scale_shape[-1] != groups or \
+            (shape[0] != scale_shape[0] if n == 2 else shape[:-1] != scale_shape[:-1]):
         _no("%s has uint8 codes [..., %d] and scales [..., %d] for %d columns", name, 16 * groups, groups, columns)
     if (codes.stride(-1) != 1 and groups) or (scales.stride(-1) != 1 and groups > 1):
         _no("%s: a row's bytes are to be neighbours", name)
@@ -337,13 +341,13 @@ def _mx4(name, m, device=None):
 def _mx4_rows(name, m):
     """The rows of an Mx4 as (device, codes [rows, ...], scales [rows, ...])."""
     device, groups = _mx4(name, m)
-    codes, scales = m.codes, m.scales
+    codes, scales, columns = m
     if codes.dim() != 2:
         codes, scales = codes.reshape(-1, 16 * groups) if groups else codes.new_empty(0, 0), scales.reshape(-1, groups) if groups else scales.new_empty(0, 0)
     if codes.stride(0) < 0 or scales.stride(0) < 0:
         codes, scales = codes.contiguous(), scales.contiguous()
-    if codes.shape[0] >> 31 or m.columns >> 31:
-        _no("%s: %d rows of %d are too many for one call", name, codes.shape[0], m.columns)
+    if (codes.shape[0] | columns) >> 31:
+        _no("%s: %d rows of %d are too many for one call", name, codes.shape[0], columns)
     return device, codes, scales
 
 
@@ -354,9 +358,13 @@ def mx4_quantize(x):
     kind = _TYPES.get(x.dtype)
     if kind is None:
         _no("x is float32, bfloat16 or float16")
-    groups, shape = -(-columns // 32), x.shape[:-1]
-    codes = torch.empty((*shape, 16 * groups), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*shape, groups), dtype=torch.uint8, device=x.device)
+    groups = -(-columns // 32)
+    if x.dim() == 2:          # (sizes as arguments: see token_logprobs)
+        codes = x2.new_empty(rows, 16 * groups, dtype=torch.uint8)
+        scales = codes.new_empty(rows, groups)
+    else:
+        codes = x2.new_empty((*x.shape[:-1], 16 * groups), dtype=torch.uint8)
+        scales = codes.new_empty((*x.shape[:-1], groups))
     if rows and columns:
         _call(device, lib(True).nb200_dev_mx4_quantize, _MX4_ROWS(codes.data_ptr(), scales.data_ptr(), 16 * groups, groups, x2.data_ptr(), stride, kind, rows, columns))
     return Mx4(codes, scales, columns)
@@ -368,9 +376,10 @@ def mx4_read(m, dtype=torch.float32):
     kind = _TYPES.get(dtype)
     if kind is None:
         _no("rows are float32, bfloat16 or float16")
-    out = torch.empty((*m.codes.shape[:-1], m.columns), dtype=dtype, device=codes.device)
-    if out.numel():
-        _call(device, lib(True).nb200_dev_mx4_read, _MX4_ROWS(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0), out.data_ptr(), m.columns, kind, codes.shape[0], m.columns))
+    rows, columns = codes.shape[0], m.columns
+    out = codes.new_empty(rows, columns, dtype=dtype) if m.codes.dim() == 2 else codes.new_empty((*m.codes.shape[:-1], columns), dtype=dtype)
+    if rows and columns:
+        _call(device, lib(True).nb200_dev_mx4_read, _MX4_ROWS(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0), out.data_ptr(), columns, kind, rows, columns))
     return out
 
 
@@ -381,24 +390,25 @@ def _product(x, w, offsets, dtype):
     if offsets is None:
         if wc.dim() != 2:
             _no("w is an Mx4 of [outputs, columns]")
-        w_expert = ws_expert = 0
+        outputs, w_expert, ws_expert, w_stride, ws_stride = wc.shape[0], 0, 0, wc.stride(0), ws.stride(0)
     else:
         if wc.dim() != 3 or not wc.shape[0]:
             _no("w is an Mx4 of [experts, outputs, columns]")
-        experts, w_expert, ws_expert = wc.shape[0], wc.stride(0), ws.stride(0)
+        experts, outputs, _ = wc.shape
+        w_expert, w_stride, _ = wc.stride()
+        ws_expert, ws_stride, _ = ws.stride()
         _cuda("offsets", offsets, device)
         if offsets.dim() != 1 or offsets.shape[0] != experts + 1 or offsets.dtype != torch.int32:
             _no("offsets are [experts + 1] of int32")
         offsets = offsets.contiguous()
-    outputs, w_stride, ws_stride = wc.shape[-2], wc.stride(-2), ws.stride(-2)
     if isinstance(x, Mx4):
         at, x2, xs = _mx4_rows("x", x)
-        shape, kind, rows, given = x.codes.shape[:-1], 3, x2.shape[0], x.columns
+        given_x, kind, rows, given = x.codes, 3, x2.shape[0], x.columns
         x_stride, xs_at, xs_stride = x2.stride(0), xs.data_ptr(), xs.stride(0)
         dtype = dtype or torch.bfloat16
     else:
         at, x2, rows, given, x_stride = _rows_of("x", x)
-        shape, kind, xs_at, xs_stride = x.shape[:-1], _TYPES.get(x.dtype), 0, 0
+        given_x, kind, xs_at, xs_stride = x, _TYPES.get(x.dtype), 0, 0
         if kind is None:
             _no("x is float32, bfloat16, float16 or an Mx4")
         dtype = dtype or x.dtype
@@ -406,14 +416,14 @@ def _product(x, w, offsets, dtype):
         _no("x is on another device")
     if given != columns:
         _no("x has %d columns, w %d", given, columns)
-    if offsets is not None and len(shape) != 1:
+    if offsets is not None and given_x.dim() != 2:
         _no("x is [rows, columns]")
     out_kind = _TYPES.get(dtype)
     if out_kind is None:
         _no("results are float32, bfloat16 or float16")
-    out = torch.empty((*shape, outputs), dtype=dtype, device=wc.device)
-    if not out.numel():
-        return out
+    out = x2.new_empty(rows, outputs, dtype=dtype) if given_x.dim() == 2 else x2.new_empty((*given_x.shape[:-1], outputs), dtype=dtype)
+    if not rows or not outputs:
+        return out.zero_() if out.numel() else out
     if not columns:
         return out.zero_()
     try:
@@ -422,15 +432,12 @@ def _product(x, w, offsets, dtype):
     except struct.error:
         _no("strides are not negative, counts numbers of 32 bits")
     L, need = lib(True), C.c_uint64()
-    _call(device, _product_room, L, p, need)
+    if L.nb200_dev_mx4_product_workspace(p, C.byref(need)):          # (sizes alone: no device is asked)
+        E._check(-1)
     need = need.value
-    room = wc.new_empty(need, dtype=torch.uint8) if need else None
+    room = wc.new_empty(need) if need else None
     _call(device, L.nb200_dev_mx4_product, p, room.data_ptr() if need else None, need)
     return out
-
-
-def _product_room(L, p, need, stream):
-    return L.nb200_dev_mx4_product_workspace(p, C.byref(need))
 
 
 def mx4_product(x, w, dtype=None):
@@ -459,9 +466,8 @@ def experts_sort(ids, experts):
     n = ids.numel()
     if n >> 31:
         _no("%d places are too many for one call", n)
-    order = torch.empty(n, dtype=torch.int32, device=ids.device)
     place = torch.empty_like(ids, dtype=torch.int32)
-    offsets = order.new_empty(experts + 1)
+    order, offsets = place.new_empty(n), place.new_empty(experts + 1)
     _call(device, lib(True).nb200_dev_experts_sort, order.data_ptr(), offsets.data_ptr(), place.data_ptr(), ids.data_ptr(), ids.element_size(), n, experts)
     return Routing(order, offsets, place)
 
@@ -471,11 +477,12 @@ def _routing(routing, device):
     order, _, place = routing
     _cuda("order", order, device)
     _cuda("place", place, device)
-    if order.dim() != 1 or order.dtype != torch.int32 or place.dtype != torch.int32 or place.dim() not in (1, 2) or place.numel() != order.shape[0]:
+    shape, n = place.shape, order.shape[0] if order.dim() == 1 else -1
+    if order.dtype is not torch.int32 or place.dtype is not torch.int32 or len(shape) not in (1, 2) or place.numel() != n:
         _no("a routing has order [tokens * top] and place [tokens, top] of int32")
-    if order.shape[0] >> 31:
-        _no("%d places are too many for one call", order.shape[0])
-    return order.contiguous(), place.contiguous(), place.shape[0], place.shape[1] if place.dim() == 2 else 1
+    if n >> 31:
+        _no("%d places are too many for one call", n)
+    return order if order.is_contiguous() else order.contiguous(), place if place.is_contiguous() else place.contiguous(), shape[0], shape[1] if len(shape) == 2 else 1
 
 
 def _gather(x, order, tokens, top):
@@ -564,7 +571,8 @@ def experts_combine(y, routing, weights=None):
         _cuda("weights", weights, device)
         if weights.shape != routing.place.shape or not weights.is_floating_point():
             _no("weights are [tokens, top] of numbers")
-        weights = weights.float().contiguous()
+        if weights.dtype is not torch.float32 or not weights.is_contiguous():
+            weights = weights.float().contiguous()
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         return _Combine.apply(y, weights, order, place, tokens, top)
     return _combine(y, place, weights, tokens, top)
