@@ -48,8 +48,8 @@ UNITS = {
     "ops.cu": ["ops.h", "pairs.cuh", "portions.h", "family.h", "../../include/nano_b200.h"],
     "kv4.cu": ["kv4.cuh", "kv4.h", "ops.h", "portions.h", "family.h", "../../include/nano_b200.h"],
     "kv4_tc.cu": ["kv4.cuh", "kv4.h", "ops.h", "pairs.cuh", "tc_ptx.cuh", "family.h"],
-    "mx4.cu": ["mx4.h", "ops.h", "portions.h", "rows.cuh", "family.h", "../../include/nano_b200.h"],
-    "mx4_tc.cu": ["mx4.h", "ops.h", "tc_ptx.cuh", "family.h"],
+    "mx4.cu": ["mx4.cuh", "mx4.h", "ops.h", "portions.h", "rows.cuh", "family.h", "../../include/nano_b200.h"],
+    "mx4_tc.cu": ["mx4.cuh", "mx4.h", "rows.cuh", "ops.h", "tc_ptx.cuh", "family.h"],
     "experts.cu": ["ops.h", "portions.h", "rows.cuh", "family.h", "../../include/nano_b200.h"],
     "sample.cu": ["kernels.cuh", "expf_ref.cuh", "sample_host.h"],
 }

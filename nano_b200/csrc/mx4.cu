@@ -6,26 +6,13 @@
 #include <algorithm>
 
 #include "family.h"
+#include "mx4.cuh"
 #include "mx4.h"
 #include "portions.h"
 #include "rows.cuh"
 
 namespace nb {
 namespace {
-
-// two numbers to two codes, the first in the lower four bits: nearest, ties to even, beyond 6 (NaN too) to 6
-__device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
-    uint32_t r;
-    asm("{\n.reg .b8 c;\ncvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\ncvt.u32.u8 %0, c;\n}" : "=r"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-// what two codes stand for, as fp16: exact
-__device__ __forceinline__ __half2 numbers_of(uint32_t byte) {
-    uint32_t r;
-    asm("{\n.reg .b8 c;\ncvt.u8.u32 c, %1;\ncvt.rn.f16x2.e2m1x2 %0, c;\n}" : "=r"(r) : "r"(byte));
-    return *reinterpret_cast<__half2 *>(&r);
-}
-__device__ __forceinline__ float scale_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fc00000u) : e == 0u ? __uint_as_float(1u << 22) : __uint_as_float(e << 23); }
 
 // ------------------------------------------------------------------------------------------------
 // Quantisation.  A thread has 32 bytes of a group (a quarter of its fp32 numbers, half of its 16-bit ones): the largest magnitude's bits by one or two exchanges; of a number 2^(f - 127) m,
@@ -57,8 +44,8 @@ __device__ __forceinline__ void quantise(const Mx4Rows &a, uint32_t per_row, uin
     for (uint32_t j = 0; j < P; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);          // (NaN above infinity above all others)
 #pragma unroll
     for (uint32_t s = 1; s < SHARE; s *= 2u) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
-    const uint32_t f = top >> 23, e = f == 255u ? 255u : f > 2u ? f - 2u : 0u;
-    const float by = __uint_as_float((254u - min(e, 252u)) << 23);          // 2^(127 - e)
+    const uint32_t e = scale_byte(top);
+    const float by = inverse_of(e);
     uint32_t w[P / 8] = {};
 #pragma unroll
     for (uint32_t j = 0; j < P / 2; j++) w[j / 4] |= codes_of(x[2 * j] * by, x[2 * j + 1] * by) << (8u * (j % 4u));

@@ -22,6 +22,7 @@ cudaError_t mx4_read_launch(const Mx4Rows &a, cudaStream_t stream);
 // How a product is run: by sizes, types and alignment alone
 struct Mx4Plan {
     uint32_t tn, ks, per, pairs;          // rows of X in a tile; blocks that share a tile's depth (0: the kernel for many tiles); steps to each; tiles of rows, over all experts at most
+    bool raw;          // the product reads numbers and quantises them itself: nothing is made before it
     bool x_codes, x_scales, w_scales, x_second;          // what a kernel makes before: codes of x, its scales (in the second order?) and those of w in the second order
     uint64_t x_scales_at, w_scales_at, bytes;          // in the workspace; codes come first
 };

@@ -10,9 +10,12 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "family.h"
+#include "mx4.cuh"
 #include "mx4.h"
+#include "rows.cuh"
 #include "tc_ptx.cuh"
 
 namespace nb {
@@ -153,11 +156,78 @@ __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles,
     return bring_scales<TN, 1, 1>(r, tiles, s0, ns, next);
 }
 
+// Rows of X that are numbers, up to 16 of them: the same four warps quantise all that their block needs of them while W's first stages are on their way, a group to a thread, into swizzled rows as a
+// bulk copy would leave them.  Every block of a tile does so for itself: a launch and a wait less than quantising first.
+struct RawRows { const void *x; uint64_t stride; uint32_t r0, live, columns; };
+constexpr uint32_t kRawSteps = 10, kRawStep = 16u * 128u, kRawScales = 16u * kStageGroups;          // steps of the depth that a block has room for; bytes of codes and of scales of one
+template <typename T>
+__device__ __forceinline__ void quantise_rows(const RawRows &x, uint32_t s0, uint32_t ns, uint32_t codes, uint32_t scales) {
+    const uint32_t tid = threadIdx.x & (kScaleThreads - 1u), per_row = ns * kStageGroups;
+    for (uint32_t i = tid; i < x.live * per_row; i += kScaleThreads) {
+        const uint32_t row = i / per_row, g = i - row * per_row, step = g / kStageGroups, c = g % kStageGroups, k = (s0 * kStageGroups + g) * kMx4Group;
+        const T *first = static_cast<const T *>(x.x) + (uint64_t)(x.r0 + row) * x.stride;
+        float v[kMx4Group];
+        if ((reinterpret_cast<uintptr_t>(first) & 15u) == 0 && k + kMx4Group <= x.columns) load_row<EVEN>(first, x.columns, (int)k, v);
+        else load_row<ANY>(first, x.columns, (int)k, v);
+        uint32_t tops[4] = {};
+#pragma unroll
+        for (uint32_t j = 0; j < kMx4Group; j++) tops[j % 4u] = max(tops[j % 4u], __float_as_uint(v[j]) & 0x7fffffffu);
+        const uint32_t e = scale_byte(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+        const float by = inverse_of(e);
+        uint32_t w[4] = {};
+#pragma unroll
+        for (uint32_t j = 0; j < kMx4Group / 2; j++) w[j / 4] |= codes_of(v[2 * j] * by, v[2 * j + 1] * by) << (8u * (j % 4u));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(codes + step * kRawStep + row * 128u + ((c ^ (row & 7u)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + step * kRawScales + row * kStageGroups + c), "r"(e) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // plain stores, read by the tensor core
+}
+// (codes of a group that is NaN may be anything: its scale makes every product NaN, and rows behind the last have no results)
+template <int WU>
+__device__ __forceinline__ bool bring_w_scales(const ScaleRing &r, const ScaleRows &w, uint32_t x_scales, uint32_t s0, uint32_t ns) {
+    using Z = Tile<16>;
+    const uint32_t tid = threadIdx.x & (kScaleThreads - 1u), warp = tid >> 5, lane = tid & 31u;
+    const uint8_t *w_row = w.base + (tid < w.live ? tid : 0u) * w.stride;
+    uint4 v[2];
+    auto ask = [&](uint32_t i, uint4 &to) { const uint32_t step = s0 + i; if (i < ns) to = scales16<WU>(w_row + (step >> 1) * r.w_step + (step & 1u) * 8u, step * kStageGroups, r.groups); };
+    ask(0, v[0]); ask(2, v[1]);
+    bool ok = true;
+    uint32_t st = 0, turn = 0;
+    for (uint32_t i0 = 0; i0 < ns; i0 += 4u)
+#pragma unroll
+        for (uint32_t d = 0; d < 2; d++) {
+            const uint32_t i = i0 + 2u * d, at = r.staged + d * kRows * 16u;
+            if (i >= ns) return ok;
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + tid * 8u), "r"(v[d].x), "r"(v[d].y) : "memory");
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + kRows * 8u + tid * 8u), "r"(v[d].z), "r"(v[d].w) : "memory");
+            ok = ok && (!turn || soon_warp(r.empty + st * 8u, (turn - 1u) & 1u));
+            if (bar_any(kScaleBar, kScaleThreads, !ok)) return false;
+            ask(i + 4u, v[d]);
+            for (uint32_t h = 0; h < min(2u, ns - i); h++) {
+                if (h && turn) { ok = soon_warp(r.empty + st * 8u, (turn - 1u) & 1u); if (!ok) break; }
+                tc_fence_after();
+                uint32_t wv[8], xv[8] = {};
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wv[j]), "=r"(wv[4 + j]) : "r"(at + h * kRows * 8u + (j * 32u + lane) * 8u) : "memory");
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(xv[0]), "=r"(xv[4]) : "r"(x_scales + (i + h) * kRawScales + (lane & 15u) * 8u) : "memory");
+                const uint32_t to = r.tmem + ((warp * 32u) << 16) + st * Z::scale_cols;
+                tc_st8(to, wv);
+                tc_st8(to + 8u, xv);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(r.full + st * 8u);
+                if (++st == r.stages) { st = 0; turn++; }
+            }
+        }
+    return ok;
+}
+
 // a stage's products
 template <int TN>
-__device__ __forceinline__ void stage_products(uint32_t at, uint32_t d, uint32_t scales, bool first) {
+__device__ __forceinline__ void stage_products(uint32_t w_at, uint32_t x_at, uint32_t d, uint32_t scales, bool first) {
     using Z = Tile<TN>;
-    const uint64_t wd = tc_desc(at), xd = tc_desc(at + Z::x_at);
+    const uint64_t wd = tc_desc(w_at), xd = tc_desc(x_at);
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++)
         mma_mx4(d, wd + 2u * k, xd + 2u * k, idesc_of(TN, (k & 1u) * 2u), scales + (k >> 1) * 4u, scales + 8u + (k >> 1) * Z::blocks * 4u, !first || k > 0);
@@ -236,20 +306,23 @@ __device__ __forceinline__ void finish_parts(const Mx4Product &p, uint32_t at, u
 // ------------------------------------------------------------------------------------------------
 template <int TN> struct Few {
     static constexpr uint32_t stages = TN <= 32 ? 5 : TN <= 64 ? 4 : 3, cols = cols_for(Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols);          // up to 107 KB: two blocks to an SM
-    static constexpr uint32_t smem = stages * Tile<TN>::bytes + 1024u;
+    // codes that bulk copies read come with W's stage by stage; numbers are quantised to a place of their own
+    static __host__ __device__ constexpr uint32_t stage(uint32_t x) { return x == T_MX4 ? Tile<TN>::bytes : Tile<TN>::x_at; }
+    static __host__ __device__ constexpr uint32_t smem(uint32_t x) { return stages * stage(x) + (x == T_MX4 ? 0u : kRawSteps * kRawStep) + 1024u; }
 };
-template <int TN>
+// X: what the rows of X are, codes that bulk copies read or numbers
+template <int TN, uint32_t X>
 __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs t) {
     using Z = Tile<TN>;
-    constexpr uint32_t ST = Few<TN>::stages;
+    constexpr uint32_t ST = Few<TN>::stages, SB = Few<TN>::stage(X);
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 1];
-    __shared__ __align__(16) uint8_t staged[2 * Z::staged];
+    __shared__ __align__(16) uint8_t staged[X == T_MX4 ? 2u * Z::staged : 2u * kRows * 16u + kRawSteps * kRawScales];
     __shared__ uint32_t tmem_s, bad_s;
     __shared__ Span span_s;
     const Mx4Product &p = t.p;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, part = blockIdx.z, n0 = blockIdx.x % t.wtiles * kRows, pair = blockIdx.x / t.wtiles;
-    const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u, full = smem_u32(bars), empty = full + ST * 8u, done = full + 2u * ST * 8u;
+    const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u, full = smem_u32(bars), empty = full + ST * 8u, done = full + 2u * ST * 8u, raw_at = ring + ST * SB;
     const uint32_t s0 = min(t.steps, part * t.per), ns = min(t.steps, s0 + t.per) - s0;
     Span span{0u, pair * TN, min(pair * TN + TN, p.rows)};
     if (p.offsets) {
@@ -267,10 +340,10 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     }
     auto weights = [&](uint32_t i) {
         const uint32_t st = i % ST;
-        mbar_expect(full + st * 8u, Z::bytes);
-        tma_3d(ring + st * Z::bytes, &t.wmap, (s0 + i) * (kDepth / 2u), n0, span.e, full + st * 8u);
+        mbar_expect(full + st * 8u, SB);
+        tma_3d(ring + st * SB, &t.wmap, (s0 + i) * (kDepth / 2u), n0, span.e, full + st * 8u);
     };
-    const uint32_t npre = min(ST, ns);
+    const uint32_t npre = min(ST, ns), rows = span.r1 - span.r0;
     if (threadIdx.x == 128u) {
         bad_s = 0;
         for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, 5); mbar_init(empty + i * 8u, 1); }
@@ -292,7 +365,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
                     if (!soon(empty + st * 8u, ((i / ST) - 1u) & 1u)) { bad_s = 1; break; }
                     weights(i);
                 }
-                tma_3d(ring + st * Z::bytes + Z::x_at, &t.xmap, (s0 + i) * (kDepth / 2u), span.r0, 0, full + st * 8u);
+                if (X == T_MX4) tma_3d(ring + st * SB + Z::x_at, &t.xmap, (s0 + i) * (kDepth / 2u), span.r0, 0, full + st * 8u);
             }
         }
     } else if (warp == 5) {
@@ -303,7 +376,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
                 ok = soon(full + st * 8u, (i / ST) & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                stage_products<TN>(ring + st * Z::bytes, tmem, scales_at + st * Z::scale_cols, i == 0);
+                stage_products<TN>(ring + st * SB, X == T_MX4 ? ring + st * SB + Z::x_at : raw_at + i * kRawStep, tmem, scales_at + st * Z::scale_cols, i == 0);
                 tc_commit(empty + st * 8u);
             }
             if (ok) tc_commit(done); else bad_s = 1;          // (the waits on it run out too)
@@ -311,13 +384,19 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     } else {
         pdl_wait();
         const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_step, t.x_step, t.w_unit, t.x_unit};
-        if (!bring_scales<TN>(r, 1, s0, ns, [&](ScaleRows &w, ScaleRows &x) {
-                w = ScaleRows{p.ws + span.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
-                x = ScaleRows{p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0};
-            })) bad_s = 1;
+        const ScaleRows w_rows{p.ws + span.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
+        bool brought;
+        if constexpr (X == T_MX4) brought = bring_scales<TN>(r, 1, s0, ns, [&](ScaleRows &w, ScaleRows &x) { w = w_rows; x = ScaleRows{p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0}; });
+        else {
+            typedef std::conditional_t<X == T_F32, float, std::conditional_t<X == T_BF16, __nv_bfloat16, __half>> T;
+            const uint32_t x_scales = r.staged + 2u * kRows * 16u;
+            quantise_rows<T>(RawRows{p.x, p.x_stride, span.r0, rows, p.columns}, s0, ns, raw_at, x_scales);
+            brought = r.w_unit >= 8u ? bring_w_scales<8>(r, w_rows, x_scales, s0, ns) : r.w_unit >= 4u ? bring_w_scales<4>(r, w_rows, x_scales, s0, ns) : bring_w_scales<1>(r, w_rows, x_scales, s0, ns);
+        }
+        if (!brought) bad_s = 1;
     }
     __syncwarp();
-    const uint32_t quad = warp & 3u, n = n0 + quad * 32u + lane, rows = span.r1 - span.r0;
+    const uint32_t quad = warp & 3u, n = n0 + quad * 32u + lane;
     bool ok = true;
     if (warp < 4) { ok = ns == 0 || soon_warp(done, 0); tc_fence_after(); if (!ok) bad_s = 1; }
     float *mine = reinterpret_cast<float *>(raw + (ring - smem_u32(raw))) + quad * 32u + lane;          // partial tiles, [TN][128], where the stages were
@@ -445,7 +524,7 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
                     ok = soon(full + st * 8u, phase);
                     if (!ok) break;
                     tc_fence_after();
-                    stage_products<TN>(ring + st * Z::bytes, tmem + set * Z::sum_cols, scales_at + st * Z::scale_cols, i == 0);
+                    stage_products<TN>(ring + st * Z::bytes, ring + st * Z::bytes + Z::x_at, tmem + set * Z::sum_cols, scales_at + st * Z::scale_cols, i == 0);
                     tc_commit(empty + st * 8u);
                     if (++st == ST) { st = 0; phase ^= 1u; }
                 }
@@ -565,12 +644,12 @@ uint32_t unit_of(const void *base, uint64_t stride, uint64_t expert, uint64_t st
 constexpr uint32_t kSms = 148;
 
 // ks 0: the kernel for many tiles
-template <int TN>
+template <int TN, uint32_t X>
 cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
     static std::atomic<uint64_t> asked[2];          // devices (of the first 64) whose shared-memory limit has been raised
-    const bool many = t.ks == 0;
-    void (*const kernel)(TcArgs) = many ? k_mx4_many<TN> : TN <= 128 ? k_mx4_few<TN <= 128 ? TN : 128> : nullptr;
-    const uint32_t smem = many ? Many<TN>::smem : Few<TN <= 128 ? TN : 128>::smem;
+    const bool many = X == T_MX4 && t.ks == 0;
+    void (*const kernel)(TcArgs) = many ? k_mx4_many<TN> : TN <= 128 ? k_mx4_few<TN <= 128 ? TN : 128, X> : nullptr;
+    const uint32_t smem = many ? Many<TN>::smem : Few<TN <= 128 ? TN : 128>::smem(X);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev > 63 || !(asked[many].load(std::memory_order_acquire) >> dev & 1u))) {
@@ -578,7 +657,7 @@ cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
         if (e == cudaSuccess && dev <= 63) asked[many].fetch_or(1ull << dev, std::memory_order_release);
     }
     if (e != cudaSuccess) return e;
-    if (!map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, TN) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
+    if ((X == T_MX4 && !map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, TN)) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
         return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(many ? Many<TN>::threads : 192u); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
@@ -626,6 +705,10 @@ Mx4Plan mx4_plan(const Mx4Product &a) {
     r.per = (steps + std::max(1u, r.ks) - 1u) / std::max(1u, r.ks);
     r.x_second = r.ks <= 1u || r.per % 2u == 0;          // (two steps of the depth are sixteen scales)
     const bool codes = a.x_type == T_MX4;
+    // Numbers are quantised by the product itself where a block has few of them (64 rows x steps: four groups to a thread).  us, so / by a kernel before: 1 x 9728 x 2560 7.9 / 8.6, 16 12.4 / 9.2,
+    // 1 x 4096 x 4096 7.3 / 8.5; and a launch less of the host's time, 10.9 / 14.7 a call
+    const uint32_t mine = std::min(16u, a.experts ? std::min(a.rows, 4u * each) : a.rows);
+    if (!codes && r.tn == 16u && r.ks && r.per <= kRawSteps && mine * r.per <= 64u) { r.raw = true; return r; }
     r.x_codes = !codes || a.columns % 2u;
     r.w_scales = r.tn == 256u && (uint64_t)r.pairs >= 4u * (uint64_t)std::max(1u, a.experts);
     r.x_scales = r.x_codes || (codes && r.tn == 256u);
@@ -641,13 +724,17 @@ cudaError_t mx4_tc_launch(const Mx4Product &a, const Mx4Plan &plan, uint64_t xs_
     t.pairs = plan.pairs; t.ks = plan.ks; t.per = plan.per;
     const bool odd = t.ks > 1 && t.per % 2u;
     t.w_step = ws_step; t.x_step = xs_step;
+    if (plan.raw) {
+        t.w_unit = unit_of(a.ws, a.ws_stride, a.ws_expert, ws_step, t.groups, odd);
+        return a.x_type == T_F32 ? launch_of<16, T_F32>(t, stream) : a.x_type == T_BF16 ? launch_of<16, T_BF16>(t, stream) : launch_of<16, T_F16>(t, stream);
+    }
     t.w_unit = unit_of(a.ws, a.ws_stride, a.ws_expert, ws_step, t.groups, odd); t.x_unit = unit_of(a.xs, a.xs_stride, 0, xs_step, t.groups, odd);
     switch (plan.tn) {
-        case 16: return launch_of<16>(t, stream);
-        case 32: return launch_of<32>(t, stream);
-        case 64: return launch_of<64>(t, stream);
-        case 128: return launch_of<128>(t, stream);
-        default: return launch_of<256>(t, stream);
+        case 16: return launch_of<16, T_MX4>(t, stream);
+        case 32: return launch_of<32, T_MX4>(t, stream);
+        case 64: return launch_of<64, T_MX4>(t, stream);
+        case 128: return launch_of<128, T_MX4>(t, stream);
+        default: return launch_of<256, T_MX4>(t, stream);
     }
 }
 

@@ -506,16 +506,22 @@ def _combine(y, place, weights, tokens, top):
     return out
 
 
+def _once(grad):
+    """No gradient of a gradient (torch's once_differentiable, without its microseconds)."""
+    if grad.requires_grad and torch.is_grad_enabled():
+        _no("the operators of experts have no gradients of gradients")
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order, place, tokens, top):
-        ctx.save_for_backward(place)
+        ctx.save_for_backward(place)          # (so that a routing changed in between is noticed)
         ctx.sizes = tokens, top
         return _gather(x, order, tokens, top)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _once(grad)
         return _combine(grad, ctx.saved_tensors[0], None, *ctx.sizes), None, None, None, None
 
 
@@ -527,8 +533,8 @@ class _Combine(torch.autograd.Function):
         return _combine(y, place, weights, tokens, top)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _once(grad)
         y, weights, order, place = ctx.saved_tensors
         tokens, top = ctx.sizes
         device, grad, _, columns, grad_stride = _rows_of("the gradient", grad)
