@@ -24,7 +24,7 @@ namespace {
 constexpr uint32_t kRows = 128, kDepth = 256, kStageGroups = kDepth / kMx4Group, kMostExperts = 1024;          // rows of W in a tile; columns of a stage
 template <int TN> struct Tile {
     static constexpr uint32_t blocks = (TN + 127) / 128;          // of 128 rows, as tensor memory holds scales: row r's word in lane r % 32, column r / 32
-    static constexpr uint32_t x_at = kRows * 128u, bytes = x_at + TN * 128u;          // of a stage
+    static constexpr uint32_t x_at = kRows * 128u;          // in a stage
     static constexpr uint32_t scale_cols = 8u + 8u * blocks, sum_cols = TN < 32 ? 32 : TN;          // of tensor memory
     static constexpr uint32_t staged = (kRows + 128u * blocks) * 16u;          // two stages' scales, sixteen to a row, on their way
 };
@@ -36,13 +36,19 @@ __device__ __forceinline__ bool soon(uint32_t bar, uint32_t parity) { return mba
 __device__ __forceinline__ bool soon_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, soon(bar, parity)); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// d (+)= a b^T: 64 columns of 128 rows of codes and of the instruction's N, each with its two scales
+// d (+)= a b^T: 64 columns of 128 rows of codes and of the instruction's N, each with its two scales.  PAIR: two blocks' 128 rows each, and half of the N rows in each block's shared memory; sums and
+// scales of a block's rows, and those of all N, are in its own tensor memory
+template <bool PAIR>
 __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %6, 0;\ntcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add) : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %6, 0;\ntcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %6, 0;\ntcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add) : "memory");
 }
 // e2m1 x e2m1, scales in 8 bits of exponent, N columns; scales from byte `id` (0 or 2) of their words
-__host__ __device__ constexpr uint32_t idesc_of(uint32_t n, uint32_t id) { return (id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((kRows >> 4) << 24) | (id << 29); }
+__host__ __device__ constexpr uint32_t idesc_of(uint32_t m, uint32_t n, uint32_t id) { return (id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (id << 29); }
 
 // Sixteen neighbouring scales of a row, from group g (a multiple of 16, or of 8 for UNIT 8) on; zeros behind its last.  UNIT: bytes that one load may bring, for every row and every g
 template <int UNIT>
@@ -75,9 +81,14 @@ constexpr uint32_t kAhead = 2, kScaleThreads = 128, kScaleBar = 1;
 __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
+__device__ __forceinline__ void arrive_at(uint32_t bar, uint32_t rank) {          // at the same barrier of block `rank`
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(bar), "r"(rank));
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
+}
 struct ScaleRows { const uint8_t *base; uint64_t stride; uint32_t live; };          // rows [0, live); what lies behind them counts for nothing
 struct ScaleRing { uint32_t staged, tmem, stages, full, empty, groups; uint64_t w_step, x_step; uint32_t w_unit, x_unit; };
-template <int TN, int WU, int XU, typename F>
+template <int TN, bool PAIR, int WU, int XU, typename F>
 __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles, uint32_t s0, uint32_t ns, F &next) {
     using Z = Tile<TN>;
     constexpr uint32_t XR = Z::blocks;          // rows of X to a thread
@@ -136,7 +147,7 @@ __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles,
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(r.full + st * 8u);
+                if (lane == 0) { if constexpr (PAIR) arrive_at(r.full + st * 8u, 0); else mbar_arrive(r.full + st * 8u); }
                 if (++st == r.stages) { st = 0; turn++; }
             }
             done = done + count == ns ? 0u : done + count;
@@ -144,16 +155,16 @@ __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles,
     return ok;
 }
 // next(w, x) names the rows of the next of `tiles` tiles, of which steps [s0, s0 + ns) of the depth are wanted
-template <int TN, typename F>
+template <int TN, bool PAIR, typename F>
 __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles, uint32_t s0, uint32_t ns, F next) {
     if (r.x_unit == 16u) {
-        if (r.w_unit == 16u) return bring_scales<TN, 16, 16>(r, tiles, s0, ns, next);
-        if (r.w_unit >= 4u) return bring_scales<TN, 4, 16>(r, tiles, s0, ns, next);
-        return bring_scales<TN, 1, 16>(r, tiles, s0, ns, next);
+        if (r.w_unit == 16u) return bring_scales<TN, PAIR, 16, 16>(r, tiles, s0, ns, next);
+        if (r.w_unit >= 4u) return bring_scales<TN, PAIR, 4, 16>(r, tiles, s0, ns, next);
+        return bring_scales<TN, PAIR, 1, 16>(r, tiles, s0, ns, next);
     }
-    if (r.w_unit >= 8u && r.x_unit >= 8u) return bring_scales<TN, 8, 8>(r, tiles, s0, ns, next);
-    if (r.w_unit >= 4u && r.x_unit >= 4u) return bring_scales<TN, 4, 4>(r, tiles, s0, ns, next);
-    return bring_scales<TN, 1, 1>(r, tiles, s0, ns, next);
+    if (r.w_unit >= 8u && r.x_unit >= 8u) return bring_scales<TN, PAIR, 8, 8>(r, tiles, s0, ns, next);
+    if (r.w_unit >= 4u && r.x_unit >= 4u) return bring_scales<TN, PAIR, 4, 4>(r, tiles, s0, ns, next);
+    return bring_scales<TN, PAIR, 1, 1>(r, tiles, s0, ns, next);
 }
 
 // Rows of X that are numbers, up to 16 of them: the same four warps quantise all that their block needs of them while W's first stages are on their way, a group to a thread, into swizzled rows as a
@@ -224,13 +235,13 @@ __device__ __forceinline__ bool bring_w_scales(const ScaleRing &r, const ScaleRo
 }
 
 // a stage's products
-template <int TN>
+template <int TN, bool PAIR = false>
 __device__ __forceinline__ void stage_products(uint32_t w_at, uint32_t x_at, uint32_t d, uint32_t scales, bool first) {
     using Z = Tile<TN>;
     const uint64_t wd = tc_desc(w_at), xd = tc_desc(x_at);
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++)
-        mma_mx4(d, wd + 2u * k, xd + 2u * k, idesc_of(TN, (k & 1u) * 2u), scales + (k >> 1) * 4u, scales + 8u + (k >> 1) * Z::blocks * 4u, !first || k > 0);
+        mma_mx4<PAIR>(d, wd + 2u * k, xd + 2u * k, idesc_of(PAIR ? 2u * kRows : kRows, TN, (k & 1u) * 2u), scales + (k >> 1) * 4u, scales + 8u + (k >> 1) * Z::blocks * 4u, !first || k > 0);
 }
 
 __device__ __forceinline__ uint32_t clamp_row(int32_t o, uint32_t rows) { return o < 0 ? 0u : min((uint32_t)o, rows); }
@@ -307,7 +318,7 @@ __device__ __forceinline__ void finish_parts(const Mx4Product &p, uint32_t at, u
 template <int TN> struct Few {
     static constexpr uint32_t stages = TN <= 32 ? 5 : TN <= 64 ? 4 : 3, cols = cols_for(Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols);          // up to 107 KB: two blocks to an SM
     // codes that bulk copies read come with W's stage by stage; numbers are quantised to a place of their own
-    static __host__ __device__ constexpr uint32_t stage(uint32_t x) { return x == T_MX4 ? Tile<TN>::bytes : Tile<TN>::x_at; }
+    static __host__ __device__ constexpr uint32_t stage(uint32_t x) { return (kRows + (x == T_MX4 ? TN : 0u)) * 128u; }
     static __host__ __device__ constexpr uint32_t smem(uint32_t x) { return stages * stage(x) + (x == T_MX4 ? 0u : kRawSteps * kRawStep) + 1024u; }
 };
 // X: what the rows of X are, codes that bulk copies read or numbers
@@ -386,7 +397,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
         const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_step, t.x_step, t.w_unit, t.x_unit};
         const ScaleRows w_rows{p.ws + span.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
         bool brought;
-        if constexpr (X == T_MX4) brought = bring_scales<TN>(r, 1, s0, ns, [&](ScaleRows &w, ScaleRows &x) { w = w_rows; x = ScaleRows{p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0}; });
+        if constexpr (X == T_MX4) brought = bring_scales<TN, false>(r, 1, s0, ns, [&](ScaleRows &w, ScaleRows &x) { w = w_rows; x = ScaleRows{p.xs + (uint64_t)span.r0 * p.xs_stride, p.xs_stride, span.r1 - span.r0}; });
         else {
             typedef std::conditional_t<X == T_F32, float, std::conditional_t<X == T_BF16, __nv_bfloat16, __half>> T;
             const uint32_t x_scales = r.staged + 2u * kRows * 16u;
@@ -437,30 +448,49 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
 // Many tiles: a block to each SM takes tiles in turn.  Codes and scales run ahead of the products over the tiles' borders, and a tile's results are written while the next one's products run: in
 // another set of columns of tensor memory (tiles of up to 128 rows of X), or, of 256, after the sums have been read out at once, 128 columns to a thread.
 // ------------------------------------------------------------------------------------------------
-template <int TN> struct Many {
-    static constexpr uint32_t stages = TN <= 16 ? 11 : TN <= 32 ? 10 : TN <= 64 ? 8 : TN <= 128 ? 6 : 4, sets = TN <= 128 ? 2 : 1, drain = TN <= 32 ? 4 : 8, columns = TN / (drain / 4);          // (columns of a thread)
+// PAIR: two blocks of a cluster share tiles of 256 x TN, 128 rows of W and half of the rows of X to each: a block's shared memory takes in and gives out two thirds of the bytes, and so does L2
+// (8192 x 8192 x 8192 225 us, 4.9 PFLOP/s, instead of 244 with a block to a tile of 128 x 256; 8192 x 9728 x 2560 103 instead of 106).  The
+// first block issues the products of both; all copies and scales count on its barriers.
+template <int TN, bool PAIR> struct Many {
+    static constexpr uint32_t stages = PAIR ? 6 : TN <= 16 ? 11 : TN <= 32 ? 10 : TN <= 64 ? 8 : TN <= 128 ? 6 : 4, sets = TN <= 128 ? 2 : 1, drain = TN <= 32 ? 4 : 8, columns = TN / (drain / 4);          // (columns of a thread)
     static constexpr uint32_t tma = 4 + drain, mma = 5 + drain;          // warps 0-3: scales, then those that write results, then one each
-    static constexpr uint32_t cols = cols_for(sets * Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols), threads = 32u * (drain + 6u), smem = stages * Tile<TN>::bytes + 1024u;
+    static constexpr uint32_t x_rows = PAIR ? TN / 2 : TN, bytes = (kRows + x_rows) * 128u;          // of a stage
+    static constexpr uint32_t cols = cols_for(sets * Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols), threads = 32u * (drain + 6u), smem = stages * bytes + 1024u;
 };
-template <int TN>
-__global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_constant__ TcArgs t) {
+// a bulk copy to this block's memory that counts on the first block's barrier
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(bar), "r"(0));
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(there) : "memory");
+}
+__device__ __forceinline__ void commit_both(uint32_t bar) {          // to the barrier of both blocks
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+template <int TN, bool PAIR>
+__global__ void __launch_bounds__(Many<TN, PAIR>::threads, 1) k_mx4_many(const __grid_constant__ TcArgs t) {
     using Z = Tile<TN>;
-    using Y = Many<TN>;
-    constexpr uint32_t ST = Y::stages, SETS = Y::sets;
+    using Y = Many<TN, PAIR>;
+    constexpr uint32_t ST = Y::stages, SETS = Y::sets, SB = Y::bytes, WIDE = PAIR ? 2u * kRows : kRows;          // WIDE: rows of W in a tile
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 2 * SETS];
     __shared__ __align__(16) uint8_t staged[2 * Z::staged];
     __shared__ uint32_t tmem_s, bad_s, pairs_s[kMostExperts + 1];          // of (expert, TN rows): those before an expert's
     const Mx4Product &p = t.p;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = PAIR ? blockIdx.x & 1u : 0u, first_tile = PAIR ? blockIdx.x / 2u : blockIdx.x, stride = PAIR ? gridDim.x / 2u : gridDim.x;
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u, full = smem_u32(bars), empty = full + ST * 8u, sums = full + 2u * ST * 8u, room = sums + SETS * 8u;
     if (threadIdx.x == 0) {
         bad_s = 0;
-        for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, 5); mbar_init(empty + i * 8u, 1); }
-        for (uint32_t i = 0; i < SETS; i++) { mbar_init(sums + i * 8u, 1); mbar_init(room + i * 8u, Y::drain); }
+        for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, PAIR ? 9 : 5); mbar_init(empty + i * 8u, 1); }
+        for (uint32_t i = 0; i < SETS; i++) { mbar_init(sums + i * 8u, 1); mbar_init(room + i * 8u, PAIR ? 2u * Y::drain : Y::drain); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == Y::mma) { tc_alloc(smem_u32(&tmem_s), Y::cols); tc_relinquish(); }
+    if (warp == Y::mma) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(Y::cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else { tc_alloc(smem_u32(&tmem_s), Y::cols); tc_relinquish(); }
+    }
     if (p.offsets && warp == Y::tma) {
         uint32_t run = 0;
         for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
@@ -475,9 +505,10 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();          // both blocks' barriers are there
     tc_fence_after();
     const uint32_t tmem = tmem_s, scales_at = tmem + SETS * Z::sum_cols, ns = t.steps;
-    const uint64_t tiles = (uint64_t)t.wtiles * (p.offsets ? pairs_s[p.experts] : t.pairs), mine = tiles > blockIdx.x ? (tiles - 1u - blockIdx.x) / gridDim.x + 1u : 0u;
+    const uint64_t tiles = (uint64_t)t.wtiles * (p.offsets ? pairs_s[p.experts] : t.pairs), mine = tiles > first_tile ? (tiles - 1u - first_tile) / stride + 1u : 0u;
     uint32_t e_now = 0;
     auto span = [&](uint64_t tile) {          // tiles come in ascending order
         const uint32_t pair = (uint32_t)(tile / t.wtiles);
@@ -490,12 +521,13 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
         if (lane == 0) {
             bool ok = true, waited = false;
             uint32_t st = 0, turn = 0;
-            for (uint64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            for (uint64_t tile = first_tile; tile < tiles && ok; tile += stride) {
                 const Span s = span(tile);
-                const uint32_t n0 = (uint32_t)(tile % t.wtiles) * kRows;
+                const uint32_t n0 = (uint32_t)(tile % t.wtiles) * WIDE + rank * kRows;
                 auto weights = [&](uint32_t i, uint32_t at) {
-                    mbar_expect(full + at * 8u, Z::bytes);
-                    tma_3d(ring + at * Z::bytes, &t.wmap, i * (kDepth / 2u), n0, s.e, full + at * 8u);
+                    if (rank == 0) mbar_expect(full + at * 8u, PAIR ? 2u * SB : SB);          // of both blocks
+                    if constexpr (PAIR) tma_pair(ring + at * SB, &t.wmap, i * (kDepth / 2u), n0, s.e, full + at * 8u);
+                    else tma_3d(ring + at * SB, &t.wmap, i * (kDepth / 2u), n0, s.e, full + at * 8u);
                 };
                 uint32_t early = 0;
                 if (!waited) {          // the first tile's weights do not depend on the kernel before, which quantises the rows
@@ -507,13 +539,14 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
                     ok = !turn || soon(empty + st * 8u, (turn - 1u) & 1u);
                     if (!ok) { bad_s = 1; break; }
                     if (i >= early) weights(i, st);
-                    tma_3d(ring + st * Z::bytes + Z::x_at, &t.xmap, i * (kDepth / 2u), s.r0, 0, full + st * 8u);
+                    if constexpr (PAIR) tma_pair(ring + st * SB + Z::x_at, &t.xmap, i * (kDepth / 2u), s.r0 + rank * Y::x_rows, 0, full + st * 8u);
+                    else tma_3d(ring + st * SB + Z::x_at, &t.xmap, i * (kDepth / 2u), s.r0, 0, full + st * 8u);
                     if (++st == ST) { st = 0; turn++; }
                 }
             }
         }
     } else if (warp == Y::mma) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             bool ok = true;
             uint32_t st = 0, phase = 0, set = 0, turn = 0;
             for (uint64_t n = 0; n < mine && ok; n++) {
@@ -524,33 +557,33 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
                     ok = soon(full + st * 8u, phase);
                     if (!ok) break;
                     tc_fence_after();
-                    stage_products<TN>(ring + st * Z::bytes, ring + st * Z::bytes + Z::x_at, tmem + set * Z::sum_cols, scales_at + st * Z::scale_cols, i == 0);
-                    tc_commit(empty + st * 8u);
+                    stage_products<TN, PAIR>(ring + st * SB, ring + st * SB + Z::x_at, tmem + set * Z::sum_cols, scales_at + st * Z::scale_cols, i == 0);
+                    if constexpr (PAIR) commit_both(empty + st * 8u); else tc_commit(empty + st * 8u);
                     if (++st == ST) { st = 0; phase ^= 1u; }
                 }
-                if (ok) tc_commit(sums + set * 8u);
+                if (ok) { if constexpr (PAIR) commit_both(sums + set * 8u); else tc_commit(sums + set * 8u); }
                 if (++set == SETS) { set = 0; turn++; }
             }
             if (!ok) bad_s = 1;
         }
     } else if (warp < 4) {
         pdl_wait();
-        uint64_t tile = blockIdx.x;
+        uint64_t tile = first_tile;
         const ScaleRing r{smem_u32(staged), scales_at, ST, full, empty, t.groups, t.w_step, t.x_step, t.w_unit, t.x_unit};
-        if (!bring_scales<TN>(r, (uint32_t)mine, 0, ns, [&](ScaleRows &w, ScaleRows &x) {
+        if (!bring_scales<TN, PAIR>(r, (uint32_t)mine, 0, ns, [&](ScaleRows &w, ScaleRows &x) {
                 const Span s = span(tile);
-                const uint32_t n0 = (uint32_t)(tile % t.wtiles) * kRows;
-                w = ScaleRows{p.ws + s.e * p.ws_expert + (uint64_t)n0 * p.ws_stride, p.ws_stride, p.outputs - n0};
+                const uint32_t n0 = (uint32_t)(tile % t.wtiles) * WIDE + rank * kRows, from = min(n0, p.outputs - 1u);          // (the second block's rows may lie behind the last)
+                w = ScaleRows{p.ws + s.e * p.ws_expert + (uint64_t)from * p.ws_stride, p.ws_stride, p.outputs - from};
                 x = ScaleRows{p.xs + (uint64_t)s.r0 * p.xs_stride, p.xs_stride, s.r1 - s.r0};
-                tile += gridDim.x;
+                tile += stride;
             })) bad_s = 1;
     } else {
         constexpr uint32_t CO = Y::columns, LD = CO < 32 ? 16 : 32, HELD = CO < 64 ? CO : 64;          // sums that a thread reads at once: 64 of fp32, all in 16 bits
         const uint32_t quad = warp & 3u, c0 = ((warp - 4u) >> 2) * CO;
         bool ok = true;
         for (uint64_t i = 0; i < mine; i++) {
-            const uint64_t tile = blockIdx.x + i * gridDim.x;
-            const uint32_t set = (uint32_t)i % SETS, n = (uint32_t)(tile % t.wtiles) * kRows + quad * 32u + lane;
+            const uint64_t tile = first_tile + i * stride;
+            const uint32_t set = (uint32_t)i % SETS, n = (uint32_t)(tile % t.wtiles) * WIDE + rank * kRows + quad * 32u + lane;
             const Span s = span(tile);
             ok = ok && soon_warp(sums + set * 8u, (uint32_t)(i / SETS) & 1u);
             tc_fence_after();
@@ -562,7 +595,7 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
                 } else if constexpr (LD == 16) tc_ld16(from + c, v);
                 else tc_ld32(from + c, v);
             };
-            auto free = [&] { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(room + set * 8u); };
+            auto free = [&] { tc_fence_before(); __syncwarp(); if (lane == 0) { if constexpr (PAIR) arrive_at(room + set * 8u, 0); else mbar_arrive(room + set * 8u); } };
             if (p.out_type == T_F32) {
 #pragma unroll
                 for (uint32_t h = 0; h < CO; h += HELD) {
@@ -604,12 +637,16 @@ __global__ void __launch_bounds__(Many<TN>::threads, 1) k_mx4_many(const __grid_
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    tc_fence_after();
     if (bad_s) {          // copies still in flight land in this block's shared memory before it is given back
         const long long t0 = clock64();
         while (clock64() - t0 < 20000000ll) __nanosleep(1000);
     }
-    if (warp == Y::mma) tc_dealloc(tmem, Y::cols);
+    if constexpr (PAIR) cluster_sync_all();          // nor while the other block's products read it
+    tc_fence_after();
+    if (warp == Y::mma) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Y::cols));
+        else tc_dealloc(tmem, Y::cols);
+    }
 }
 
 // ---- host side ----
@@ -646,10 +683,11 @@ constexpr uint32_t kSms = 148;
 // ks 0: the kernel for many tiles
 template <int TN, uint32_t X>
 cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
+    constexpr bool PAIR = TN == 256;
     static std::atomic<uint64_t> asked[2];          // devices (of the first 64) whose shared-memory limit has been raised
     const bool many = X == T_MX4 && t.ks == 0;
-    void (*const kernel)(TcArgs) = many ? k_mx4_many<TN> : TN <= 128 ? k_mx4_few<TN <= 128 ? TN : 128, X> : nullptr;
-    const uint32_t smem = many ? Many<TN>::smem : Few<TN <= 128 ? TN : 128>::smem(X);
+    void (*const kernel)(TcArgs) = many ? k_mx4_many<TN, PAIR> : TN <= 128 ? k_mx4_few<TN <= 128 ? TN : 128, X> : nullptr;
+    const uint32_t smem = many ? Many<TN, PAIR>::smem : Few<TN <= 128 ? TN : 128>::smem(X);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev > 63 || !(asked[many].load(std::memory_order_acquire) >> dev & 1u))) {
@@ -657,20 +695,20 @@ cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
         if (e == cudaSuccess && dev <= 63) asked[many].fetch_or(1ull << dev, std::memory_order_release);
     }
     if (e != cudaSuccess) return e;
-    if ((X == T_MX4 && !map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, TN)) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
+    if ((X == T_MX4 && !map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, many ? Many<TN, PAIR>::x_rows : TN)) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
         return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
-    cfg.blockDim = dim3(many ? Many<TN>::threads : 192u); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
-    cfg.gridDim = many ? dim3((uint32_t)std::min<uint64_t>(kSms, (uint64_t)t.wtiles * t.pairs)) : dim3(t.wtiles * (t.pairs + (t.p.offsets ? 1u : 0u)), 1, t.ks);
+    cfg.blockDim = dim3(many ? Many<TN, PAIR>::threads : 192u); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = PAIR ? dim3(2u * (uint32_t)std::min<uint64_t>(kSms / 2u, (uint64_t)t.wtiles * t.pairs)) : many ? dim3((uint32_t)std::min<uint64_t>(kSms, (uint64_t)t.wtiles * t.pairs)) : dim3(t.wtiles * (t.pairs + (t.p.offsets ? 1u : 0u)), 1, t.ks);
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
     if (t.made) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
-    if (t.ks > 1) {
+    if (t.ks > 1 || PAIR) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = 1; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs++].val.clusterDim.z = t.ks;
+        attr[cfg.numAttrs].val.clusterDim.x = PAIR ? 2 : 1; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs++].val.clusterDim.z = PAIR ? 1 : t.ks;
     }
     return cudaLaunchKernelEx(&cfg, kernel, t);
 }
@@ -734,7 +772,7 @@ cudaError_t mx4_tc_launch(const Mx4Product &a, const Mx4Plan &plan, uint64_t xs_
         case 32: return launch_of<32, T_MX4>(t, stream);
         case 64: return launch_of<64, T_MX4>(t, stream);
         case 128: return launch_of<128, T_MX4>(t, stream);
-        default: return launch_of<256, T_MX4>(t, stream);
+        default: t.wtiles = (a.outputs + 2u * kRows - 1u) / (2u * kRows); return launch_of<256, T_MX4>(t, stream);
     }
 }
 

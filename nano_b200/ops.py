@@ -326,16 +326,17 @@ def _rows_of(name, x):
 def _mx4(name, m, device=None):
     """(device, groups) of an Mx4"""
     codes, scales, columns = m
-    device = _cuda(name, codes, device)
-    _cuda(name, scales, device)
-    groups = -(-columns // 32)
-    shape, scale_shape, n = codes.shape, scales.shape, codes.dim()
+    at = _cuda(name, codes, device)
+    groups, n = -(-columns // 32), codes.dim()
+    shape, scale_shape = codes.shape, scales.shape
     if codes.dtype is not _U8 or scales.dtype is not _U8 or not n or scales.dim() != n or shape[-1] != 16 * groups or scale_shape[-1] != groups or \
             (shape[0] != scale_shape[0] if n == 2 else shape[:-1] != scale_shape[:-1]):
         _no("%s has uint8 codes [..., %d] and scales [..., %d] for %d columns", name, 16 * groups, groups, columns)
-    if (codes.stride(-1) != 1 and groups) or (scales.stride(-1) != 1 and groups > 1):
+    if not (scales.is_cuda and scales.get_device() == at):
+        _cuda(name, scales, at)
+    if not (codes.is_contiguous() and scales.is_contiguous()) and ((codes.stride(-1) != 1 and groups) or (scales.stride(-1) != 1 and groups > 1)):
         _no("%s: a row's bytes are to be neighbours", name)
-    return device, groups
+    return at, groups
 
 
 def _mx4_rows(name, m):
