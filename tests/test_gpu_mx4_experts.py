@@ -4,6 +4,9 @@ Tolerances.  Quantisation is exact: its scales and numbers are fixed.  A product
 2^-23 of the sum of their magnitudes S at each addition: K 2^-23 S, and half a step of the result's type.  A token's sum over its `top` experts is off by top + 1 roundings of 2^-24 of its terms'
 magnitudes, a scalar product over D columns by D + 1 of them, and each by half a step of its type."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -482,3 +485,161 @@ def test_refusals():
         y = x.clone().requires_grad_()
         g, = torch.autograd.grad((ops.experts_gather(y, r) ** 2).sum(), y, create_graph=True)
         torch.autograd.grad(g.sum(), y)
+
+
+# ---------------- further sizes, strides and orders of calls ----------------
+@pytest.mark.parametrize("rows,outputs,columns", [(3001, 4000, 1000), (1024, 9728, 256), (2048, 5001, 777), (700, 20000, 96), (4096, 2600, 3333)])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_large_products(rows, outputs, columns, kind):
+    """Many tiles: shared by two blocks, and by one, with outputs that end inside a tile."""
+    x, w = random_mx4(rows, columns, seed=rows), random_mx4(outputs, columns, seed=3)
+    x.scales.clamp_(max=129)          # (sums within fp16)
+    w.scales.sub_(5)
+    check_product(x, w, DT[kind])
+
+
+@pytest.mark.parametrize("counts", [[700, 0, 255, 1, 256, 257] * 3, [5000, 1, 0, 3], [300] * 40])
+def test_large_products_of_experts(counts):
+    x, w = random_mx4(sum(counts) + 7, 512, seed=1), random_mx4(len(counts), 1000, 512, seed=2)
+    check_product(x, w, torch.bfloat16, offsets_of(counts))
+    got = check_product(x, w, torch.float32, offsets_of(counts, first=7))
+    assert (got[:7] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 6, 18, 200])
+@pytest.mark.parametrize("columns", [189, 191, 61, 1])
+def test_what_fills_up_a_group_does_not_count(rows, columns):
+    """Rows of an odd number of columns out of longer ones: the rest of the last group, and of its last byte, holds other numbers."""
+    G = -(-columns // 32)
+    x, w = random_mx4(rows, 512, seed=5), random_mx4(130, 512, seed=6)
+    a, b = ops.Mx4(x.codes[:, :16 * G], x.scales[:, :G], columns), ops.Mx4(w.codes[:, :16 * G], w.scales[:, :G], columns)
+    check_product(a, b, torch.float32)
+    we = ops.Mx4(b.codes.expand(2, 130, 16 * G), b.scales.expand(2, 130, G), columns)          # one matrix for all experts
+    check_product(a, we, torch.float32, offsets_of([rows // 2, rows - rows // 2]))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 2, 4, 6, 16, 17, 40])
+@pytest.mark.parametrize("offset,columns", [(0, 640), (1, 640), (3, 517), (8, 96), (2, 2500)])
+def test_products_of_rows_of_numbers_anywhere(kind, rows, offset, columns):
+    big = randn(rows, columns + offset + 5, seed=rows, kind=kind)
+    big[:, :offset] = math.nan
+    big[:, offset + columns:] = math.nan
+    w = ops.mx4_quantize(randn(300, columns, seed=2))
+    x = big[:, offset:offset + columns]
+    got = check_product(x, w, torch.float32)
+    assert torch.equal(got, ops.mx4_product(ops.mx4_quantize(x), w, torch.float32)) or columns == 2500          # (a depth may be split otherwise)
+    check_product(x.t().contiguous().t(), w, torch.float32)
+    check_product(x[:1].expand(rows, columns), w, torch.float32)
+
+
+def test_sort_of_many_places_and_experts():
+    ids = torch.randint(0, 1100, (20000, 5), device="cuda", generator=gen(1))
+    for a, b in zip(ops.experts_sort(ids, 1024), sorted_reference(ids, 1024)):
+        assert torch.equal(a.cpu(), b)
+
+
+def state_of_all(seed):
+    s = dict(x=randn(40, 200, seed=seed), big=randn(600, 512, seed=seed, kind="bf16"), ids=torch.randint(-1, 6, (40, 3), device="cuda", generator=gen(seed)), weights=torch.softmax(randn(40, 3, seed=seed), 1))
+    s["w"], s["wide"], s["we"] = ops.mx4_quantize(randn(300, 200, seed=seed)), ops.mx4_quantize(randn(20000, 512, seed=seed)), ops.mx4_quantize(randn(6, 200, 200, seed=seed))
+    return s
+
+
+def run_of_all(s):
+    r = ops.experts_sort(s["ids"], 6)
+    y = ops.experts_product(ops.experts_gather(s["x"], r), s["we"], r.offsets)
+    return [*r, y, ops.experts_combine(y, r, s["weights"]), ops.mx4_product(s["x"][:2], s["w"]), ops.mx4_product(s["x"], s["w"]), ops.mx4_product(ops.mx4_quantize(s["x"]), s["w"]),
+            ops.mx4_product(s["big"], s["wide"]), ops.mx4_read(ops.mx4_quantize(s["x"][:, 1:]))]
+
+
+def test_two_graphs_that_share_memory():
+    a, b = state_of_all(21), state_of_all(22)
+    want = [[t.clone() for t in run_of_all(s)] for s in (a, b)]
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], torch.cuda.graph_pool_handle()
+    for s in (a, b):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(run_of_all(s))
+        graphs.append(graph)
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(outs[i], want[i]))
+        assert torch.equal(run_of_all(a)[4], want[0][4])
+
+
+def test_all_on_four_streams_at_once():
+    states = [state_of_all(30 + i) for i in range(4)]
+    want = [[t.clone() for t in run_of_all(s)] for s in states]
+    streams = [torch.cuda.Stream() for _ in states]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, stream in zip(states, streams):
+            with torch.cuda.stream(stream):
+                got.append(run_of_all(s))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(g, w))
+
+
+def test_a_captured_step_that_learns():
+    """Forward and backward in one graph, as a training loop captures them."""
+    x, w = randn(64, 96, seed=1).requires_grad_(), randn(64, 2, seed=2).requires_grad_()
+    ids = torch.randint(0, 5, (64, 2), device="cuda", generator=gen(3))
+
+    def step():
+        r = ops.experts_sort(ids, 5)
+        out = ops.experts_combine(torch.tanh(ops.experts_gather(x, r)), r, w)
+        return torch.autograd.grad(out.square().sum(), [x, w])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (5, 6):
+        with torch.no_grad():
+            x.copy_(randn(64, 96, seed=seed))
+        ids.copy_(torch.randint(-1, 5, (64, 2), device="cuda", generator=gen(seed)))
+        graph.replay()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
+def test_a_routing_changed_in_between_is_noticed():
+    _, r = routing_of(8, 2, 4)
+    x = randn(8, 16).requires_grad_()
+    xs = ops.experts_gather(x, r)
+    r.place.fill_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(xs, x, torch.ones_like(xs))
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import test_gpu_mx4_experts as t
+s = t.state_of_all(1)
+ids = torch.randint(0, 1000, (20000, 4), device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = t.run_of_all(s) + list(t.ops.experts_sort(ids, 1000))
+graph.replay()
+torch.cuda.synchronize()
+want = t.run_of_all(s) + list(t.ops.experts_sort(ids, 1000))
+assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(out, want))
+print("the same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=os.path.dirname(here), tests=here)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
