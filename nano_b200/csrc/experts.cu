@@ -127,44 +127,61 @@ __global__ void __launch_bounds__(kSortThreads) k_experts_sort(const SortArgs a,
 // shifted out of two of the row's.
 // ------------------------------------------------------------------------------------------------
 constexpr uint32_t kMoveThreads = 256, kMoveUnits = 4;
-struct GatherArgs { uint8_t *out; const uint8_t *x; const int32_t *order; uint64_t out_stride, x_stride; uint32_t bytes, top, tokens; };
-__device__ __forceinline__ const uint8_t *token_row(const GatherArgs &a, uint32_t r) {          // null: none
+struct GatherArgs { uint8_t *out; const uint8_t *x; const int32_t *order; uint64_t out_stride, x_stride; uint32_t bytes, top, tokens, margin; };
+__device__ __forceinline__ uint32_t token_of(const GatherArgs &a, uint32_t r) {          // `tokens` and more: none
     const int32_t o = __ldg(a.order + r);
-    const uint32_t t = (uint32_t)o / a.top;
-    return o >= 0 && t < a.tokens ? a.x + t * a.x_stride : nullptr;
+    return o >= 0 ? (uint32_t)o / a.top : 0xffffffffu;
 }
-__global__ void __launch_bounds__(kMoveThreads) k_experts_gather(const GatherArgs a, const uint32_t per_row, const uint32_t items) {
+__global__ void __launch_bounds__(kMoveThreads) k_experts_gather(const GatherArgs a, const Divider per_row, const uint32_t items) {
     uint4 v[kMoveUnits] = {};
     const uint32_t i0 = blockIdx.x * kMoveThreads * kMoveUnits + threadIdx.x;
 #pragma unroll
     for (uint32_t j = 0; j < kMoveUnits; j++) {
-        const uint32_t i = i0 + j * kMoveThreads, r = i / per_row;
+        const uint32_t i = i0 + j * kMoveThreads, r = per_row.over(i);
         if (i >= items) break;
-        if (const uint8_t *row = token_row(a, r)) v[j] = __ldg(reinterpret_cast<const uint4 *>(row) + (i - r * per_row));
+        const uint32_t t = token_of(a, r);
+        if (t < a.tokens) v[j] = __ldg(reinterpret_cast<const uint4 *>(a.x + t * a.x_stride) + (i - r * per_row.d));
     }
 #pragma unroll
     for (uint32_t j = 0; j < kMoveUnits; j++) {
-        const uint32_t i = i0 + j * kMoveThreads, r = i / per_row;
+        const uint32_t i = i0 + j * kMoveThreads, r = per_row.over(i);
         if (i >= items) break;
-        reinterpret_cast<uint4 *>(a.out + (uint64_t)r * a.out_stride)[i - r * per_row] = v[j];
+        reinterpret_cast<uint4 *>(a.out + (uint64_t)r * a.out_stride)[i - r * per_row.d] = v[j];
     }
 }
-__global__ void __launch_bounds__(kMoveThreads) k_experts_gather_any(const GatherArgs a, const uint32_t per_row, const uint32_t items) {
-    const uint32_t i = blockIdx.x * kMoveThreads + threadIdx.x, r = i / per_row;
-    if (i >= items) return;
-    uint8_t *to = a.out + (uint64_t)r * a.out_stride;
-    const uint8_t *row = token_row(a, r);
-    const int k = piece_at(to, i - r * per_row);
-    if (k >= (int)a.bytes) return;
-    if (k >= 0 && (uint32_t)k + 16u <= a.bytes) {
-        uint32_t w[4] = {};
-        if (row && inside<16, uint8_t>(a.bytes, k)) load_words<4, true>(row + k, w);
-        else if (row)
+// UNIT: bytes that every row's start and length are multiples of
+template <typename UNIT>
+__global__ void __launch_bounds__(kMoveThreads) k_experts_gather_any(const GatherArgs a, const Divider per_row, const uint32_t items) {
+    constexpr int S = sizeof(UNIT), U = 2;
+    union Piece { uint32_t w[4]; UNIT u[16 / S]; };
+    Piece v[U] = {};
+    int k[U];
+    uint8_t *to[U];
+    const uint32_t i0 = blockIdx.x * kMoveThreads * U + threadIdx.x;
 #pragma unroll
-            for (int j = 0; j < 16; j++) w[j / 4] |= (uint32_t)__ldg(row + k + j) << (8 * (j % 4));
-        *reinterpret_cast<uint4 *>(to + k) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else
-        for (int j = max(k, 0); j < min(k + 16, (int)a.bytes); j++) to[j] = row ? __ldg(row + j) : (uint8_t)0;
+    for (uint32_t u = 0; u < U; u++) {
+        const uint32_t i = i0 + u * kMoveThreads, r = per_row.over(i);
+        k[u] = 0x7fffffff - 16;
+        if (i >= items) continue;
+        to[u] = a.out + (uint64_t)r * a.out_stride;
+        k[u] = piece_at(to[u], i - r * per_row.d);
+        if (k[u] >= (int)a.bytes) continue;
+        const uint32_t t = token_of(a, r);
+        if (t >= a.tokens) continue;
+        const uint8_t *row = a.x + t * a.x_stride;
+        if (between(t, a.tokens, a.margin) || inside<16, uint8_t>(a.bytes, k[u])) load_words<4, (S < 2)>(row + k[u], v[u].w);
+        else
+#pragma unroll
+            for (int j = 0; j < 16; j += S) if (k[u] + j >= 0 && k[u] + j < (int)a.bytes) v[u].u[j / S] = *reinterpret_cast<const UNIT *>(row + k[u] + j);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) {
+        if (k[u] >= (int)a.bytes) continue;
+        if (k[u] >= 0 && (uint32_t)k[u] + 16u <= a.bytes) *reinterpret_cast<uint4 *>(to[u] + k[u]) = make_uint4(v[u].w[0], v[u].w[1], v[u].w[2], v[u].w[3]);
+        else
+#pragma unroll
+            for (int j = 0; j < 16; j += S) if (k[u] + j >= 0 && k[u] + j < (int)a.bytes) *reinterpret_cast<UNIT *>(to[u] + k[u] + j) = v[u].u[j / S];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -174,6 +191,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_experts_gather_any(const Gathe
 struct CombineArgs {
     void *out; const void *y; const float *weights; const int32_t *place, *order; uint64_t out_stride, y_stride; uint32_t tokens, top, rows, columns;
     const void *grad; void *dy; float *dweights; uint64_t grad_stride, dy_stride;
+    uint32_t y_margin, grad_margin;          // (margin_rows)
 };
 template <typename T, Where WHERE>
 __device__ __forceinline__ void combine_piece(const CombineArgs &a, T *out, uint64_t first, int c) {
@@ -190,21 +208,27 @@ __device__ __forceinline__ void combine_piece(const CombineArgs &a, T *out, uint
             for (int k = 0; k < P; k++) sum[k] = fmaf(w, y[k], sum[k]);
         }
     }
-    store_piece<WHERE>(out, a.columns, c, sum);
+    store_piece<WHERE == EVEN ? EVEN : ANY>(out, a.columns, c, sum);
 }
 // BORDERS: every row starts on a 16-byte border and is whole pieces
 template <typename T, bool BORDERS>
-__global__ void __launch_bounds__(kMoveThreads) k_experts_combine(const CombineArgs a, const uint32_t per_row, const uint32_t items) {
+__global__ void __launch_bounds__(kMoveThreads) k_experts_combine(const CombineArgs a, const Divider per_row, const uint32_t items) {
     constexpr int P = 16 / sizeof(T);
-    const uint32_t i = blockIdx.x * kMoveThreads + threadIdx.x, t = i / per_row;
+    const uint32_t i = blockIdx.x * kMoveThreads + threadIdx.x, t = per_row.over(i);
     if (i >= items) return;
     T *out = static_cast<T *>(a.out) + t * a.out_stride;
-    if constexpr (BORDERS) combine_piece<T, EVEN>(a, out, (uint64_t)t * a.top, (int)((i - t * per_row) * P));
+    const uint64_t first = (uint64_t)t * a.top;
+    if constexpr (BORDERS) combine_piece<T, EVEN>(a, out, first, (int)((i - t * per_row.d) * P));
     else {
-        const int c = piece_at(out, i - t * per_row);
+        const int c = piece_at(out, i - t * per_row.d);
         if (c >= (int)a.columns) return;
-        if (inside<P, T>(a.columns, c)) combine_piece<T, INSIDE>(a, out, (uint64_t)t * a.top, c);
-        else combine_piece<T, ANY>(a, out, (uint64_t)t * a.top, c);
+        bool plain = inside<P, T>(a.columns, c);
+        if (!plain) {
+            plain = true;
+            for (uint32_t j = 0; j < a.top; j++) { const uint32_t r = (uint32_t)__ldg(a.place + first + j); plain = plain && (r >= a.rows || between(r, a.rows, a.y_margin)); }
+        }
+        if (plain) combine_piece<T, INSIDE>(a, out, first, c);
+        else combine_piece<T, ANY>(a, out, first, c);
     }
 }
 
@@ -218,13 +242,16 @@ __device__ __forceinline__ float grad_piece(const GradRow<T> &r, int c) {
         if (r.weigh) {
             float v[P];
             load_row<WHERE>(r.y, r.columns, c, v);
+            if (WHERE == INSIDE && (c < 0 || (uint32_t)(c + P) > r.columns))
+#pragma unroll
+                for (int k = 0; k < P; k++) if (c + k < 0 || (uint32_t)(c + k) >= r.columns) d[k] = v[k] = 0.0f;
 #pragma unroll
             for (int k = 0; k < P; k++) dot = fmaf(d[k], v[k], dot);
         }
 #pragma unroll
         for (int k = 0; k < P; k++) d[k] *= r.w;
     }
-    if (r.wanted) store_piece<WHERE>(r.dy, r.columns, c, d);
+    if (r.wanted) store_piece<WHERE == EVEN ? EVEN : ANY>(r.dy, r.columns, c, d);
     return dot;
 }
 // LANES threads to a row
@@ -244,12 +271,12 @@ __global__ void __launch_bounds__(kMoveThreads) k_experts_combine_grad(const Com
 #pragma unroll 4
             for (uint32_t c = lane * P; c < a.columns; c += LANES * P) dot += grad_piece<EVEN>(row, (int)c);
         } else {
-            // pieces [b0, b1) are inside, whatever borders the other rows have; those before and behind go number by number
-            const uint32_t head = (uint32_t)-piece_at(row.dy, 0), pieces = (a.columns + head + P - 1u) / P, b0 = head ? 2u : 1u, b1 = a.columns + head >= 2u * P ? (a.columns + head - 2u * P) / P + 1u : 0u;
-#pragma unroll 4
-            for (uint32_t b = b0 + lane; b < b1; b += LANES) dot += grad_piece<INSIDE>(row, piece_at(row.dy, b));
-            const uint32_t ends = b1 > b0 ? b0 + (pieces - b1) : pieces;
-            for (uint32_t b = lane; b < ends; b += LANES) dot += grad_piece<ANY>(row, piece_at(row.dy, b1 > b0 && b >= b0 ? b1 + (b - b0) : b));
+            const uint32_t pieces = (a.columns + (uint32_t)-piece_at(row.dy, 0) + P - 1u) / P;
+            if (!known || (between(r, a.rows, a.y_margin) && between(t, a.tokens, a.grad_margin))) {
+#pragma unroll 2
+                for (uint32_t b = lane; b < pieces; b += LANES) dot += grad_piece<INSIDE>(row, piece_at(row.dy, b));
+            } else
+                for (uint32_t b = lane; b < pieces; b += LANES) dot += grad_piece<ANY>(row, piece_at(row.dy, b));
         }
     }
     if (!a.dweights) return;
@@ -269,8 +296,8 @@ cudaError_t combine_launch(const CombineArgs &a, cudaStream_t stream) {
         b.place += (uint64_t)t0 * a.top;
         if (a.weights) b.weights += (uint64_t)t0 * a.top;
         const uint32_t items = nt * per_row, blocks = (items + kMoveThreads - 1u) / kMoveThreads;
-        if (all) k_experts_combine<T, true><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
-        else k_experts_combine<T, false><<<blocks, kMoveThreads, 0, stream>>>(b, per_row, items);
+        if (all) k_experts_combine<T, true><<<blocks, kMoveThreads, 0, stream>>>(b, Divider::of(per_row), items);
+        else k_experts_combine<T, false><<<blocks, kMoveThreads, 0, stream>>>(b, Divider::of(per_row), items);
         return cudaGetLastError();
     });
 }
@@ -278,11 +305,11 @@ template <typename T>
 cudaError_t grad_launch(const CombineArgs &a, cudaStream_t stream) {
     const bool even = on_borders<T>(a.dy, a.dy_stride, a.rows) && on_borders<T>(a.y, a.y_stride, a.rows) && on_borders<T>(a.grad, a.grad_stride, a.tokens) && a.columns * sizeof(T) % 16u == 0;
     const uint32_t pieces = (a.columns * (uint32_t)sizeof(T) + 15u) / 16u, n = a.tokens * a.top, all = std::max(n, a.rows);
-    // threads to a row: as many as it has pieces, up to a warp (rows and places are at most 2^30)
+    // Threads to a row: as many as it has pieces, up to a warp; eight for rows of up to 64 pieces that start anywhere, whose ends are stores of single numbers (rows and places are at most 2^30).
+    // us with 8 / 32: 131072 rows of 267 bf16 numbers 61 / 127, but 32768 of 2047 133 / 108, 8000 of 2534 fp32 158 / 62
     auto go = [&](auto kernel, uint32_t lanes) { kernel<<<(uint32_t)(((uint64_t)all * lanes + kMoveThreads - 1u) / kMoveThreads), kMoveThreads, 0, stream>>>(a, n); return cudaGetLastError(); };
-    if (pieces <= 4u) return even ? go(k_experts_combine_grad<T, 4, true>, 4) : go(k_experts_combine_grad<T, 4, false>, 4);
-    if (pieces <= 8u) return even ? go(k_experts_combine_grad<T, 8, true>, 8) : go(k_experts_combine_grad<T, 8, false>, 8);
-    return even ? go(k_experts_combine_grad<T, 32, true>, 32) : go(k_experts_combine_grad<T, 32, false>, 32);
+    if (!even) return pieces <= 64u ? go(k_experts_combine_grad<T, 8, false>, 8) : go(k_experts_combine_grad<T, 32, false>, 32);
+    return pieces <= 4u ? go(k_experts_combine_grad<T, 4, true>, 4) : pieces <= 8u ? go(k_experts_combine_grad<T, 8, true>, 8) : go(k_experts_combine_grad<T, 32, true>, 32);
 }
 
 }  // namespace
@@ -326,7 +353,8 @@ int combine_checked(const nb200_experts_rows *p, bool gradient, nb::CombineArgs 
     auto aligned = [&](const void *x, uint32_t to) { return reinterpret_cast<uintptr_t>(x) % to == 0; };
     if (!aligned(p->out, size) || !aligned(p->y, size) || !aligned(p->grad, size) || !aligned(p->dy, size)) return fail(NB200_EINVAL, "rows are not aligned to their type");
     if (!aligned(p->weights, 4) || !aligned(p->place, 4) || !aligned(p->order, 4) || !aligned(p->dweights, 4)) return fail(NB200_EINVAL, "weights and places are not aligned to their type");
-    *a = nb::CombineArgs{p->out, p->y, p->weights, p->place, p->order, p->out_stride, p->y_stride, p->tokens, p->top, p->rows, p->columns, p->grad, p->dy, p->dweights, p->grad_stride, p->dy_stride};
+    *a = nb::CombineArgs{p->out, p->y, p->weights, p->place, p->order, p->out_stride, p->y_stride, p->tokens, p->top, p->rows, p->columns, p->grad, p->dy, p->dweights, p->grad_stride, p->dy_stride,
+                          nb::margin_rows(p->y_stride * size), nb::margin_rows(p->grad_stride * size)};
     if (gradient) {
         if (p->rows > (uint64_t)p->tokens * p->top) return fail(NB200_EINVAL, "%u rows of %u places", p->rows, p->tokens * p->top);
         const bool some = p->rows && p->columns;
@@ -361,14 +389,22 @@ int nb200_dev_experts_gather(void *out, uint64_t out_stride, const void *x, uint
     if (reinterpret_cast<uintptr_t>(order) % 4u) return fail(NB200_EINVAL, "order is not aligned to its type");
     if (n > 1 && out_stride < row_bytes) return fail(NB200_EINVAL, "rows of the result overlap");
     if (nb200_device_count() <= 0) return fail(NB200_ENODEV, "no CUDA device: nano_b200 has no CPU path");
-    const bool even = (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(x) | out_stride | x_stride | row_bytes) % 16u == 0;
-    const uint32_t bytes = (uint32_t)row_bytes, per_row = even ? bytes / 16u : nb::most_pieces<uint8_t>(bytes, false);
+    const uint64_t at = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(x) | out_stride | x_stride | row_bytes;
+    uint32_t unit = 16;
+    while (at % unit) unit /= 2u;
+    const uint32_t bytes = (uint32_t)row_bytes, per_row = unit == 16u ? bytes / 16u : nb::most_pieces<uint8_t>(bytes, false);
+    const nb::Divider by = nb::Divider::of(per_row);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     NB_CK(nb::in_portions(n, std::max(1u, 0x7fffff00u / per_row), [&](uint32_t r0, uint32_t rows) {
-        const nb::GatherArgs a{static_cast<uint8_t *>(out) + r0 * out_stride, static_cast<const uint8_t *>(x), order + r0, out_stride, x_stride, bytes, top, tokens};
-        const uint32_t items = rows * per_row, each = nb::kMoveThreads * nb::kMoveUnits;
-        if (even) nb::k_experts_gather<<<(items + each - 1u) / each, nb::kMoveThreads, 0, s>>>(a, per_row, items);
-        else nb::k_experts_gather_any<<<(items + nb::kMoveThreads - 1u) / nb::kMoveThreads, nb::kMoveThreads, 0, s>>>(a, per_row, items);
+        const nb::GatherArgs a{static_cast<uint8_t *>(out) + r0 * out_stride, static_cast<const uint8_t *>(x), order + r0, out_stride, x_stride, bytes, top, tokens, nb::margin_rows(x_stride)};
+        const uint32_t items = rows * per_row, each = nb::kMoveThreads * (unit >= 16u ? nb::kMoveUnits : 2u), blocks = (items + each - 1u) / each;
+        switch (unit) {
+            case 16: nb::k_experts_gather<<<blocks, nb::kMoveThreads, 0, s>>>(a, by, items); break;
+            case 8: nb::k_experts_gather_any<uint2><<<blocks, nb::kMoveThreads, 0, s>>>(a, by, items); break;
+            case 4: nb::k_experts_gather_any<uint32_t><<<blocks, nb::kMoveThreads, 0, s>>>(a, by, items); break;
+            case 2: nb::k_experts_gather_any<uint16_t><<<blocks, nb::kMoveThreads, 0, s>>>(a, by, items); break;
+            default: nb::k_experts_gather_any<uint8_t><<<blocks, nb::kMoveThreads, 0, s>>>(a, by, items);
+        }
         return cudaGetLastError();
     }));
     return 0;

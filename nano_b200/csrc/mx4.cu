@@ -27,10 +27,10 @@ __device__ __forceinline__ void fill_scales(const Mx4Rows &a, uint32_t row, uint
 }
 template <typename T> constexpr uint32_t kEach = 32u / sizeof(T);          // numbers to a thread
 template <typename T>
-__device__ __forceinline__ void quantise(const Mx4Rows &a, uint32_t per_row, uint32_t items, uint32_t i) {          // by all threads of a warp
+__device__ __forceinline__ void quantise(const Mx4Rows &a, const Divider &per_row, uint32_t items, uint32_t i) {          // by all threads of a warp
     constexpr uint32_t P = kEach<T>, SHARE = kMx4Group / P;          // threads to a group
     const bool live = i < items;
-    const uint32_t row = live ? i / per_row : 0u, q = live ? i - row * per_row : 0u;
+    const uint32_t row = live ? per_row.over(i) : 0u, q = live ? i - row * per_row.d : 0u;
     float x[P] = {};
     if (live) {
         const T *first = static_cast<const T *>(a.x) + (uint64_t)row * a.x_stride;
@@ -39,29 +39,29 @@ __device__ __forceinline__ void quantise(const Mx4Rows &a, uint32_t per_row, uin
         else if (inside<P, T>(a.columns, k)) load_row<INSIDE>(first, a.columns, k, x);
         else load_row<ANY>(first, a.columns, k, x);
     }
-    uint32_t top = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < P; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);          // (NaN above infinity above all others)
+    uint32_t top = top_bits(x);          // (as whole numbers NaN stands above infinity, above all others)
 #pragma unroll
     for (uint32_t s = 1; s < SHARE; s *= 2u) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
     const uint32_t e = scale_byte(top);
     const float by = inverse_of(e);
-    uint32_t w[P / 8] = {};
 #pragma unroll
-    for (uint32_t j = 0; j < P / 2; j++) w[j / 4] |= codes_of(x[2 * j] * by, x[2 * j + 1] * by) << (8u * (j % 4u));
+    for (uint32_t j = 0; j < P; j++) x[j] *= by;
+    uint32_t w[P / 8];
+#pragma unroll
+    for (uint32_t j = 0; j < P / 8; j++) w[j] = codes_of(x + 8 * j);
     if (!live) return;
     uint8_t *to = a.codes + (uint64_t)row * a.code_stride + q * (P / 2u);
     if constexpr (P == 8) *reinterpret_cast<uint32_t *>(to) = e == 255u ? 0u : w[0];
     else *reinterpret_cast<uint2 *>(to) = e == 255u ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
-    if (q % SHARE == 0) { *scale_at(a, row, q / SHARE) = (uint8_t)e; fill_scales(a, row, q / SHARE, per_row / SHARE); }
+    if (q % SHARE == 0) { *scale_at(a, row, q / SHARE) = (uint8_t)e; fill_scales(a, row, q / SHARE, per_row.d / SHARE); }
 }
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, const uint32_t per_row, const uint32_t items) { quantise<T>(a, per_row, items, blockIdx.x * kThreads + threadIdx.x); }
+__global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, const Divider per_row, const uint32_t items) { quantise<T>(a, per_row, items, blockIdx.x * kThreads + threadIdx.x); }
 
 // And back, by pieces of 16 bytes of the result, 64 bytes to a thread, whose loads are under way at once: the codes of a piece's numbers are nibbles of two neighbouring words, its scales one or two
-// (of one word and one where rows start on borders).  8192 rows of 2560 fp32 numbers FIGURE us
+// (of one word and one where rows start on borders).  8192 rows of 2560 fp32 numbers 16 us (5.9 TB/s), 8191 of 2570 22
 template <typename T, bool BORDERS>
-__global__ void __launch_bounds__(kThreads) k_mx4_read(const Mx4Rows a, const uint32_t per_row, const uint32_t items) {
+__global__ void __launch_bounds__(kThreads) k_mx4_read(const Mx4Rows a, const Divider per_row, const uint32_t items) {
     constexpr int P = 16 / sizeof(T), U = 4;
     const uint32_t groups = (a.columns + kMx4Group - 1u) / kMx4Group, i0 = blockIdx.x * (kThreads * U) + threadIdx.x;
     uint32_t lo[U], hi[U], e0[U], e1[U];
@@ -69,9 +69,9 @@ __global__ void __launch_bounds__(kThreads) k_mx4_read(const Mx4Rows a, const ui
     int k[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const uint32_t i = i0 + u * kThreads, row = i < items ? i / per_row : 0u;
+        const uint32_t i = i0 + u * kThreads, row = i < items ? per_row.over(i) : 0u;
         first[u] = static_cast<T *>(a.x) + (uint64_t)row * a.x_stride;
-        k[u] = i >= items ? 0x7fffffff - P : BORDERS ? (int)((i - row * per_row) * P) : piece_at(first[u], i - row * per_row);
+        k[u] = i >= items ? 0x7fffffff - P : BORDERS ? (int)((i - row * per_row.d) * P) : piece_at(first[u], i - row * per_row.d);
         const uint32_t from = k[u] >= (int)a.columns ? 0u : (uint32_t)max(k[u], 0), at = from / 8u, g = from / kMx4Group;
         const uint8_t *scales = a.scales + (uint64_t)row * a.scale_stride;
         const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.codes + (uint64_t)row * a.code_stride);
@@ -114,10 +114,11 @@ template <typename T>
 cudaError_t read_launch_t(const Mx4Rows &a, cudaStream_t stream) {
     const bool borders = on_borders<T>(a.x, a.x_stride, a.rows);
     const uint32_t per_row = most_pieces<T>(a.columns, borders);
+    const Divider by = Divider::of(per_row);
     return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
         blocks = (blocks + 3u) / 4u;
-        if (borders) k_mx4_read<T, true><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
-        else k_mx4_read<T, false><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
+        if (borders) k_mx4_read<T, true><<<blocks, kThreads, 0, stream>>>(b, by, items);
+        else k_mx4_read<T, false><<<blocks, kThreads, 0, stream>>>(b, by, items);
     });
 }
 
@@ -153,16 +154,16 @@ __device__ __forceinline__ void clean(const Mx4Rows &a, const Codes &from, uint3
     *scale_at(a, row, g) = from.scales[(uint64_t)row * from.scale_stride + g];
     fill_scales(a, row, g, groups);
 }
-struct Prepare { Mx4Rows rows; Codes codes; Scales xs, ws; uint64_t x_items, w_items; uint32_t per_row, first; };
+struct Prepare { Mx4Rows rows; Codes codes; Scales xs, ws; uint64_t x_items, w_items; uint32_t per_row, first; Divider by; };
 enum { kOfF32, kOfBf16, kOfF16, kOfCodes, kOfScales };          // what x is: numbers, codes to be cleaned, codes whose scales are put in order
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) k_mx4_prepare(const __grid_constant__ Prepare a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // the product sets itself up and brings its first weights meanwhile
     if (blockIdx.x >= a.first) { second_order(a.ws, (uint64_t)(blockIdx.x - a.first) * kThreads + threadIdx.x, a.w_items); return; }
     const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    if constexpr (KIND == kOfF32) quantise<float>(a.rows, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
-    else if constexpr (KIND == kOfBf16) quantise<__nv_bfloat16>(a.rows, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
-    else if constexpr (KIND == kOfF16) quantise<__half>(a.rows, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
+    if constexpr (KIND == kOfF32) quantise<float>(a.rows, a.by, (uint32_t)a.x_items, (uint32_t)i);
+    else if constexpr (KIND == kOfBf16) quantise<__nv_bfloat16>(a.rows, a.by, (uint32_t)a.x_items, (uint32_t)i);
+    else if constexpr (KIND == kOfF16) quantise<__half>(a.rows, a.by, (uint32_t)a.x_items, (uint32_t)i);
     else if constexpr (KIND == kOfCodes) clean(a.rows, a.codes, a.per_row, (uint32_t)a.x_items, (uint32_t)i);
     else second_order(a.xs, i, a.x_items);
 }
@@ -171,10 +172,11 @@ __global__ void __launch_bounds__(kThreads) k_mx4_prepare(const __grid_constant_
 
 cudaError_t mx4_quantize_launch(const Mx4Rows &a, cudaStream_t stream) {
     const uint32_t per_row = mx4_groups(a.columns) * (a.type == T_F32 ? 4u : 2u);
+    const Divider by = Divider::of(std::max(1u, per_row));
     return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
-        if (a.type == T_F32) k_mx4_quantize<float><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
-        else if (a.type == T_BF16) k_mx4_quantize<__nv_bfloat16><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
-        else k_mx4_quantize<__half><<<blocks, kThreads, 0, stream>>>(b, per_row, items);
+        if (a.type == T_F32) k_mx4_quantize<float><<<blocks, kThreads, 0, stream>>>(b, by, items);
+        else if (a.type == T_BF16) k_mx4_quantize<__nv_bfloat16><<<blocks, kThreads, 0, stream>>>(b, by, items);
+        else k_mx4_quantize<__half><<<blocks, kThreads, 0, stream>>>(b, by, items);
     });
 }
 cudaError_t mx4_read_launch(const Mx4Rows &a, cudaStream_t stream) {
@@ -192,6 +194,7 @@ cudaError_t mx4_prepare_launch(const Mx4Product &p, const Mx4Plan &plan, uint8_t
     a.xs = Scales{p.xs, p.xs_stride, 0, xs, p.rows, groups, chunks, p.x_type == T_MX4 ? unit(p.xs, p.xs_stride, 0) : 1u};
     const uint32_t kind = p.x_type != T_MX4 ? p.x_type : plan.x_codes ? (uint32_t)kOfCodes : (uint32_t)kOfScales;
     a.per_row = kind == kOfF32 ? groups * 4u : kind < kOfCodes ? groups * 2u : kind == kOfCodes ? groups : chunks;
+    a.by = Divider::of(a.per_row);
     // x in portions whose items are counted in 31 bits, w's scales with the first
     return in_portions(plan.x_codes || plan.x_scales ? p.rows : 1u, std::max(1u, 0x7fffff00u / a.per_row), [&](uint32_t r0, uint32_t n) {
         Prepare b = a;

@@ -5,11 +5,21 @@
 
 namespace nb {
 
-// two numbers to two codes, the first in the lower four bits: nearest, ties to even, beyond 6 (NaN too) to 6
-__device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
+// eight numbers to eight codes, the first in the lowest four bits: nearest, ties to even, beyond 6 (NaN too) to 6
+__device__ __forceinline__ uint32_t codes_of(const float *x) {
     uint32_t r;
-    asm("{\n.reg .b8 c;\ncvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\ncvt.u32.u8 %0, c;\n}" : "=r"(r) : "f"(lo), "f"(hi));
+    asm("{\n.reg .b8 a, b, c, d;\ncvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\ncvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        "mov.b32 %0, {a, b, c, d};\n}" : "=r"(r) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
     return r;
+}
+// the largest magnitude of three, NaN if one is
+__device__ __forceinline__ float top_of(float a, float b, float c) { float r; asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+template <uint32_t N>
+__device__ __forceinline__ uint32_t top_bits(const float (&x)[N]) {          // its bits, of N numbers (a multiple of 8)
+    float t[4] = {};
+#pragma unroll
+    for (uint32_t j = 0; j < N; j += 2) t[j / 2 % 4u] = top_of(t[j / 2 % 4u], x[j], x[j + 1]);
+    return __float_as_uint(top_of(top_of(t[0], t[1], t[2]), t[3], 0.0f)) & 0x7fffffffu;
 }
 // what two codes stand for, as fp16: exact
 __device__ __forceinline__ __half2 numbers_of(uint32_t byte) {

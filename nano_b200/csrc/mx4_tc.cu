@@ -180,14 +180,11 @@ __device__ __forceinline__ void quantise_rows(const RawRows &x, uint32_t s0, uin
         float v[kMx4Group];
         if ((reinterpret_cast<uintptr_t>(first) & 15u) == 0 && k + kMx4Group <= x.columns) load_row<EVEN>(first, x.columns, (int)k, v);
         else load_row<ANY>(first, x.columns, (int)k, v);
-        uint32_t tops[4] = {};
-#pragma unroll
-        for (uint32_t j = 0; j < kMx4Group; j++) tops[j % 4u] = max(tops[j % 4u], __float_as_uint(v[j]) & 0x7fffffffu);
-        const uint32_t e = scale_byte(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+        const uint32_t e = scale_byte(top_bits(v));
         const float by = inverse_of(e);
-        uint32_t w[4] = {};
 #pragma unroll
-        for (uint32_t j = 0; j < kMx4Group / 2; j++) w[j / 4] |= codes_of(v[2 * j] * by, v[2 * j + 1] * by) << (8u * (j % 4u));
+        for (uint32_t j = 0; j < kMx4Group; j++) v[j] *= by;
+        const uint32_t w[4] = {codes_of(v), codes_of(v + 8), codes_of(v + 16), codes_of(v + 24)};
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(codes + step * kRawStep + row * 128u + ((c ^ (row & 7u)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + step * kRawScales + row * kStageGroups + c), "r"(e) : "memory");
     }

@@ -1,11 +1,22 @@
-// rows.cuh -- rows of numbers that start anywhere (mx4.cu, experts.cu): neighbours read as whole 16-byte pieces of memory, of which the wanted part is shifted out, and written as whole pieces.  Nothing
-// outside a row is touched: its ends go number by number.
+// rows.cuh -- rows of numbers that start anywhere (mx4.cu, experts.cu): neighbours read as whole 16-byte pieces of memory, of which the wanted part is shifted out, and written as whole pieces.  What
+// lies beside a row is never written, and read (without being used) only between the first and the last row of its tensor.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
 namespace nb {
+
+// n / d and the rest, for n below 2^31: m = ceil(2^(31 + s) / d), 2^(s - 1) < d <= 2^s, is off by less than 2^-31 of 2^(31 + s) / d, so the quotient is never a whole one too large
+struct Divider {
+    uint32_t d, m, s;
+    static Divider of(uint32_t d) {
+        uint32_t s = 0;
+        while (s < 31u && (1u << s) < d) s++;
+        return Divider{d, (uint32_t)(((1ull << (31u + s)) + d - 1u) / d), s};
+    }
+    __device__ __forceinline__ uint32_t over(uint32_t n) const { return (uint32_t)((uint64_t)n * m >> (31u + s)); }
+};
 
 template <typename T> struct Num;
 template <> struct Num<float> {
@@ -56,7 +67,7 @@ __device__ __forceinline__ void widen_words(const uint32_t (&w)[W], float (&x)[P
 }
 
 // Numbers k .. k + P - 1 (16 or 32 bytes) of the row of n numbers at `first`.  EVEN: rows start on 16-byte borders and n is a multiple of P.  INSIDE: so far from the row's ends (`inside`) that
-// every piece read belongs to it.  ANY: zeros outside of the row (k may be negative)
+// every piece read belongs to it, or in a row between the first and the last of its tensor (`between`): numbers outside of the row are anything.  ANY: zeros outside of the row (k may be negative)
 enum Where { EVEN, INSIDE, ANY };
 template <int P, typename T> __device__ __forceinline__ bool inside(uint32_t n, int k) { constexpr int Q = 16 / (int)sizeof(T); return k >= Q && (uint32_t)(k + P + Q) <= n; }
 template <Where WHERE, int P, typename T>
@@ -86,6 +97,9 @@ __device__ __forceinline__ void store_piece(T *first, uint32_t n, int k, const f
         for (int i = 0; i < P; i++) if (k + i >= 0 && (uint32_t)(k + i) < n) first[k + i] = Num<T>::narrow(x[i]);
 }
 
+// rows at each end of a tensor beside which 32 bytes of it need not lie; all, where rows lie upon one another.  The pieces of a row between them may be read from its first number's to its last's
+inline uint32_t margin_rows(uint64_t stride_bytes) { return stride_bytes ? (uint32_t)((31u + stride_bytes) / stride_bytes) : 0xffffffffu; }
+__device__ __forceinline__ bool between(uint32_t r, uint32_t rows, uint32_t margin) { return r >= margin && r < rows && rows - r > margin; }
 // all rows on 16-byte borders
 template <typename T> inline bool on_borders(const void *at, uint64_t stride, uint32_t rows) { return (reinterpret_cast<uintptr_t>(at) | (rows > 1 ? stride * sizeof(T) : 0u)) % 16u == 0; }
 
