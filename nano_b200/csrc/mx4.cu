@@ -231,7 +231,7 @@ int rows_checked(const nb200_mx4_rows *p, nb::Mx4Rows *a) {
     if (!p->rows) return 0;
     if (!p->codes || !p->scales || !p->x) return fail(NB200_EINVAL, "null argument");
     const uint64_t groups = nb::mx4_groups(p->columns);
-    if (reinterpret_cast<uintptr_t>(p->codes) % 16u || p->code_stride % 16u) return fail(NB200_EINVAL, "codes start and go on in multiples of 16 bytes");
+    if (reinterpret_cast<uintptr_t>(p->codes) % 16u || (p->rows > 1 && p->code_stride % 16u)) return fail(NB200_EINVAL, "codes start and go on in multiples of 16 bytes");
     if (reinterpret_cast<uintptr_t>(p->x) % nb::elem_size(p->type)) return fail(NB200_EINVAL, "numbers are not aligned to their type");
     if (p->rows > 1 && (p->code_stride < groups * 16u || p->scale_stride < groups)) return fail(NB200_EINVAL, "rows of codes or scales overlap");
     *a = nb::Mx4Rows{static_cast<uint8_t *>(p->codes), static_cast<uint8_t *>(p->scales), p->code_stride, p->scale_stride, 16, p->x, p->x_stride, p->type, p->rows, p->columns};
@@ -250,7 +250,7 @@ int product_checked(const nb200_mx4_product *p, nb::Mx4Product *a) {
     const bool codes = p->x_type == NB200_T_MX4;
     const uint64_t groups = nb::mx4_groups(p->columns), row = groups * 16u;
     if (!p->x || !p->w || !p->w_scales || !p->out || (codes && !p->x_scales) || (p->experts && !p->offsets)) return fail(NB200_EINVAL, "null argument");
-    if (reinterpret_cast<uintptr_t>(p->w) % 16u || p->w_stride % 16u || p->w_expert % 16u || (codes && (reinterpret_cast<uintptr_t>(p->x) % 16u || p->x_stride % 16u)))
+    if (reinterpret_cast<uintptr_t>(p->w) % 16u || (p->outputs > 1 && p->w_stride % 16u) || (p->experts > 1 && p->w_expert % 16u) || (codes && (reinterpret_cast<uintptr_t>(p->x) % 16u || (p->rows > 1 && p->x_stride % 16u))))
         return fail(NB200_EINVAL, "codes start and go on in multiples of 16 bytes");
     if (p->w_stride >> 38 || p->w_expert >> 38 || (codes && p->x_stride >> 38)) return fail(NB200_EINVAL, "strides of codes are below 2^38 bytes");
     if ((p->outputs > 1 && p->w_stride < row) || (codes && p->rows > 1 && p->x_stride < row)) return fail(NB200_EINVAL, "rows of codes overlap");

@@ -662,8 +662,8 @@ Encode encoder() {
 // rows of codes in boxes of 128 bytes x `box`; what lies behind a row's last whole byte reads as zeros
 bool map_of(CUtensorMap *m, const void *base, uint32_t columns, uint64_t rows, uint64_t experts, uint64_t stride, uint64_t expert, uint32_t box) {
     const uint64_t bytes = (columns + 1u) / 2u, least = (bytes + 15u) & ~15ull;
-    if (rows == 1) stride = std::max<uint64_t>(stride, least);
-    if (experts == 1) expert = std::max<uint64_t>(stride, least);
+    if (rows == 1) stride = least;
+    if (experts <= 1) expert = least;
     const cuuint64_t dims[3] = {bytes, rows, experts}, strides[2] = {stride, expert};
     const cuuint32_t boxes[3] = {kDepth / 2u, box, 1}, step[3] = {1, 1, 1};
     const Encode e = encoder();

@@ -533,6 +533,30 @@ def test_products_of_rows_of_numbers_anywhere(kind, rows, offset, columns):
     check_product(x[:1].expand(rows, columns), w, torch.float32)
 
 
+def test_one_row_of_a_tensor_of_any_stride():
+    """The stride of a single row is of no account."""
+    K = 300
+    x, w = random_mx4(1, K, seed=1), random_mx4(1, K, seed=2)
+
+    def odd(m):
+        codes, scales = (torch.empty(1000, dtype=torch.uint8, device="cuda").as_strided(t.shape, (7, 1)) for t in (m.codes, m.scales))
+        codes.copy_(m.codes), scales.copy_(m.scales)
+        return ops.Mx4(codes, scales, K)
+    near(ops.mx4_read(odd(x)), values(x).float(), 0.0, "read")
+    check_product(odd(x), odd(w), torch.float32)
+    check_product(odd(x), random_mx4(50, K, seed=3), torch.float32)
+    one = ops.Mx4(odd(w).codes[None], odd(w).scales[None], K)
+    check_product(odd(x), one, torch.float32, offsets_of([1]))
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_products_of_small_and_large_scales(rows):
+    """Numbers from 2^-100 to 2^100 in one product, each output of one size."""
+    x, w = random_mx4(rows, 96, seed=1), random_mx4(201, 96, seed=2)
+    w.scales[:] = torch.arange(27, 228, device="cuda").to(torch.uint8)[:, None]
+    check_product(x, w, torch.float32)
+
+
 def test_sort_of_many_places_and_experts():
     ids = torch.randint(0, 1100, (20000, 5), device="cuda", generator=gen(1))
     for a, b in zip(ops.experts_sort(ids, 1024), sorted_reference(ids, 1024)):
