@@ -76,11 +76,11 @@ def test_product_refusals():
     refused(L.nb200_dev_mx4_product_workspace(product(), None), "null")
     assert L.nb200_dev_mx4_product_workspace(product(), C.byref(need)) == 0 and need.value == 0
     assert L.nb200_dev_mx4_product_workspace(product(x_type=1), C.byref(need)) == 0 and need.value == 0          # few rows are quantised on the way
-    assert L.nb200_dev_mx4_product_workspace(product(x_type=1, columns=100, rows=50), C.byref(need)) == 0 and need.value >= 50 * 4 * 17
+    assert L.nb200_dev_mx4_product_workspace(product(x_type=1, columns=100, rows=5000), C.byref(need)) == 0 and need.value >= 5000 * 4 * 17
     n, text = need.value, "%d are needed" % need.value
-    refused(L.nb200_dev_mx4_product(product(x_type=1, columns=100, rows=50), P, n - 1, None), text)
-    refused(L.nb200_dev_mx4_product(product(x_type=1, columns=100, rows=50), None, n, None), text)
-    refused(L.nb200_dev_mx4_product(product(x_type=1, columns=100, rows=50), P + 8, n, None), text)
+    refused(L.nb200_dev_mx4_product(product(x_type=1, columns=100, rows=5000), P, n - 1, None), text)
+    refused(L.nb200_dev_mx4_product(product(x_type=1, columns=100, rows=5000), None, n, None), text)
+    refused(L.nb200_dev_mx4_product(product(x_type=1, columns=100, rows=5000), P + 8, n, None), text)
 
 
 def sort(order=P, offsets=P, place=P, ids=P, id_bytes=8, n=10, experts=4):
