@@ -325,6 +325,8 @@ def _rows_of(name, x):
 
 def _mx4(name, m, device=None):
     """(device, groups) of an Mx4"""
+    if not isinstance(m, Mx4):
+        _no("%s is an Mx4", name)
     codes, scales, columns = m
     at = _cuda(name, codes, device)
     groups, n = -(-columns // 32), codes.dim()
@@ -385,8 +387,8 @@ def mx4_read(m, dtype=torch.float32):
 
 
 def _product(x, w, offsets, dtype):
-    wc, ws, columns = w
     device, groups = _mx4("w", w)
+    wc, ws, columns = w
     experts = 0
     if offsets is None:
         if wc.dim() != 2:
@@ -475,6 +477,8 @@ def experts_sort(ids, experts):
 
 def _routing(routing, device):
     """(order, place, tokens, top), contiguous"""
+    if not isinstance(routing, Routing):
+        _no("a routing is what experts_sort gives")
     order, _, place = routing
     _cuda("order", order, device)
     _cuda("place", place, device)
@@ -507,9 +511,9 @@ def _combine(y, place, weights, tokens, top):
     return out
 
 
-def _once(grad):
-    """No gradient of a gradient (torch's once_differentiable, without its microseconds)."""
-    if grad.requires_grad and torch.is_grad_enabled():
+def _once(grad, *factors):
+    """No gradient of a gradient, by the one that comes in or by what it is multiplied with."""
+    if torch.is_grad_enabled() and (grad.requires_grad or any(f is not None and f.requires_grad for f in factors)):
         _no("the operators of experts have no gradients of gradients")
 
 
@@ -529,22 +533,26 @@ class _Gather(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, order, place, tokens, top):
-        ctx.save_for_backward(y, weights, order, place)
+        by_y, by_weights = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(y if by_weights else None, weights if by_y else None, order, place)          # (what a gradient is multiplied with)
         ctx.sizes = tokens, top
         return _combine(y, place, weights, tokens, top)
 
     @staticmethod
     def backward(ctx, grad):
-        _once(grad)
         y, weights, order, place = ctx.saved_tensors
+        _once(grad, y, weights)
         tokens, top = ctx.sizes
+        by_y, by_weights = ctx.needs_input_grad[:2]
         device, grad, _, columns, grad_stride = _rows_of("the gradient", grad)
-        _, y, rows, _, y_stride = _rows_of("y", y)
-        dy = y.new_empty(rows, columns) if ctx.needs_input_grad[0] else None
-        dw = None if weights is None or not ctx.needs_input_grad[1] else torch.empty_like(weights)
-        _call(device, lib(True).nb200_dev_experts_combine_grad, _EXPERTS_ROWS(0, 0, y.data_ptr(), y_stride, 0 if weights is None else weights.data_ptr(), place.data_ptr(), order.data_ptr(),
-                                                                              _TYPES[y.dtype], tokens, top, rows, columns, grad.data_ptr(), grad_stride, 0 if dy is None else dy.data_ptr(), columns,
-                                                                              0 if dw is None else dw.data_ptr()))
+        rows, y_stride = order.shape[0], 0
+        if y is not None:
+            _, y, _, _, y_stride = _rows_of("y", y)
+        dy = grad.new_empty(rows, columns) if by_y else None
+        dw = torch.empty_like(place, dtype=torch.float32) if by_weights else None
+        _call(device, lib(True).nb200_dev_experts_combine_grad, _EXPERTS_ROWS(0, 0, 0 if y is None else y.data_ptr(), y_stride, 0 if weights is None else weights.data_ptr(), place.data_ptr(),
+                                                                              order.data_ptr(), _TYPES[grad.dtype], tokens, top, rows, columns, grad.data_ptr(), grad_stride,
+                                                                              0 if dy is None else dy.data_ptr(), columns, 0 if dw is None else dw.data_ptr()))
         return dy, dw, None, None, None, None
 
 

@@ -667,3 +667,59 @@ def test_the_first_calls_of_a_process_may_be_captured():
     here = os.path.dirname(os.path.abspath(__file__))
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=os.path.dirname(here), tests=here)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
+
+
+# ---------------- what a backward pass keeps, and what it cannot give ----------------
+def test_combine_keeps_what_its_gradients_need():
+    """Rows that nothing is multiplied with may change before the backward pass, weights too where only theirs is wanted; what a wanted gradient reads may not."""
+    ids = torch.tensor([[0, 3], [1, -1], [2, 0]], device="cuda")
+    r = ops.experts_sort(ids, 4)
+    y0, w0, g = torch.randn(6, 24, device="cuda"), torch.rand(3, 2, device="cuda"), torch.randn(3, 24, device="cuda")
+
+    def run(y_grad, w_grad, change):
+        leaf, weights = y0.clone().requires_grad_(y_grad), w0.clone().requires_grad_(w_grad)
+        y, w = leaf * 1, weights * 1
+        out = ops.experts_combine(y, r, w)
+        with torch.no_grad():
+            for name in change:
+                {"y": y, "w": w}[name].zero_()
+        out.backward(g)
+        return leaf.grad, weights.grad
+
+    dy, dw = run(True, True, "")
+    known = (r.order >= 0)[:, None]
+    assert torch.equal(dy, torch.where(known, g[r.order.long().clamp(min=0) // 2] * w0.flatten()[r.order.long().clamp(min=0)][:, None], 0))
+    only_y, none = run(True, False, "y")
+    assert torch.equal(only_y, dy) and none is None
+    none, only_w = run(False, True, "w")
+    assert torch.equal(only_w, dw) and none is None
+    for kinds, change in (((True, True), "y"), ((True, True), "w"), ((True, False), "w"), ((False, True), "y")):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            run(*kinds, change)
+
+
+def test_no_gradients_of_gradients():
+    """A graph of the gradient is refused where the gradient depends on something that has one: it would be lost."""
+    ids = torch.tensor([[0, 3], [1, -1], [2, 0]], device="cuda")
+    r = ops.experts_sort(ids, 4)
+    y, w = torch.randn(6, 24, device="cuda", requires_grad=True), torch.rand(3, 2, device="cuda", requires_grad=True)
+    for leaf in (y, w):
+        with pytest.raises(NB200Error, match="gradients of gradients"):
+            torch.autograd.grad(ops.experts_combine(y, r, w).sum(), leaf, create_graph=True)
+    g, = torch.autograd.grad(ops.experts_combine(y, r, w.detach()).sum(), y, create_graph=True)          # of y's nothing depends on y
+    want, = torch.autograd.grad(ops.experts_combine(y, r, w.detach()).sum(), y)
+    assert torch.equal(g, want) and not g.requires_grad
+    x = torch.randn(3, 24, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(ops.experts_gather(x, r).sum(), x, create_graph=True)
+    assert torch.equal(g, torch.tensor([2.0, 1.0, 2.0], device="cuda")[:, None].expand(3, 24))
+
+
+def test_arguments_of_other_kinds_are_refused():
+    x = torch.zeros(3, 64, device="cuda")
+    w, ids = ops.mx4_quantize(x), torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    for f in (lambda: ops.mx4_read(x), lambda: ops.mx4_product(x, x), lambda: ops.mx4_product(w, tuple(w)), lambda: ops.experts_product(x, x[None], torch.tensor([0, 3], dtype=torch.int32, device="cuda"))):
+        with pytest.raises(NB200Error, match="is an Mx4"):
+            f()
+    for f in (lambda: ops.experts_gather(x, ids), lambda: ops.experts_gather(w, ids), lambda: ops.experts_combine(torch.zeros(6, 4, device="cuda"), tuple(ops.experts_sort(ids, 2)))):
+        with pytest.raises(NB200Error, match="what experts_sort gives"):
+            f()
