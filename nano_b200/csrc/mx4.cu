@@ -58,42 +58,65 @@ __device__ __forceinline__ void quantise(const Mx4Rows &a, const Divider &per_ro
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_mx4_quantize(const Mx4Rows a, const Divider per_row, const uint32_t items) { quantise<T>(a, per_row, items, blockIdx.x * kThreads + threadIdx.x); }
 
-// And back, by pieces of 16 bytes of the result, 64 bytes to a thread, whose loads are under way at once: the codes of a piece's numbers are nibbles of two neighbouring words, its scales one or two
-// (of one word and one where rows start on borders).  8192 rows of 2560 fp32 numbers 16 us (5.9 TB/s), 8191 of 2570 22
+// And back, by pieces of 32 bytes of the result, two to a thread, whose loads are under way at once: the codes of a piece's numbers are nibbles of neighbouring words, its scales one or two (of its
+// own words and one where rows start on borders of 32 bytes).  8192 rows of 2560 fp32 numbers 15.6 us (6.1 TB/s), 8191 of 2570
+// 18.3 (with pieces of 16 bytes 16.2 and 22.4); in bf16 8192 of 2560 7.8, 8191 of 2561 12.3
+constexpr uint32_t kReadPieces = 2;
 template <typename T, bool BORDERS>
 __global__ void __launch_bounds__(kThreads) k_mx4_read(const Mx4Rows a, const Divider per_row, const uint32_t items) {
-    constexpr int P = 16 / sizeof(T), U = 4;
+    constexpr int P = 32 / sizeof(T), W = P / 8, U = (int)kReadPieces;
     const uint32_t groups = (a.columns + kMx4Group - 1u) / kMx4Group, i0 = blockIdx.x * (kThreads * U) + threadIdx.x;
-    uint32_t lo[U], hi[U], e0[U], e1[U];
+    uint32_t w[U][W + 1], e0[U], e1[U];
     T *first[U];
     int k[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const uint32_t i = i0 + u * kThreads, row = i < items ? per_row.over(i) : 0u;
         first[u] = static_cast<T *>(a.x) + (uint64_t)row * a.x_stride;
-        k[u] = i >= items ? 0x7fffffff - P : BORDERS ? (int)((i - row * per_row.d) * P) : piece_at(first[u], i - row * per_row.d);
+        k[u] = i >= items ? 0x7fffffff - P : (int)((i - row * per_row.d) * P) - (BORDERS ? 0 : (int)((reinterpret_cast<uintptr_t>(first[u]) & 31u) / sizeof(T)));
         const uint32_t from = k[u] >= (int)a.columns ? 0u : (uint32_t)max(k[u], 0), at = from / 8u, g = from / kMx4Group;
         const uint8_t *scales = a.scales + (uint64_t)row * a.scale_stride;
         const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.codes + (uint64_t)row * a.code_stride);
-        lo[u] = __ldg(codes + at);
+        if (BORDERS && W == 2) { const uint2 v = __ldg(reinterpret_cast<const uint2 *>(codes + at)); w[u][0] = v.x; w[u][W - 1] = v.y; }
+        else {
+#pragma unroll
+            for (int j = 0; j < W + (BORDERS ? 0 : 1); j++) w[u][j] = __ldg(codes + min(at + j, groups * 4u - 1u));
+        }
         e0[u] = scales[g];
-        if (!BORDERS) { hi[u] = __ldg(codes + min(at + 1u, groups * 4u - 1u)); e1[u] = scales[min((from + P - 1u) / kMx4Group, groups - 1u)]; }
+        if (!BORDERS) e1[u] = scales[min((from + P - 1u) / kMx4Group, groups - 1u)];
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (k[u] >= (int)a.columns) continue;
-        const uint32_t from = (uint32_t)max(k[u], 0), border = (from / kMx4Group + 1u) * kMx4Group;
-        uint32_t w = BORDERS ? lo[u] >> (4u * (from % 8u)) : __funnelshift_r(lo[u], hi[u], 4u * (from % 8u));
-        if (!BORDERS && k[u] < 0) w <<= -4 * k[u];          // (the row's first piece: its numbers are the last of it)
+        const uint32_t from = (uint32_t)max(k[u], 0), border = (from / kMx4Group + 1u) * kMx4Group, bits = 4u * (from % 8u);
+        uint64_t v = W == 2 ? (uint64_t)w[u][W - 1] << 32 | w[u][0] : w[u][0];
+        if (!BORDERS) {
+            if (W == 2) v = (uint64_t)__funnelshift_r(w[u][W - 1], w[u][W], bits) << 32 | __funnelshift_r(w[u][0], w[u][W - 1], bits);
+            else v = __funnelshift_r(w[u][0], w[u][1], bits);
+            if (k[u] < 0) v <<= -4 * k[u];          // (the row's first piece: its numbers are the last of it)
+        }
         const float s0 = scale_of(e0[u]), s1 = BORDERS ? s0 : scale_of(e1[u]);
         float x[P];
 #pragma unroll
         for (int j = 0; j < P; j += 2) {
-            const float2 n = __half22float2(numbers_of(w >> (4 * j)));
-            x[j] = n.x * (k[u] + j < (int)border ? s0 : s1);
-            x[j + 1] = n.y * (k[u] + j + 1 < (int)border ? s0 : s1);
+            const float2 n = __half22float2(numbers_of((uint32_t)(v >> (4 * j))));
+            x[j] = n.x * (BORDERS || k[u] + j < (int)border ? s0 : s1);
+            x[j + 1] = n.y * (BORDERS || k[u] + j + 1 < (int)border ? s0 : s1);
         }
-        store_piece<ANY>(first[u], a.columns, k[u], x);
+        union { uint32_t w[8]; T v[P]; } out;
+#pragma unroll
+        for (int j = 0; j < P; j++) out.v[j] = Num<T>::narrow(x[j]);
+        if (k[u] >= 0 && (uint32_t)k[u] + P <= a.columns) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(first[u] + k[u]), "r"(out.w[0]), "r"(out.w[1]), "r"(out.w[2]), "r"(out.w[3]), "r"(out.w[4]), "r"(out.w[5]), "r"(out.w[6]), "r"(out.w[7]) : "memory");
+        } else
+#pragma unroll
+            for (int h = 0; h < P; h += P / 2) {
+                const int kh = k[u] + h;
+                if (kh >= 0 && (uint32_t)kh + P / 2 <= a.columns) *reinterpret_cast<uint4 *>(first[u] + kh) = make_uint4(out.w[h / (P / 8)], out.w[h / (P / 8) + 1], out.w[h / (P / 8) + 2], out.w[h / (P / 8) + 3]);
+                else
+#pragma unroll
+                    for (int j = 0; j < P / 2; j++) if (kh + j >= 0 && kh + j < (int)a.columns) first[u][kh + j] = out.v[h + j];
+            }
     }
 }
 
@@ -112,11 +135,12 @@ cudaError_t by_rows(const Mx4Rows &a, uint32_t per_row, F f) {
 }
 template <typename T>
 cudaError_t read_launch_t(const Mx4Rows &a, cudaStream_t stream) {
-    const bool borders = on_borders<T>(a.x, a.x_stride, a.rows);
-    const uint32_t per_row = most_pieces<T>(a.columns, borders);
+    constexpr uint32_t P = 32u / sizeof(T);
+    const bool borders = (reinterpret_cast<uintptr_t>(a.x) | (a.rows > 1 ? a.x_stride * sizeof(T) : 0u)) % 32u == 0;
+    const uint32_t per_row = borders ? (a.columns + P - 1u) / P : (a.columns + 2u * P - 2u) / P;
     const Divider by = Divider::of(per_row);
     return by_rows(a, per_row, [&](const Mx4Rows &b, uint32_t items, uint32_t blocks) {
-        blocks = (blocks + 3u) / 4u;
+        blocks = (blocks + kReadPieces - 1u) / kReadPieces;
         if (borders) k_mx4_read<T, true><<<blocks, kThreads, 0, stream>>>(b, by, items);
         else k_mx4_read<T, false><<<blocks, kThreads, 0, stream>>>(b, by, items);
     });
