@@ -76,7 +76,8 @@ __device__ __forceinline__ uint4 scales16(const uint8_t *at, uint32_t g, uint32_
 
 // Four warps bring the scales of tile after tile to tensor memory: a thread loads those of one row of W and of one or two of X, eight at a time and kAhead stages ahead, the four exchange them
 // through shared memory, and each writes all of them to its quarter of the lanes.  (tcgen05.cp, which replicates by itself, takes its turn with the products, some 55 cycles for each 128 x 4
-// scales, a quarter of a stage of 128 x 256: 8192 x 8192 x 8192 took 266 us with it.)
+// scales, a quarter of a stage of 128 x 256: 8192 x 8192 x 8192 took 266 us with it.)  Pairs of SMs, whose ring has six stages, hand two of them over at once: one wait for the
+// stores of both (213 us of 227); shorter rings would run dry.
 constexpr uint32_t kAhead = 2, kScaleThreads = 128, kScaleBar = 1;
 __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
@@ -127,29 +128,45 @@ __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles,
                 asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + (j * kScaleThreads + tid) * 8u), "r"(v[d][j].x), "r"(v[d][j].y) : "memory");
                 asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + Z::staged / 2u + (j * kScaleThreads + tid) * 8u), "r"(v[d][j].z), "r"(v[d][j].w) : "memory");
             }
+            const uint32_t st1 = st + 1u == r.stages ? 0u : st + 1u, turn1 = st1 ? turn : turn + 1u;          // the second of the two
             ok = ok && (!turn || soon_warp(r.empty + st * 8u, (turn - 1u) & 1u));
+            if constexpr (PAIR) ok = ok && (count < 2u || !turn1 || soon_warp(r.empty + st1 * 8u, (turn1 - 1u) & 1u));
             if (bar_any(kScaleBar, kScaleThreads, !ok)) return false;          // one verdict for the four warps, which meet here
             ask(v[d]);
-            for (uint32_t h = 0; h < count; h++) {
-                if (h && turn) {          // (the others learn of a wait that runs out where they meet again)
-                    ok = soon_warp(r.empty + st * 8u, (turn - 1u) & 1u);
-                    if (!ok) break;
-                }
-                tc_fence_after();
+            auto write = [&](uint32_t from, uint32_t st) {
                 uint32_t w[8], x[8 * XR];          // [half of the stage][row / 32]
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j]), "=r"(w[4 + j]) : "r"(at + h * (Z::staged / 2u) + (j * 32u + lane) * 8u) : "memory");
+                for (uint32_t j = 0; j < 4; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j]), "=r"(w[4 + j]) : "r"(from + (j * 32u + lane) * 8u) : "memory");
 #pragma unroll
-                for (uint32_t j = 0; j < 4 * XR; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[j]), "=r"(x[4 * XR + j]) : "r"(at + h * (Z::staged / 2u) + (kRows + j * 32u + lane) * 8u) : "memory");
+                for (uint32_t j = 0; j < 4 * XR; j++) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[j]), "=r"(x[4 * XR + j]) : "r"(from + (kRows + j * 32u + lane) * 8u) : "memory");
                 const uint32_t to = r.tmem + ((warp * 32u) << 16) + st * Z::scale_cols;
                 tc_st8(to, w);
                 if constexpr (XR == 1) tc_st8(to + 8u, x); else tc_st16(to + 8u, x);
+            };
+            if constexpr (PAIR) {
+                tc_fence_after();
+                write(at, st);
+                if (count == 2u) write(at + Z::staged / 2u, st1);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) { if constexpr (PAIR) arrive_at(r.full + st * 8u, 0); else mbar_arrive(r.full + st * 8u); }
-                if (++st == r.stages) { st = 0; turn++; }
-            }
+                if (lane < count) arrive_at(r.full + (lane ? st1 : st) * 8u, 0);
+                st += count;
+                if (st >= r.stages) { st -= r.stages; turn++; }
+            } else
+                for (uint32_t h = 0; h < count; h++) {
+                    if (h && turn) {          // (the others learn of a wait that runs out where they meet again)
+                        ok = soon_warp(r.empty + st * 8u, (turn - 1u) & 1u);
+                        if (!ok) break;
+                    }
+                    tc_fence_after();
+                    write(at + h * (Z::staged / 2u), st);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(r.full + st * 8u);
+                    if (++st == r.stages) { st = 0; turn++; }
+                }
             done = done + count == ns ? 0u : done + count;
         }
     return ok;
