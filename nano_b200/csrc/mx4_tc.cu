@@ -77,7 +77,7 @@ __device__ __forceinline__ uint4 scales16(const uint8_t *at, uint32_t g, uint32_
 // Four warps bring the scales of tile after tile to tensor memory: a thread loads those of one row of W and of one or two of X, eight at a time and kAhead stages ahead, the four exchange them
 // through shared memory, and each writes all of them to its quarter of the lanes.  (tcgen05.cp, which replicates by itself, takes its turn with the products, some 55 cycles for each 128 x 4
 // scales, a quarter of a stage of 128 x 256: 8192 x 8192 x 8192 took 266 us with it.)  Pairs of SMs, whose ring has six stages, hand two of them over at once: one wait for the
-// stores of both (213 us of 227); shorter rings would run dry.
+// stores of both (8192 x 8192 x 8192 212 us, one by one 227); shorter rings would run dry.
 constexpr uint32_t kAhead = 2, kScaleThreads = 128, kScaleBar = 1;
 __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
 // another set of columns of tensor memory (tiles of up to 128 rows of X), or, of 256, after the sums have been read out at once, 128 columns to a thread.
 // ------------------------------------------------------------------------------------------------
 // PAIR: two blocks of a cluster share tiles of 256 x TN, 128 rows of W and half of the rows of X to each: a block's shared memory takes in and gives out two thirds of the bytes, and so does L2
-// (8192 x 8192 x 8192 225 us, 4.9 PFLOP/s, instead of 244 with a block to a tile of 128 x 256; 8192 x 9728 x 2560 103 instead of 106).  The
+// (8192 x 8192 x 8192 212 us, 5.2 PFLOP/s, instead of 244 with a block to a tile of 128 x 256; 8192 x 9728 x 2560 100 instead of 106).  The
 // first block issues the products of both; all copies and scales count on its barriers.
 template <int TN, bool PAIR> struct Many {
     static constexpr uint32_t stages = PAIR ? 6 : TN <= 16 ? 11 : TN <= 32 ? 10 : TN <= 64 ? 8 : TN <= 128 ? 6 : 4, sets = TN <= 128 ? 2 : 1, drain = TN <= 32 ? 4 : 8, columns = TN / (drain / 4);          // (columns of a thread)
