@@ -723,3 +723,13 @@ def test_arguments_of_other_kinds_are_refused():
     for f in (lambda: ops.experts_gather(x, ids), lambda: ops.experts_gather(w, ids), lambda: ops.experts_combine(torch.zeros(6, 4, device="cuda"), tuple(ops.experts_sort(ids, 2)))):
         with pytest.raises(NB200Error, match="what experts_sort gives"):
             f()
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 4, 8, 16])
+def test_sort_at_the_borders_of_blocks(blocks):
+    """Lists of just as many places as so many blocks take, and one more or less; of one expert, and of many."""
+    for n in (1024 * blocks - 1, 1024 * blocks, 1024 * blocks + 1):
+        for experts in (1, 33, 1024):
+            ids = torch.randint(-1, experts + 1, (n,), device="cuda", generator=torch.Generator("cuda").manual_seed(n))
+            for a, b in zip(ops.experts_sort(ids, experts), sorted_reference(ids, experts)):
+                assert torch.equal(a.cpu(), b.reshape(a.shape)), (n, experts)
