@@ -359,7 +359,7 @@ int combine_checked(const nb200_experts_rows *p, bool gradient, nb::CombineArgs 
     if (gradient) {
         if (p->rows > (uint64_t)p->tokens * p->top) return fail(NB200_EINVAL, "%u rows of %u places", p->rows, p->tokens * p->top);
         const bool some = p->rows && p->columns;
-        if ((p->dy && p->rows && (!p->order || (some && !p->grad))) || (p->dweights && p->tokens && p->top && (!p->place || (some && (!p->order || !p->y || !p->grad))))) return fail(NB200_EINVAL, "null argument");
+        if ((p->dy && p->rows && (!p->order || (some && !p->grad))) || (p->dweights && p->tokens && p->top && (!p->place || (p->rows && !p->order) || (some && (!p->y || !p->grad))))) return fail(NB200_EINVAL, "null argument");
         if (p->dy && p->rows > 1 && p->dy_stride < p->columns) return fail(NB200_EINVAL, "rows of the gradient overlap");
     } else if (p->tokens && p->columns) {
         if (!p->out || (p->top && (!p->place || (p->rows && !p->y)))) return fail(NB200_EINVAL, "null argument");

@@ -152,3 +152,15 @@ def test_no_cpu_fallback():
               lambda: ops.experts_combine(torch.zeros(2, 4), ops.Routing(*[torch.zeros(4, dtype=torch.int32)] * 3))):
         with pytest.raises(E.NB200Error, match="CUDA tensor"):
             f()
+
+
+def test_gradient_of_weights_wants_order_whatever_the_columns():
+    """The kernel reads order for every row, of rows without columns too; without rows it reads none."""
+    call = E.lib().nb200_dev_experts_combine_grad
+    none = dict(columns=0, dy=None, dy_stride=0, grad=None, y=None)
+    refused(call(combined(order=None, **none), None), "null")
+    refused(call(combined(place=None, **none), None), "null")
+    refused(call(combined(order=None, dy=None), None), "null")
+    if E.device_count() <= 0:          # (these would be launched)
+        assert call(combined(**none), None) == ENODEV
+        assert call(combined(order=None, rows=0, **none), None) == ENODEV
