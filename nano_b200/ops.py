@@ -15,7 +15,7 @@
     experts_combine  experts' rows back to their tokens, weighted and summed
 
 Calls run on the current stream of the tensors' device, wait for nothing and may be captured into a CUDA graph.  Outputs are new tensors; only those of experts_gather and experts_combine
-carry gradients.
+carry gradients, backwards and once.
 Arguments that an operator does not take are refused with NB200Error before anything is queued; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -26,6 +26,7 @@ from array import array
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import engine as E
 from .engine import NB200Error, lib
@@ -511,8 +512,15 @@ def _combine(y, place, weights, tokens, top):
     return out
 
 
+def _no_tangents(*inputs):
+    """No derivatives in forward mode (which autograd.Function is not asked for where no input requires a gradient)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in inputs):
+        _no("the operators of experts have no derivatives in forward mode")
+
+
 def _once(grad, *factors):
     """No gradient of a gradient, by the one that comes in or by what it is multiplied with."""
+    _no_tangents(grad)
     if torch.is_grad_enabled() and (grad.requires_grad or any(f is not None and f.requires_grad for f in factors)):
         _no("the operators of experts have no gradients of gradients")
 
@@ -558,7 +566,7 @@ class _Combine(torch.autograd.Function):
 
 def experts_gather(x, routing):
     """Tokens' rows in the order of their experts: x [tokens, columns] (any type, or an Mx4) -> [tokens * top, columns], row r that of token order[r] / top, zeros behind the last place that has an
-    expert.  A token's gradient is the sum, in 32 bits, of those of its rows (float32, bfloat16 and float16)."""
+    expert.  A token's gradient is the sum, in 32 bits, of those of its rows (float32, bfloat16 and float16); forward mode is refused."""
     if isinstance(x, Mx4):
         device, _ = _mx4("x", x)
         order, _, tokens, top = _routing(routing, device)
@@ -568,6 +576,7 @@ def experts_gather(x, routing):
     order, place, tokens, top = _routing(routing, _cuda("x", x))
     if x.dim() != 2:
         _no("x is [tokens, columns]")
+    _no_tangents(x)
     if x.requires_grad and torch.is_grad_enabled():
         if x.dtype not in _TYPES:
             _no("rows with gradients are float32, bfloat16 or float16")
@@ -577,7 +586,7 @@ def experts_gather(x, routing):
 
 def experts_combine(y, routing, weights=None):
     """Experts' rows back to their tokens: y [rows, columns] (float32, bfloat16 or float16), rows as experts_gather gives them, weights [tokens, top] (ones unless given) ->
-    [tokens, columns], sum over j of weights[t, j] y[place[t, j]] in 32 bits, rounded once to y's type; a place without an expert adds nothing.  Gradients go to y and weights."""
+    [tokens, columns], sum over j of weights[t, j] y[place[t, j]] in 32 bits, rounded once to y's type; a place without an expert adds nothing.  Gradients go to y and weights; forward mode is refused."""
     device = _cuda("y", y)
     order, place, tokens, top = _routing(routing, device)
     if y.dim() != 2 or y.shape[0] != order.shape[0] or y.dtype not in _TYPES:
@@ -588,6 +597,7 @@ def experts_combine(y, routing, weights=None):
             _no("weights are [tokens, top] of numbers")
         if weights.dtype is not torch.float32 or not weights.is_contiguous():
             weights = weights.float().contiguous()
+    _no_tangents(y, weights)
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         return _Combine.apply(y, weights, order, place, tokens, top)
     return _combine(y, place, weights, tokens, top)

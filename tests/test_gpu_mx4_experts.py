@@ -733,3 +733,30 @@ def test_sort_at_the_borders_of_blocks(blocks):
             ids = torch.randint(-1, experts + 1, (n,), device="cuda", generator=torch.Generator("cuda").manual_seed(n))
             for a, b in zip(ops.experts_sort(ids, experts), sorted_reference(ids, experts)):
                 assert torch.equal(a.cpu(), b.reshape(a.shape)), (n, experts)
+
+
+def test_no_derivatives_in_forward_mode():
+    """A tangent that comes in, with an input or with a gradient on its way back, is refused: it would be lost.  Inputs without one go on inside a level too."""
+    forward = torch.autograd.forward_ad
+    ids = torch.tensor([[0, 3], [1, -1], [2, 0]], device="cuda")
+    r = ops.experts_sort(ids, 4)
+    x, y, w = randn(3, 24, seed=1), randn(6, 24, seed=2), randn(3, 2, seed=3)
+    leaf = x.clone().requires_grad_()
+    rows, weights = y.clone().requires_grad_(), w.clone().requires_grad_()
+    with forward.dual_level():
+        def dual(t):
+            return forward.make_dual(t, torch.ones_like(t))
+        refused = [lambda: ops.experts_gather(dual(x), r), lambda: ops.experts_gather(dual(x.double()), r), lambda: ops.experts_gather(dual(leaf), r), lambda: ops.experts_combine(dual(y), r), lambda: ops.experts_combine(dual(y), r, w),
+                   lambda: ops.experts_combine(y, r, dual(w)), lambda: ops.experts_combine(rows, r, dual(w)), lambda: ops.experts_combine(y, r, dual(w.double())), lambda: torch.autograd.grad(ops.experts_gather(leaf, r), leaf, dual(y)),
+                   lambda: torch.autograd.grad(ops.experts_combine(rows, r, weights), rows, dual(x)), lambda: torch.autograd.grad(ops.experts_combine(rows, r, weights), weights, dual(x))]
+        for f in refused:
+            with pytest.raises(NB200Error, match="forward mode"):
+                f()
+            with torch.no_grad(), pytest.raises(NB200Error, match="forward mode"):          # (which is not what forward mode goes by)
+                refused[0]()
+        inside = ops.experts_gather(x, r), ops.experts_combine(y, r, w), torch.autograd.grad(ops.experts_combine(rows, r, weights).sum(), [rows, weights])
+    assert torch.equal(inside[0], ops.experts_gather(x, r)) and torch.equal(inside[1], ops.experts_combine(y, r, w))
+    for a, b in zip(inside[2], torch.autograd.grad(ops.experts_combine(rows, r, weights).sum(), [rows, weights])):
+        assert torch.equal(a, b)
+    with pytest.raises(NB200Error, match="forward mode"):
+        torch.func.jvp(lambda v: ops.experts_gather(v, r), (x,), (torch.ones_like(x),))
