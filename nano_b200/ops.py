@@ -308,6 +308,8 @@ class Routing(NamedTuple):
 def _rows_of(name, x):
     """A tensor [..., columns] of numbers as (device, tensor of neighbouring numbers, rows, columns, stride from row to row)."""
     device = _cuda(name, x)
+    if x.is_neg() or x.is_conj():          # (a view that leaves that to whoever reads it)
+        x = x.resolve_neg().resolve_conj()
     if x.dim() == 2:
         rows, columns = x.shape
         stride, one = x.stride()
@@ -595,8 +597,8 @@ def experts_combine(y, routing, weights=None):
         _cuda("weights", weights, device)
         if weights.shape != routing.place.shape or not weights.is_floating_point():
             _no("weights are [tokens, top] of numbers")
-        if weights.dtype is not torch.float32 or not weights.is_contiguous():
-            weights = weights.float().contiguous()
+        if weights.dtype is not torch.float32 or not weights.is_contiguous() or weights.is_neg():
+            weights = weights.float().contiguous().resolve_neg()
     _no_tangents(y, weights)
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         return _Combine.apply(y, weights, order, place, tokens, top)

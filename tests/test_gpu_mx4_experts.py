@@ -760,3 +760,30 @@ def test_no_derivatives_in_forward_mode():
         assert torch.equal(a, b)
     with pytest.raises(NB200Error, match="forward mode"):
         torch.func.jvp(lambda v: ops.experts_gather(v, r), (x,), (torch.ones_like(x),))
+
+
+def test_conjugated_and_negated_views():
+    """Views whose numbers are not yet what they stand for in memory."""
+    ids = torch.tensor([[0, 3], [1, -1], [2, 0]], device="cuda")
+    r = ops.experts_sort(ids, 4)
+    x, y, w, g = randn(3, 96, seed=1), randn(6, 96, seed=2), randn(3, 2, seed=3), randn(3, 96, seed=4)
+    m, me = ops.mx4_quantize(randn(40, 96, seed=5)), ops.mx4_quantize(randn(4, 40, 96, seed=6))
+    neg = torch._neg_view
+    assert neg(x).is_neg() and neg(x).is_contiguous()
+    z = torch.complex(x, x.flip(0))
+    for v in (z.conj(), z.conj()[:, 3:90], neg(z.conj())):
+        assert torch.equal(ops.experts_gather(v, r), ops.experts_gather(v.clone().resolve_conj().resolve_neg(), r))
+    assert torch.equal(ops.experts_gather(z.conj(), r)[0], z[0].conj().resolve_conj())
+    for a, b in ((neg(x), -x), (neg(x)[:, 3:77], -x[:, 3:77]), (neg(x[0]), -x[0]), (neg(x).view(3, 2, 48), -x.view(3, 2, 48))):
+        assert all(torch.equal(s, t) for s, t in zip(ops.mx4_quantize(a)[:2], ops.mx4_quantize(b)[:2]))
+    for f in (lambda v: ops.mx4_product(v, m), lambda v: ops.experts_gather(v, r)):
+        assert torch.equal(f(neg(x)), f(-x))
+    assert torch.equal(ops.experts_product(neg(y), me, r.offsets), ops.experts_product(-y, me, r.offsets))
+    want = ops.experts_combine(-y, r, -w)
+    assert torch.equal(ops.experts_combine(neg(y), r, neg(w)), want) and torch.equal(ops.experts_combine(neg(y), r, neg(w.double())), ops.experts_combine(-y, r, -w.double()))
+    leaf, weights = y.clone().requires_grad_(), w.clone().requires_grad_()
+    for a, b in zip(torch.autograd.grad(ops.experts_combine(neg(leaf), r, neg(weights)), [leaf, weights], neg(g)), torch.autograd.grad(ops.experts_combine(-leaf, r, -weights), [leaf, weights], -g)):
+        assert torch.equal(a, b)
+    leaf = x.clone().requires_grad_()
+    for a, b in zip(torch.autograd.grad(ops.experts_gather(neg(leaf), r), leaf, neg(y)), torch.autograd.grad(ops.experts_gather(-leaf, r), leaf, -y)):
+        assert torch.equal(a, b)
