@@ -307,21 +307,25 @@ __device__ __forceinline__ void put_rows(const Mx4Product &p, uint64_t row, uint
 }
 
 // Of a tile whose parts lie in the blocks of a cluster, block `part` finishes J rows in every J * ks: the parts added up in the order of the depth.  As many rows at once as there may be: a
-// word of another block is some 200 ns away
+// word of another block is some 200 ns away.  lost: 0, or NaN in a block without its sums, whose part may be anything
 template <int J>
-__device__ __forceinline__ void finish_parts(const Mx4Product &p, uint32_t at, uint32_t part, uint32_t ks, uint32_t r0, uint32_t n, uint32_t rows) {
+__device__ __forceinline__ void finish_parts(const Mx4Product &p, uint32_t at, uint32_t lost, uint32_t part, uint32_t ks, uint32_t r0, uint32_t n, uint32_t rows) {
     for (uint32_t j = part * J; j < rows; j += ks * J) {
-        float f[J] = {};
+        float f[J] = {}, none = 0.0f;
 #pragma unroll 2
         for (uint32_t q = 0; q < ks; q++) {
-            uint32_t peer;
+            uint32_t peer, peer_lost;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + j * kRows * 4u), "r"(q));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer_lost) : "r"(lost), "r"(q));
+            none += ld_cluster_f32(peer_lost);
             float v[J];
 #pragma unroll
             for (uint32_t i = 0; i < J; i++) v[i] = ld_cluster_f32(peer + i * kRows * 4u);          // (a part has all TN rows' places)
 #pragma unroll
             for (uint32_t i = 0; i < J; i++) f[i] += v[i];
         }
+#pragma unroll
+        for (uint32_t i = 0; i < J; i++) f[i] += none;          // (a sum that began with +0 is not -0: adding 0 changes none)
         put_rows<J>(p, r0 + j, n, f, rows - j);
     }
 }
@@ -344,6 +348,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     __shared__ __align__(8) uint64_t bars[2 * ST + 1];
     __shared__ __align__(16) uint8_t staged[X == T_MX4 ? 2u * Z::staged : 2u * kRows * 16u + kRawSteps * kRawScales];
     __shared__ uint32_t tmem_s, bad_s;
+    __shared__ float lost_s;
     __shared__ Span span_s;
     const Mx4Product &p = t.p;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, part = blockIdx.z, n0 = blockIdx.x % t.wtiles * kRows, pair = blockIdx.x / t.wtiles;
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     };
     const uint32_t npre = min(ST, ns), rows = span.r1 - span.r0;
     if (threadIdx.x == 128u) {
-        bad_s = 0;
+        bad_s = 0; lost_s = 0.0f;
         for (uint32_t i = 0; i < ST; i++) { mbar_init(full + i * 8u, 5); mbar_init(empty + i * 8u, 1); }
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -423,8 +428,8 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     __syncwarp();
     const uint32_t quad = warp & 3u, n = n0 + quad * 32u + lane;
     bool ok = true;
-    if (warp < 4) { ok = ns == 0 || soon_warp(done, 0); tc_fence_after(); if (!ok) bad_s = 1; }
-    float *mine = reinterpret_cast<float *>(raw + (ring - smem_u32(raw))) + quad * 32u + lane;          // partial tiles, [TN][128], where the stages were
+    if (warp < 4) { ok = ns == 0 || soon_warp(done, 0); tc_fence_after(); if (!ok) { bad_s = 1; lost_s = NAN; } }
+    float *mine = reinterpret_cast<float *>(raw + (ring - smem_u32(raw))) + quad * 32u + lane;          // partial tiles, [TN][128], where the stages were (and, where a wait ran out, copies may still land)
     if (warp < 4) {
 #pragma unroll 1
         for (uint32_t c = 0; c < TN; c += 16u) {
@@ -443,8 +448,8 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
     if (t.ks > 1) {          // every block of the cluster finishes some of the tile's rows, in turn, its parts added up in the order of the depth
         cluster_sync_all();
         if (warp < 4 && n < p.outputs) {
-            if (TN >= 32 && rows > 4u * t.ks) finish_parts<16>(p, smem_u32(mine), part, t.ks, span.r0, n, rows);
-            else finish_parts<4>(p, smem_u32(mine), part, t.ks, span.r0, n, rows);
+            if (TN >= 32 && rows > 4u * t.ks) finish_parts<16>(p, smem_u32(mine), smem_u32(&lost_s), part, t.ks, span.r0, n, rows);
+            else finish_parts<4>(p, smem_u32(mine), smem_u32(&lost_s), part, t.ks, span.r0, n, rows);
         }
         cluster_sync_all();          // no block leaves while another reads its part
     }
