@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_experts_combine_grad(const Com
             for (uint32_t c = lane * P; c < a.columns; c += LANES * P) dot += grad_piece<EVEN>(row, (int)c);
         } else {
             const uint32_t pieces = (a.columns + (uint32_t)-piece_at(row.dy, 0) + P - 1u) / P;
-            if (!known || (between(r, a.rows, a.y_margin) && between(t, a.tokens, a.grad_margin))) {
+            if (!known || ((!row.weigh || between(r, a.rows, a.y_margin)) && between(t, a.tokens, a.grad_margin))) {          // (y is read for the weights' gradient alone)
 #pragma unroll 2
                 for (uint32_t b = lane; b < pieces; b += LANES) dot += grad_piece<INSIDE>(row, piece_at(row.dy, b));
             } else

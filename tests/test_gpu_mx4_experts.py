@@ -787,3 +787,20 @@ def test_conjugated_and_negated_views():
     leaf = x.clone().requires_grad_()
     for a, b in zip(torch.autograd.grad(ops.experts_gather(neg(leaf), r), leaf, neg(y)), torch.autograd.grad(ops.experts_gather(-leaf, r), leaf, -y)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("columns", [1, 7, 36, 267, 1001])
+def test_gradient_of_rows_alone_at_odd_widths(kind, columns):
+    """Rows that start anywhere, their gradient among NaN: without the weights' gradient y is not there to be read."""
+    _, r = routing_of(90, 3, 5, seed=columns)
+    wide = torch.full((90, columns + 9), math.nan, device="cuda", dtype=DT[kind])
+    g, w = wide[:, 5:5 + columns], randn(90, 2 + 1, seed=2)
+    g.copy_(randn(90, columns, seed=1, kind=kind))
+    y = randn(270, columns, seed=3, kind=kind).requires_grad_()
+    o = r.order.clamp(min=0).long()
+    for weights in (w, None):
+        dy, = torch.autograd.grad(ops.experts_combine(y, r, weights), y, g)
+        factor = torch.ones(270, device="cuda") if weights is None else w.flatten()[o]
+        want = torch.where((r.order >= 0)[:, None], (g.float()[o // 3] * factor[:, None]).to(y.dtype), torch.zeros((), device="cuda", dtype=y.dtype))
+        assert torch.equal(dy, want)          # (one product in 32 bits, rounded once)
