@@ -471,7 +471,8 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
 // (8192 x 8192 x 8192 212 us, 5.2 PFLOP/s, instead of 244 with a block to a tile of 128 x 256; 8192 x 9728 x 2560 100 instead of 106).  The
 // first block issues the products of both; all copies and scales count on its barriers.
 template <int TN, bool PAIR> struct Many {
-    static constexpr uint32_t stages = PAIR ? 6 : TN <= 16 ? 11 : TN <= 32 ? 10 : TN <= 64 ? 8 : TN <= 128 ? 6 : 4, sets = TN <= 128 ? 2 : 1, drain = TN <= 32 ? 4 : 8, columns = TN / (drain / 4);          // (columns of a thread)
+    static_assert(PAIR == (TN == 256));
+    static constexpr uint32_t stages = TN <= 16 ? 11 : TN <= 32 ? 10 : TN <= 64 ? 8 : 6, sets = TN <= 128 ? 2 : 1, drain = TN <= 32 ? 4 : 8, columns = TN / (drain / 4);          // (columns of a thread)
     static constexpr uint32_t tma = 4 + drain, mma = 5 + drain;          // warps 0-3: scales, then those that write results, then one each
     static constexpr uint32_t x_rows = PAIR ? TN / 2 : TN, bytes = (kRows + x_rows) * 128u;          // of a stage
     static constexpr uint32_t cols = cols_for(sets * Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols), threads = 32u * (drain + 6u), smem = stages * bytes + 1024u;
@@ -702,11 +703,13 @@ constexpr uint32_t kSms = 148;
 // ks 0: the kernel for many tiles
 template <int TN, uint32_t X>
 cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
-    constexpr bool PAIR = TN == 256;
+    constexpr bool PAIR = TN == 256, CODES = X == T_MX4;
     static std::atomic<uint64_t> asked[2];          // devices (of the first 64) whose shared-memory limit has been raised
-    const bool many = X == T_MX4 && t.ks == 0;
-    void (*const kernel)(TcArgs) = many ? k_mx4_many<TN, PAIR> : TN <= 128 ? k_mx4_few<TN <= 128 ? TN : 128, X> : nullptr;
-    const uint32_t smem = many ? Many<TN, PAIR>::smem : Few<TN <= 128 ? TN : 128>::smem(X);
+    const bool many = PAIR || (CODES && t.ks == 0);
+    void (*kernel)(TcArgs) = nullptr;
+    uint32_t smem = 0, threads = 192, x_rows = TN;
+    if constexpr (CODES) if (many) { kernel = k_mx4_many<TN, PAIR>; smem = Many<TN, PAIR>::smem; threads = Many<TN, PAIR>::threads; x_rows = Many<TN, PAIR>::x_rows; }
+    if constexpr (!PAIR) if (!many) { kernel = k_mx4_few<TN, X>; smem = Few<TN>::smem(X); }
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev > 63 || !(asked[many].load(std::memory_order_acquire) >> dev & 1u))) {
@@ -714,10 +717,10 @@ cudaError_t launch_of(TcArgs &t, cudaStream_t stream) {
         if (e == cudaSuccess && dev <= 63) asked[many].fetch_or(1ull << dev, std::memory_order_release);
     }
     if (e != cudaSuccess) return e;
-    if ((X == T_MX4 && !map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, many ? Many<TN, PAIR>::x_rows : TN)) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
+    if ((CODES && !map_of(&t.xmap, t.p.x, t.p.columns, t.p.rows, 1, t.p.x_stride, 0, x_rows)) || !map_of(&t.wmap, t.p.w, t.p.columns, t.p.outputs, std::max(1u, t.p.experts), t.p.w_stride, t.p.w_expert, kRows))
         return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
-    cfg.blockDim = dim3(many ? Many<TN, PAIR>::threads : 192u); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cfg.gridDim = PAIR ? dim3(2u * (uint32_t)std::min<uint64_t>(kSms / 2u, (uint64_t)t.wtiles * t.pairs)) : many ? dim3((uint32_t)std::min<uint64_t>(kSms, (uint64_t)t.wtiles * t.pairs)) : dim3(t.wtiles * (t.pairs + (t.p.offsets ? 1u : 0u)), 1, t.ks);
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
