@@ -804,3 +804,43 @@ def test_gradient_of_rows_alone_at_odd_widths(kind, columns):
         factor = torch.ones(270, device="cuda") if weights is None else w.flatten()[o]
         want = torch.where((r.order >= 0)[:, None], (g.float()[o // 3] * factor[:, None]).to(y.dtype), torch.zeros((), device="cuda", dtype=y.dtype))
         assert torch.equal(dy, want)          # (one product in 32 bits, rounded once)
+
+
+@pytest.mark.parametrize("columns", [1, 33, 70, 160, 1000])
+@pytest.mark.parametrize("dropped", [0.0, 0.3, 1.0])
+def test_gather_of_rows_in_4_bits(columns, dropped):
+    """Codes and scales of odd numbers of groups, out of wider rows too, and places without an expert: those stand for zeros."""
+    G = -(-columns // 32)
+    for tokens, top in ((1, 1), (37, 3), (500, 2)):
+        _, r = routing_of(tokens, top, 9, seed=tokens, dropped=dropped)
+        wide = random_mx4(tokens, 32 * (G + 3), seed=columns)
+        live, o = (r.order >= 0)[:, None], r.order.clamp(min=0).long() // top
+        for x in (random_mx4(tokens, columns, seed=columns), ops.Mx4(wide.codes[:, 16:16 + 16 * G], wide.scales[:, 1:1 + G], columns)):
+            got = ops.experts_gather(x, r)
+            assert got.columns == columns and torch.equal(got.codes, torch.where(live, x.codes[o], 0)) and torch.equal(got.scales, torch.where(live, x.scales[o], 0))
+            near(ops.mx4_read(got), torch.where(live, values(x)[o], 0.0).float(), 0.0, "gathered")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 2, 4, 6, 16, 17, 40])
+def test_deep_rows_quantised_on_the_way_and_before(rows, kind):
+    """The two may share the depth out otherwise.  An instruction adds two groups' sums to what is there, three roundings of at most 2^-23 of the magnitudes' sum S; a depth of 2500 is 40 instructions and at
+    most 8 parts: either side is off by (3 x 40 + 8) 2^-23 S."""
+    K = 2500
+    x, w = randn(rows, K, seed=rows, kind=kind), ops.mx4_quantize(randn(300, K, seed=2))
+    size = quantised(x)[1].abs() @ values(w).abs().T
+    near(ops.mx4_product(x, w, torch.float32), ops.mx4_product(ops.mx4_quantize(x), w, torch.float32), 2 * (3 * 40 + 8) * 2.0 ** -23 * size, "quantised on the way")
+
+
+def test_which_calls_carry_gradients():
+    """Rows in 4 bits and their products carry none; a gradient that is to pass them is the caller's to give."""
+    x, w = randn(5, 64, seed=1).requires_grad_(), randn(2, 40, 64, seed=2).requires_grad_()
+    m = ops.mx4_quantize(w)
+    r = ops.experts_sort(torch.tensor([0, 1, 1, -1, 0], device="cuda"), 2)
+    rows = ops.experts_gather(x, r)
+    assert rows.requires_grad and ops.experts_combine(rows, r).requires_grad
+    y = ops.experts_product(rows, m, r.offsets)
+    assert not any(t.requires_grad for t in (m.codes, m.scales, ops.mx4_read(m), ops.mx4_product(x, ops.Mx4(m.codes[0], m.scales[0], 64)), y))
+    weights = torch.rand(5, device="cuda").requires_grad_()
+    g, = torch.autograd.grad(ops.experts_combine(y, r, weights).sum(), weights)          # those of the weights go by the rows as they are
+    near(g, by_token(y, r.place).sum(-1), (40 + 1) * 2.0 ** -24 * by_token(y, r.place).abs().sum(-1), "gradient of weights")
