@@ -359,7 +359,7 @@ def _mx4_rows(name, m):
 
 def mx4_quantize(x):
     """x [..., columns] (float32, bfloat16 or float16; rows of a matrix may lie any stride apart) as an Mx4.  Of a group's largest magnitude a the scale is 2^(floor(log2 a) - 2); a number becomes the
-    nearest code, of two as near the one with an even number, and what lies beyond 6 becomes 6.  A group with a NaN or an infinity is NaN."""
+    nearest code, of two as near the one with an even number, and what lies beyond 6 becomes 6.  A group with a NaN or an infinity is NaN.  No gradient passes."""
     device, x2, rows, columns, stride = _rows_of("x", x)
     kind = _TYPES.get(x.dtype)
     if kind is None:
@@ -377,7 +377,7 @@ def mx4_quantize(x):
 
 
 def mx4_read(m, dtype=torch.float32):
-    """What an Mx4 stands for: [..., columns]."""
+    """What an Mx4 stands for: [..., columns], without a gradient."""
     device, codes, scales = _mx4_rows("m", m)
     kind = _TYPES.get(dtype)
     if kind is None:
@@ -448,13 +448,14 @@ def _product(x, w, offsets, dtype):
 
 def mx4_product(x, w, dtype=None):
     """x w^T: x [..., columns], an Mx4 or numbers (float32, bfloat16 or float16) that the call quantises as mx4_quantize does; w an Mx4 of [outputs, columns] -> [..., outputs] of dtype (x's; bfloat16
-    where x is an Mx4).  Products are exact, sums have 32 bits."""
+    where x is an Mx4).  Products are exact, sums have 32 bits.  No gradient goes to x, whether it asks for one or not."""
     return _product(x, w, None, dtype)
 
 
 def experts_product(x, w, offsets, dtype=None):
     """Rows sorted by expert times their experts' matrices: x [rows, columns] as in mx4_product, w an Mx4 of [experts, outputs, columns], offsets [experts + 1] (int32, Routing.offsets): rows
-    offsets[e] .. offsets[e + 1] - 1 are multiplied with w[e], what lies outside of all becomes zeros -> [rows, outputs].  At most 1024 experts."""
+    offsets[e] .. offsets[e + 1] - 1 are multiplied with w[e], what lies outside of all becomes zeros -> [rows, outputs].  At most 1024 experts.  No gradient goes to x,
+    whether it asks for one or not: between experts_gather and experts_combine it ends here."""
     if offsets is None:
         _no("offsets are [experts + 1] of int32")
     return _product(x, w, offsets, dtype)
