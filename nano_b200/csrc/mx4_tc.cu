@@ -187,7 +187,10 @@ __device__ __forceinline__ bool bring_scales(const ScaleRing &r, uint32_t tiles,
 // Rows of X that are numbers, up to 16 of them: the same four warps quantise all that their block needs of them while W's first stages are on their way, a group to a thread, into swizzled rows as a
 // bulk copy would leave them.  Every block of a tile does so for itself: a launch and a wait less than quantising first.
 struct RawRows { const void *x; uint64_t stride; uint32_t r0, live, columns; };
-constexpr uint32_t kRawSteps = 10, kRawStep = 16u * 128u, kRawScales = 16u * kStageGroups;          // steps of the depth that a block has room for; bytes of codes and of scales of one
+constexpr uint32_t kRawStep = 16u * 128u, kRawScales = 16u * kStageGroups, kRawStages = 5;          // bytes of codes and of scales of a step of the depth; stages of W
+// Steps of the depth that a block has room for where an SM has two blocks of 113 KB: beside W's stages and their alignment, two stages' scales of W and the barriers, 13.  us, so / by a kernel before, with
+// 11 steps: 1 x 9728 x 2816 7.9 / 8.7 (10.5 / 15 a call), 1 x 16000 x 2816 9.1 / 9.4
+constexpr uint32_t kRawSteps = (113u * 1024u - kRawStages * kRows * 128u - 1024u - 2u * kRows * 16u - 256u) / (kRawStep + kRawScales);
 template <typename T>
 __device__ __forceinline__ void quantise_rows(const RawRows &x, uint32_t s0, uint32_t ns, uint32_t codes, uint32_t scales) {
     const uint32_t tid = threadIdx.x & (kScaleThreads - 1u), per_row = ns * kStageGroups;
@@ -334,7 +337,7 @@ __device__ __forceinline__ void finish_parts(const Mx4Product &p, uint32_t at, u
 // Few tiles: a tile's depth is shared by a cluster of ks blocks, each of which finishes some of its rows.  grid (tiles of W x (pairs + 1 with experts), 1, ks)
 // ------------------------------------------------------------------------------------------------
 template <int TN> struct Few {
-    static constexpr uint32_t stages = TN <= 32 ? 5 : TN <= 64 ? 4 : 3, cols = cols_for(Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols);          // up to 107 KB: two blocks to an SM
+    static constexpr uint32_t stages = TN <= 32 ? kRawStages : TN <= 64 ? 4 : 3, cols = cols_for(Tile<TN>::sum_cols + stages * Tile<TN>::scale_cols);          // up to 107 KB: two blocks to an SM
     // codes that bulk copies read come with W's stage by stage; numbers are quantised to a place of their own
     static __host__ __device__ constexpr uint32_t stage(uint32_t x) { return (kRows + (x == T_MX4 ? TN : 0u)) * 128u; }
     static __host__ __device__ constexpr uint32_t smem(uint32_t x) { return stages * stage(x) + (x == T_MX4 ? 0u : kRawSteps * kRawStep) + 1024u; }

@@ -844,3 +844,13 @@ def test_which_calls_carry_gradients():
     weights = torch.rand(5, device="cuda").requires_grad_()
     g, = torch.autograd.grad(ops.experts_combine(y, r, weights).sum(), weights)          # those of the weights go by the rows as they are
     near(g, by_token(y, r.place).sum(-1), (40 + 1) * 2.0 ** -24 * by_token(y, r.place).abs().sum(-1), "gradient of weights")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,outputs,columns", [(1, 9728, 2561), (1, 9728, 2816), (2, 5000, 2999), (4, 9728, 3328), (5, 300, 3327), (1, 9728, 3329), (5, 2000, 3329), (1, 19500, 3328), (3, 9728, 6656), (1, 9728, 6657), (1, 9728, 7000)])
+def test_few_rows_as_deep_as_a_block_has_room_for(kind, rows, outputs, columns):
+    x = randn(rows, columns + 3, seed=rows, kind=kind)[:, 3:]
+    check_product(x, ops.mx4_quantize(randn(outputs, columns, seed=2)), torch.float32)
+    if rows > 1:
+        w = ops.mx4_quantize(randn(3, 500, columns, seed=3))
+        check_product(x, w, torch.float32, offsets_of([1, 0, rows - 1]))

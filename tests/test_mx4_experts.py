@@ -164,3 +164,14 @@ def test_gradient_of_weights_wants_order_whatever_the_columns():
     if E.device_count() <= 0:          # (these would be launched)
         assert call(combined(**none), None) == ENODEV
         assert call(combined(order=None, rows=0, **none), None) == ENODEV
+
+
+def test_one_row_needs_no_workspace_up_to_the_room_of_a_block():
+    """Thirteen steps of 256 columns, twice as many where two blocks share them: at no depth below that is a launch put before the product."""
+    need = C.c_uint64(7)
+    for kind in (0, 1, 2):
+        for outputs in (1, 1000, 9728, 128 * 148):
+            for columns in range(32, 6656 + 1, 32):
+                groups = columns // 32
+                p = product(x_type=kind, x_scales=None, x_stride=columns, columns=columns, rows=1, outputs=outputs, w_stride=16 * groups, ws_stride=groups, out_stride=outputs)
+                assert E.lib().nb200_dev_mx4_product_workspace(p, C.byref(need)) == 0 and need.value == 0, (kind, outputs, columns)
