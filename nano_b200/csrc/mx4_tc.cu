@@ -3,7 +3,8 @@
 // out^T = W X^T in tiles of 128 rows of W x TN rows of X: tcgen05.mma kind::mxf4 takes 64 columns of both and two scales for each row, which lie in tensor memory.
 // A stage is 256 columns: codes by cp.async.bulk.tensor into 128-byte-swizzled rows, scales by four warps.  A lane of tensor memory is an output column, so a warp's stores of one row are
 // neighbours.
-// Every wait has a limit; a block in which one runs out leaves with NaN in its results.
+// Every wait has a limit; a block in which one runs out leaves with NaN in its results, those of a tile that it shares among them.
+// Products are named rows x outputs x columns, times are those on the device with W in memory, not in L2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(192) k_mx4_few(const __grid_constant__ TcArgs 
 // another set of columns of tensor memory (tiles of up to 128 rows of X), or, of 256, after the sums have been read out at once, 128 columns to a thread.
 // ------------------------------------------------------------------------------------------------
 // PAIR: two blocks of a cluster share tiles of 256 x TN, 128 rows of W and half of the rows of X to each: a block's shared memory takes in and gives out two thirds of the bytes, and so does L2
-// (8192 x 8192 x 8192 212 us, 5.2 PFLOP/s, instead of 244 with a block to a tile of 128 x 256; 8192 x 9728 x 2560 100 instead of 106).  The
+// (8192 x 8192 x 8192 225 us instead of 244 with a block to a tile of 128 x 256, 8192 x 9728 x 2560 102 instead of 106; with scales handed over in twos 212, 5.2 PFLOP/s, and 100).  The
 // first block issues the products of both; all copies and scales count on its barriers.
 template <int TN, bool PAIR> struct Many {
     static_assert(PAIR == (TN == 256));
@@ -747,8 +748,10 @@ Mx4Plan mx4_plan(const Mx4Product &a) {
     auto pairs = [&](uint32_t tn) { return a.experts ? std::min(a.rows, a.rows / tn + std::min(a.rows, a.experts)) : (a.rows + tn - 1u) / tn; };
     // Tiles of tn rows of X, ks blocks to one: what takes least by a model of the time in us, fitted to products of 1 to 1024 rows with 1024 x 2048 up to 20000 x 1024 and 2560 x 9728.  A step of the depth
     // takes `one` in the kernel for few tiles (once more for each 296 blocks, which begin anew, a quarter more where SMs have two), parts of a tile and their exchange some more; in the kernel for many tiles `step`,
-    // a tile `tile`.  us as measured, few / many: 1 x 9728 x 2560 7.8 / 8.4 (16 rows), 128 9.8 / 9.0 (128 rows), 256 11.0 / 12.9; split 1 / 2 / 4 / 8: 1 x 2560 x 9728 17.7 / 11.5 / 8.6 / 8.7,
+    // a tile `tile`.  us as measured, with X in codes, few / many: 1 x 9728 x 2560 7.8 / 8.4 (16 rows), 128 9.8 / 9.0 (128 rows), 256 11.0 / 12.9; split 1 / 2 / 4 / 8: 1 x 2560 x 9728 17.7 / 11.5 / 8.6 / 8.7,
     // 1 x 9728 x 2560 7.8 / 7.8 / 10.3 / 15.1; 64 / 128 / 256 rows: 512 x 9728 x 2560 22.3 / 17.8 / 16.6, 128 9.3 / 9.0 / 10.6
+    // Bytes have no term of their own: a block's step brings 18 to 64 KB in the time above, and rounds of tiles took longer than W's bytes in all that was measured (24 x 151936 x 1024 20.9 us, its bytes 14.8;
+    // 132 rows of 64 experts of 1024 x 2048, 44 of them asked for, 17.4 and 7.6)
     struct Cost { uint32_t tn; float one, step, tile; };
     constexpr Cost costs[5] = {{16, 0.40f, 0.33f, 0.40f}, {32, 0.42f, 0.34f, 0.45f}, {64, 0.45f, 0.36f, 0.50f}, {128, 0.60f, 0.34f, 1.1f}, {256, 0.0f, 0.50f, 1.3f}};
     float best = 3e38f;
@@ -768,8 +771,8 @@ Mx4Plan mx4_plan(const Mx4Product &a) {
     r.per = (steps + std::max(1u, r.ks) - 1u) / std::max(1u, r.ks);
     r.x_second = r.ks <= 1u || r.per % 2u == 0;          // (two steps of the depth are sixteen scales)
     const bool codes = a.x_type == T_MX4;
-    // Numbers are quantised by the product itself where a block has few of them (64 rows x steps: four groups to a thread).  us, so / by a kernel before: 1 x 9728 x 2560 7.9 / 8.6, 16 12.4 / 9.2,
-    // 1 x 4096 x 4096 7.3 / 8.5; and a launch less of the host's time, 10.9 / 14.7 a call
+    // Numbers are quantised by the product itself where a block has few of them (64 rows x steps: four groups to a thread).  us, so / by a kernel before: 1 x 9728 x 2560 7.6 / 8.4, 1 x 4096 x 4096 7.0 / 7.3,
+    // 6 x 9728 x 2560 9.3 / 8.4, 16 12.4 / 9.2; and a launch less of the host's time, 10.9 / 15.2 a call, which is what six rows have it for
     const uint32_t mine = std::min(16u, a.experts ? std::min(a.rows, 4u * each) : a.rows);
     if (!codes && r.tn == 16u && r.ks && r.per <= kRawSteps && mine * r.per <= 64u) { r.raw = true; return r; }
     r.x_codes = !codes || a.columns % 2u;
